@@ -113,6 +113,21 @@ typedef struct xt_buffer {
 int xt_gpu_run_buffers(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, void* stream,
                        char** err);
 
+/* Bytes of device memory, beside its buffers, that a launch of `func` works in:
+ * 0 for most programs.  Attention of few rows over many keys gives the keys to
+ * several workgroups, whose partial results meet there. */
+int xt_workspace_bytes(xt_module* m, const char* func, size_t* bytes, char** err);
+
+/* xt_gpu_run and xt_gpu_run_buffers with that workspace: `work_bytes` of device
+ * memory, 16-byte aligned, the launch's own until it has run (two launches that
+ * may run at once, or two captured graphs, need one each).  Without it (NULL, as
+ * in the two calls above) a program runs without splitting: the same result
+ * within rounding, slower. */
+int xt_gpu_run_with(xt_module* m, const char* func, void* const* bufs, const size_t* buf_bytes, int nbufs, void* work,
+                    size_t work_bytes, void* stream, char** err);
+int xt_gpu_run_buffers_with(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, void* work,
+                            size_t work_bytes, void* stream, char** err);
+
 #ifdef __cplusplus
 }
 #endif

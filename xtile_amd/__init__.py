@@ -9,8 +9,10 @@ reference lowers nova further to command text for its "x1" NPU (the
 hand-written HIP kernels: ``compile`` validates and plans the launch, and
 ``launch`` runs the program on the GPU over caller-owned device tensors.
 
-Extensions over the reference API: ``float16`` / ``bfloat16`` dtypes,
-``canonicalize``, ``plan``, ``signature`` and ``launch``.
+Extensions over the reference API: ``float16`` / ``bfloat16`` / ``int32``
+dtypes, ``canonicalize``, ``plan``, ``signature``, ``workspace`` and ``launch``,
+and the ops ``rms_norm``, ``row_scale``, ``quantize``, ``matmul_q4`` (with
+``pack_q4`` / ``unpack_q4``) and ``attend``.
 """
 
 from __future__ import annotations
@@ -29,6 +31,7 @@ from .dsl import (
     DType,
     add,
     astype,
+    attend,
     bfloat16,
     bid,
     convert as _convert_impl,
@@ -37,15 +40,20 @@ from .dsl import (
     float16,
     float32,
     int8,
+    int32,
     kernel,
     load,
     load_conv2d,
     matmul,
+    matmul_q4,
     max,
     mma,
     mul,
+    quantize,
     reciprocal,
     reshape,
+    rms_norm,
+    row_scale,
     rsqrt,
     sigmoid,
     silu,
@@ -169,6 +177,50 @@ def compile(module: Any):
     return module
 
 
+def workspace(module: Any, func: str | None = None) -> int:
+    """Bytes of device memory beside its buffers that a launch of `func` works in
+    (0 for most programs).  ``launch`` takes them from torch's allocator for the
+    time of the launch; a caller of the C ABI hands them over."""
+    return _native.workspace(module, func)
+
+
+# Nibble i of four bytes (low nibble of a byte first) holds weight _Q4_ORDER[i] of
+# eight: nibbles i and i + 4, which one mask takes out of a 32-bit word together,
+# are neighbours along K.
+_Q4_ORDER = (0, 2, 4, 6, 1, 3, 5, 7)
+
+
+def pack_q4(values):
+    """Integer weights -8..7 (a tensor [..., K], K a multiple of 8) as ``matmul_q4``
+    reads them: int8 [..., K / 2], two weights a byte, each 8 more than its value.
+    Of every eight weights the bytes hold, low nibble first: 0 2 4 6 1 3 5 7."""
+    import torch
+
+    if not isinstance(values, torch.Tensor) or values.dtype.is_floating_point or values.dtype.is_complex:
+        raise TypeError("pack_q4 expects a tensor of integers")
+    if values.dim() < 1 or values.shape[-1] % 8:
+        raise ValueError("pack_q4 expects a last dim that is a multiple of 8")
+    if values.numel() and (int(values.min()) < -8 or int(values.max()) > 7):
+        raise ValueError("pack_q4 expects values from -8 to 7")
+    u = (values.to(torch.int16) + 8).reshape(*values.shape[:-1], values.shape[-1] // 8, 8)[..., list(_Q4_ORDER)]
+    packed = u[..., 0::2] | (u[..., 1::2] << 4)
+    return packed.to(torch.uint8).view(torch.int8).reshape(*values.shape[:-1], values.shape[-1] // 2)
+
+
+def unpack_q4(packed):
+    """The int8 weights -8..7 [..., K] that ``pack_q4`` laid out as [..., K / 2]."""
+    import torch
+
+    if not isinstance(packed, torch.Tensor) or packed.dtype != torch.int8:
+        raise TypeError("unpack_q4 expects an int8 tensor")
+    if packed.dim() < 1 or packed.shape[-1] % 4:
+        raise ValueError("unpack_q4 expects a last dim that is a multiple of 4")
+    u = packed.contiguous().view(torch.uint8).reshape(*packed.shape[:-1], packed.shape[-1] // 4, 4)
+    nibbles = torch.stack((u & 15, u >> 4), dim=-1).reshape(*u.shape[:-1], 8)
+    order = [_Q4_ORDER.index(i) for i in range(8)]
+    return (nibbles[..., order].to(torch.int8) - 8).reshape(*packed.shape[:-1], 2 * packed.shape[-1])
+
+
 _TORCH_DTYPES = None
 
 
@@ -249,7 +301,15 @@ def _launch_checked(module: Any, buffers: tuple, func: str | None, stream: Any) 
     with torch.cuda.device(device):
         s = stream if stream is not None else torch.cuda.current_stream(device)
         handle = s.cuda_stream if hasattr(s, "cuda_stream") else int(s)
-        _native.launch(module, sig["name"], ptrs, sizes, handle)
+        nwork = _native.workspace(module, sig["name"])
+        if not nwork:
+            _native.launch(module, sig["name"], ptrs, sizes, handle)
+            return
+        # allocated on the launch's stream, so that what torch hands the memory to
+        # next runs behind the launch, and inside a capture it is the graph's own
+        with torch.cuda.stream(torch.cuda.ExternalStream(handle, device) if handle else torch.cuda.default_stream(device)):
+            work = torch.empty(nwork, dtype=torch.uint8, device=device)
+            _native.launch(module, sig["name"], ptrs, sizes, handle, work.data_ptr(), nwork)
 
 
 def convert(kernel_fn, *, args, grid, double_buffering=False):
@@ -306,6 +366,7 @@ __all__ = [
     "Module",
     "add",
     "astype",
+    "attend",
     "bfloat16",
     "bid",
     "canonicalize",
@@ -316,12 +377,14 @@ __all__ = [
     "exp",
     "float16",
     "float32",
+    "int32",
     "int8",
     "kernel",
     "launch",
     "load",
     "load_conv2d",
     "matmul",
+    "matmul_q4",
     "max",
     "mma",
     "mul",
@@ -330,10 +393,14 @@ __all__ = [
     "nova_optimize",
     "nova_threading",
     "nova_to_x1",
+    "pack_q4",
     "parse",
     "plan",
+    "quantize",
     "reciprocal",
     "reshape",
+    "rms_norm",
+    "row_scale",
     "rsqrt",
     "save_compile_results",
     "save_ir",
@@ -346,6 +413,8 @@ __all__ = [
     "sum",
     "tanh",
     "transpose",
+    "unpack_q4",
+    "workspace",
     "xt_serialize",
     "xt_to_nova",
 ]

@@ -104,6 +104,21 @@ SIGNATURES["xt_gpu_run_buffers"] = (
 )
 
 
+SIGNATURES["xt_workspace_bytes"] = (
+    ctypes.c_int,
+    [ctypes.c_void_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_void_p)],
+)
+SIGNATURES["xt_gpu_run_with"] = (
+    ctypes.c_int,
+    [*SIGNATURES["xt_gpu_run"][1][:5], ctypes.c_void_p, ctypes.c_size_t, *SIGNATURES["xt_gpu_run"][1][5:]],
+)
+SIGNATURES["xt_gpu_run_buffers_with"] = (
+    ctypes.c_int,
+    [*SIGNATURES["xt_gpu_run_buffers"][1][:4], ctypes.c_void_p, ctypes.c_size_t,
+     *SIGNATURES["xt_gpu_run_buffers"][1][4:]],
+)
+
+
 def _load() -> ctypes.CDLL:
     path = os.environ.get("XTILE_AMD_LIB", str(_LIB_PATH))
     if not os.path.exists(path):
@@ -296,8 +311,21 @@ def plan(module: object, func: str | None = None) -> tuple[str, float, float]:
     return _take_string(out), nbytes.value, nflops.value
 
 
-def launch(module: object, func: str | None, ptrs, sizes, stream: int = 0) -> None:
-    """Enqueue `func` on `stream` with device pointers `ptrs` (memref order)."""
+def workspace(module: object, func: str | None = None) -> int:
+    """Bytes of device memory beside its buffers that a launch of `func` works in."""
+    handle = _unwrap(module)
+    out = ctypes.c_size_t()
+    err = ctypes.c_void_p()
+    st = lib.xt_workspace_bytes(handle.ptr, (func or "").encode(), ctypes.byref(out), ctypes.byref(err))
+    msg = _take_string(err)
+    if st != XT_OK:
+        _raise(st, msg, "planning failed")
+    return out.value
+
+
+def launch(module: object, func: str | None, ptrs, sizes, stream: int = 0, work: int = 0, work_bytes: int = 0) -> None:
+    """Enqueue `func` on `stream` with device pointers `ptrs` (memref order) and,
+    where the program uses one, `work_bytes` of workspace at `work`."""
     handle = _unwrap(module)
     n = len(ptrs)
     if len(sizes) != n:
@@ -305,12 +333,14 @@ def launch(module: object, func: str | None, ptrs, sizes, stream: int = 0) -> No
     arr_p = (ctypes.c_void_p * n)(*ptrs)
     arr_s = (ctypes.c_size_t * n)(*sizes)
     err = ctypes.c_void_p()
-    st = lib.xt_gpu_run(
+    st = lib.xt_gpu_run_with(
         handle.ptr,
         (func or "").encode(),
         arr_p,
         arr_s,
         n,
+        ctypes.c_void_p(work or None),
+        work_bytes,
         ctypes.c_void_p(stream or None),
         ctypes.byref(err),
     )

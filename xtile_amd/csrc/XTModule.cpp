@@ -170,8 +170,23 @@ py::tuple plan(py::object module, py::object func) {
   return py::make_tuple(desc, nbytes, nflops);
 }
 
+size_t workspace(py::object module, py::object func) {
+  xt_module* m = unwrap(module);
+  const std::string f = func_arg(func);
+  size_t bytes = 0;
+  char* err = nullptr;
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = xt_workspace_bytes(m, f.c_str(), &bytes, &err);
+  }
+  const std::string msg = take(err);
+  if (st != XT_OK) raise_status(st, msg, "planning failed");
+  return bytes;
+}
+
 void launch(py::object module, py::object func, const std::vector<uintptr_t>& ptrs, const std::vector<size_t>& sizes,
-            uintptr_t stream) {
+            uintptr_t stream, uintptr_t work, size_t work_bytes) {
   xt_module* m = unwrap(module);
   if (ptrs.size() != sizes.size()) throw py::value_error("ptrs and sizes differ in length");
   const std::string f = func_arg(func);
@@ -181,8 +196,8 @@ void launch(py::object module, py::object func, const std::vector<uintptr_t>& pt
   int st;
   {
     py::gil_scoped_release nogil;
-    st = xt_gpu_run(m, f.c_str(), bufs.data(), sizes.data(), (int)bufs.size(), reinterpret_cast<void*>(stream),
-                    &err);
+    st = xt_gpu_run_with(m, f.c_str(), bufs.data(), sizes.data(), (int)bufs.size(), reinterpret_cast<void*>(work),
+                         work_bytes, reinterpret_cast<void*>(stream), &err);
   }
   const std::string msg = take(err);
   if (st != XT_OK) raise_status(st, msg, "launch failed");
@@ -212,7 +227,10 @@ PYBIND11_MODULE(_xtile, m) {
   m.def("signature", &signature, py::arg("module"), py::arg("func") = py::none());
   m.def("plan", &plan, py::arg("module"), py::arg("func") = py::none(),
         "(kernel description, algorithmic bytes, algorithmic FLOPs) of one launch.");
+  m.def("workspace", &workspace, py::arg("module"), py::arg("func") = py::none(),
+        "Bytes of device memory beside its buffers that a launch of func works in.");
   m.def("launch", &launch, py::arg("module"), py::arg("func"), py::arg("ptrs"), py::arg("sizes"),
-        py::arg("stream") = 0, "Enqueue func on stream (a hipStream_t as an integer) over device pointers.");
+        py::arg("stream") = 0, py::arg("work") = 0, py::arg("work_bytes") = 0,
+        "Enqueue func on stream (a hipStream_t as an integer) over device pointers.");
   m.def("version", []() { return std::string(xt_version()); });
 }

@@ -162,12 +162,14 @@ bool get_grid(const Func& f, int32_t grid[3]) {
 }
 
 bool is_pure_op(const std::string& n) {
-  // Ops carrying the `Pure` trait in include/xt/XTOps.td plus arith.constant.
+  // Ops carrying the `Pure` trait in include/xt/XTOps.td plus arith.constant and
+  // the ops this backend adds.
   static const char* pure[] = {"xt.get_tile_block_id", "xt.add", "xt.sub", "xt.mul",
                                "xt.exp", "xt.cos", "xt.sin", "xt.reciprocal", "xt.rsqrt",
                                "xt.sigmoid", "xt.tanh", "xt.silu", "xt.itof", "xt.ftoi",
                                "xt.matmul", "xt.mma", "xt.reduce_sum", "xt.reduce_max",
-                               "xt.reshape", "xt.transpose", "xt.permute", "arith.constant"};
+                               "xt.reshape", "xt.transpose", "xt.permute", "arith.constant",
+                               "xt.rms_norm", "xt.row_scale", "xt.quantize", "xt.matmul_q4", "xt.attend"};
   for (const char* p : pure)
     if (n == p) return true;
   return false;
@@ -242,6 +244,11 @@ const std::unordered_map<std::string, OpInfo>& op_table() {
       {"xt.reshape", {Fmt::Arith, 1, 1, 1}},
       {"xt.transpose", {Fmt::Arith, 1, 1, 1}},
       {"xt.permute", {Fmt::Permute, 1, 1, 1}},
+      {"xt.rms_norm", {Fmt::Arith, 2, 2, 1}},
+      {"xt.row_scale", {Fmt::Arith, 1, 1, 1}},
+      {"xt.quantize", {Fmt::Arith, 2, 2, 1}},
+      {"xt.matmul_q4", {Fmt::Arith, 3, 4, 1}},
+      {"xt.attend", {Fmt::Arith, 3, 9, 1}},
       {"func.return", {Fmt::Return, 0, -1, 0}},
       {"cf.br", {Fmt::Br, 0, -1, 0}},
       {"cf.cond_br", {Fmt::CondBr, 1, 1, 0}},

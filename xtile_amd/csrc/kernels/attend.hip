@@ -1,0 +1,133 @@
+// Masked attention, softmax(scores) v with the scores' cap, distance bias and masks
+// (xtile_amd.dsl.attend states them), in one pass over the keys: a running maximum
+// m and total l of a row, and its sum of weighted values, rescaled where m grows:
+//   s = q . k;  m' = max(m, s);  l = l e^(m - m') + sum e^(s - m');  o likewise
+// Scores and sums are held in 32 bits in units of log2; weights are rounded to the
+// values' type for the second product.
+//
+// The products run transposed, scores^T = K Q^T and result^T = V^T P^T, on 32 x 32
+// MFMA tiles: a lane then holds one query row, so the running maximum and total are
+// one register each, reduced within the lane and with one swap of lane halves, and
+// the weights leave the first product in the registers in which the second takes
+// them (keys in the order of the accumulator's registers; the values are read in
+// that order by transposing LDS reads).
+//
+// All heads that share a key head are one list of rows, token by token, so they
+// read the keys once.  128 rows a workgroup, the keys shared through LDS by its four
+// waves; up to 32 rows (single tokens), every wave takes tiles of keys of its own.
+// Tiles that no row sees are not read: the visible ones are two runs, the prefix
+// and the band between window and diagonal, cut to the keys whose documents may be
+// the rows'.  Few rows over many keys are split over workgroups that leave their
+// m, l and sums in the workspace, and a second kernel joins them.
+#include "attend_kernels.h"
+
+#include "launch.h"
+
+namespace xtk {
+
+extern template hipError_t run_attend<32>(bool, bool, const AttendArgs&, hipStream_t);
+extern template hipError_t run_attend<64>(bool, bool, const AttendArgs&, hipStream_t);
+extern template hipError_t run_attend<96>(bool, bool, const AttendArgs&, hipStream_t);
+extern template hipError_t run_attend<128>(bool, bool, const AttendArgs&, hipStream_t);
+extern template hipError_t run_attend<160>(bool, bool, const AttendArgs&, hipStream_t);
+extern template hipError_t run_attend<192>(bool, bool, const AttendArgs&, hipStream_t);
+extern template hipError_t run_attend<224>(bool, bool, const AttendArgs&, hipStream_t);
+extern template hipError_t run_attend<256>(bool, bool, const AttendArgs&, hipStream_t);
+
+hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipStream_t s, std::string& why) {
+  const xt::AttendPlan& t = p.attend;
+  // a workgroup reads its own query rows before it stores them, so the result may
+  // lie over q, element for element; over nothing else
+  auto apart = [&](int in) {
+    if (in < 0 || (in != t.o.arg && !buffers_meet(p, bufs, t.o.arg, in))) return true;
+    const xt::TileAddr &a = t.q.addr, &b = t.o.addr;
+    if (in == t.q.arg && bufs[in] == bufs[t.o.arg] && t.q.head == t.o.head && t.q.row == t.o.row && a.c0 == b.c0 &&
+        a.sx == b.sx && a.sy == b.sy && a.sz == b.sz)
+      return true;
+    why = "buffer " + std::to_string(t.o.arg) + " is stored and meets buffer " + std::to_string(in) +
+          ", which the program reads elsewhere";
+    return false;
+  };
+  for (const xt::AttendAccess* a : {&t.q, &t.k, &t.v, &t.extra[0], &t.extra[1], &t.extra[2], &t.extra[3], &t.extra[4],
+                                    &t.extra[5]})
+    if (!apart(a->arg)) return hipErrorInvalidValue;
+  auto off = [](const xt::AttendAccess& a) { return TileOff{a.addr.c0, a.addr.sx, a.addr.sy, a.addr.sz}; };
+  auto bytes = [&](const xt::AttendAccess& a) { return static_cast<unsigned char*>(bufs[a.arg]); };
+  AttendArgs a{};
+  a.q = bytes(t.q);
+  a.k = bytes(t.k);
+  a.v = bytes(t.v);
+  a.o = bytes(t.o);
+  a.tq = off(t.q);
+  a.tk = off(t.k);
+  a.tv = off(t.v);
+  a.to = off(t.o);
+  a.q_head = t.q.head;
+  a.q_row = t.q.row;
+  a.o_head = t.o.head;
+  a.o_row = t.o.row;
+  a.ldk = t.k.row;
+  a.ldv = t.v.row;
+  if (t.extra[0].arg >= 0) {
+    a.slopes = static_cast<const float*>(bufs[t.extra[0].arg]);
+    a.tslopes = off(t.extra[0]);
+    a.slope_step = t.extra[0].row;
+  }
+  auto ints = [&](int e, const int*& at, TileOff& o) {
+    if (t.extra[e].arg < 0) return;
+    at = static_cast<const int*>(bufs[t.extra[e].arg]);
+    o = off(t.extra[e]);
+  };
+  ints(1, a.start, a.tstart);
+  ints(2, a.length, a.tlength);
+  ints(3, a.prefix, a.tprefix);
+  ints(4, a.qdocs, a.tqdocs);
+  ints(5, a.kdocs, a.tkdocs);
+  a.qdoc_step = t.extra[4].row;
+  a.heads = static_cast<int>(t.heads);
+  a.rows = static_cast<int>(t.heads * t.rows);
+  a.keys = static_cast<int>(t.keys);
+  const bool few = a.rows <= xt::kAttendFewRows;
+  const int per = static_cast<int>(few ? xt::kAttendFewRows : xt::kAttendRows);
+  a.tiles = (a.rows + per - 1) / per;
+  a.splits = work ? t.splits : 1;
+  a.work = static_cast<float*>(work);
+  const long long blocks = grid_blocks(p), nwg = blocks * a.tiles * a.splits;
+  if (!grid_fits(nwg, 256) || (a.splits > 1 && !grid_fits(blocks * a.rows, 256))) {
+    why = "attend: " + std::to_string(nwg) + " workgroups exceed one launch";
+    return hipErrorInvalidValue;
+  }
+  a.nwg = static_cast<int>(nwg);
+  a.blocks = block_decode(p.grid[0], p.grid[1], false);
+  a.d_heads = div31(a.heads);
+  a.d_work = div31(a.tiles * a.splits);
+  a.d_splits = div31(a.splits);
+  a.scale_log2 = t.scale * 1.44269504088896340736f;
+  if (t.cap > 0) {
+    a.cap_in = 2.0f * t.scale * 1.44269504088896340736f / t.cap;
+    a.cap_log2 = t.cap * 1.44269504088896340736f;
+  }
+  a.causal = t.causal;
+  a.window = static_cast<int>(std::min<int64_t>(t.window, 1 << 30));
+  // DMA takes 16-byte aligned rows, of which 64 lie within a descriptor's 4 GiB;
+  // other rows go through registers
+  auto chunks = [&](const xt::AttendAccess& x) {
+    const xt::TileAddr& d = x.addr;
+    return reinterpret_cast<uintptr_t>(bufs[x.arg]) % 16 == 0 && x.row % 8 == 0 && d.c0 % 8 == 0 && d.sx % 8 == 0 &&
+           d.sy % 8 == 0 && d.sz % 8 == 0;
+  };
+  a.dma = chunks(t.k) && chunks(t.v);
+  const bool b = t.elem == xt::Elem::BF16;
+  switch (t.d) {
+    case 32: return run_attend<32>(b, few, a, s);
+    case 64: return run_attend<64>(b, few, a, s);
+    case 96: return run_attend<96>(b, few, a, s);
+    case 128: return run_attend<128>(b, few, a, s);
+    case 160: return run_attend<160>(b, few, a, s);
+    case 192: return run_attend<192>(b, few, a, s);
+    case 224: return run_attend<224>(b, few, a, s);
+    default: return run_attend<256>(b, few, a, s);
+  }
+}
+
+}  // namespace xtk

@@ -1,0 +1,775 @@
+// The attention kernels: see attend.hip for the mathematics and the choices.
+#pragma once
+
+#include "common.h"
+
+namespace xtk {
+
+struct AttendArgs {
+  const unsigned char* q;
+  const unsigned char* k;
+  const unsigned char* v;
+  unsigned char* o;
+  const float* slopes;
+  const int *start, *length, *prefix, *qdocs, *kdocs;
+  TileOff tq, tk, tv, to, tslopes, tstart, tlength, tprefix, tqdocs, tkdocs;  // element offsets
+  long long q_head, q_row, o_head, o_row, ldk, ldv, slope_step, qdoc_step;   // strides in elements
+  BlockDecode blocks;
+  Div31 d_heads, d_work, d_splits;  // d_work: row tiles x splits of a Block
+  int heads, rows, keys;            // rows: query rows of a Block, heads x tokens
+  int tiles, splits, nwg;
+  float scale_log2;  // scale * log2 e, what the products are multiplied by without a cap
+  float cap_in, cap_log2;  // 2 scale log2 e / cap and cap * log2 e; cap_log2 0: no cap
+  int causal, window, dma;
+  float* work;
+};
+
+// attend_*.hip, one instantiation each for d of 32, 64, ... 256.
+template <int D>
+hipError_t run_attend(bool bf16, bool few, const AttendArgs& a, hipStream_t s);
+
+}  // namespace xtk
+
+#ifdef XTK_ATTEND_KERNELS
+
+#include "launch.h"
+
+namespace xtk {
+namespace {
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) unsigned char lds_t;
+typedef unsigned u4a __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u2a __attribute__((ext_vector_type(2), aligned(2)));
+
+constexpr int kFar = 1 << 30;  // positions are held within this
+
+// Four bytes a lane into LDS by DMA; as dma16.
+__device__ __forceinline__ void dma4(i32x4 rsrc, unsigned lds, unsigned voff) {
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
+}
+
+__device__ __forceinline__ float both_halves(float v, bool is_max) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float a = __builtin_bit_cast(float, (unsigned)r[0]), b = __builtin_bit_cast(float, (unsigned)r[1]);
+  return is_max ? fmaxf(a, b) : a + b;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float16v mma(uint4v a, uint4v b, float16v c) {
+  if constexpr (BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+template <bool BF16>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  if constexpr (BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, b2{(__bf16)a, (__bf16)b});
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, h2{(_Float16)a, (_Float16)b});
+  }
+}
+
+// What one wave's 32 query rows see, and its running softmax.  Lane (c = lane % 32,
+// h = lane / 32) holds row c; of a tile of 32 keys it holds the scores of keys
+// 8 (r / 4) + 4 h + r % 4 in register r, and of the result columns
+// 32 n + 8 (r / 4) + 4 h + r % 4 in register r of acc[n].
+template <int D, bool BF16>
+struct Rows {
+  static constexpr int N = D / 32, KK = D / 16;
+  static constexpr int PITCH = 2 * D;  // bytes of a key row in LDS
+
+  // Where a key row's 16-byte chunks lie in LDS: chunk c at c ^ ksw (keys), c ^ vsw
+  // (values), so that the 16 rows of a fragment read, and the four rows of a
+  // transposing read, fall into distinct banks for every D.
+  static __device__ __forceinline__ int ksw(int row) {
+    return D % 128 == 0 ? row & 15 : D % 64 == 0 ? (row >> 1) & 7 : (row >> 2) & 3;
+  }
+  static __device__ __forceinline__ int vsw(int row) {
+    return D % 128 == 0 ? 4 * (row & 3) : D % 64 == 0 ? 4 * ((row >> 1) & 1) : 0;
+  }
+
+  int lane, col, hi;
+  int row, token;        // this lane's row of the Block (the last one past the end) and its token
+  int pos, above, below; // sees key j when below < j <= above (or j < prefix)
+  int p0, p1;            // positions of the wave's first and last row
+  float slope;           // times log2 e
+  int doc;
+  uint4v q[KK];
+  float16v acc[N];
+  float m, l;
+  int vkey, vchunk;      // LDS offset of this lane's part of a value fragment
+
+  __device__ __forceinline__ void begin(const AttendArgs& p, int first, int bx, int by, int bz, int start) {
+    lane = threadIdx.x & 63;
+    col = lane & 31;
+    hi = lane >> 5;
+    row = min(first + col, p.rows - 1);
+    token = (int)p.d_heads((unsigned)row);
+    const int head = row - token * p.heads;
+    pos = start + token;
+    p0 = start + (int)p.d_heads((unsigned)min(first, p.rows - 1));
+    p1 = start + (int)p.d_heads((unsigned)min(first + 31, p.rows - 1));
+    above = p.causal ? min(pos, kFar) : kFar;
+    below = p.window ? max(pos - p.window, -1) : -1;
+    slope = p.slopes ? p.slopes[p.tslopes.at(bx, by, bz) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
+    doc = p.qdocs ? p.qdocs[p.tqdocs.at(bx, by, bz) + token * p.qdoc_step] : 0;
+    const unsigned char* at = p.q + (p.tq.at(bx, by, bz) + head * p.q_head + token * p.q_row + 8 * hi) * 2;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) q[kk] = (uint4v)(*reinterpret_cast<const u4a*>(at + kk * 32));
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][r] = 0.0f;
+    m = -__builtin_inff();
+    l = 0.0f;
+    const int g = lane >> 4, li = lane & 15;
+    const int key = 4 * hi + (li >> 2), chunk = 2 * (g & 1) + ((li & 3) >> 1);
+    vkey = key * PITCH;
+    vchunk = ((chunk ^ vsw(key)) << 4) + 8 * (li & 1);
+  }
+
+  __device__ __forceinline__ uint4v key_fragment(const unsigned char* K, int kt, int kk) const {
+    const int r = kt * 32 + col;
+    return *reinterpret_cast<const uint4v*>(K + r * PITCH + (((2 * kk + hi) ^ ksw(col)) << 4));
+  }
+
+  // Values of keys 32 kt + 16 u + {4 h + 0..3, 8 + 4 h + 0..3}, column 32 n + c.
+  __device__ __forceinline__ uint4v value_fragment(const unsigned char* V, int kt, int u, int n) const {
+    // vsw moves whole groups of four chunks, the bits that n sets
+    const int at = vkey + (vchunk ^ (n << 6)) + (kt * 32 + u * 16) * PITCH;
+    lds_t* const f = (lds_t*)(V + at);
+    const uint2v lo = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     reinterpret_cast<short4v __attribute__((address_space(3)))*>(f)));
+    const uint2v up = __builtin_bit_cast(
+        uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    reinterpret_cast<short4v __attribute__((address_space(3)))*>(f + 8 * PITCH)));
+    return uint4v{lo[0], lo[1], up[0], up[1]};
+  }
+
+  // Whether the wave's rows see all of keys [key0, key0 + n), or none of them.
+  __device__ __forceinline__ bool sees_all(const AttendArgs& p, int key0, int n, int len, int pre) const {
+    return key0 + n <= len && !p.qdocs &&
+           (key0 + n <= pre ||
+            ((!p.causal || key0 + n - 1 <= p0) && (!p.window || key0 > p1 - p.window)));
+  }
+  __device__ __forceinline__ bool sees_none(const AttendArgs& p, int key0, int n, int pre) const {
+    return key0 >= pre && ((p.causal && key0 > p1) || (p.window && key0 + n - 1 <= p0 - p.window));
+  }
+
+  // T tiles of 32 keys from key0 on.  docs: their documents in LDS, or null, then
+  // p.kdocs at doc_at.
+  template <int T>
+  __device__ __forceinline__ void tile(const AttendArgs& p, const unsigned char* K, const unsigned char* V,
+                                       const int* docs, const int* kdocs, int key0, int len, int pre) {
+    float16v s[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int t = 0; t < T; ++t) s[t] = mma<BF16>(key_fragment(K, t, kk), q[kk], s[t]);
+
+    float mul = p.scale_log2;
+    if (p.cap_log2 > 0.0f) {
+      // cap tanh(z) = cap (1 - 2 / (e^2z + 1)); off by a few 2^-24 cap
+      mul = 1.0f;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[t][r] = fmaf(-2.0f * p.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[t][r] * p.cap_in) + 1.0f),
+                         p.cap_log2);
+    }
+    if (p.slopes) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const float away = (float)(pos - (key0 + t * 32 + 4 * hi));
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[t][r] = fmaf(-slope, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[t][r] * mul);
+      }
+      mul = 1.0f;
+    }
+    unsigned seen[T];  // of a tile that is masked in part: bit r for register r
+    bool part = false;
+    if (!sees_all(p, key0, 32 * T, len, pre)) {
+      unsigned all = 0xffffu;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const int base = key0 + t * 32 + 4 * hi;
+        const int a = above - base, b = below - base, f = pre - base, n = len - base;
+        unsigned bits = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int c = 8 * (r >> 2) + (r & 3);
+          if (((c <= a && c > b) || c < f) && c < n) bits |= 1u << r;
+        }
+        if (p.qdocs) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            int d[4];
+            if (docs) {
+              const int4* at = reinterpret_cast<const int4*>(docs + t * 32 + 4 * hi + 8 * w);
+              d[0] = at->x, d[1] = at->y, d[2] = at->z, d[3] = at->w;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) d[e] = base + 8 * w + e < len ? kdocs[base + 8 * w + e] : 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (d[e] != doc) bits &= ~(1u << (4 * w + e));
+          }
+        }
+        seen[t] = bits;
+        all &= bits;
+      }
+      part = __builtin_amdgcn_ballot_w64(all != 0xffffu) != 0;
+      if (part) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[t][r] = (seen[t] >> r) & 1 ? s[t][r] : -__builtin_inff();
+      }
+    }
+
+    // the running maximum, in units of log2
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+    const float now = fmaxf(m, both_halves(top, true) * mul);
+    const float use = now == -__builtin_inff() ? 0.0f : now;
+    if (__builtin_amdgcn_ballot_w64(now > m) != 0) {
+      const float alpha = __builtin_amdgcn_exp2f(m - use);
+      l *= alpha;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+    }
+    m = now;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], mul, -use));
+        sum += s[t][r];
+      }
+    l += sum;
+
+    uint4v w[T][2];  // the weights rounded to the values' type: off by half a step each, as the result is
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[t][u][e] = pack2<BF16>(s[t][8 * u + 2 * e], s[t][8 * u + 2 * e + 1]);
+    if (part && !finite_values<T>(V)) {
+      masked_values<T>(V, w, seen);
+      return;
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n] = mma<BF16>(value_fragment(V, t, u, n), w[t][u], acc[n]);
+  }
+
+  static constexpr unsigned kExp = BF16 ? 0x7f80u : 0x7c00u;
+
+  // A weight of 0 times a hidden infinity or NaN would be NaN: a tile that is
+  // masked in part is looked through for them.
+  template <int T>
+  __device__ __forceinline__ bool finite_values(const unsigned char* V) const {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    us2 most = {0, 0};
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const uint4v v = value_fragment(V, t, u, n);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, v[e] & (kExp | kExp << 16)));
+        }
+    return __builtin_amdgcn_ballot_w64(most[0] == kExp || most[1] == kExp) == 0;
+  }
+
+  // Such a tile: the finite values as ever, and what a row sees of +inf, -inf and
+  // NaN counted by products with ones.
+  template <int T>
+  __device__ __forceinline__ void masked_values(const unsigned char* V, const uint4v (&w)[T][2],
+                                                const unsigned (&seen)[T]) {
+    constexpr unsigned one = BF16 ? 0x3f80u : 0x3c00u;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      float16v up, down;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) up[r] = down[r] = 0.0f;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4v v = value_fragment(V, t, u, n);
+          uint4v fine, plus, minus, sees;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            fine[e] = plus[e] = minus[e] = sees[e] = 0;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const unsigned b = (v[e] >> (16 * x)) & 0xffffu;
+              const bool odd = (b & kExp) == kExp, nan = odd && (b & ~(kExp | 0x8000u)) != 0;
+              fine[e] |= (odd ? 0u : b) << (16 * x);
+              plus[e] |= (odd && (nan || !(b & 0x8000u)) ? one : 0u) << (16 * x);
+              minus[e] |= (odd && (nan || (b & 0x8000u)) ? one : 0u) << (16 * x);
+              sees[e] |= ((seen[t] >> (8 * u + 2 * e + x)) & 1 ? one : 0u) << (16 * x);
+            }
+          }
+          acc[n] = mma<BF16>(fine, w[t][u], acc[n]);
+          up = mma<BF16>(plus, sees, up);
+          down = mma<BF16>(minus, sees, down);
+        }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (up[r] > 0.0f) acc[n][r] += __builtin_inff();
+        if (down[r] > 0.0f) acc[n][r] -= __builtin_inff();
+      }
+    }
+  }
+};
+
+// The tiles of BN keys that a workgroup's rows may see: tiles [a0, a0 + na) of the
+// prefix, then [b0, b0 + nb).
+struct Tiles {
+  int a0, na, b0, n;
+  __device__ __forceinline__ int at(int i) const { return i < na ? a0 + i : b0 + (i - na); }
+};
+
+// p0, p1: the workgroup's first and last position; [d0, d1): the keys whose
+// documents may be its rows'.
+__device__ __forceinline__ Tiles tiles_of(const AttendArgs& p, int bn, int p0, int p1, int len, int pre, int d0, int d1) {
+  const int b0 = max(p.window ? max(0, p0 - p.window + 1) : 0, d0);
+  const int b1 = min(p.causal ? min(len, max(p1, -1) + 1) : len, d1);
+  const int a1 = min(pre, d1);
+  Tiles t;
+  t.a0 = d0 / bn;
+  t.na = a1 > d0 ? (a1 + bn - 1) / bn - t.a0 : 0;
+  t.b0 = max(b0 / bn, t.na ? t.a0 + t.na : 0);
+  t.n = t.na + (b1 > b0 ? max(0, (b1 + bn - 1) / bn - t.b0) : 0);
+  return t;
+}
+
+// The smallest and largest over the workgroup's threads; `mem`: two ints a wave.
+template <int W>
+__device__ __forceinline__ void span(int& lo, int& hi, int* mem) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o, 64));
+    hi = max(hi, __shfl_xor(hi, o, 64));
+  }
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    mem[2 * wave] = lo;
+    mem[2 * wave + 1] = hi;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    lo = min(lo, mem[2 * w]);
+    hi = max(hi, mem[2 * w + 1]);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  __syncthreads();
+}
+
+// Keys [d0, d1) outside of which no key's document lies between those of tokens
+// t0 to t1: all that packed documents need not read.
+template <int W>
+__device__ __forceinline__ void document_keys(const AttendArgs& p, const int* qdocs, const int* kdocs, int t0, int t1,
+                                              int keys, int* mem, int& d0, int& d1) {
+  int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+  for (int t = t0 + (int)threadIdx.x; t <= t1; t += 64 * W) {
+    const int d = qdocs[t * p.qdoc_step];
+    lo = min(lo, d);
+    hi = max(hi, d);
+  }
+  span<W>(lo, hi, mem);
+  int first = keys, last = -1;
+  for (int j = threadIdx.x; j < keys; j += 64 * W) {
+    const int d = kdocs[j];
+    if (d >= lo && d <= hi) {
+      first = min(first, j);
+      last = max(last, j);
+    }
+  }
+  span<W>(first, last, mem);
+  d0 = first;
+  d1 = last + 1;
+}
+
+struct BlockAt {
+  int x, y, z, tile, split, start, len, pre;
+  long long block;
+};
+
+__device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
+  BlockAt b;
+  const int id = xcd_contiguous(blockIdx.x, p.nwg);
+  const int blk = (int)p.d_work((unsigned)id);
+  const int rest = id - blk * p.tiles * p.splits;
+  const int tile = (int)p.d_splits((unsigned)rest);
+  b.split = rest - tile * p.splits;
+  b.tile = p.tiles - 1 - tile;  // a causal Block's last rows see the most keys: they go first
+  b.block = blk;
+  p.blocks(blk, b.x, b.y, b.z);
+  b.start = p.start ? min(max(p.start[p.tstart.at(b.x, b.y, b.z)], -kFar), kFar - 1) : 0;
+  b.len = p.length ? min(max(p.length[p.tlength.at(b.x, b.y, b.z)], 0), p.keys) : p.keys;
+  b.pre = p.prefix ? min(max(p.prefix[p.tprefix.at(b.x, b.y, b.z)], 0), b.len) : 0;
+  b.start = __builtin_amdgcn_readfirstlane(b.start);
+  b.len = __builtin_amdgcn_readfirstlane(b.len);
+  b.pre = __builtin_amdgcn_readfirstlane(b.pre);
+  return b;
+}
+
+// BN keys of D values each from an array to LDS, by STEP waves: instruction i of a
+// wave fills 1 KB, lane L at byte 16 L, with the chunk that belongs there.  Rows past
+// `left` become zeros.
+template <int D, int BN, bool VALUES, int STEP>
+struct Fill {
+  typedef Rows<D, false> R;
+  static constexpr int IN = BN * D * 2 / 1024 / STEP;
+  static_assert(IN * 1024 * STEP == BN * D * 2, "whole instructions");
+  const unsigned char* base;
+  unsigned pitch;
+  unsigned off[IN];
+  int lane, first;
+
+  __device__ __forceinline__ void begin(const unsigned char* b, long long ld, int wave) {
+    base = b;
+    pitch = (unsigned)(ld * 2);
+    lane = threadIdx.x & 63;
+    first = wave;
+#pragma unroll
+    for (int i = 0; i < IN; ++i) {
+      const int pos = (i * STEP + first) * 1024 + lane * 16, row = pos / (2 * D), c = (pos % (2 * D)) >> 4;
+      off[i] = (unsigned)row * pitch + ((c ^ (VALUES ? R::vsw(row) : R::ksw(row))) << 4);
+    }
+  }
+
+  __device__ __forceinline__ void issue(bool dma, int key0, int left, unsigned char* to) const {
+    const unsigned char* from = base + (long long)key0 * pitch;
+    if (dma) {
+      const i32x4 rs = raw_rsrc(from, (unsigned)(min(left, BN) - 1) * pitch + 2 * D);
+      const unsigned at = __builtin_amdgcn_readfirstlane(lds_addr(to) + first * 1024);
+#pragma unroll
+      for (int i = 0; i < IN; ++i) dma16(rs, at + i * STEP * 1024, off[i], 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < IN; ++i) {
+        const int pos = (i * STEP + first) * 1024 + lane * 16;
+        uint4v v = {0, 0, 0, 0};
+        if (pos / (2 * D) < left) v = (uint4v)(*reinterpret_cast<const u4a*>(from + off[i]));
+        *reinterpret_cast<uint4v*>(to + pos) = v;
+      }
+    }
+  }
+};
+
+// Every LDS access of this wave is done, then the barrier: a bare s_barrier, since
+// __syncthreads would also wait for the DMA in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Four neighbouring result columns of a row, rounded once.
+template <bool BF16>
+__device__ __forceinline__ void store4(const AttendArgs& p, const BlockAt& b, int row, int d, float x, float y, float z,
+                                       float w) {
+  const int token = (int)p.d_heads((unsigned)row), head = row - token * p.heads;
+  unsigned char* const at = p.o + (p.to.at(b.x, b.y, b.z) + head * p.o_head + token * p.o_row + d) * 2;
+  *reinterpret_cast<u2a*>(at) = u2a{pack2<BF16>(x, y), pack2<BF16>(z, w)};
+}
+
+// The workspace: D sums of each (row, split), then a maximum and a total each.
+__device__ __forceinline__ float* sums_of(const AttendArgs& p, int D, long long row, int split) {
+  return p.work + (row * p.splits + split) * D;
+}
+__device__ __forceinline__ float* total_of(const AttendArgs& p, int D, long long rows, long long row, int split) {
+  return p.work + rows * p.splits * D + 2 * (row * p.splits + split);
+}
+
+// More than 32 rows: 128 of them, 32 a wave, the keys in tiles of 64 that the waves
+// share, two of them in LDS.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs p, long long all_rows) {
+  constexpr int BN = 64, KB = BN * D * 2, STAGE = 2 * KB + 256;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const BlockAt b = block_at(p);
+  const int first = b.tile * 128, last = min(first + 127, p.rows - 1);
+  const int t0 = (int)p.d_heads((unsigned)first), t1 = (int)p.d_heads((unsigned)last);
+  const int* const kdocs = p.kdocs ? p.kdocs + p.tkdocs.at(b.x, b.y, b.z) : nullptr;
+  int d0 = 0, d1 = b.len;
+  if (kdocs)
+    document_keys<4>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, t0, t1, b.len, reinterpret_cast<int*>(lds), d0, d1);
+  const Tiles tiles = tiles_of(p, BN, b.start + t0, b.start + t1, b.len, b.pre, d0, d1);
+  const int i0 = (int)((long long)tiles.n * b.split / p.splits), i1 = (int)((long long)tiles.n * (b.split + 1) / p.splits);
+
+  Fill<D, BN, false, 4> fk;
+  Fill<D, BN, true, 4> fv;
+  fk.begin(p.k + p.tk.at(b.x, b.y, b.z) * 2, p.ldk, wave);
+  fv.begin(p.v + p.tv.at(b.x, b.y, b.z) * 2, p.ldv, wave);
+  Rows<D, BF16> rows;
+  rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start);
+
+  auto issue = [&](int i, unsigned char* at) {
+    const int key0 = tiles.at(i) * BN, left = b.len - key0;
+    fk.issue(p.dma, key0, left, at);
+    fv.issue(p.dma, key0, left, at + KB);
+    if (kdocs) dma4(raw_rsrc(kdocs + key0, (unsigned)min(left, BN) * 4), lds_addr(at + 2 * KB), (threadIdx.x & 63) * 4);
+  };
+  constexpr int PER = 2 * (D / 32);
+  if (i0 < i1) issue(i0, lds);
+  for (int i = i0; i < i1; ++i) {
+    unsigned char* const at = lds + ((i - i0) & 1) * STAGE;
+    const bool more = i + 1 < i1;
+    if (more) issue(i + 1, lds + ((i + 1 - i0) & 1) * STAGE);
+    if (!more || !p.dma) XTK_WAIT_VM(0);
+    else if (kdocs) XTK_WAIT_VM(PER + 1);
+    else XTK_WAIT_VM(PER);
+    lds_barrier();
+    const int key0 = tiles.at(i) * BN;
+    if (!rows.sees_none(p, key0, BN, b.pre))
+      rows.template tile<2>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len, b.pre);
+    lds_barrier();
+  }
+
+  const float l = both_halves(rows.l, false);
+  if (first + 32 * wave + rows.col >= p.rows) return;
+  if (p.splits == 1) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = l == 0.0f ? 0.0f : rows.acc[n][4 * w + e] * inv;
+        store4<BF16>(p, b, rows.row, 32 * n + 8 * w + 4 * rows.hi, o[0], o[1], o[2], o[3]);
+      }
+    return;
+  }
+  const long long row = b.block * p.rows + rows.row;
+  float* const sums = sums_of(p, D, row, b.split);
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      *reinterpret_cast<float4v*>(sums + 32 * n + 8 * w + 4 * rows.hi) =
+          float4v{rows.acc[n][4 * w], rows.acc[n][4 * w + 1], rows.acc[n][4 * w + 2], rows.acc[n][4 * w + 3]};
+  if (rows.hi == 0) {
+    float* const t = total_of(p, D, all_rows, row, b.split);
+    t[0] = rows.m;
+    t[1] = l;
+  }
+}
+
+// Waves of a workgroup of few rows, and tiles of 32 keys in a wave's ring: what
+// fills 160 KB of LDS, twice over where that leaves enough in flight.
+template <int D>
+struct Few {
+  static constexpr int W = D <= 160 ? 4 : 2, TILE = 32 * D * 4;
+  static constexpr int NS = D == 32 ? 4 : D == 64 ? 2 : D == 96 || D == 192 ? 3 : 2;
+  static constexpr int LDS = W * NS * TILE;
+  static_assert(LDS <= 160 * 1024 && W * 256 + W * 32 * (D + 4) * 4 <= LDS, "rings, then the waves' results");
+  static_assert((NS - 1) * (D / 8) < 64, "vmcnt is six bits");
+};
+
+// Up to 32 rows: every wave has them all and takes tiles of 32 keys in turn, each in
+// a ring of its own, so that nothing but its own loads makes a wave wait.
+template <int D, bool BF16>
+__global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p, long long all_rows) {
+  typedef Few<D> F;
+  constexpr int W = F::W, NS = F::NS, KB = 32 * D * 2, PER = D / 8;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[F::LDS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const BlockAt b = block_at(p);
+  const int t1 = (int)p.d_heads((unsigned)(p.rows - 1));
+  const int* const kdocs = p.kdocs ? p.kdocs + p.tkdocs.at(b.x, b.y, b.z) : nullptr;
+  int d0 = 0, d1 = b.len;
+  if (kdocs)
+    document_keys<W>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, 0, t1, b.len, reinterpret_cast<int*>(lds), d0, d1);
+  const Tiles tiles = tiles_of(p, 32, b.start, b.start + t1, b.len, b.pre, d0, d1);
+  const int i0 = (int)((long long)tiles.n * b.split / p.splits), i1 = (int)((long long)tiles.n * (b.split + 1) / p.splits);
+  const int mine = max(0, (i1 - i0 - wave + W - 1) / W);
+
+  Fill<D, 32, false, 1> fk;
+  Fill<D, 32, true, 1> fv;
+  fk.begin(p.k + p.tk.at(b.x, b.y, b.z) * 2, p.ldk, 0);
+  fv.begin(p.v + p.tv.at(b.x, b.y, b.z) * 2, p.ldv, 0);
+  unsigned char* const ring = lds + wave * NS * F::TILE;
+  auto key_of = [&](int j) { return tiles.at(i0 + wave + j * W) * 32; };
+  auto issue = [&](int j, int slot) {
+    unsigned char* const at = ring + slot * F::TILE;
+    const int key0 = key_of(j);
+    fk.issue(p.dma, key0, b.len - key0, at);
+    fv.issue(p.dma, key0, b.len - key0, at + KB);
+  };
+  Rows<D, BF16> rows;
+  rows.begin(p, 0, b.x, b.y, b.z, b.start);
+#pragma unroll
+  for (int j = 0; j < NS; ++j)
+    if (j < mine) issue(j, j);
+  int slot = 0;
+  for (int j = 0; j < mine; ++j) {
+    const int ahead = p.dma ? min(mine - 1 - j, NS - 1) : 0;
+    switch (ahead) {
+      case 0: XTK_WAIT_VM(0); break;
+      case 1: XTK_WAIT_VM(PER); break;
+      case 2: XTK_WAIT_VM(NS > 2 ? 2 * PER : 0); break;
+      default: XTK_WAIT_VM(NS > 3 ? 3 * PER : 0); break;
+    }
+    asm volatile("" ::: "memory");
+    unsigned char* const at = ring + slot * F::TILE;
+    rows.template tile<1>(p, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
+    // every fragment is in registers before the slot is filled again
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (j + NS < mine) issue(j + NS, slot);
+    slot = slot + 1 == NS ? 0 : slot + 1;
+  }
+
+  // the waves' results meet in the rings
+  float* const total = reinterpret_cast<float*>(lds);
+  float* const part = total + W * 64;
+  const float own = both_halves(rows.l, false);
+  __syncthreads();
+  if (rows.hi == 0) {
+    total[(wave * 32 + rows.col) * 2] = rows.m;
+    total[(wave * 32 + rows.col) * 2 + 1] = own;
+  }
+  __syncthreads();
+  auto joined = [&](int c, float& m, float& l) {
+    m = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = fmaxf(m, total[(w * 32 + c) * 2]);
+    const float use = m == -__builtin_inff() ? 0.0f : m;
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) l += total[(w * 32 + c) * 2 + 1] * __builtin_amdgcn_exp2f(total[(w * 32 + c) * 2] - use);
+    return use;
+  };
+  float m, l;
+  const float f = __builtin_amdgcn_exp2f(rows.m - joined(rows.col, m, l));
+  if (rows.col < p.rows) {
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        *reinterpret_cast<float4v*>(part + (wave * 32 + rows.col) * (D + 4) + 32 * n + 8 * w + 4 * rows.hi) =
+            float4v{rows.acc[n][4 * w] * f, rows.acc[n][4 * w + 1] * f, rows.acc[n][4 * w + 2] * f,
+                    rows.acc[n][4 * w + 3] * f};
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.rows * (D / 4); e += 64 * W) {
+    const int c = e / (D / 4), d = 4 * (e % (D / 4));
+    float4v o = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < W; ++w) o += *reinterpret_cast<const float4v*>(part + (w * 32 + c) * (D + 4) + d);
+    joined(c, m, l);
+    if (p.splits == 1) {
+      const float inv = 1.0f / l;
+      if (l == 0.0f) o = float4v{0, 0, 0, 0};
+      else o *= inv;
+      store4<BF16>(p, b, c, d, o[0], o[1], o[2], o[3]);
+    } else {
+      const long long row = b.block * p.rows + c;
+      *reinterpret_cast<float4v*>(sums_of(p, D, row, b.split) + d) = o;
+      if (d == 0) {
+        float* const t = total_of(p, D, all_rows, row, b.split);
+        t[0] = m;
+        t[1] = l;
+      }
+    }
+  }
+}
+
+// The splits of a row joined: a workgroup of four waves a row, each a quarter of the
+// splits, in a fixed order.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs p, long long all_rows) {
+  __shared__ float part[4][D];
+  __shared__ float totals[4];
+  const long long row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  BlockAt b;
+  const int blk = (int)p.d_work((unsigned)row);
+  const int r = (int)(row - (long long)blk * p.rows);
+  p.blocks(blk, b.x, b.y, b.z);
+  float m = -__builtin_inff();
+  for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, *total_of(p, D, all_rows, row, s));
+  m = wave_reduce<true>(m);
+  if (m == -__builtin_inff()) m = 0.0f;
+  const int s0 = p.splits * wave / 4, s1 = p.splits * (wave + 1) / 4;
+  float l = 0.0f;
+  float4v o = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = s0; s < s1; ++s) {
+    const float* t = total_of(p, D, all_rows, row, s);
+    const float f = __builtin_amdgcn_exp2f(t[0] - m);
+    l += t[1] * f;
+    if (lane < D / 4) o += f * *reinterpret_cast<const float4v*>(sums_of(p, D, row, s) + 4 * lane);
+  }
+  if (lane < D / 4) *reinterpret_cast<float4v*>(&part[wave][4 * lane]) = o;
+  if (lane == 0) totals[wave] = l;
+  __syncthreads();
+  if (threadIdx.x >= D / 4) return;
+  l = 0.0f;
+  o = float4v{0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    l += totals[w];
+    o += *reinterpret_cast<const float4v*>(&part[w][4 * lane]);
+  }
+  if (l == 0.0f) o = float4v{0, 0, 0, 0};
+  else o *= 1.0f / l;
+  store4<BF16>(p, b, r, 4 * lane, o[0], o[1], o[2], o[3]);
+}
+
+template <int D, bool BF16>
+hipError_t run_attend_elem(bool few, const AttendArgs& a, hipStream_t s) {
+  const long long blocks = a.nwg / ((long long)a.tiles * a.splits), all_rows = blocks * a.rows;
+  if (few) attend_few_kernel<D, BF16><<<a.nwg, 64 * Few<D>::W, 0, s>>>(a, all_rows);
+  else attend_rows_kernel<D, BF16><<<a.nwg, 256, 0, s>>>(a, all_rows);
+  if (a.splits > 1) {
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    AttendArgs j = a;
+    j.d_work = div31(static_cast<unsigned>(a.rows));
+    attend_join_kernel<D, BF16><<<static_cast<unsigned>(all_rows), 256, 0, s>>>(j, all_rows);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+template <int D>
+hipError_t run_attend(bool bf16, bool few, const AttendArgs& a, hipStream_t s) {
+  return bf16 ? run_attend_elem<D, true>(few, a, s) : run_attend_elem<D, false>(few, a, s);
+}
+
+}  // namespace xtk
+
+#endif

@@ -77,6 +77,22 @@ inline bool accesses_meet(const xt::Plan& p, void* const* bufs, const xt::Access
   return first(x) < past(y) && first(y) < past(x);
 }
 
+// Whether a result may be stored while an operand is read: their buffers do not
+// meet, or, where every thread has read what it stores over (`in_place`), they are
+// the same elements at the same places.
+inline bool result_apart(const xt::Plan& p, void* const* bufs, const xt::Access2D& out, const xt::Access2D& in,
+                         bool in_place, std::string& why) {
+  if (out.arg != in.arg && !buffers_meet(p, bufs, out.arg, in.arg)) return true;
+  auto same = [](const xt::Access2D& a, const xt::Access2D& b) {
+    return a.elem == b.elem && a.rows == b.rows && a.cols == b.cols && a.ld == b.ld && a.addr.c0 == b.addr.c0 &&
+           a.addr.sx == b.addr.sx && a.addr.sy == b.addr.sy && a.addr.sz == b.addr.sz;
+  };
+  if (in_place && bufs[out.arg] == bufs[in.arg] && same(out, in)) return true;
+  why = "buffer " + std::to_string(out.arg) + " is stored and meets buffer " + std::to_string(in.arg) +
+        ", which the program reads elsewhere";
+  return false;
+}
+
 // Blocks of the plan's grid, in 64 bits (three int32 axes).
 inline long long grid_blocks(const xt::Plan& p) {
   return static_cast<long long>(p.grid[0]) * p.grid[1] * p.grid[2];
@@ -108,6 +124,11 @@ bool conv_blocks_cover_output(const xt::Plan& p, long long es);
 // The few-input-channel conv kernel (conv_small.hip), same contract.
 bool launch_conv2d_small(const xt::Plan& p, void* const* bufs, hipStream_t s, bool ahead, hipError_t& e);
 hipError_t launch_tilevm(const xt::Plan& p, void* const* bufs, hipStream_t s, std::string& why);
+
+hipError_t launch_rms_norm(const xt::Plan& p, void* const* bufs, hipStream_t s, std::string& why);
+hipError_t launch_matmul_q4(const xt::Plan& p, void* const* bufs, hipStream_t s, std::string& why);
+// `work`: the plan's workspace, or null (the keys are then not split).
+hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipStream_t s, std::string& why);
 
 // Fused tile programs (fused_jit.cpp): compile_fused fills fp.code from
 // fp.source with hiprtc (or the code-object cache); launch_fused runs it.

@@ -1,0 +1,412 @@
+// Root-mean-square norm of rows, with the residual's addition and, where asked
+// for, rows in 8 bits:
+//   h = x + r;  y = h / sqrt(mean(h^2) + eps) * gamma
+//   s = max |y| / 127;  q = rint(y / s)
+//
+// One pass: a group of threads holds its row in registers as f32 (h is rounded
+// only where it is stored), so x, r and gamma are read once and nothing is read
+// back.  The sum of squares and the largest |h gamma| are found together, since
+// max |y| = max |h gamma| / sqrt(...): one exchange over the group serves both.
+//
+// HBM bounds it for many rows, one group's latency for one row.  A row takes
+// 64 threads (rows to 1024 values, no barrier), 256 (to 8192) or 1024; longer
+// rows are read again for the second half (rms_norm_long_kernel).
+#include <vector>
+
+#include "common.h"
+#include "launch.h"
+
+namespace xtk {
+namespace {
+
+enum { kF32 = 0, kF16 = 1, kBF16 = 2, kI8 = 3 };
+
+struct NormArgs {
+  const void* x;
+  const void* r;
+  const void* gamma;
+  void* sum;
+  void* y;
+  float* scale;
+  TileOff tx, tr, tg, tsum, ty, tscale;
+  long long ldx, ldr, ldsum, ldy, ldscale;
+  BlockDecode blocks;
+  Div31 per;  // rows of a Block
+  int block_rows, rows, cols;
+  int gamma_elem, y_elem;
+  float eps;
+};
+
+// Eight values at element alignment; the first n of them where fewer are left.
+template <int ELEM>
+__device__ __forceinline__ void load8(const void* base, long long at, int n, float (&v)[8]) {
+  if constexpr (ELEM == kF32) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    const float* q = static_cast<const float*>(base) + at;
+    if (n >= 8) {
+      const f4 a = *reinterpret_cast<const f4*>(q), b = *reinterpret_cast<const f4*>(q + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? q[i] : 0.0f;
+    }
+  } else if constexpr (ELEM == kF16) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8), aligned(2)));
+    const _Float16* q = static_cast<const _Float16*>(base) + at;
+    if (n >= 8) {
+      const h8 a = *reinterpret_cast<const h8*>(q);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)q[i] : 0.0f;
+    }
+  } else {
+    typedef unsigned short s8 __attribute__((ext_vector_type(8), aligned(2)));
+    const unsigned short* q = static_cast<const unsigned short*>(base) + at;
+    if (n >= 8) {
+      const s8 a = *reinterpret_cast<const s8*>(q);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, (unsigned)a[i] << 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? __builtin_bit_cast(float, (unsigned)q[i] << 16) : 0.0f;
+    }
+  }
+}
+
+// Rounded once, to nearest even, to the stored type.
+template <int ELEM>
+__device__ __forceinline__ void store8(void* base, long long at, int n, const float (&v)[8]) {
+  if constexpr (ELEM == kF32) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    float* q = static_cast<float*>(base) + at;
+    if (n >= 8) {
+      *reinterpret_cast<f4*>(q) = f4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f4*>(q + 4) = f4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) q[i] = v[i];
+    }
+  } else if constexpr (ELEM == kF16) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8), aligned(2)));
+    _Float16* q = static_cast<_Float16*>(base) + at;
+    if (n >= 8) {
+      h8 a;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = (_Float16)v[i];
+      *reinterpret_cast<h8*>(q) = a;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) q[i] = (_Float16)v[i];
+    }
+  } else {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8), aligned(2)));
+    __bf16* q = static_cast<__bf16*>(base) + at;
+    if (n >= 8) {
+      b8 a;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = (__bf16)v[i];
+      *reinterpret_cast<b8*>(q) = a;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) q[i] = (__bf16)v[i];
+    }
+  }
+}
+
+__device__ __forceinline__ void load8_of(int elem, const void* base, long long at, int n, float (&v)[8]) {
+  if (elem == kF32) load8<kF32>(base, at, n, v);
+  else if (elem == kF16) load8<kF16>(base, at, n, v);
+  else load8<kBF16>(base, at, n, v);
+}
+
+// y / s to int8, half to even.  `inv` is 1 / s, 0 where s is too small for a
+// normal reciprocal: those rows divide.
+__device__ __forceinline__ int to_i8(float y, float s, float inv) {
+  const float v = inv != 0.0f ? y * inv : s != 0.0f ? y / s : 0.0f;
+  int i;  // saturates, NaN to 0; assembly because a C++ cast of such values is undefined
+  asm("v_cvt_i32_f32 %0, %1" : "=v"(i) : "v"(__builtin_rintf(v)));
+  return min(max(i, -127), 127);
+}
+
+__device__ __forceinline__ void store_y8(const NormArgs& p, long long at, int n, const float (&y)[8], float s, float inv) {
+  if (p.y_elem == kF32) {
+    store8<kF32>(p.y, at, n, y);
+  } else if (p.y_elem == kF16) {
+    store8<kF16>(p.y, at, n, y);
+  } else if (p.y_elem == kBF16) {
+    store8<kBF16>(p.y, at, n, y);
+  } else {
+    signed char* q = static_cast<signed char*>(p.y) + at;
+    unsigned w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((unsigned)to_i8(y[i], s, inv) & 255u) << (8 * (i & 3));
+    if (n >= 8) {
+      typedef unsigned u2 __attribute__((ext_vector_type(2), aligned(1)));
+      *reinterpret_cast<u2*>(q) = u2{w[0], w[1]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) q[i] = (signed char)(w[i >> 2] >> (8 * (i & 3)));
+    }
+  }
+}
+
+// The larger of two magnitudes as their bits: NaN is above infinity, so it stays.
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+  return v;
+}
+
+// The sum and the largest magnitude over the T threads of a row (every lane active).
+template <int T>
+__device__ __forceinline__ void row_reduce(float& ss, unsigned& top, bool want_top) {
+  ss = wave_reduce<false>(ss);
+  if (want_top) top = wave_umax(top);
+  if constexpr (T > 64) {
+    __shared__ float part[T / 64];
+    __shared__ unsigned tops[T / 64];
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+      part[wave] = ss;
+      tops[wave] = top;
+    }
+    __syncthreads();
+    ss = 0;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+      ss += part[w];
+      top = max(top, tops[w]);
+    }
+  }
+}
+
+struct RowAt {
+  long long x, r, g, sum, y, scale;
+};
+
+__device__ __forceinline__ RowAt row_at(const NormArgs& p, int row) {
+  const int b = (int)p.per((unsigned)row);
+  const int i = row - b * p.block_rows;
+  int bx, by, bz;
+  p.blocks(b, bx, by, bz);
+  return RowAt{p.tx.at(bx, by, bz) + i * p.ldx,     p.tr.at(bx, by, bz) + i * p.ldr,
+               p.tg.at(bx, by, bz),                 p.tsum.at(bx, by, bz) + i * p.ldsum,
+               p.ty.at(bx, by, bz) + i * p.ldy,     p.tscale.at(bx, by, bz) + i * p.ldscale};
+}
+
+__device__ __forceinline__ float inverse_root(const NormArgs& p, float ss) {
+  return 1.0f / sqrtf(ss / (float)p.cols + p.eps);
+}
+
+// T threads a row, NV vectors of eight values each.
+template <int ELEM, int T, int NV>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(NormArgs p) {
+  constexpr int R = T < 256 ? 256 / T : 1;  // rows of a workgroup
+  const int row = R == 1 ? (int)blockIdx.x : __builtin_amdgcn_readfirstlane(blockIdx.x * R + threadIdx.x / T);
+  if (R > 1 && row >= p.rows) return;  // whole waves, and no barrier below for them
+  const RowAt at = row_at(p, row);
+  const int t = R == 1 ? threadIdx.x : threadIdx.x % T;
+  const bool quantize = p.y_elem == kI8;
+  float h[NV][8], g[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * T + t) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[i][e] = 0.0f, g[i][e] = 0.0f;
+    if (c < p.cols) load8<ELEM>(p.x, at.x + c, p.cols - c, h[i]);
+  }
+  if (p.r) {
+    float r[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * T + t) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[i][e] = 0.0f;
+      if (c < p.cols) load8<ELEM>(p.r, at.r + c, p.cols - c, r[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[i][e] += r[i][e];
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * T + t) * 8;
+    if (c < p.cols) load8_of(p.gamma_elem, p.gamma, at.g + c, p.cols - c, g[i]);
+  }
+  float ss = 0.0f;
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float s8 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s8 = fmaf(h[i][e], h[i][e], s8);
+    ss += s8;
+  }
+  if (quantize) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        top = max(top, __builtin_bit_cast(unsigned, h[i][e] * g[i][e]) & 0x7fffffffu);
+  }
+  row_reduce<T>(ss, top, quantize);
+  const float inv = inverse_root(p, ss);
+  float s = 0.0f, is = 0.0f;
+  if (quantize) {
+    s = __builtin_bit_cast(float, top) * inv / 127.0f;
+    is = s >= 1.0e-37f ? 1.0f / s : 0.0f;
+    if (t == 0) p.scale[at.scale] = s;
+    if (s != s) is = s;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * T + t) * 8;
+    if (c >= p.cols) continue;
+    if (p.sum) store8<ELEM>(p.sum, at.sum + c, p.cols - c, h[i]);
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = h[i][e] * inv * g[i][e];
+    store_y8(p, at.y + c, p.cols - c, y, s, is);
+  }
+}
+
+// Rows that the registers of a workgroup do not hold: x and r are read twice,
+// the second time from L2.  Nothing is stored before the second pass, and then by
+// the thread that has just read those values again, since it may lie over x or r.
+template <int ELEM>
+__global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs p) {
+  constexpr int T = 1024;
+  const RowAt at = row_at(p, blockIdx.x);
+  const int t = threadIdx.x;
+  const bool quantize = p.y_elem == kI8;
+  float ss = 0.0f;
+  unsigned top = 0;
+  auto row8 = [&](int c, float (&h)[8], float (&g)[8]) {
+    float r[8];
+    load8<ELEM>(p.x, at.x + c, p.cols - c, h);
+    if (p.r) {
+      load8<ELEM>(p.r, at.r + c, p.cols - c, r);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] += r[e];
+    }
+    load8_of(p.gamma_elem, p.gamma, at.g + c, p.cols - c, g);
+  };
+  for (int c = t * 8; c < p.cols; c += T * 8) {
+    float h[8], g[8], s8 = 0.0f;
+    row8(c, h, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s8 = fmaf(h[e], h[e], s8);
+      top = max(top, __builtin_bit_cast(unsigned, h[e] * g[e]) & 0x7fffffffu);
+    }
+    ss += s8;
+  }
+  row_reduce<T>(ss, top, quantize);
+  const float inv = inverse_root(p, ss);
+  float s = 0.0f, is = 0.0f;
+  if (quantize) {
+    s = __builtin_bit_cast(float, top) * inv / 127.0f;
+    is = s >= 1.0e-37f ? 1.0f / s : 0.0f;
+    if (t == 0) p.scale[at.scale] = s;
+    if (s != s) is = s;
+  }
+  for (int c = t * 8; c < p.cols; c += T * 8) {
+    float h[8], g[8], y[8];
+    row8(c, h, g);
+    if (p.sum) store8<ELEM>(p.sum, at.sum + c, p.cols - c, h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = h[e] * inv * g[e];
+    store_y8(p, at.y + c, p.cols - c, y, s, is);
+  }
+}
+
+template <int ELEM, int T>
+void run(const NormArgs& a, int nv, hipStream_t s) {
+  constexpr int threads = T < 256 ? 256 : T;
+  const int wgs = T < 256 ? (a.rows + 256 / T - 1) / (256 / T) : a.rows;
+  if (nv <= 1) rms_norm_kernel<ELEM, T, 1><<<wgs, threads, 0, s>>>(a);
+  else if (nv <= 2) rms_norm_kernel<ELEM, T, 2><<<wgs, threads, 0, s>>>(a);
+  else rms_norm_kernel<ELEM, T, 4><<<wgs, threads, 0, s>>>(a);
+}
+
+template <int ELEM>
+void run_elem(const NormArgs& a, hipStream_t s) {
+  const int v = (a.cols + 7) / 8;  // vectors of a row
+  if (v <= 128) run<ELEM, 64>(a, (v + 63) / 64, s);
+  else if (v <= 1024) run<ELEM, 256>(a, (v + 255) / 256, s);
+  else if (v <= 4096) run<ELEM, 1024>(a, (v + 1023) / 1024, s);
+  else rms_norm_long_kernel<ELEM><<<a.rows, 1024, 0, s>>>(a);
+}
+
+int elem_of(xt::Elem e) {
+  return e == xt::Elem::F32 ? kF32 : e == xt::Elem::F16 ? kF16 : e == xt::Elem::BF16 ? kBF16 : kI8;
+}
+
+}  // namespace
+
+hipError_t launch_rms_norm(const xt::Plan& p, void* const* bufs, hipStream_t s, std::string& why) {
+  const xt::NormPlan& n = p.norm;
+  // a result may lie over x or r: every thread stores over what it has read, and
+  // nothing that another reads
+  std::vector<const xt::Access2D*> ins = {&n.x, &n.gamma}, outs = {&n.y};
+  if (n.residual) ins.push_back(&n.r);
+  if (n.keep_sum) outs.push_back(&n.sum);
+  if (n.quantize) outs.push_back(&n.scale);
+  for (size_t i = 0; i < outs.size(); ++i) {
+    for (const xt::Access2D* in : ins)
+      if (!result_apart(p, bufs, *outs[i], *in, in != &n.gamma, why)) return hipErrorInvalidValue;
+    for (size_t j = 0; j < i; ++j)
+      if (buffers_meet(p, bufs, outs[i]->arg, outs[j]->arg)) {
+        why = "buffers " + std::to_string(outs[j]->arg) + " and " + std::to_string(outs[i]->arg) +
+              " are both stored and meet";
+        return hipErrorInvalidValue;
+      }
+  }
+  auto off = [](const xt::Access2D& a) { return TileOff{a.addr.c0, a.addr.sx, a.addr.sy, a.addr.sz}; };
+  NormArgs a{};
+  a.x = bufs[n.x.arg];
+  a.r = n.residual ? bufs[n.r.arg] : nullptr;
+  a.gamma = bufs[n.gamma.arg];
+  a.sum = n.keep_sum ? bufs[n.sum.arg] : nullptr;
+  a.y = bufs[n.y.arg];
+  a.scale = n.quantize ? static_cast<float*>(bufs[n.scale.arg]) : nullptr;
+  a.tx = off(n.x);
+  a.tr = off(n.r);
+  a.tg = off(n.gamma);
+  a.tsum = off(n.sum);
+  a.ty = off(n.y);
+  a.tscale = off(n.scale);
+  a.ldx = n.x.ld;
+  a.ldr = n.r.ld;
+  a.ldsum = n.sum.ld;
+  a.ldy = n.y.ld;
+  a.ldscale = n.scale.ld;
+  a.blocks = block_decode(p.grid[0], p.grid[1], false);
+  a.per = div31(static_cast<unsigned>(n.x.rows));
+  a.block_rows = static_cast<int>(n.x.rows);
+  const long long rows = grid_blocks(p) * n.x.rows;
+  a.rows = static_cast<int>(rows);
+  a.cols = static_cast<int>(n.x.cols);
+  a.gamma_elem = elem_of(n.gamma.elem);
+  a.y_elem = elem_of(n.y.elem);
+  a.eps = n.eps;
+  const int t = a.cols <= 1024 ? 64 : a.cols <= 8192 ? 256 : 1024;
+  if (!grid_fits(rows, t)) {
+    why = "rms_norm: " + std::to_string(rows) + " rows exceed one launch";
+    return hipErrorInvalidValue;
+  }
+  if (n.x.elem == xt::Elem::F32) run_elem<kF32>(a, s);
+  else if (n.x.elem == xt::Elem::F16) run_elem<kF16>(a, s);
+  else run_elem<kBF16>(a, s);
+  return hipGetLastError();
+}
+
+}  // namespace xtk

@@ -3,15 +3,21 @@
 // A launch through the Python checks (signature JSON, six attribute reads and
 // a size product a tensor, a device context manager, ctypes arrays) took 12-16
 // us of host time, several times what a small kernel runs; this call takes the
-// tensors' fields from their C++ objects and hands them to xt_gpu_run_buffers.
+// tensors' fields from their C++ objects and hands them to xt_gpu_run_buffers_with.
 //
-//   bind(run, free, type)                xt_gpu_run_buffers and xt_free of the library
-//                                        that owns the module handles, as addresses,
-//                                        and the handles' type (None: capsules)
+//   bind(run, free, type, workspace)     xt_gpu_run_buffers_with, xt_free and
+//                                        xt_workspace_bytes of the library that owns
+//                                        the module handles, as addresses, and the
+//                                        handles' type (None: capsules)
 //   launch(handle, buffers, func, stream) True when the program was enqueued.
 //                                        False when anything is not the plain
 //                                        case: the caller then takes the checked
 //                                        path, which launches it or raises.
+//
+// A program's workspace comes from torch's caching allocator and goes back to it
+// once the launch is enqueued: the allocator hands memory on within one stream,
+// in order, and keeps a captured graph's to that graph.  So it is taken here only
+// for a launch on the current stream; another stream's is the checked path's.
 //
 // The plain case: every buffer exactly a torch.Tensor with storage of its own
 // (no subclass, no functorch or functionalisation wrapper), contiguous, of its
@@ -20,6 +26,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -32,10 +39,12 @@
 
 namespace {
 
-typedef int (*RunFn)(xt_module*, const char*, const xt_buffer*, int, void*, char**);
+typedef int (*RunFn)(xt_module*, const char*, const xt_buffer*, int, void*, size_t, void*, char**);
+typedef int (*WorkFn)(xt_module*, const char*, size_t*, char**);
 typedef void (*FreeFn)(void*);
 RunFn g_run = nullptr;
 FreeFn g_free = nullptr;
+WorkFn g_work = nullptr;
 PyTypeObject* g_handle = nullptr;  // the ctypes binding's NativeModule; nullptr: capsules
 PyObject* g_ptr_name = nullptr;    // "_ptr"
 
@@ -135,10 +144,21 @@ PyObject* launch_plain(PyObject* const* args) {
   }
   char* err = nullptr;
   int st = XT_ERR_ARGUMENT;
+  const bool current = stream == static_cast<void*>(c10::hip::getCurrentHIPStream(device).stream());
   Py_BEGIN_ALLOW_THREADS;
   try {
-    st = g_run(m, func, b, static_cast<int>(n), stream, &err);
-  } catch (const std::exception&) {  // out of memory while planning
+    size_t need = 0;
+    st = g_work(m, func, &need, &err);
+    if (st == XT_OK && need == 0) {
+      st = g_run(m, func, b, static_cast<int>(n), nullptr, 0, stream, &err);
+    } else if (st == XT_OK && current) {
+      const c10::DataPtr work = c10::hip::HIPCachingAllocator::get()->allocate(need);
+      st = g_run(m, func, b, static_cast<int>(n), work.get(), need, stream, &err);
+    } else {
+      st = XT_ERR_ARGUMENT;
+    }
+  } catch (const std::exception&) {  // out of memory: the checked path says so
+    st = XT_ERR_ARGUMENT;
   }
   Py_END_ALLOW_THREADS;
   const std::string text = err ? err : "launch failed";
@@ -165,11 +185,13 @@ PyObject* launch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  void* run = nargs == 3 && PyLong_Check(args[0]) ? PyLong_AsVoidPtr(args[0]) : nullptr;
-  void* release = nargs == 3 && PyLong_Check(args[1]) ? PyLong_AsVoidPtr(args[1]) : nullptr;
+  void* run = nargs == 4 && PyLong_Check(args[0]) ? PyLong_AsVoidPtr(args[0]) : nullptr;
+  void* release = nargs == 4 && PyLong_Check(args[1]) ? PyLong_AsVoidPtr(args[1]) : nullptr;
+  void* work = nargs == 4 && PyLong_Check(args[3]) ? PyLong_AsVoidPtr(args[3]) : nullptr;
   if (PyErr_Occurred()) return nullptr;
-  if (!run || !release || (args[2] != Py_None && !PyType_Check(args[2]))) {
-    PyErr_SetString(PyExc_ValueError, "bind(address of xt_gpu_run_buffers, address of xt_free, handle type or None)");
+  if (!run || !release || !work || (args[2] != Py_None && !PyType_Check(args[2]))) {
+    PyErr_SetString(PyExc_ValueError, "bind(address of xt_gpu_run_buffers_with, address of xt_free, handle type or None, "
+                                      "address of xt_workspace_bytes)");
     return nullptr;
   }
   PyObject* const was = reinterpret_cast<PyObject*>(g_handle);
@@ -181,6 +203,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Py_XDECREF(was);
   g_run = reinterpret_cast<RunFn>(run);
   g_free = reinterpret_cast<FreeFn>(release);
+  g_work = reinterpret_cast<WorkFn>(work);
   Py_RETURN_NONE;
 }
 
@@ -188,7 +211,7 @@ PyMethodDef kMethods[] = {
     {"launch", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(launch)), METH_FASTCALL,
      "launch(handle, buffers, func, stream) -> bool: whether the program was enqueued"},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL,
-     "bind(xt_gpu_run_buffers, xt_free, type): the library's functions, as addresses, and its handles' type"},
+     "bind(xt_gpu_run_buffers_with, xt_free, type, xt_workspace_bytes): the library's functions, as addresses, and its handles' type"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_launch", "xt.launch over torch tensors", -1, kMethods,

@@ -10,6 +10,11 @@
 //              f16/bf16/i8 in, f32 or i8 out (kernels/matmul.py:6-19)
 //   Conv2d     store(load_conv2d(S, load F))         i8/f16/bf16 in, f32/bf16 out
 //              (kernels/conv2d.py:10-37; conv slice math lib/xt/XTToNova.cpp:110-142)
+//   RmsNorm    rms_norm of a loaded tile or of the sum of two, to rows of floats
+//              or through row_scale and quantize to rows in 8 bits (no reference
+//              counterpart, like the two below)
+//   MatmulQ4   store(matmul_q4(load X, load W, load S[, load R]))
+//   Attend     store(attend(load Q, load K, load V, ...)), reshapes in between
 #include "plan.h"
 
 #include <algorithm>
@@ -522,6 +527,306 @@ bool match_gemm_form(const Analysis& an, Plan& p, std::string& err, bool ragged)
 
 bool match_gemm(const Analysis& an, Plan& p, std::string& err) { return match_gemm_form(an, p, err, false); }
 
+// -- RmsNorm, MatmulQ4, Attend ---------------------------------------------------
+
+const Op* load_of(const Analysis& an, int v) {
+  const Op* o = def_of(an, v);
+  return o && o->name == "xt.load" ? o : nullptr;
+}
+
+// The arguments a program stores to, each once and none that `also` reads.
+bool stored_apart(const std::vector<int>& stored, const std::vector<int>& also, const char* what, std::string& err) {
+  for (size_t i = 0; i < stored.size(); ++i) {
+    const bool twice = std::count(stored.begin(), stored.end(), stored[i]) > 1;
+    if (twice || std::count(also.begin(), also.end(), stored[i])) {
+      err = std::string(what) + " programs store each result to an argument of its own; argument #" +
+            std::to_string(stored[i]) + (twice ? " is stored twice" : " is also an operand");
+      return false;
+    }
+  }
+  return true;
+}
+
+bool match_rms_norm(const Analysis& an, Plan& p, std::string& err) {
+  int nn, ns, nq, nst;
+  const Op* norm = only(an, "xt.rms_norm", nn);
+  const Op* rs = only(an, "xt.row_scale", ns);
+  const Op* qz = only(an, "xt.quantize", nq);
+  only(an, "xt.store", nst);
+  if (nn == 0) {
+    if (ns + nq) err = "row_scale and quantize run on the result of an rms_norm";
+    return false;
+  }
+  const char* form =
+      "rms_norm programs must be store(rms_norm(x, gamma)) or the stores of its row_scale and quantize, x a loaded "
+      "tile or the sum of two, which may be stored too";
+  err = form;
+  if (nn != 1 || ns > 1 || nq != ns) return false;
+  NormPlan& n = p.norm;
+  n = NormPlan{};
+  const Op* h = def_of(an, norm->operands[0]);
+  const Op* lg = load_of(an, norm->operands[1]);
+  const Op *lx = h, *lr = nullptr;
+  if (h && h->name == "xt.add") {
+    n.residual = true;
+    lx = load_of(an, h->operands[0]);
+    lr = load_of(an, h->operands[1]);
+  }
+  if (!lx || lx->name != "xt.load" || !lg || (n.residual && (!lr || lr == lx))) return false;
+  const Type& t = an.f.type_of(norm->operands[0]);
+  if (n.residual && (an.f.type_of(lx->results[0]) != t || an.f.type_of(lr->results[0]) != t)) return false;
+  n.quantize = ns == 1;
+  if (n.quantize && (rs->operands[0] != norm->results[0] || qz->operands[0] != norm->results[0] ||
+                     qz->operands[1] != rs->results[0]))
+    return false;
+  std::vector<int> stored;
+  const Op* st_y = nullptr;
+  const Op* st_s = nullptr;
+  const Op* st_h = nullptr;
+  for (const Op* o : an.compute) {
+    if (o->name != "xt.store") continue;
+    const int v = o->operands[0];
+    const Op** slot = n.residual && v == h->results[0]                          ? &st_h
+                      : v == (n.quantize ? qz->results[0] : norm->results[0]) ? &st_y
+                      : n.quantize && v == rs->results[0]                     ? &st_s
+                                                                              : nullptr;
+    if (!slot || *slot) return false;
+    *slot = o;
+    stored.push_back(an.arg_index(o->operands[1]));
+  }
+  n.keep_sum = st_h != nullptr;
+  if (!st_y || (n.quantize && !st_s)) return false;
+  // loads, the sum, the norm, the two 8-bit ops and the stores, and nothing else
+  const int ops = 3 + (n.residual ? 2 : 0) + (n.quantize ? 2 : 0) + nst;
+  if (count_ops(an) != ops) return false;
+  err.clear();
+  if (!access_of(an, *lx, n.x, err) || (n.residual && !access_of(an, *lr, n.r, err)) ||
+      !access_of(an, *lg, n.gamma, err) || !access_of(an, *st_y, n.y, err) ||
+      (n.keep_sum && !access_of(an, *st_h, n.sum, err)) || (n.quantize && !access_of(an, *st_s, n.scale, err)))
+    return false;
+  if (!stored_apart(stored, {n.gamma.arg}, "rms_norm", err)) return false;
+  n.eps = static_cast<float>(find_attr(norm->attrs, "eps")->f);
+  const double blocks = double(p.grid[0]) * p.grid[1] * p.grid[2], elems = double(t.numel());
+  if (blocks * double(n.x.rows) >= 2147483648.0 || n.x.cols >= (int64_t(1) << 30)) {
+    err = "rms_norm takes fewer than 2^31 rows of fewer than 2^30 columns";
+    return false;
+  }
+  p.kind = PlanKind::RmsNorm;
+  p.algo_bytes = blocks * (elems * (elem_bytes(n.x.elem) * (1 + n.residual + n.keep_sum) + elem_bytes(n.y.elem)) +
+                           (n.quantize ? 4.0 * double(n.x.rows) : 0)) +
+                 double(n.gamma.cols) * elem_bytes(n.gamma.elem);
+  p.algo_flops = 6 * blocks * elems;
+  return true;
+}
+
+bool match_q4(const Analysis& an, Plan& p, std::string& err) {
+  int nm, nst;
+  const Op* mm = only(an, "xt.matmul_q4", nm);
+  const Op* st = only(an, "xt.store", nst);
+  if (nm == 0) return false;
+  err = "matmul_q4 programs must be store(matmul_q4(x, w, scales[, row scales])) with loaded operands";
+  const int operands = static_cast<int>(mm->operands.size());
+  if (nm != 1 || nst != 1 || st->operands[0] != mm->results[0]) return false;
+  const Op* ld[4] = {};
+  std::set<const Op*> distinct;
+  for (int i = 0; i < operands; ++i) {
+    if (!(ld[i] = load_of(an, mm->operands[i]))) return false;
+    distinct.insert(ld[i]);
+  }
+  if (count_ops(an) != static_cast<int>(distinct.size()) + 2) return false;
+  err.clear();
+  Q4Plan& q = p.q4;
+  q = Q4Plan{};
+  q.row_scale = operands == 4;
+  Access2D* acc[4] = {&q.x, &q.w, &q.scales, &q.rows};
+  std::vector<int> read;
+  for (int i = 0; i < operands; ++i) {
+    if (!access_of(an, *ld[i], *acc[i], err)) return false;
+    read.push_back(acc[i]->arg);
+  }
+  if (!access_of(an, *st, q.y, err) || !stored_apart({q.y.arg}, read, "matmul_q4", err)) return false;
+  q.K = q.x.cols;
+  q.group = q.K / q.scales.cols;
+  if (q.y.rows >= (int64_t(1) << 30) || q.y.cols >= (int64_t(1) << 30) || q.K >= (int64_t(1) << 24)) {
+    err = "matmul_q4 takes tiles of fewer than 2^30 rows and columns and K below 2^24";
+    return false;
+  }
+  p.kind = PlanKind::MatmulQ4;
+  const double blocks = double(p.grid[0]) * p.grid[1] * p.grid[2];
+  p.algo_flops = blocks * 2.0 * double(q.y.rows) * double(q.y.cols) * double(q.K);
+  read.push_back(q.y.arg);
+  for (int arg : read) {  // minimum HBM traffic: each argument once
+    const Type& t = an.f.type_of(an.f.args[arg]);
+    p.algo_bytes += double(t.numel()) * elem_bytes(t.elem);
+  }
+  return true;
+}
+
+// `shape` over the elements of a tile with dims `tile` and strides `st`, in row-major
+// order: its strides, where each of its dims is one run of evenly spaced elements.
+bool reshaped_strides(const std::vector<int64_t>& tile, const std::vector<int64_t>& st,
+                      const std::vector<int64_t>& shape, std::vector<int64_t>& out) {
+  std::vector<std::pair<int64_t, int64_t>> src;  // (extent, stride), innermost first
+  for (size_t i = tile.size(); i-- > 0;)
+    if (tile[i] > 1) src.push_back({tile[i], st[i]});
+  size_t at = 0;
+  out.assign(shape.size(), 0);
+  for (size_t i = shape.size(); i-- > 0;) {
+    int64_t have = 1;
+    while (have < shape[i]) {
+      if (at == src.size()) return false;
+      auto& s = src[at];
+      if (have == 1) out[i] = s.second;
+      else if (s.second != out[i] * have) return false;
+      const int64_t want = shape[i] / have;
+      if (shape[i] % have) return false;
+      if (s.first <= want) {
+        if (want % s.first) return false;
+        have *= s.first;
+        ++at;
+      } else {  // a part of this dim; the rest is an outer dim's
+        if (s.first % want) return false;
+        have *= want;
+        s = {s.first / want, s.second * want};
+      }
+    }
+  }
+  return at == src.size();
+}
+
+// The load or store `o` of a tile that the program sees as `shape`.
+bool attend_access(const Analysis& an, const Op& o, const std::vector<int64_t>& shape, AttendAccess& a,
+                   std::vector<int64_t>& strides, std::string& err) {
+  const bool is_load = o.name == "xt.load";
+  const int mem_v = is_load ? o.operands[0] : o.operands[1];
+  const Type& mem = an.f.type_of(mem_v);
+  const Type& ten = is_load ? an.f.type_of(o.results[0]) : an.f.type_of(o.operands[0]);
+  a.arg = an.arg_index(mem_v);
+  if (a.arg < 0) {
+    err = o.name + " must access a function argument";
+    return false;
+  }
+  a.elem = mem.elem;
+  int shared = 0;
+  if (is_load)
+    if (const Attr* sh = find_attr(o.attrs, "shared")) shared = static_cast<int>(sh->i);
+  const std::vector<int> cv(o.operands.begin() + (is_load ? 1 : 2), o.operands.end());
+  if (!tile_origin(an, cv, shared, ten.shape, mem.shape, o.name + " of argument #" + std::to_string(a.arg), a.addr,
+                   nullptr, err))
+    return false;
+  if (!reshaped_strides(ten.shape, strides_of(mem.shape), shape, strides)) {
+    err = o.name + " of argument #" + std::to_string(a.arg) + ": the tile's dims do not reshape to evenly spaced rows";
+    return false;
+  }
+  return true;
+}
+
+bool match_attend(const Analysis& an, Plan& p, std::string& err) {
+  int na, nst;
+  const Op* at = only(an, "xt.attend", na);
+  const Op* st = only(an, "xt.store", nst);
+  if (na == 0) return false;
+  err = "attend programs must be store(attend(...)) with loaded operands, reshapes in between";
+  if (na != 1 || nst != 1) return false;
+  std::set<const Op*> seen = {at, st};
+  auto through = [&](int v) {  // past reshapes
+    const Op* o = def_of(an, v);
+    while (o && o->name == "xt.reshape") {
+      seen.insert(o);
+      o = def_of(an, o->operands[0]);
+    }
+    return o;
+  };
+  if (through(st->operands[0]) != at) return false;
+  AttendPlan& a = p.attend;
+  a = AttendPlan{};
+  const Type &tq = an.f.type_of(at->operands[0]), &tk = an.f.type_of(at->operands[1]);
+  a.elem = tq.elem;
+  a.keys = tk.shape[0];
+  a.d = tk.shape[1];
+  a.heads = tq.rank() == 3 ? tq.shape[0] : tq.shape[1] / a.d;
+  a.rows = tq.rank() == 3 ? tq.shape[1] : tq.shape[0];
+  const bool token = tq.rank() == 2;
+  const std::vector<int64_t> hrd = token ? std::vector<int64_t>{a.rows, a.heads, a.d}
+                                         : std::vector<int64_t>{a.heads, a.rows, a.d};
+  const Attr* extras = find_attr(at->attrs, "extras");
+  std::vector<int> read;
+  std::vector<int64_t> s;
+  auto rows_of = [&](const Op* o, AttendAccess& x) {
+    if (!attend_access(an, *o, hrd, x, s, err)) return false;
+    x.head = s[token ? 1 : 0];
+    x.row = s[token ? 0 : 1];
+    return true;
+  };
+  err.clear();
+  AttendAccess* kv[2] = {&a.k, &a.v};
+  for (size_t i = 0, e = 0; i < at->operands.size(); ++i) {
+    const Op* ld = through(at->operands[i]);
+    if (!ld || ld->name != "xt.load") {
+      err = "attend operands must be loaded tiles, reshapes in between";
+      return false;
+    }
+    seen.insert(ld);
+    if (i == 0) {
+      if (!rows_of(ld, a.q)) return false;
+    } else if (i < 3) {
+      if (!attend_access(an, *ld, {a.keys, a.d}, *kv[i - 1], s, err)) return false;
+      kv[i - 1]->row = s[0];
+    } else {
+      while (!extras->ints[e]) ++e;
+      const Type& t = an.f.type_of(at->operands[i]);
+      if (!attend_access(an, *ld, t.shape, a.extra[e], s, err)) return false;
+      a.extra[e].row = s[1];
+      ++e;
+    }
+    if (i) read.push_back(an.arg_index(ld->operands[0]));
+  }
+  if (!rows_of(st, a.o)) return false;
+  if (seen.size() != an.compute.size()) {
+    err = "attend programs must be store(attend(...)) with loaded operands and nothing else";
+    return false;
+  }
+  if (!stored_apart({a.o.arg}, read, "attend", err)) return false;
+  if (a.d % 32 || a.d > 256) {
+    err = "the HIP attend kernel takes heads of 32 to 256 columns, a multiple of 32; got " + std::to_string(a.d);
+    return false;
+  }
+  const double blocks = double(p.grid[0]) * p.grid[1] * p.grid[2];
+  const int64_t rows = a.heads * a.rows;
+  if (a.keys >= (int64_t(1) << 30) || double(a.heads) * double(a.rows) >= double(1 << 30) ||
+      blocks * double(rows) >= 2147483648.0) {
+    err = "the HIP attend kernel takes fewer than 2^30 keys, and than 2^31 rows over the grid";
+    return false;
+  }
+  if (a.k.row >= (int64_t(1) << 24) || a.v.row >= (int64_t(1) << 24) || (a.extra[5].arg >= 0 && a.extra[5].row > 1)) {
+    err = "the HIP attend kernel takes keys and values in rows less than 2^24 elements apart, and documents of the keys "
+          "side by side";
+    return false;
+  }
+  a.scale = static_cast<float>(find_attr(at->attrs, "scale")->f);
+  if (const Attr* c = find_attr(at->attrs, "cap")) a.cap = static_cast<float>(c->f);
+  if (const Attr* c = find_attr(at->attrs, "causal")) a.causal = c->i != 0;
+  if (const Attr* w = find_attr(at->attrs, "window")) a.window = w->i;
+  p.kind = PlanKind::Attend;
+  a.splits = attend_splits(p);
+  if (a.splits > 1) p.workspace = static_cast<int64_t>(blocks) * rows * a.splits * (a.d + 2) * 4;
+  // every pair is counted: masks are known at the launch, causal rows before it
+  double pairs = double(rows) * double(a.keys);
+  if (a.causal && a.extra[1].arg < 0 && a.extra[3].arg < 0) {
+    pairs = 0;
+    for (int64_t r = 0; r < a.rows; ++r) pairs += double(std::min(r + 1, a.keys));
+    pairs *= double(a.heads);
+  }
+  p.algo_flops = blocks * pairs * 4.0 * double(a.d);
+  read.push_back(a.q.arg);
+  read.push_back(a.o.arg);
+  for (int arg : read) {
+    const Type& t = an.f.type_of(an.f.args[arg]);
+    p.algo_bytes += double(t.numel()) * elem_bytes(t.elem);
+  }
+  return true;
+}
+
 // -- Conv2d ----------------------------------------------------------------------
 
 bool match_conv(const Analysis& an, Plan& p, std::string& err) {
@@ -963,6 +1268,26 @@ std::string Plan::describe() const {
       os << fused->layout << " insts=" << vm.inst.size();
       if (gemm_ragged) os << " gemm k=" << gemm_k;
       break;
+    case PlanKind::RmsNorm:
+      os << "rms_norm " << elem_name(norm.x.elem) << "->" << elem_name(norm.y.elem) << (norm.residual ? " residual" : "")
+         << " tile=" << norm.x.rows << "x" << norm.x.cols;
+      break;
+    case PlanKind::MatmulQ4:
+      os << "matmul_q4 " << elem_name(q4.x.elem) << "->" << elem_name(q4.y.elem) << " tile=" << q4.y.rows << "x"
+         << q4.y.cols << " k=" << q4.K << " group=" << q4.group;
+      break;
+    case PlanKind::Attend: {
+      os << "attend " << elem_name(attend.elem) << " heads=" << attend.heads << " rows=" << attend.rows
+         << " keys=" << attend.keys << " d=" << attend.d;
+      if (attend.cap > 0) os << " cap";
+      if (attend.causal) os << " causal";
+      if (attend.window) os << " window=" << attend.window;
+      static const char* names[6] = {"slopes", "start", "length", "prefix", "docs", ""};
+      for (int e = 0; e < 5; ++e)
+        if (attend.extra[e].arg >= 0) os << " " << names[e];
+      if (attend.splits > 1) os << " splits=" << attend.splits;
+      break;
+    }
     case PlanKind::Conv2d:
       os << "conv2d_nhwc " << elem_name(conv.elem) << "->" << elem_name(conv.out_elem) << " tile=" << conv.TB
          << "x" << conv.TH << "x" << conv.TW << "x" << conv.TC << " filter=" << conv.KH << "x" << conv.KW << "x"
@@ -1006,6 +1331,18 @@ GemmCover gemm_cover(const Plan& p, int64_t w, bool is_m) {
     }
   }
   return c;
+}
+
+int attend_splits(const Plan& p) {
+  const AttendPlan& a = p.attend;
+  const int64_t rows = a.heads * a.rows, per = rows <= kAttendFewRows ? kAttendFewRows : kAttendRows;
+  const double tiles = double(p.grid[0]) * p.grid[1] * p.grid[2] * double((rows + per - 1) / per);
+  // Four workgroups a CU, so that sequences of different lengths even out, but
+  // no fewer than 256 keys each.
+  const double want = 1024 / tiles;
+  const int64_t most = a.keys / 256;
+  if (want < 2 || most < 2) return 1;
+  return static_cast<int>(std::min<double>(std::min<double>(want, double(most)), 256));
 }
 
 bool gemm_tile(const GemmCover& m, const GemmCover& n, bool over_a, bool over_b) {
@@ -1079,7 +1416,7 @@ bool build_plan(const Module& m, const std::string& func, Plan& p, std::string& 
   // the tile interpreter, and the first reason is reported if that fails too
   err.clear();
   std::string first;
-  for (auto match : {match_ew, match_softmax, match_gemm, match_conv}) {
+  for (auto match : {match_ew, match_softmax, match_gemm, match_conv, match_rms_norm, match_q4, match_attend}) {
     std::string why;
     if (match(an, p, why)) return true;
     if (first.empty()) first = why;

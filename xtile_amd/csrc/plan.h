@@ -41,7 +41,7 @@ struct Coord {
   int64_t value = 0;
 };
 
-enum class PlanKind { EwBinary, RowSoftmax, Gemm, Conv2d, TileVM, Fused };
+enum class PlanKind { EwBinary, RowSoftmax, Gemm, Conv2d, TileVM, Fused, RmsNorm, MatmulQ4, Attend };
 enum class EwOp { Add = 0, Sub = 1, Mul = 2 };
 
 struct ConvPlan {
@@ -114,6 +114,48 @@ struct FusedPlan {
   int attend_threads = 0, attend_workgroups = 0;
 };
 
+// store(rms_norm(load x [+ load r], load gamma)), the sum stored too where there
+// is one and its store is wanted, or the norm's int8 rows and their scales.
+struct NormPlan {
+  bool residual = false, keep_sum = false, quantize = false;
+  Access2D x, r, gamma, sum, y, scale;  // y: the int8 rows with `quantize`; scale: (R, 1)
+  float eps = 0;
+};
+
+// store(matmul_q4(load x, load w, load scales[, load row_scale])).
+struct Q4Plan {
+  bool row_scale = false;
+  Access2D x, w, scales, rows, y;
+  int64_t K = 0, group = 0;
+};
+
+// One operand of an attend program as heads x rows x D (or rows x columns) of a
+// strided array; strides in elements, D contiguous.
+struct AttendAccess {
+  int arg = -1;
+  Elem elem = Elem::None;
+  TileAddr addr;
+  int64_t head = 0, row = 0;
+};
+
+// store([reshape] attend([reshape] load q, k, v, extras)).
+struct AttendPlan {
+  Elem elem = Elem::None;
+  int64_t heads = 0, rows = 0, keys = 0, d = 0;  // of a Block; `heads` query heads share its keys
+  AttendAccess q, k, v, o;
+  AttendAccess extra[6];  // slopes, start, length, prefix, q_docs, k_docs; arg -1: absent
+  float scale = 1, cap = 0;  // cap 0: none
+  bool causal = false;
+  int64_t window = 0;        // 0: none
+  // Few rows over many keys: workgroups a row tile that split the keys between
+  // them where the launch is given a workspace (1: never).
+  int splits = 1;
+};
+
+// Rows of one attend workgroup: up to 32 take one wave's width with the keys
+// dealt to the waves, more take 128 with the keys shared.
+constexpr int64_t kAttendFewRows = 32, kAttendRows = 128;
+
 struct Plan {
   PlanKind kind = PlanKind::EwBinary;
   std::string func;
@@ -137,6 +179,10 @@ struct Plan {
   // kernel for ragged sizes runs it where the buffers allow.
   bool gemm_ragged = false;
   ConvPlan conv;
+  NormPlan norm;
+  Q4Plan q4;
+  AttendPlan attend;
+  int64_t workspace = 0;  // bytes a launch may work in beside its buffers
   VmPlan vm;
   std::shared_ptr<FusedPlan> fused;  // Fused: the generated kernel (vm keeps the accesses)
   std::string unfused;               // TileVM: why the program is not fused
@@ -192,6 +238,9 @@ GemmCover gemm_cover(const Plan& p, int64_t w, bool is_m);
 // B) in LDS before it stores, and another tile of the Block would still read
 // them.
 bool gemm_tile(const GemmCover& m, const GemmCover& n, bool over_a, bool over_b);
+
+// Workgroups that share an attend tile's keys, of a plan whose sizes are set.
+int attend_splits(const Plan& p);
 
 // Builds the plan of function `func` (empty name: the only function).
 // Returns false and sets `error` when the program is not one the HIP

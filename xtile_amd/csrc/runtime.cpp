@@ -59,11 +59,17 @@ int get_plan(xt_module* m, const std::string& func, std::shared_ptr<const xt::Pl
   return XT_OK;
 }
 
-// Enqueues a plan over buffers known to hold its memrefs.
-int run_plan(const xt::Plan& p, void* const* bufs, void* stream, char** err) {
+// Enqueues a plan over buffers known to hold its memrefs.  `work` is its workspace,
+// or null.
+int run_plan(const xt::Plan& p, void* const* bufs, void* work, size_t work_bytes, void* stream, char** err) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   std::string why;
   hipError_t e = hipSuccess;
+  if (work && p.workspace &&
+      (work_bytes < static_cast<size_t>(p.workspace) || reinterpret_cast<uintptr_t>(work) % 16))
+    return fail(err, XT_ERR_ARGUMENT,
+                "@" + p.func + " works in " + std::to_string(p.workspace) + " bytes at a multiple of 16, got " +
+                    std::to_string(work_bytes));
   switch (p.kind) {
     case xt::PlanKind::EwBinary: e = xtk::launch_ew_binary(p, bufs, s, why); break;
     case xt::PlanKind::RowSoftmax: e = xtk::launch_row_softmax(p, bufs, s, why); break;
@@ -71,6 +77,9 @@ int run_plan(const xt::Plan& p, void* const* bufs, void* stream, char** err) {
     case xt::PlanKind::Conv2d: e = xtk::launch_conv2d(p, bufs, s, why); break;
     case xt::PlanKind::TileVM: e = xtk::launch_tilevm(p, bufs, s, why); break;
     case xt::PlanKind::Fused: e = xtk::launch_fused(p, bufs, s, why); break;
+    case xt::PlanKind::RmsNorm: e = xtk::launch_rms_norm(p, bufs, s, why); break;
+    case xt::PlanKind::MatmulQ4: e = xtk::launch_matmul_q4(p, bufs, s, why); break;
+    case xt::PlanKind::Attend: e = xtk::launch_attend(p, bufs, work, s, why); break;
   }
   if (!why.empty()) return fail(err, XT_ERR_ARGUMENT, why);
   if (e != hipSuccess)
@@ -202,8 +211,26 @@ int xt_plan(xt_module* m, const char* func, char** out_desc, double* algo_bytes,
   return XT_OK;
 }
 
+int xt_workspace_bytes(xt_module* m, const char* func, size_t* bytes, char** err) {
+  if (!m || !bytes) return fail(err, XT_ERR_TYPE, "expected an xtile module");
+  std::shared_ptr<const xt::Plan> plan;
+  std::lock_guard<std::mutex> lock(m->mu);
+  int st = get_plan(m, func_key(func), plan, err);
+  if (st == XT_OK) *bytes = static_cast<size_t>(plan->workspace);
+  return st;
+}
+
 int xt_gpu_run(xt_module* m, const char* func, void* const* bufs, const size_t* buf_bytes,
                int nbufs, void* stream, char** err) {
+  return xt_gpu_run_with(m, func, bufs, buf_bytes, nbufs, nullptr, 0, stream, err);
+}
+
+int xt_gpu_run_buffers(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, void* stream, char** err) {
+  return xt_gpu_run_buffers_with(m, func, bufs, nbufs, nullptr, 0, stream, err);
+}
+
+int xt_gpu_run_with(xt_module* m, const char* func, void* const* bufs, const size_t* buf_bytes, int nbufs, void* work,
+                    size_t work_bytes, void* stream, char** err) {
   if (!m) return fail(err, XT_ERR_TYPE, "expected an xtile module");
   std::shared_ptr<const xt::Plan> plan;
   {
@@ -226,10 +253,11 @@ int xt_gpu_run(xt_module* m, const char* func, void* const* bufs, const size_t* 
                   "buffer " + std::to_string(k) + " holds " + std::to_string(buf_bytes[k]) +
                       " bytes; " + t.str() + " needs " + std::to_string(need));
   }
-  return run_plan(p, bufs, stream, err);
+  return run_plan(p, bufs, work, work_bytes, stream, err);
 }
 
-int xt_gpu_run_buffers(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, void* stream, char** err) {
+int xt_gpu_run_buffers_with(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, void* work,
+                            size_t work_bytes, void* stream, char** err) {
   if (!m) return fail(err, XT_ERR_TYPE, "expected an xtile module");
   std::shared_ptr<const xt::Plan> plan;
   {
@@ -251,7 +279,7 @@ int xt_gpu_run_buffers(xt_module* m, const char* func, const xt_buffer* bufs, in
     if (!same) return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is not a " + t.str());
     ptrs[k] = bufs[k].ptr;
   }
-  return run_plan(p, ptrs, stream, err);
+  return run_plan(p, ptrs, work, work_bytes, stream, err);
 }
 
 }  // extern "C"

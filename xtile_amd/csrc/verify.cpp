@@ -9,8 +9,10 @@
 //   reductions                       lib/xt/XTOps.cpp:274-307
 //   reshape / transpose / permute    lib/xt/XTOps.cpp:309-397
 // Extension (not in the reference): matmul and load_conv2d also accept
-// f16 x f16 and bf16 x bf16 inputs with an f32 result.
+// f16 x f16 and bf16 x bf16 inputs with an f32 result; the ops rms_norm,
+// row_scale, quantize, matmul_q4 and attend.
 #include <algorithm>
+#include <cmath>
 
 #include "ir.h"
 
@@ -57,6 +59,79 @@ struct Verifier {
     const Attr* a = find_attr(o.attrs, name);
     if (!a) fail(o.loc, o.name, std::string("requires attribute '") + name + "'");
     return a;
+  }
+
+  static bool narrow_or_f32(Elem e) { return e == Elem::F32 || e == Elem::F16 || e == Elem::BF16; }
+
+  // A finite f32 attribute, positive (or, zero_ok, not negative).
+  bool number_attr(const Op& o, const Attr* a, const char* name, bool zero_ok) {
+    const double v = a->kind == Attr::Float ? static_cast<double>(static_cast<float>(a->f)) : -1;
+    if (a->kind != Attr::Float || a->type.elem != Elem::F32 || !std::isfinite(v) || v < 0 || (!zero_ok && v == 0))
+      return fail(o.loc, o.name, std::string(name) + " attribute must be a finite, " +
+                                     (zero_ok ? "non-negative" : "positive") + " f32");
+    return true;
+  }
+
+  // Rank-2 statically shaped tensors throughout.
+  bool rank2(const Func& f, const Op& o) {
+    for (const std::vector<int>* vs : {&o.operands, &o.results})
+      for (int v : *vs) {
+        const Type& t = f.type_of(v);
+        if (!t.is_tensor()) return fail(o.loc, o.name, "requires ranked tensor operands and result");
+        if (t.rank() != 2) return fail(o.loc, o.name, "requires rank-2 tensors");
+      }
+    return true;
+  }
+
+  bool verify_attend(const Func& f, const Op& o) {
+    const std::string& n = o.name;
+    auto T = [&](int v) -> const Type& { return f.type_of(v); };
+    for (int v : o.operands)
+      if (!T(v).is_tensor()) return fail(o.loc, n, "requires ranked tensor operands and result");
+    const Type &q = T(o.operands[0]), &k = T(o.operands[1]), &v = T(o.operands[2]);
+    if (q != T(o.results[0])) return fail(o.loc, n, "requires query and result tensor types to match");
+    if ((q.elem != Elem::F16 && q.elem != Elem::BF16) || k.elem != q.elem || v.elem != q.elem)
+      return fail(o.loc, n, "requires f16 or bf16 query, key and value tensors of one type");
+    if (k.rank() != 2 || k != v) return fail(o.loc, n, "requires (keys, D) key and value tensors of one shape");
+    const int64_t nk = k.shape[0], d = k.shape[1];
+    int64_t heads, rows;
+    if (q.rank() == 3 && q.shape[2] == d) {
+      heads = q.shape[0];
+      rows = q.shape[1];
+    } else if (q.rank() == 2 && q.shape[1] % d == 0) {
+      heads = q.shape[1] / d;
+      rows = q.shape[0];
+    } else {
+      return fail(o.loc, n, "requires a (heads, rows, D) or (rows, heads * D) query tensor");
+    }
+    const Attr* scale = need_attr(o, "scale");
+    const Attr* extras = need_attr(o, "extras");
+    if (!scale || !extras) return false;
+    if (!number_attr(o, scale, "scale", false)) return false;
+    if (const Attr* cap = find_attr(o.attrs, "cap"))
+      if (!number_attr(o, cap, "cap", false)) return false;
+    if (const Attr* c = find_attr(o.attrs, "causal"))
+      if (c->kind != Attr::Bool) return fail(o.loc, n, "causal attribute must be true or false");
+    if (const Attr* w = find_attr(o.attrs, "window"))
+      if (w->kind != Attr::Int || w->i <= 0 || w->i > 0x7fffffff)
+        return fail(o.loc, n, "window attribute must be positive and below 2^31");
+    if (extras->kind != Attr::DenseArray || extras->ints.size() != 6)
+      return fail(o.loc, n, "extras attribute must have exactly 6 entries");
+    size_t count = 3;
+    for (int64_t e : extras->ints) {
+      if (e != 0 && e != 1) return fail(o.loc, n, "extras attribute entries must be 0 or 1");
+      count += static_cast<size_t>(e);
+    }
+    if (count != o.operands.size()) return fail(o.loc, n, "extras attribute does not match the operand count");
+    if (extras->ints[4] != extras->ints[5]) return fail(o.loc, n, "q_docs and k_docs come together");
+    static const char* names[6] = {"slopes", "start", "length", "prefix", "q_docs", "k_docs"};
+    const int64_t cols[6] = {heads, 1, 1, 1, rows, nk};
+    for (size_t e = 0, at = 3; e < 6; ++e) {
+      if (!extras->ints[e]) continue;
+      const Type want = Type::tensor(e == 0 ? Elem::F32 : Elem::I32, {1, cols[e]});
+      if (T(o.operands[at++]) != want) return fail(o.loc, n, std::string(names[e]) + " must be a " + want.str());
+    }
+    return true;
   }
 
   bool verify_op(const Func& f, const Op& o) {
@@ -306,6 +381,50 @@ struct Verifier {
                       "permute result shape must match the input shape reordered by permutation");
       return true;
     }
+    if (n == "xt.rms_norm") {
+      if (!rank2(f, o)) return false;
+      const Type &x = T(o.operands[0]), &g = T(o.operands[1]), &r = T(o.results[0]);
+      if (x.shape != r.shape) return fail(o.loc, n, "requires operand and result tensor shapes to match");
+      if (g.shape[0] != 1 || g.shape[1] != x.shape[1])
+        return fail(o.loc, n, "requires a (1, C) gamma matching the operand's columns");
+      if (!narrow_or_f32(x.elem) || !narrow_or_f32(g.elem) || !narrow_or_f32(r.elem))
+        return fail(o.loc, n, "requires f32, f16 or bf16 element types");
+      const Attr* eps = need_attr(o, "eps");
+      return eps && number_attr(o, eps, "eps", true);
+    }
+    if (n == "xt.row_scale") {
+      if (!rank2(f, o)) return false;
+      const Type &x = T(o.operands[0]), &r = T(o.results[0]);
+      if (!narrow_or_f32(x.elem)) return fail(o.loc, n, "requires an f32, f16 or bf16 operand");
+      if (r != Type::tensor(Elem::F32, {x.shape[0], 1}))
+        return fail(o.loc, n, "requires an f32 result with one value a row");
+      return true;
+    }
+    if (n == "xt.quantize") {
+      if (!rank2(f, o)) return false;
+      const Type &x = T(o.operands[0]), &s = T(o.operands[1]), &r = T(o.results[0]);
+      if (!narrow_or_f32(x.elem)) return fail(o.loc, n, "requires an f32, f16 or bf16 operand");
+      if (s != Type::tensor(Elem::F32, {x.shape[0], 1}))
+        return fail(o.loc, n, "requires an f32 scale with one value a row");
+      if (r != Type::tensor(Elem::I8, x.shape)) return fail(o.loc, n, "requires an i8 result of the operand's shape");
+      return true;
+    }
+    if (n == "xt.matmul_q4") {
+      if (!rank2(f, o)) return false;
+      const Type &x = T(o.operands[0]), &w = T(o.operands[1]), &s = T(o.operands[2]), &r = T(o.results[0]);
+      if ((x.elem != Elem::I8 && x.elem != Elem::F16 && x.elem != Elem::BF16) || w.elem != Elem::I8 ||
+          !narrow_or_f32(s.elem) || !narrow_or_f32(r.elem))
+        return fail(o.loc, n, "requires an i8, f16 or bf16 lhs, i8 weights and f32, f16 or bf16 scales and result");
+      if (x.shape[1] != 2 * w.shape[1]) return fail(o.loc, n, "requires two weights a byte: weight columns half the lhs's");
+      if (s.shape[0] != w.shape[0] || x.shape[1] % s.shape[1] || (x.shape[1] / s.shape[1]) % 32)
+        return fail(o.loc, n, "requires (N, K / G) scales for groups of G weights, G a multiple of 32");
+      if (r.shape[0] != x.shape[0] || r.shape[1] != w.shape[0])
+        return fail(o.loc, n, "result shape must match matmul output shape");
+      if (o.operands.size() == 4 && T(o.operands[3]) != Type::tensor(Elem::F32, {x.shape[0], 1}))
+        return fail(o.loc, n, "requires an f32 row scale with one value a row");
+      return true;
+    }
+    if (n == "xt.attend") return verify_attend(f, o);
     if (n == "func.return") {
       if (o.operands.size() != f.result_types.size())
         return fail(o.loc, n, "has " + std::to_string(o.operands.size()) +

@@ -20,11 +20,16 @@ Reference behaviour followed here (file:line into the reference tree):
 Extension (not in the reference, documented as such): `float16` and
 `bfloat16` dtypes.  Narrow-float `matmul` and `load_conv2d` produce a float32
 result, mirroring the reference's int8 -> float32 rule (xtile/dsl.py:369-370).
+Also an extension: `int32` arrays (positions, lengths, documents), and the
+operators of a language model's layer, each one op over whole tiles:
+`rms_norm`, `row_scale` and `quantize` (rows in 8 bits), `matmul_q4` (4-bit
+weights) and `attend` (masked attention).
 """
 
 from __future__ import annotations
 
 import inspect
+import math
 from dataclasses import dataclass
 from typing import Callable, Sequence
 
@@ -45,8 +50,11 @@ int8 = DType(name="int8", mlir_name="i8")
 # Extension dtypes (MFMA input types on gfx950).
 float16 = DType(name="float16", mlir_name="f16")
 bfloat16 = DType(name="bfloat16", mlir_name="bf16")
+# Extension dtype of what `attend` takes beside its tiles: positions, lengths, documents.
+int32 = DType(name="int32", mlir_name="i32")
 
 _NARROW_FLOATS = (float16, bfloat16)
+_FLOATS = (float32, *_NARROW_FLOATS)
 
 
 def _all_positive_ints(values: object) -> bool:
@@ -235,6 +243,35 @@ class _Compute:
             f"{self.result.ssa_name} = {self.op_name}({operand_names}){attr} : "
             f"{operand_types} -> {_tensor_type(self.result.shape, self.result.dtype)}"
         )
+
+
+@dataclass(frozen=True)
+class _Operator:
+    """A tensor -> tensor op with attributes of its own (`attrs`: names and their text)."""
+
+    op_name: str
+    result: TensorValue
+    operands: tuple[TensorValue, ...]
+    attrs: tuple[tuple[str, str], ...] = ()
+
+    def render(self, names: dict[int, str]) -> str:
+        attr = " {" + ", ".join(f"{k} = {v}" for k, v in sorted(self.attrs)) + "}" if self.attrs else ""
+        operand_names = ", ".join(v.ssa_name for v in self.operands)
+        operand_types = ", ".join(_tensor_type(v.shape, v.dtype) for v in self.operands)
+        return (
+            f"{self.result.ssa_name} = {self.op_name}({operand_names}){attr} : "
+            f"{operand_types} -> {_tensor_type(self.result.shape, self.result.dtype)}"
+        )
+
+
+def _float_text(value: float) -> str:
+    """An f32 attribute's text, as the printer of the native IR writes it."""
+    text = f"{value:.6e}"
+    if float(text) != value:
+        text = f"{value:.17g}"
+        if not any(c in text for c in ".en"):
+            text += ".0"
+    return text + " : f32"
 
 
 def _coords_text(index: tuple) -> str:
@@ -563,6 +600,118 @@ class TraceContext:
         self.ops.append(_Compute("xt.transpose", result, (value,)))
         return result
 
+    # -- operators of a language model's layer (extension) ------------------
+
+    @staticmethod
+    def _number(op: str, name: str, value: object, positive: bool = True) -> float:
+        if isinstance(value, bool) or not isinstance(value, (int, float)):
+            raise TypeError(f"{op} requires {name} to be a number")
+        if not math.isfinite(value) or value < 0 or (positive and value == 0) or value > 3.4028234663852886e38:
+            raise ValueError(f"{op} requires {name} to be finite and {'positive' if positive else 'non-negative'}")
+        return float(value)
+
+    def rms_norm(self, value, gamma, eps: float = 1e-6, dtype: DType | None = None) -> TensorValue:
+        self._need_tensor(value)
+        self._need_tensor(gamma)
+        dtype = value.dtype if dtype is None else dtype
+        if len(value.shape) != 2:
+            raise ValueError("xt.rms_norm currently supports rank-2 tensors only")
+        if gamma.shape != (1, value.shape[1]):
+            raise ValueError("xt.rms_norm requires a (1, C) gamma matching the value's columns")
+        if value.dtype not in _FLOATS or gamma.dtype not in _FLOATS or dtype not in _FLOATS:
+            raise TypeError("xt.rms_norm requires float32, float16 or bfloat16 tensors and result")
+        eps = self._number("xt.rms_norm", "eps", eps, positive=False)
+        result = self._value("rms", value.shape, dtype)
+        self.ops.append(_Operator("xt.rms_norm", result, (value, gamma), (("eps", _float_text(eps)),)))
+        return result
+
+    def row_scale(self, value) -> TensorValue:
+        self._need_tensor(value)
+        if len(value.shape) != 2:
+            raise ValueError("xt.row_scale currently supports rank-2 tensors only")
+        if value.dtype not in _FLOATS:
+            raise TypeError("xt.row_scale requires a float32, float16 or bfloat16 tensor")
+        result = self._value("row_scale", (value.shape[0], 1), float32)
+        self.ops.append(_Operator("xt.row_scale", result, (value,)))
+        return result
+
+    def quantize(self, value, scale) -> TensorValue:
+        self._need_tensor(value)
+        self._need_tensor(scale)
+        if len(value.shape) != 2:
+            raise ValueError("xt.quantize currently supports rank-2 tensors only")
+        if scale.shape != (value.shape[0], 1):
+            raise ValueError("xt.quantize requires a (R, 1) scale matching the value's rows")
+        if value.dtype not in _FLOATS or scale.dtype != float32:
+            raise TypeError("xt.quantize requires a float tensor and a float32 scale")
+        result = self._value("quantized", value.shape, int8)
+        self.ops.append(_Operator("xt.quantize", result, (value, scale)))
+        return result
+
+    def matmul_q4(self, value, weight, scales, row_scale=None, dtype: DType = float32) -> TensorValue:
+        operands = (value, weight, scales) if row_scale is None else (value, weight, scales, row_scale)
+        for v in operands:
+            self._need_tensor(v)
+        if any(len(v.shape) != 2 for v in operands):
+            raise ValueError("xt.matmul_q4 currently supports rank-2 tensors only")
+        (m, k), (n, half) = value.shape, weight.shape
+        if value.dtype not in (int8, *_NARROW_FLOATS) or weight.dtype != int8 or scales.dtype not in _FLOATS:
+            raise TypeError("xt.matmul_q4 requires an int8, float16 or bfloat16 value, int8 weights and float scales")
+        if dtype not in _FLOATS:
+            raise TypeError("xt.matmul_q4 requires a float32, float16 or bfloat16 result")
+        if k != 2 * half:
+            raise ValueError("xt.matmul_q4 requires two weights a byte: weight columns half the value's")
+        if scales.shape[0] != n or k % scales.shape[1] or (k // scales.shape[1]) % 32:
+            raise ValueError("xt.matmul_q4 requires (N, K / G) scales for groups of G weights, G a multiple of 32")
+        if row_scale is not None and (row_scale.shape != (m, 1) or row_scale.dtype != float32):
+            raise ValueError("xt.matmul_q4 requires a float32 (M, 1) row scale")
+        result = self._value("matmul", (m, n), dtype)
+        self.ops.append(_Operator("xt.matmul_q4", result, operands))
+        return result
+
+    def attend(self, q, k, v, scale, cap=None, causal=False, window=None, slopes=None, start=None, length=None,
+               prefix=None, q_docs=None, k_docs=None) -> TensorValue:
+        extras = (slopes, start, length, prefix, q_docs, k_docs)
+        for t in (q, k, v, *(e for e in extras if e is not None)):
+            self._need_tensor(t)
+        if q.dtype not in _NARROW_FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError("xt.attend requires float16 or bfloat16 tensors of one dtype")
+        if len(k.shape) != 2 or k.shape != v.shape:
+            raise ValueError("xt.attend requires (keys, D) key and value tensors of one shape")
+        nk, d = k.shape
+        if len(q.shape) == 3 and q.shape[2] == d:
+            heads, rows = q.shape[0], q.shape[1]
+        elif len(q.shape) == 2 and q.shape[1] % d == 0:
+            heads, rows = q.shape[1] // d, q.shape[0]
+        else:
+            raise ValueError("xt.attend requires a (heads, rows, D) or (rows, heads * D) query tensor")
+        if (q_docs is None) != (k_docs is None):
+            raise ValueError("xt.attend requires q_docs and k_docs together")
+        wants = ((1, heads), (1, 1), (1, 1), (1, 1), (1, rows), (1, nk))
+        for name, t, shape in zip(("slopes", "start", "length", "prefix", "q_docs", "k_docs"), extras, wants):
+            dtype = float32 if name == "slopes" else int32
+            if t is not None and (t.shape != shape or t.dtype != dtype):
+                raise ValueError(f"xt.attend requires {name} of shape {shape} and dtype {dtype.name}")
+        attrs = [("scale", _float_text(self._number("xt.attend", "scale", scale)))]
+        if cap is not None:
+            attrs.append(("cap", _float_text(self._number("xt.attend", "cap", cap))))
+        if not isinstance(causal, bool):
+            raise TypeError("xt.attend requires causal to be True or False")
+        if causal:
+            attrs.append(("causal", "true"))
+        if window is not None:
+            if isinstance(window, bool) or not isinstance(window, int):
+                raise TypeError("xt.attend requires window to be an integer")
+            if not 0 < window < 2**31:
+                raise ValueError("xt.attend requires window to be positive and below 2**31")
+            attrs.append(("window", f"{window} : i64"))
+        present = ", ".join("1" if e is not None else "0" for e in extras)
+        attrs.append(("extras", f"array<i32: {present}>"))
+        result = self._value("attend", q.shape, q.dtype)
+        operands = (q, k, v, *(e for e in extras if e is not None))
+        self.ops.append(_Operator("xt.attend", result, operands, tuple(attrs)))
+        return result
+
     # -- emission ---------------------------------------------------------
 
     def _arg_names(self) -> dict[int, str]:
@@ -727,6 +876,50 @@ def reshape(input_value, *, shape):
 
 def transpose(input_value):
     return _trace("transpose").transpose(input_value)
+
+
+def rms_norm(value, gamma, *, eps: float = 1e-6, dtype: DType | None = None):
+    """`value / sqrt(mean(value ** 2) + eps) * gamma`, row by row: a (R, C) tile and
+    a (1, C) gamma.  Held in 32 bits, rounded once where it is stored."""
+    return _trace("rms_norm").rms_norm(value, gamma, eps=eps, dtype=dtype)
+
+
+def row_scale(value):
+    """(R, 1) float32 scales of a tile's rows in 8 bits: the largest magnitude of
+    a row over 127."""
+    return _trace("row_scale").row_scale(value)
+
+
+def quantize(value, scale):
+    """`value / scale` to the nearest int8 (half to even), at most 127 in
+    magnitude; 0 in rows whose scale is 0 and where the quotient is NaN."""
+    return _trace("quantize").quantize(value, scale)
+
+
+def matmul_q4(value, weight, scales, *, row_scale=None, dtype: DType = float32):
+    """`value @ w.T` with 4-bit weights: value (M, K), weight (N, K / 2) int8 as
+    `pack_q4` lays them out, scales (N, K / G) with one scale a group of G weights
+    of a row.  `row_scale` (M, 1) multiplies the rows of the result: with the int8
+    rows of `quantize` it is their scale."""
+    return _trace("matmul_q4").matmul_q4(value, weight, scales, row_scale=row_scale, dtype=dtype)
+
+
+def attend(q, k, v, *, scale, cap=None, causal=False, window=None, slopes=None, start=None, length=None, prefix=None,
+           q_docs=None, k_docs=None):
+    """`softmax(scores) v` over the keys that each query row sees.
+
+    q is (heads, rows, D) or (rows, heads * D); its heads share k and v, (keys,
+    D).  Row t of q is at position `start + t` (start: a (1, 1) int32 tile, 0
+    without it), key j at position j.  The score of a pair is `scale * q . k`,
+    with `cap` `cap * tanh(score / cap)`, less `slopes[head] * distance` with
+    `slopes`, a (1, heads) float32 tile.  Row at p sees key j when all hold:
+    j < length (a (1, 1) int32 tile); their documents are equal (q_docs (1,
+    rows), k_docs (1, keys), int32); and j < prefix (a (1, 1) int32 tile), or
+    j <= p if `causal` and p - j < window if `window` is given.  Rows that see
+    nothing, or only scores of minus infinity, are 0.  What hidden keys and
+    values hold, NaN included, has no effect."""
+    return _trace("attend").attend(q, k, v, scale, cap=cap, causal=causal, window=window, slopes=slopes, start=start,
+                                   length=length, prefix=prefix, q_docs=q_docs, k_docs=k_docs)
 
 
 def convert(kernel_fn, *, args, grid, double_buffering, parse_module):

@@ -11,6 +11,9 @@ the tile sizes of the five benchmark configurations:
   C4 conv2d   f16 NHWC 32x56x56x64, 3x3x64x64 filter, stride 1, pad 1 -> f32
   C5 matmul   bf16 4096x11008x4096 -> f32, 256x128 tiles, grid (86, 16, 1),
               A shared along axis 0 (`shared = 1`)
+
+Beside them: `layernorm`, `column_softmax`, `bias_add` and `attention`, and the
+operators of a language model's layer: `rms_norm`, `matmul_q4`, `masked_attention`.
 """
 
 from __future__ import annotations
@@ -19,6 +22,7 @@ from . import (
     Array,
     add as tile_add,
     astype,
+    attend,
     bfloat16,
     bid,
     cdiv,
@@ -27,13 +31,18 @@ from . import (
     float16,
     float32,
     int8,
+    int32,
     kernel,
     load,
     load_conv2d,
     matmul,
+    matmul_q4 as tile_matmul_q4,
     max as tile_max,
     mul as tile_mul,
+    quantize,
     reciprocal,
+    rms_norm as tile_rms_norm,
+    row_scale as tile_row_scale,
     rsqrt,
     reshape,
     store,
@@ -322,6 +331,129 @@ def attention(heads: int, nq: int, nk: int, d: int, tq: int = 64, qk=float16):
     va = Array(shape=(heads, nk, d), dtype=float32)
     oa = Array(shape=(heads, nq, d), dtype=float32)
     return convert(attention_kernel, args=(qa, ka, va, oa, tq, d, nk), grid=(nq // tq, heads, 1))
+
+
+# -- operators of a language model's layer -------------------------------------
+
+
+def rms_norm(rows: int, cols: int, dtype=bfloat16, *, residual: bool = True, quantize: bool = False, eps: float = 1e-6,
+             gamma=None, trow: int = 1):
+    """Root-mean-square norm of rows, after the residual's addition, to rows of the
+    input's type or to int8 rows with a float32 scale each.
+
+    Buffers: x, [the residual], gamma (1, cols) of dtype `gamma` (default: `dtype`),
+    [the sum], then y, or the int8 rows and their (rows, 1) scales.  The sum is
+    held in 32 bits for the norm and rounded where it is stored; it may be stored
+    over x or the residual (pass one tensor twice)."""
+    if rows % trow:
+        raise ValueError("trow must divide rows")
+    x = Array(shape=(rows, cols), dtype=dtype)
+    g = Array(shape=(1, cols), dtype=gamma or dtype)
+    rows8, scales = Array(shape=(rows, cols), dtype=int8), Array(shape=(rows, 1), dtype=float32)
+    to_rows8 = quantize
+    ins = 2 if residual else 1
+
+    def body(args):
+        r = bid(0)
+        h = load(args[0], index=(r, 0), shape=(trow, cols))
+        if residual:
+            h = tile_add(h, load(args[1], index=(r, 0), shape=(trow, cols)))
+            store(args[3], index=(r, 0), tile=h)
+        y = tile_rms_norm(h, load(args[ins], index=(0, 0), shape=(1, cols), shared=1), eps=eps)
+        if to_rows8:
+            s = tile_row_scale(y)
+            store(args[-2], index=(r, 0), tile=_quantize(y, s))
+            store(args[-1], index=(r, 0), tile=s)
+        else:
+            store(args[-1], index=(r, 0), tile=y)
+
+    arrays = [x] * ins + [g] + ([x] if residual else []) + ([rows8, scales] if quantize else [x])
+    return convert(_named("rms_norm_kernel", body, len(arrays)), args=tuple(arrays), grid=(rows // trow, 1, 1))
+
+
+def matmul_q4(m: int, n: int, k: int, *, group: int = 128, dtype=bfloat16, scales=float16, out=float32,
+              row_scale: bool = False):
+    """x (m, k) against n rows of k 4-bit weights with a scale for each `group` of a row.
+
+    Buffers: x of `dtype` (float16, bfloat16 or int8), the weights (n, k / 2) int8
+    from `pack_q4`, their scales (n, k / group), [row scales (m, 1) float32], y (m, n)."""
+    if group < 1 or k % group:
+        raise ValueError("group must divide k")
+    arrays = [Array(shape=(m, k), dtype=dtype), Array(shape=(n, k // 2), dtype=int8),
+              Array(shape=(n, k // group), dtype=scales)]
+    if row_scale:
+        arrays.append(Array(shape=(m, 1), dtype=float32))
+
+    def body(args):
+        tiles = [load(a, index=(0, 0), shape=t.shape) for a, t in zip(args, arrays)]
+        y = tile_matmul_q4(*tiles[:3], row_scale=tiles[3] if row_scale else None, dtype=out)
+        store(args[-1], index=(0, 0), tile=y)
+
+    args = (*arrays, Array(shape=(m, n), dtype=out))
+    return convert(_named("matmul_q4_kernel", body, len(args)), args=args, grid=(1, 1, 1))
+
+
+def masked_attention(batch: int, kv_heads: int, group: int, nq: int, nk: int, d: int, *, dtype=bfloat16, scale=None,
+                     cap=None, causal: bool = False, window=None, slopes: bool = False, start: bool = False,
+                     length: bool = False, prefix: bool = False, docs: bool = False, token_major: bool = False):
+    """Attention of `group` query heads to each key head, one Block a key head.
+
+    Buffers: q and the result [batch, kv_heads * group, nq, d], k and v [batch,
+    kv_heads, nk, d], or, `token_major`, [batch, nq, kv_heads * group * d] and
+    [batch, nk, kv_heads * d]; between v and the result, where asked for: slopes
+    (kv_heads, group) float32; start, length, prefix (batch, 1) int32; the documents
+    of the queries (batch, nq) and of the keys (batch, nk) int32.  Their meaning is
+    `attend`'s.  `scale` defaults to d ** -0.5."""
+    if min(batch, kv_heads, group, nq, nk, d) < 1:
+        raise ValueError("masked_attention sizes must be positive")
+    heads = kv_heads * group
+    q_shape = (batch, nq, heads * d) if token_major else (batch, heads, nq, d)
+    k_shape = (batch, nk, kv_heads * d) if token_major else (batch, kv_heads, nk, d)
+    per_batch = Array(shape=(batch, 1), dtype=int32)
+    named = {"slopes": (slopes, Array(shape=(kv_heads, group), dtype=float32)), "start": (start, per_batch),
+             "length": (length, per_batch), "prefix": (prefix, per_batch),
+             "q_docs": (docs, Array(shape=(batch, nq), dtype=int32)),
+             "k_docs": (docs, Array(shape=(batch, nk), dtype=int32))}
+    extras = {name: array for name, (wanted, array) in named.items() if wanted}
+    scale = d**-0.5 if scale is None else scale
+
+    def body(args):
+        h, b = bid(0), bid(1)
+        if token_major:
+            q = reshape(load(args[0], index=(b, 0, h), shape=(1, nq, group * d)), shape=(nq, group * d))
+            k, v = (reshape(load(a, index=(b, 0, h), shape=(1, nk, d)), shape=(nk, d)) for a in args[1:3])
+        else:
+            q = reshape(load(args[0], index=(b, h, 0, 0), shape=(1, group, nq, d)), shape=(group, nq, d))
+            k, v = (reshape(load(a, index=(b, h, 0, 0), shape=(1, 1, nk, d)), shape=(nk, d)) for a in args[1:3])
+        tiles = {}
+        for (name, array), arg in zip(extras.items(), args[3:]):
+            index, shape = ((h, 0), (1, group)) if name == "slopes" else ((b, 0), (1, array.shape[1]))
+            tiles[name] = load(arg, index=index, shape=shape)
+        o = attend(q, k, v, scale=scale, cap=cap, causal=causal, window=window, **tiles)
+        if token_major:
+            store(args[-1], index=(b, 0, h), tile=reshape(o, shape=(1, nq, group * d)))
+        else:
+            store(args[-1], index=(b, h, 0, 0), tile=reshape(o, shape=(1, group, nq, d)))
+
+    qa, ka = Array(shape=q_shape, dtype=dtype), Array(shape=k_shape, dtype=dtype)
+    args = (qa, ka, ka, *extras.values(), qa)
+    return convert(_named("masked_attention_kernel", body, len(args)), args=args, grid=(kv_heads, batch, 1))
+
+
+_quantize = quantize
+
+
+def _named(name: str, body, count: int):
+    """A kernel of `count` positional arguments, for builders whose arrays depend on their options."""
+    import inspect
+
+    def fn(*args):
+        body(args)
+
+    fn.__name__ = name
+    params = [inspect.Parameter(f"arg{i}", inspect.Parameter.POSITIONAL_OR_KEYWORD) for i in range(count)]
+    fn.__signature__ = inspect.Signature(params)
+    return kernel(fn)
 
 
 CONFIGS = {
