@@ -20,6 +20,7 @@ struct AttendArgs {
   int tiles, splits, nwg;
   float scale_log2;  // scale * log2 e, what the products are multiplied by without a cap
   float cap_in, cap_log2;  // 2 scale log2 e / cap and cap * log2 e; cap_log2 0: no cap
+  float cap_scale, cap_near, cap_poly[5];  // scale / cap; products of at most cap_near take cap_poly (attend.hip)
   int causal, window, dma;
   float* work;
 };
@@ -43,6 +44,7 @@ typedef unsigned u4a __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned u2a __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr int kFar = 1 << 30;  // positions are held within this
+constexpr float kSlack = 8.0f;
 
 // Four bytes a lane into LDS by DMA; as dma16.
 __device__ __forceinline__ void dma4(i32x4 rsrc, unsigned lds, unsigned voff) {
@@ -99,7 +101,8 @@ struct Rows {
   int pos, above, below; // sees key j when below < j <= above (or j < prefix)
   int p0, p1;            // positions of the wave's first and last row
   float slope;           // times log2 e
-  int doc;
+  int doc, one_doc;      // this lane's document; the first lane's, where alike: all rows have that
+  bool alike;
   uint4v q[KK];
   float16v acc[N];
   float m, l;
@@ -119,19 +122,25 @@ struct Rows {
     below = p.window ? max(pos - p.window, -1) : -1;
     slope = p.slopes ? p.slopes[p.tslopes.at(bx, by, bz) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
     doc = p.qdocs ? p.qdocs[p.tqdocs.at(bx, by, bz) + token * p.qdoc_step] : 0;
+    one_doc = __builtin_amdgcn_readfirstlane(doc);
+    alike = __builtin_amdgcn_ballot_w64(doc != one_doc) == 0;
     const unsigned char* at = p.q + (p.tq.at(bx, by, bz) + head * p.q_head + token * p.q_row + 8 * hi) * 2;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) q[kk] = (uint4v)(*reinterpret_cast<const u4a*>(at + kk * 32));
+    reset();
+    const int g = lane >> 4, li = lane & 15;
+    const int key = 4 * hi + (li >> 2), chunk = 2 * (g & 1) + ((li & 3) >> 1);
+    vkey = key * PITCH;
+    vchunk = ((chunk ^ vsw(key)) << 4) + 8 * (li & 1);
+  }
+
+  __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[n][r] = 0.0f;
     m = -__builtin_inff();
     l = 0.0f;
-    const int g = lane >> 4, li = lane & 15;
-    const int key = 4 * hi + (li >> 2), chunk = 2 * (g & 1) + ((li & 3) >> 1);
-    vkey = key * PITCH;
-    vchunk = ((chunk ^ vsw(key)) << 4) + 8 * (li & 1);
   }
 
   __device__ __forceinline__ uint4v key_fragment(const unsigned char* K, int kt, int kk) const {
@@ -152,20 +161,31 @@ struct Rows {
     return uint4v{lo[0], lo[1], up[0], up[1]};
   }
 
-  // Whether the wave's rows see all of keys [key0, key0 + n), or none of them.
+  // Whether the wave's rows see all of keys [key0, key0 + n), documents aside, or none.
   __device__ __forceinline__ bool sees_all(const AttendArgs& p, int key0, int n, int len, int pre) const {
-    return key0 + n <= len && !p.qdocs &&
-           (key0 + n <= pre ||
-            ((!p.causal || key0 + n - 1 <= p0) && (!p.window || key0 > p1 - p.window)));
+    return key0 + n <= len && (key0 + n <= pre || ((!p.causal || key0 + n - 1 <= p0) && (!p.window || key0 > p1 - p.window)));
   }
   __device__ __forceinline__ bool sees_none(const AttendArgs& p, int key0, int n, int pre) const {
     return key0 >= pre && ((p.causal && key0 > p1) || (p.window && key0 + n - 1 <= p0 - p.window));
   }
 
-  // T tiles of 32 keys from key0 on.  docs: their documents in LDS, or null, then
-  // p.kdocs at doc_at.
-  template <int T>
-  __device__ __forceinline__ void tile(const AttendArgs& p, const unsigned char* K, const unsigned char* V,
+  // Of a lane's 16 registers of a tile of 32 keys, as bits, those whose key is at most
+  // x past the lane's first: register r holds key 8 (r / 4) + r % 4.
+  static __device__ __forceinline__ unsigned up_to(int x) {
+    const int y = min(max(x, -1), 31);
+    return (1u << (4 * (y >> 3) + min((y & 7) + 1, 4))) - 1u;  // -1: 4 (-1) + 4
+  }
+
+  __device__ __forceinline__ int doc_of(const int* docs, const int* kdocs, int t, int i, int base, int len) const {
+    if (docs) return docs[t * 32 + 4 * hi + i];
+    return base + i < len ? kdocs[base + i] : 0;
+  }
+
+  // T tiles of 32 keys from key0 on.  docs: their documents in LDS, or null, then from
+  // kdocs.  ODD: values that are not finite may lie in a tile that is masked in part;
+  // without it, false where that is so (the rows' results are then of no use).
+  template <int T, bool ODD>
+  __device__ __forceinline__ bool tile(const AttendArgs& p, const unsigned char* K, const unsigned char* V,
                                        const int* docs, const int* kdocs, int key0, int len, int pre) {
     float16v s[T];
 #pragma unroll
@@ -179,14 +199,31 @@ struct Rows {
 
     float mul = p.scale_log2;
     if (p.cap_log2 > 0.0f) {
-      // cap tanh(z) = cap (1 - 2 / (e^2z + 1)); off by a few 2^-24 cap
       mul = 1.0f;
+      float big = 0.0f;
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[t][r] = fmaf(-2.0f * p.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[t][r] * p.cap_in) + 1.0f),
-                         p.cap_log2);
+        for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(s[t][r]));
+      if (__builtin_amdgcn_ballot_w64(big > p.cap_near) == 0) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float z = s[t][r] * p.cap_scale, w = z * z;
+            float y = fmaf(w, p.cap_poly[4], p.cap_poly[3]);
+            y = fmaf(w, y, p.cap_poly[2]);
+            y = fmaf(w, y, p.cap_poly[1]);
+            s[t][r] = z * fmaf(w, y, p.cap_poly[0]);
+          }
+      } else {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[t][r] = fmaf(-2.0f * p.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[t][r] * p.cap_in) + 1.0f),
+                           p.cap_log2);
+      }
     }
     if (p.slopes) {
 #pragma unroll
@@ -199,45 +236,36 @@ struct Rows {
       mul = 1.0f;
     }
     unsigned seen[T];  // of a tile that is masked in part: bit r for register r
-    bool part = false;
-    if (!sees_all(p, key0, 32 * T, len, pre)) {
-      unsigned all = 0xffffu;
+    bool part = !sees_all(p, key0, 32 * T, len, pre);
+    bool by_doc = false;
+    if (kdocs) {
+      const int i = key0 + (lane & (32 * T - 1));
+      const int d = docs ? docs[lane & (32 * T - 1)] : i < len ? kdocs[i] : one_doc;
+      by_doc = !alike || __builtin_amdgcn_ballot_w64(i < len && d != one_doc) != 0;
+      part |= by_doc;
+    }
+    if (part) {
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         const int base = key0 + t * 32 + 4 * hi;
-        const int a = above - base, b = below - base, f = pre - base, n = len - base;
-        unsigned bits = 0;
+        unsigned bits = ((up_to(above - base) & ~up_to(below - base)) | up_to(pre - 1 - base)) & up_to(len - 1 - base);
+        if (by_doc) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int c = 8 * (r >> 2) + (r & 3);
-          if (((c <= a && c > b) || c < f) && c < n) bits |= 1u << r;
-        }
-        if (p.qdocs) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            int d[4];
-            if (docs) {
-              const int4* at = reinterpret_cast<const int4*>(docs + t * 32 + 4 * hi + 8 * w);
-              d[0] = at->x, d[1] = at->y, d[2] = at->z, d[3] = at->w;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) d[e] = base + 8 * w + e < len ? kdocs[base + 8 * w + e] : 0;
-            }
+          for (int w = 0; w < 4; ++w)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (d[e] != doc) bits &= ~(1u << (4 * w + e));
-          }
+              bits &= ~((doc_of(docs, kdocs, t, 8 * w + e, base, len) != doc ? 1u : 0u) << (4 * w + e));
         }
         seen[t] = bits;
-        all &= bits;
       }
-      part = __builtin_amdgcn_ballot_w64(all != 0xffffu) != 0;
-      if (part) {
 #pragma unroll
-        for (int t = 0; t < T; ++t)
+      for (int t = 0; t < T; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] = (seen[t] >> r) & 1 ? s[t][r] : -__builtin_inff();
-      }
+        for (int r = 0; r < 16; ++r) {  // -inf where the bit is clear
+          const unsigned keep = (unsigned)((int)(seen[t] << (31 - r)) >> 31);
+          const float x = s[t][r];  // a bit cast of the element itself would read element 0
+          s[t][r] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, x) & keep) | (~keep & 0xff800000u));
+        }
     }
 
     // the running maximum, in units of log2
@@ -246,17 +274,20 @@ struct Rows {
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-    const float now = fmaxf(m, both_halves(top, true) * mul);
-    const float use = now == -__builtin_inff() ? 0.0f : now;
-    if (__builtin_amdgcn_ballot_w64(now > m) != 0) {
-      const float alpha = __builtin_amdgcn_exp2f(m - use);
+    top = both_halves(top, true) * mul;
+    // weights may reach 2^kSlack: the sums are rescaled only where a row's maximum
+    // has grown by more (most tiles of a long row raise some row's by a little)
+    if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) {
+      const float now = fmaxf(m, top);
+      const float alpha = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
+      m = now;
       l *= alpha;
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
     }
-    m = now;
+    const float use = m == -__builtin_inff() ? 0.0f : m;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < T; ++t)
@@ -274,9 +305,15 @@ struct Rows {
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[t][u][e] = pack2<BF16>(s[t][8 * u + 2 * e], s[t][8 * u + 2 * e + 1]);
-    if (part && !finite_values<T>(V)) {
-      masked_values<T>(V, w, seen);
-      return;
+    bool fine = true;
+    if (part) {
+      fine = finite_values<T>(V);
+      if constexpr (ODD)
+        if (!fine) {
+          masked_values<T>(V, w, seen);
+          return true;
+        }
+      asm volatile("" ::: "memory");  // or the fragments just looked through would be kept for the products
     }
 #pragma unroll
     for (int t = 0; t < T; ++t)
@@ -284,12 +321,15 @@ struct Rows {
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int n = 0; n < N; ++n) acc[n] = mma<BF16>(value_fragment(V, t, u, n), w[t][u], acc[n]);
+    return fine;
   }
 
   static constexpr unsigned kExp = BF16 ? 0x7f80u : 0x7c00u;
 
-  // A weight of 0 times a hidden infinity or NaN would be NaN: a tile that is
-  // masked in part is looked through for them.
+  // A weight of 0 times a hidden infinity or NaN would be NaN: a tile that is masked
+  // in part is looked through for them.  Where there are any, the workgroup (or wave)
+  // goes through its keys again with ODD: a loop of its own, so that the rare path
+  // does not cost the ordinary one registers.
   template <int T>
   __device__ __forceinline__ bool finite_values(const unsigned char* V) const {
     typedef unsigned short us2 __attribute__((ext_vector_type(2)));
@@ -326,17 +366,15 @@ struct Rows {
           const uint4v v = value_fragment(V, t, u, n);
           uint4v fine, plus, minus, sees;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            fine[e] = plus[e] = minus[e] = sees[e] = 0;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const unsigned b = (v[e] >> (16 * x)) & 0xffffu;
-              const bool odd = (b & kExp) == kExp, nan = odd && (b & ~(kExp | 0x8000u)) != 0;
-              fine[e] |= (odd ? 0u : b) << (16 * x);
-              plus[e] |= (odd && (nan || !(b & 0x8000u)) ? one : 0u) << (16 * x);
-              minus[e] |= (odd && (nan || (b & 0x8000u)) ? one : 0u) << (16 * x);
-              sees[e] |= ((seen[t] >> (8 * u + 2 * e + x)) & 1 ? one : 0u) << (16 * x);
-            }
+          for (int e = 0; e < 4; ++e) {  // halves of all ones where they hold, in packed 16-bit arithmetic
+            const unsigned finite = nonzero_halves((kExp | kExp << 16) - (v[e] & (kExp | kExp << 16)));
+            const unsigned nan = nonzero_halves(v[e] & ~(kExp | kExp << 16 | 0x80008000u));
+            const unsigned below = nonzero_halves(v[e] & 0x80008000u);
+            fine[e] = v[e] & finite;
+            plus[e] = (nan | ~below) & ~finite & (one | one << 16);
+            minus[e] = (nan | below) & ~finite & (one | one << 16);
+            const unsigned b = seen[t] >> (8 * u + 2 * e);
+            sees[e] = ((b & 1u) | (b & 2u) << 15) * one;
           }
           acc[n] = mma<BF16>(fine, w[t][u], acc[n]);
           up = mma<BF16>(plus, sees, up);
@@ -348,6 +386,12 @@ struct Rows {
         if (down[r] > 0.0f) acc[n][r] -= __builtin_inff();
       }
     }
+  }
+
+  static __device__ __forceinline__ unsigned nonzero_halves(unsigned x) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    const us2 one = {1, 1};
+    return __builtin_bit_cast(unsigned, (us2)(us2{0, 0} - __builtin_elementwise_min(__builtin_bit_cast(us2, x), one)));
   }
 };
 
@@ -409,7 +453,25 @@ __device__ __forceinline__ void document_keys(const AttendArgs& p, const int* qd
   }
   span<W>(lo, hi, mem);
   int first = keys, last = -1;
-  for (int j = threadIdx.x; j < keys; j += 64 * W) {
+  typedef int i4a __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int STEP = 256 * W;  // keys a round
+  const int mine = 4 * (int)threadIdx.x;
+  int j = 0;
+  for (; j + 4 * STEP <= keys; j += 4 * STEP) {
+    i4a d[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) d[u] = *reinterpret_cast<const i4a*>(kdocs + j + u * STEP + mine);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d[u][e] >= lo && d[u][e] <= hi) {
+          const int at = j + u * STEP + mine + e;
+          first = min(first, at);
+          last = max(last, at);
+        }
+  }
+  for (j += threadIdx.x; j < keys; j += 64 * W) {
     const int d = kdocs[j];
     if (d >= lo && d <= hi) {
       first = min(first, j);
@@ -541,6 +603,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(Atte
     if (kdocs) dma4(raw_rsrc(kdocs + key0, (unsigned)min(left, BN) * 4), lds_addr(at + 2 * KB), (threadIdx.x & 63) * 4);
   };
   constexpr int PER = 2 * (D / 32);
+  bool fine = true;
   if (i0 < i1) issue(i0, lds);
   for (int i = i0; i < i1; ++i) {
     unsigned char* const at = lds + ((i - i0) & 1) * STAGE;
@@ -552,8 +615,23 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(Atte
     lds_barrier();
     const int key0 = tiles.at(i) * BN;
     if (!rows.sees_none(p, key0, BN, b.pre))
-      rows.template tile<2>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len, b.pre);
+      fine &= rows.template tile<2, false>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len,
+                                           b.pre);
     lds_barrier();
+  }
+  if (__syncthreads_or(!fine)) {
+    rows.reset();
+    for (int i = i0; i < i1; ++i) {
+      issue(i, lds);
+      XTK_WAIT_VM(0);
+      lds_barrier();
+      const int key0 = tiles.at(i) * BN;
+#pragma unroll 1
+      for (int t = 0; t < BN / 32; ++t)
+        rows.template tile<1, true>(p, lds + t * (KB / 2), lds + KB + t * (KB / 2),
+                                    reinterpret_cast<const int*>(lds + 2 * KB) + 32 * t, kdocs, key0 + 32 * t, b.len, b.pre);
+      lds_barrier();
+    }
   }
 
   const float l = both_halves(rows.l, false);
@@ -632,6 +710,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
 #pragma unroll
   for (int j = 0; j < NS; ++j)
     if (j < mine) issue(j, j);
+  bool fine = true;
   int slot = 0;
   for (int j = 0; j < mine; ++j) {
     const int ahead = p.dma ? min(mine - 1 - j, NS - 1) : 0;
@@ -643,12 +722,23 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
     }
     asm volatile("" ::: "memory");
     unsigned char* const at = ring + slot * F::TILE;
-    rows.template tile<1>(p, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
+    fine &= rows.template tile<1, false>(p, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
     // every fragment is in registers before the slot is filled again
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     if (j + NS < mine) issue(j + NS, slot);
     slot = slot + 1 == NS ? 0 : slot + 1;
+  }
+  if (!fine) {
+    rows.reset();
+    for (int j = 0; j < mine; ++j) {
+      issue(j, 0);
+      XTK_WAIT_VM(0);
+      asm volatile("" ::: "memory");
+      rows.template tile<1, true>(p, ring, ring + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 
   // the waves' results meet in the rings
@@ -706,46 +796,58 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   }
 }
 
-// The splits of a row joined: a workgroup of four waves a row, each a quarter of the
-// splits, in a fixed order.
+// The splits of a row joined, in a fixed order.  A row takes G groups of D / 4 threads
+// (a column quad each), every G-th split a group; up to 256 splits.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs p, long long all_rows) {
-  __shared__ float part[4][D];
-  __shared__ float totals[4];
+  constexpr int Q = D / 4, G = 256 / Q;
+  __shared__ float f[256];
+  __shared__ float red[8];
+  __shared__ __attribute__((aligned(16))) float part[G][D];
   const long long row = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   BlockAt b;
   const int blk = (int)p.d_work((unsigned)row);
   const int r = (int)(row - (long long)blk * p.rows);
   p.blocks(blk, b.x, b.y, b.z);
-  float m = -__builtin_inff();
-  for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, *total_of(p, D, all_rows, row, s));
-  m = wave_reduce<true>(m);
-  if (m == -__builtin_inff()) m = 0.0f;
-  const int s0 = p.splits * wave / 4, s1 = p.splits * (wave + 1) / 4;
-  float l = 0.0f;
-  float4v o = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) {
-    const float* t = total_of(p, D, all_rows, row, s);
-    const float f = __builtin_amdgcn_exp2f(t[0] - m);
-    l += t[1] * f;
-    if (lane < D / 4) o += f * *reinterpret_cast<const float4v*>(sums_of(p, D, row, s) + 4 * lane);
-  }
-  if (lane < D / 4) *reinterpret_cast<float4v*>(&part[wave][4 * lane]) = o;
-  if (lane == 0) totals[wave] = l;
+  const float2 t = tid < p.splits ? *reinterpret_cast<const float2*>(total_of(p, D, all_rows, row, tid))
+                                  : float2{-__builtin_inff(), 0.0f};
+  const int g = tid / Q, d = 4 * (tid % Q);
+  // the first sums are on their way before the maximum is known
+  float4v v[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    v[u] = g < G && g + u * G < p.splits ? *reinterpret_cast<const float4v*>(sums_of(p, D, row, g + u * G) + d)
+                                         : float4v{0, 0, 0, 0};
+  float m = wave_reduce<true>(t.x);
+  if (lane == 0) red[wave] = m;
   __syncthreads();
-  if (threadIdx.x >= D / 4) return;
-  l = 0.0f;
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (m == -__builtin_inff()) m = 0.0f;
+  const float own = __builtin_amdgcn_exp2f(t.x - m);
+  f[tid] = own;
+  const float l = wave_reduce<false>(t.y * own);
+  if (lane == 0) red[4 + wave] = l;
+  __syncthreads();
+  float4v o = {0, 0, 0, 0};
+  if (g < G) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (g + u * G < p.splits) o += f[g + u * G] * v[u];
+#pragma unroll 8
+    for (int s = g + 4 * G; s < p.splits; s += G)
+      o += f[s] * *reinterpret_cast<const float4v*>(sums_of(p, D, row, s) + d);
+    *reinterpret_cast<float4v*>(&part[g][d]) = o;
+  }
+  __syncthreads();
+  if (tid >= Q) return;
   o = float4v{0, 0, 0, 0};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    l += totals[w];
-    o += *reinterpret_cast<const float4v*>(&part[w][4 * lane]);
-  }
-  if (l == 0.0f) o = float4v{0, 0, 0, 0};
-  else o *= 1.0f / l;
-  store4<BF16>(p, b, r, 4 * lane, o[0], o[1], o[2], o[3]);
+  for (int w = 0; w < G; ++w) o += *reinterpret_cast<const float4v*>(&part[w][d]);
+  const float total = (red[4] + red[5]) + (red[6] + red[7]);
+  if (total == 0.0f) o = float4v{0, 0, 0, 0};
+  else o *= 1.0f / total;
+  store4<BF16>(p, b, r, d, o[0], o[1], o[2], o[3]);
 }
 
 template <int D, bool BF16>
