@@ -16,16 +16,18 @@
 // read the keys once.  128 rows a workgroup, the keys shared through LDS by its four
 // waves; up to 32 rows (single tokens), every wave takes tiles of keys of its own.
 // The cap: cap tanh(z), z = score / cap, as cap (1 - 2 / (e^2z + 1)), off by a few
-// 2^-24 cap, or, for a tile of scores with |z| <= 3/4 throughout (caps are set far
+// 2^-24 cap, or, for a tile of scores with |z| <= 1/2 throughout (caps are set far
 // above ordinary scores), as z times a polynomial in z^2 fitted to tanh(z) / z there
-// (relative error 5.7e-7 by fit, 6.7e-7 in 32 bits): 7 operations a score in place of
-// two transcendental ones that take four times as long each.
+// (relative error 5.4e-7 by fit, 6.2e-7 in 32 bits): five operations a score in place
+// of five of which two take twice the time.
 //
 // Tiles that no row sees are not read: the visible ones are two runs, the prefix
 // and the band between window and diagonal, cut to the keys whose documents may be
 // the rows'.  Few rows over many keys are split over workgroups that leave their
 // m, l and sums in the workspace, and a second kernel joins them.
 #include "attend_kernels.h"
+
+#include <cmath>
 
 #include "launch.h"
 
@@ -57,8 +59,13 @@ hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipSt
   for (const xt::AttendAccess* a : {&t.q, &t.k, &t.v, &t.extra[0], &t.extra[1], &t.extra[2], &t.extra[3], &t.extra[4],
                                     &t.extra[5]})
     if (!apart(a->arg)) return hipErrorInvalidValue;
-  auto off = [](const xt::AttendAccess& a) { return TileOff{a.addr.c0, a.addr.sx, a.addr.sy, a.addr.sz}; };
-  auto bytes = [&](const xt::AttendAccess& a) { return static_cast<unsigned char*>(bufs[a.arg]); };
+  auto off = [](const xt::AttendAccess& a) {  // tile steps are not negative
+    return Walk{static_cast<unsigned long long>(a.addr.sx), static_cast<unsigned long long>(a.addr.sy),
+                static_cast<unsigned long long>(a.addr.sz)};
+  };
+  auto bytes = [&](const xt::AttendAccess& a) {
+    return static_cast<unsigned char*>(bufs[a.arg]) + a.addr.c0 * xt::elem_bytes(a.elem);
+  };
   AttendArgs a{};
   a.q = bytes(t.q);
   a.k = bytes(t.k);
@@ -75,13 +82,13 @@ hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipSt
   a.ldk = t.k.row;
   a.ldv = t.v.row;
   if (t.extra[0].arg >= 0) {
-    a.slopes = static_cast<const float*>(bufs[t.extra[0].arg]);
+    a.slopes = reinterpret_cast<const float*>(bytes(t.extra[0]));
     a.tslopes = off(t.extra[0]);
     a.slope_step = t.extra[0].row;
   }
-  auto ints = [&](int e, const int*& at, TileOff& o) {
+  auto ints = [&](int e, const int*& at, Walk& o) {
     if (t.extra[e].arg < 0) return;
-    at = static_cast<const int*>(bufs[t.extra[e].arg]);
+    at = reinterpret_cast<const int*>(bytes(t.extra[e]));
     o = off(t.extra[e]);
   };
   ints(1, a.start, a.tstart);
@@ -112,10 +119,11 @@ hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipSt
   if (t.cap > 0) {
     a.cap_in = 2.0f * t.scale * 1.44269504088896340736f / t.cap;
     a.cap_log2 = t.cap * 1.44269504088896340736f;
-    a.cap_scale = t.scale / t.cap;
-    a.cap_near = 0.75f / a.cap_scale;
-    static const double poly[5] = {0.999999435, -0.333282516, 0.132589833, -0.0500563039, 0.0129296327};
-    for (int i = 0; i < 5; ++i) a.cap_poly[i] = static_cast<float>(poly[i] * t.cap * 1.44269504088896340736);
+    const double z = double(t.scale) / t.cap;  // of a product; its powers are normal numbers in this range
+    a.cap_near = z > 1e-4 && z < 1e4 ? static_cast<float>(0.5 / z) : -1.0f;
+    static const double poly[4] = {0.999999456, -0.33326318, 0.131902967, -0.0444022264};
+    for (int i = 0; i < 4; ++i)
+      a.cap_poly[i] = static_cast<float>(poly[i] * t.cap * 1.4426950408889634 * std::pow(z, 2 * i + 1));
   }
   a.causal = t.causal;
   a.window = static_cast<int>(std::min<int64_t>(t.window, 1 << 30));

@@ -5,6 +5,15 @@
 
 namespace xtk {
 
+// Element offset of a Block's tile from the argument's first one: the pointers start
+// at that, and every step is at least 0.
+struct Walk {
+  unsigned long long sx, sy, sz;
+  __device__ __forceinline__ unsigned long long at(unsigned x, unsigned y, unsigned z) const {
+    return x * sx + y * sy + z * sz;
+  }
+};
+
 struct AttendArgs {
   const unsigned char* q;
   const unsigned char* k;
@@ -12,7 +21,7 @@ struct AttendArgs {
   unsigned char* o;
   const float* slopes;
   const int *start, *length, *prefix, *qdocs, *kdocs;
-  TileOff tq, tk, tv, to, tslopes, tstart, tlength, tprefix, tqdocs, tkdocs;  // element offsets
+  Walk tq, tk, tv, to, tslopes, tstart, tlength, tprefix, tqdocs, tkdocs;
   long long q_head, q_row, o_head, o_row, ldk, ldv, slope_step, qdoc_step;   // strides in elements
   BlockDecode blocks;
   Div31 d_heads, d_work, d_splits;  // d_work: row tiles x splits of a Block
@@ -20,7 +29,7 @@ struct AttendArgs {
   int tiles, splits, nwg;
   float scale_log2;  // scale * log2 e, what the products are multiplied by without a cap
   float cap_in, cap_log2;  // 2 scale log2 e / cap and cap * log2 e; cap_log2 0: no cap
-  float cap_scale, cap_near, cap_poly[5];  // scale / cap; products of at most cap_near take cap_poly (attend.hip)
+  float cap_near, cap_poly[4];  // products of at most cap_near take cap_poly (attend.hip); cap_near < 0: none do
   int causal, window, dma;
   float* work;
 };
@@ -46,6 +55,10 @@ typedef unsigned u2a __attribute__((ext_vector_type(2), aligned(2)));
 constexpr int kFar = 1 << 30;  // positions are held within this
 constexpr float kSlack = 8.0f;
 
+// The LDS address of a pointer into LDS: the low half of its generic address (a cast
+// between address spaces compares with null first).
+__device__ __forceinline__ unsigned lds_at(const void* p) { return (unsigned)reinterpret_cast<uintptr_t>(p); }
+
 // Four bytes a lane into LDS by DMA; as dma16.
 __device__ __forceinline__ void dma4(i32x4 rsrc, unsigned lds, unsigned voff) {
   asm volatile("buffer_load_dword %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
@@ -64,6 +77,18 @@ __device__ __forceinline__ float16v mma(uint4v a, uint4v b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// l + the sum of a packed pair.
+template <bool BF16>
+__device__ __forceinline__ float add_pair(unsigned w, float l) {
+  if constexpr (BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), __builtin_bit_cast(b2, 0x3f803f80u), l, false);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), __builtin_bit_cast(h2, 0x3c003c00u), l, false);
+  }
 }
 
 template <bool BF16>
@@ -85,6 +110,7 @@ template <int D, bool BF16>
 struct Rows {
   static constexpr int N = D / 32, KK = D / 16;
   static constexpr int PITCH = 2 * D;  // bytes of a key row in LDS
+  static constexpr int VAHEAD = D < 128 ? 2 : 1;  // steps of 16 keys whose values are read ahead
 
   // Where a key row's 16-byte chunks lie in LDS: chunk c at c ^ ksw (keys), c ^ vsw
   // (values), so that the 16 rows of a fragment read, and the four rows of a
@@ -106,7 +132,7 @@ struct Rows {
   uint4v q[KK];
   float16v acc[N];
   float m, l;
-  int vkey, vchunk;      // LDS offset of this lane's part of a value fragment
+  int koff[KK], voff[N]; // LDS offsets of this lane's part of a key and of a value fragment
 
   __device__ __forceinline__ void begin(const AttendArgs& p, int first, int bx, int by, int bz, int start) {
     lane = threadIdx.x & 63;
@@ -130,8 +156,10 @@ struct Rows {
     reset();
     const int g = lane >> 4, li = lane & 15;
     const int key = 4 * hi + (li >> 2), chunk = 2 * (g & 1) + ((li & 3) >> 1);
-    vkey = key * PITCH;
-    vchunk = ((chunk ^ vsw(key)) << 4) + 8 * (li & 1);
+#pragma unroll
+    for (int n = 0; n < N; ++n) voff[n] = key * PITCH + ((((chunk ^ vsw(key)) << 4) + 8 * (li & 1)) ^ (n << 6));
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) koff[kk] = col * PITCH + (((2 * kk + hi) ^ ksw(col)) << 4);
   }
 
   __device__ __forceinline__ void reset() {
@@ -143,16 +171,20 @@ struct Rows {
     l = 0.0f;
   }
 
+  // Behind a loop: the sums as they are, or the loop would copy them to the registers
+  // that what follows wants them in, once a tile.
+  __device__ __forceinline__ void hold() {
+#pragma unroll
+    for (int n = 0; n < N; ++n) asm volatile("" : "+v"(acc[n]));
+  }
+
   __device__ __forceinline__ uint4v key_fragment(const unsigned char* K, int kt, int kk) const {
-    const int r = kt * 32 + col;
-    return *reinterpret_cast<const uint4v*>(K + r * PITCH + (((2 * kk + hi) ^ ksw(col)) << 4));
+    return *reinterpret_cast<const uint4v*>(K + koff[kk] + kt * 32 * PITCH);
   }
 
   // Values of keys 32 kt + 16 u + {4 h + 0..3, 8 + 4 h + 0..3}, column 32 n + c.
   __device__ __forceinline__ uint4v value_fragment(const unsigned char* V, int kt, int u, int n) const {
-    // vsw moves whole groups of four chunks, the bits that n sets
-    const int at = vkey + (vchunk ^ (n << 6)) + (kt * 32 + u * 16) * PITCH;
-    lds_t* const f = (lds_t*)(V + at);
+    lds_t* const f = (lds_t*)lds_at(V + voff[n] + (kt * 32 + u * 16) * PITCH);
     const uint2v lo = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                      reinterpret_cast<short4v __attribute__((address_space(3)))*>(f)));
     const uint2v up = __builtin_bit_cast(
@@ -182,9 +214,9 @@ struct Rows {
   }
 
   // T tiles of 32 keys from key0 on.  docs: their documents in LDS, or null, then from
-  // kdocs.  ODD: values that are not finite may lie in a tile that is masked in part;
-  // without it, false where that is so (the rows' results are then of no use).
-  template <int T, bool ODD>
+  // kdocs.  False where values that are not finite lie in a tile that is masked in part
+  // (the rows' results are then of no use).
+  template <int T>
   __device__ __forceinline__ bool tile(const AttendArgs& p, const unsigned char* K, const unsigned char* V,
                                        const int* docs, const int* kdocs, int key0, int len, int pre) {
     float16v s[T];
@@ -192,29 +224,58 @@ struct Rows {
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
+    // fragments AHEAD steps before their products: one LDS read takes longer than a
+    // step's products, and the scheduler would read each just before its use
+    constexpr int AHEAD = KK < 4 ? KK : 4;
+    uint4v kf[AHEAD][T];
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
+    for (int kk = 0; kk < AHEAD; ++kk)
 #pragma unroll
-      for (int t = 0; t < T; ++t) s[t] = mma<BF16>(key_fragment(K, t, kk), q[kk], s[t]);
+      for (int t = 0; t < T; ++t) kf[kk][t] = key_fragment(K, t, kk);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) s[t] = mma<BF16>(kf[kk % AHEAD][t], q[kk], s[t]);
+      if (kk + AHEAD < KK) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) kf[kk % AHEAD][t] = key_fragment(K, t, kk + AHEAD);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // the values of the first products, read behind the scores' arithmetic
+    uint4v vf[VAHEAD][N];
+#pragma unroll
+    for (int x = 0; x < VAHEAD; ++x)
+#pragma unroll
+      for (int n = 0; n < N; ++n) vf[x][n] = value_fragment(V, 0, x, n);
+    __builtin_amdgcn_sched_barrier(0);
+
+    bool part = !sees_all(p, key0, 32 * T, len, pre);
+    bool by_doc = false;
+    if (kdocs) {
+      const int i = key0 + (lane & (32 * T - 1));
+      const int d = docs ? docs[lane & (32 * T - 1)] : i < len ? kdocs[i] : one_doc;
+      by_doc = !alike || __builtin_amdgcn_ballot_w64(i < len && d != one_doc) != 0;
+      part |= by_doc;
+    }
 
     float mul = p.scale_log2;
     if (p.cap_log2 > 0.0f) {
-      mul = 1.0f;
-      float big = 0.0f;
+      float big[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(s[t][r]));
-      if (__builtin_amdgcn_ballot_w64(big > p.cap_near) == 0) {
+        for (int r = 0; r < 16; ++r) big[r & 3] = fmaxf(big[r & 3], fabsf(s[t][r]));
+      const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+      mul = 1.0f;
+      if (__builtin_amdgcn_ballot_w64(most > p.cap_near) == 0) {
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float z = s[t][r] * p.cap_scale, w = z * z;
-            float y = fmaf(w, p.cap_poly[4], p.cap_poly[3]);
-            y = fmaf(w, y, p.cap_poly[2]);
-            y = fmaf(w, y, p.cap_poly[1]);
-            s[t][r] = z * fmaf(w, y, p.cap_poly[0]);
+            const float w = s[t][r] * s[t][r];
+            s[t][r] *= fmaf(w, fmaf(w, fmaf(w, p.cap_poly[3], p.cap_poly[2]), p.cap_poly[1]), p.cap_poly[0]);
           }
       } else {
 #pragma unroll
@@ -235,16 +296,8 @@ struct Rows {
       }
       mul = 1.0f;
     }
-    unsigned seen[T];  // of a tile that is masked in part: bit r for register r
-    bool part = !sees_all(p, key0, 32 * T, len, pre);
-    bool by_doc = false;
-    if (kdocs) {
-      const int i = key0 + (lane & (32 * T - 1));
-      const int d = docs ? docs[lane & (32 * T - 1)] : i < len ? kdocs[i] : one_doc;
-      by_doc = !alike || __builtin_amdgcn_ballot_w64(i < len && d != one_doc) != 0;
-      part |= by_doc;
-    }
     if (part) {
+      unsigned seen[T];  // bit r for register r
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         const int base = key0 + t * 32 + 4 * hi;
@@ -268,13 +321,13 @@ struct Rows {
         }
     }
 
-    // the running maximum, in units of log2
-    float top = s[0][0];
+    // the running maximum, in units of log2; four chains, since each step waits for the last
+    float most[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-    top = both_halves(top, true) * mul;
+      for (int r = 0; r < 16; ++r) most[r & 3] = fmaxf(most[r & 3], s[t][r]);
+    const float top = both_halves(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), true) * mul;
     // weights may reach 2^kSlack: the sums are rescaled only where a row's maximum
     // has grown by more (most tiles of a long row raise some row's by a little)
     if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) {
@@ -287,49 +340,68 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
     }
-    const float use = m == -__builtin_inff() ? 0.0f : m;
-    float sum = 0.0f;
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], mul, -use));
-        sum += s[t][r];
-      }
-    l += sum;
-
-    uint4v w[T][2];  // the weights rounded to the values' type: off by half a step each, as the result is
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[t][u][e] = pack2<BF16>(s[t][8 * u + 2 * e], s[t][8 * u + 2 * e + 1]);
     bool fine = true;
     if (part) {
       fine = finite_values<T>(V);
-      if constexpr (ODD)
-        if (!fine) {
-          masked_values<T>(V, w, seen);
-          return true;
-        }
       asm volatile("" ::: "memory");  // or the fragments just looked through would be kept for the products
     }
+    add_values<T>(V, s, vf, mul);
+    return fine;
+  }
+
+  // Weights e^(score - m), rounded to the values' type (off by half a step each, as
+  // the result is), and their products with the values; l takes the rounded weights,
+  // so that a row's weights sum to one.  vf: the values of the first VAHEAD steps.
+  template <int T>
+  __device__ __forceinline__ void add_values(const unsigned char* V, float16v (&s)[T], uint4v (&vf)[VAHEAD][N], float mul) {
+    const float use = m == -__builtin_inff() ? 0.0f : m;
+    uint4v w[T][2];
+    auto weigh = [&](int t) {
 #pragma unroll
-    for (int t = 0; t < T; ++t)
+      for (int r = 0; r < 16; ++r) s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], mul, -use));
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int n = 0; n < N; ++n) acc[n] = mma<BF16>(value_fragment(V, t, u, n), w[t][u], acc[n]);
-    return fine;
+        for (int e = 0; e < 4; ++e) {
+          w[t][u][e] = pack2<BF16>(s[t][8 * u + 2 * e], s[t][8 * u + 2 * e + 1]);
+          l = add_pair<BF16>(w[t][u][e], l);
+        }
+    };
+    weigh(0);
+    // ahead of the other wave of the SIMD: its arithmetic fills the matrix unit's time
+    // (causal, 4096 tokens, 32 heads of 128, capped: 210 -> 188 us)
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      // the next tile's weights between this one's products
+      if (t + 1 < T) weigh(t + 1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int x = 2 * t + u;
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n] = mma<BF16>(vf[x % VAHEAD][n], w[t][u], acc[n]);
+        if (x + VAHEAD < 2 * T) {
+#pragma unroll
+          for (int n = 0; n < N; ++n) vf[x % VAHEAD][n] = value_fragment(V, (x + VAHEAD) / 2, (x + VAHEAD) % 2, n);
+        }
+      }
+      if (t + 1 < T) {
+#pragma unroll
+        for (int x = 0; x < 2 * N; ++x) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                // a product,
+          __builtin_amdgcn_sched_group_barrier(0x402, 48 / (2 * N) + 1, 0);  // its share of the arithmetic
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                // and of the reads
+        }
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
   }
 
   static constexpr unsigned kExp = BF16 ? 0x7f80u : 0x7c00u;
 
   // A weight of 0 times a hidden infinity or NaN would be NaN: a tile that is masked
-  // in part is looked through for them.  Where there are any, the workgroup (or wave)
-  // goes through its keys again with ODD: a loop of its own, so that the rare path
-  // does not cost the ordinary one registers.
+  // in part is looked through for them, and a workgroup that meets any goes through
+  // its rows again one by one (odd_rows).
   template <int T>
   __device__ __forceinline__ bool finite_values(const unsigned char* V) const {
     typedef unsigned short us2 __attribute__((ext_vector_type(2)));
@@ -346,52 +418,6 @@ struct Rows {
             most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, v[e] & (kExp | kExp << 16)));
         }
     return __builtin_amdgcn_ballot_w64(most[0] == kExp || most[1] == kExp) == 0;
-  }
-
-  // Such a tile: the finite values as ever, and what a row sees of +inf, -inf and
-  // NaN counted by products with ones.
-  template <int T>
-  __device__ __forceinline__ void masked_values(const unsigned char* V, const uint4v (&w)[T][2],
-                                                const unsigned (&seen)[T]) {
-    constexpr unsigned one = BF16 ? 0x3f80u : 0x3c00u;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      float16v up, down;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) up[r] = down[r] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint4v v = value_fragment(V, t, u, n);
-          uint4v fine, plus, minus, sees;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {  // halves of all ones where they hold, in packed 16-bit arithmetic
-            const unsigned finite = nonzero_halves((kExp | kExp << 16) - (v[e] & (kExp | kExp << 16)));
-            const unsigned nan = nonzero_halves(v[e] & ~(kExp | kExp << 16 | 0x80008000u));
-            const unsigned below = nonzero_halves(v[e] & 0x80008000u);
-            fine[e] = v[e] & finite;
-            plus[e] = (nan | ~below) & ~finite & (one | one << 16);
-            minus[e] = (nan | below) & ~finite & (one | one << 16);
-            const unsigned b = seen[t] >> (8 * u + 2 * e);
-            sees[e] = ((b & 1u) | (b & 2u) << 15) * one;
-          }
-          acc[n] = mma<BF16>(fine, w[t][u], acc[n]);
-          up = mma<BF16>(plus, sees, up);
-          down = mma<BF16>(minus, sees, down);
-        }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        if (up[r] > 0.0f) acc[n][r] += __builtin_inff();
-        if (down[r] > 0.0f) acc[n][r] -= __builtin_inff();
-      }
-    }
-  }
-
-  static __device__ __forceinline__ unsigned nonzero_halves(unsigned x) {
-    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-    const us2 one = {1, 1};
-    return __builtin_bit_cast(unsigned, (us2)(us2{0, 0} - __builtin_elementwise_min(__builtin_bit_cast(us2, x), one)));
   }
 };
 
@@ -536,7 +562,7 @@ struct Fill {
     const unsigned char* from = base + (long long)key0 * pitch;
     if (dma) {
       const i32x4 rs = raw_rsrc(from, (unsigned)(min(left, BN) - 1) * pitch + 2 * D);
-      const unsigned at = __builtin_amdgcn_readfirstlane(lds_addr(to) + first * 1024);
+      const unsigned at = __builtin_amdgcn_readfirstlane(lds_at(to) + first * 1024);
 #pragma unroll
       for (int i = 0; i < IN; ++i) dma16(rs, at + i * STEP * 1024, off[i], 0);
     } else {
@@ -572,12 +598,111 @@ __device__ __forceinline__ float* total_of(const AttendArgs& p, int D, long long
   return p.work + rows * p.splits * D + 2 * (row * p.splits + split);
 }
 
+// Rows first, first + step, ... below last over the keys of tiles [i0, i1) of bn, a
+// wave each and in vector arithmetic: the way for keys among which hidden values are
+// not finite, of which only what a row sees is ever multiplied.  Lane j of 64 keys has
+// the score of key j; then the lanes have the columns.
+template <int D, bool BF16>
+__device__ __forceinline__ void odd_rows(const AttendArgs& p, const BlockAt& b, const Tiles& tiles, int bn, int i0, int i1,
+                                         const int* kdocs, int first, int last, int step, long long all_rows) {
+  const int lane = threadIdx.x & 63;
+  auto value = [](unsigned short x) {
+    return BF16 ? __builtin_bit_cast(float, (unsigned)x << 16) : (float)__builtin_bit_cast(_Float16, x);
+  };
+  const unsigned short* const keys = reinterpret_cast<const unsigned short*>(p.k) + p.tk.at(b.x, b.y, b.z);
+  const unsigned short* const values = reinterpret_cast<const unsigned short*>(p.v) + p.tv.at(b.x, b.y, b.z);
+#pragma unroll 1
+  for (int row = first; row < last; row += step) {
+    const int token = (int)p.d_heads((unsigned)row), head = row - token * p.heads, pos = b.start + token;
+    const unsigned short* const q = reinterpret_cast<const unsigned short*>(p.q) + p.tq.at(b.x, b.y, b.z) +
+                                    head * p.q_head + token * p.q_row;
+    const float slope = p.slopes ? p.slopes[p.tslopes.at(b.x, b.y, b.z) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
+    const int doc = p.qdocs ? p.qdocs[p.tqdocs.at(b.x, b.y, b.z) + token * p.qdoc_step] : 0;
+    auto sees = [&](int j, int end) {
+      return j < end && j < b.len && (j < b.pre || ((!p.causal || j <= pos) && (!p.window || j > pos - p.window))) &&
+             (!kdocs || kdocs[j] == doc);
+    };
+    auto score = [&](int j) {
+      const unsigned short* const k = keys + (long long)j * p.ldk;
+      float s = 0.0f;
+#pragma unroll 1
+      for (int d = 0; d < D; ++d) s = fmaf(value(q[d]), value(k[d]), s);
+      s = p.cap_log2 > 0.0f ? fmaf(-2.0f * p.cap_log2,
+                                   __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.cap_in) + 1.0f), p.cap_log2)
+                            : s * p.scale_log2;
+      return p.slopes ? fmaf(-slope, fabsf((float)(pos - j)), s) : s;
+    };
+    float m = -__builtin_inff(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+      for (int i = i0; i < i1; ++i) {
+        const int key0 = tiles.at(i) * bn, j = key0 + lane;
+        const bool in = sees(j, key0 + bn);
+        const float s = in ? score(j) : -__builtin_inff();
+        if (pass == 0) {
+          m = fmaxf(m, s);
+          continue;
+        }
+        const float w = in ? __builtin_amdgcn_exp2f(s - m) : 0.0f;
+        l += w;
+        unsigned long long left = __builtin_amdgcn_ballot_w64(in);
+#pragma unroll 1
+        while (left) {
+          const int e = __builtin_ctzll(left);
+          left &= left - 1;
+          const float we = __shfl(w, e, 64);
+#pragma unroll
+          for (int c = 0; c < (D + 63) / 64; ++c)
+            if (c * 64 + lane < D) o[c] = fmaf(we, value(values[(long long)(key0 + e) * p.ldv + c * 64 + lane]), o[c]);
+        }
+      }
+      if (pass == 0) {
+        m = wave_reduce<true>(m);
+        if (m == -__builtin_inff()) m = 0.0f;
+      }
+    }
+    l = wave_reduce<false>(l);
+    const long long at = b.block * p.rows + row;
+    float* const t = p.splits > 1 ? total_of(p, D, all_rows, at, b.split) : nullptr;
+    if (t && lane == 0) {
+      t[0] = m;
+      t[1] = l;
+    }
+#pragma unroll
+    for (int c = 0; c < (D + 63) / 64; ++c) {
+      if (c * 64 + lane >= D) continue;
+      if (t) {
+        sums_of(p, D, at, b.split)[c * 64 + lane] = o[c];
+      } else {
+        const unsigned both = pack2<BF16>(l == 0.0f ? 0.0f : o[c] / l, 0.0f);
+        reinterpret_cast<unsigned short*>(p.o)[p.to.at(b.x, b.y, b.z) + head * p.o_head + token * p.o_row + c * 64 + lane] =
+            (unsigned short)both;
+      }
+    }
+  }
+}
+
+// Whether any wave of the workgroup says so; no LDS access is left out standing.
+template <int W>
+__device__ __forceinline__ bool any_wave(bool x, unsigned char* lds) {
+  int* const at = reinterpret_cast<int*>(lds);
+  if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) any |= at[w];
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(any) != 0;
+}
+
 // More than 32 rows: 128 of them, 32 a wave, the keys in tiles of 64 that the waves
 // share, two of them in LDS.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs p, long long all_rows) {
   constexpr int BN = 64, KB = BN * D * 2, STAGE = 2 * KB + 256;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
+  const bool dma = p.dma;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const BlockAt b = block_at(p);
   const int first = b.tile * 128, last = min(first + 127, p.rows - 1);
@@ -587,56 +712,49 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(Atte
   if (kdocs)
     document_keys<4>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, t0, t1, b.len, reinterpret_cast<int*>(lds), d0, d1);
   const Tiles tiles = tiles_of(p, BN, b.start + t0, b.start + t1, b.len, b.pre, d0, d1);
-  const int i0 = (int)((long long)tiles.n * b.split / p.splits), i1 = (int)((long long)tiles.n * (b.split + 1) / p.splits);
+  const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
+  const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
 
   Fill<D, BN, false, 4> fk;
   Fill<D, BN, true, 4> fv;
   fk.begin(p.k + p.tk.at(b.x, b.y, b.z) * 2, p.ldk, wave);
   fv.begin(p.v + p.tv.at(b.x, b.y, b.z) * 2, p.ldv, wave);
-  Rows<D, BF16> rows;
-  rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start);
-
   auto issue = [&](int i, unsigned char* at) {
     const int key0 = tiles.at(i) * BN, left = b.len - key0;
-    fk.issue(p.dma, key0, left, at);
-    fv.issue(p.dma, key0, left, at + KB);
-    if (kdocs) dma4(raw_rsrc(kdocs + key0, (unsigned)min(left, BN) * 4), lds_addr(at + 2 * KB), (threadIdx.x & 63) * 4);
+    fk.issue(dma, key0, left, at);
+    fv.issue(dma, key0, left, at + KB);
+    if (kdocs) dma4(raw_rsrc(kdocs + key0, (unsigned)min(left, BN) * 4), lds_at(at + 2 * KB), (threadIdx.x & 63) * 4);
   };
-  constexpr int PER = 2 * (D / 32);
-  bool fine = true;
   if (i0 < i1) issue(i0, lds);
+  Rows<D, BF16> rows;
+  rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start);
+  bool fine = true;
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) {
+    // one barrier a tile: behind it this tile has landed, and every wave is done with
+    // the one before, whose place the next one takes while this one is worked on
     unsigned char* const at = lds + ((i - i0) & 1) * STAGE;
-    const bool more = i + 1 < i1;
-    if (more) issue(i + 1, lds + ((i + 1 - i0) & 1) * STAGE);
-    if (!more || !p.dma) XTK_WAIT_VM(0);
-    else if (kdocs) XTK_WAIT_VM(PER + 1);
-    else XTK_WAIT_VM(PER);
+    XTK_WAIT_VM(0);
     lds_barrier();
+    if (i + 1 < i1) issue(i + 1, lds + ((i + 1 - i0) & 1) * STAGE);
     const int key0 = tiles.at(i) * BN;
     if (!rows.sees_none(p, key0, BN, b.pre))
-      fine &= rows.template tile<2, false>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len,
-                                           b.pre);
-    lds_barrier();
+      fine &= rows.template tile<2>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len, b.pre);
   }
-  if (__syncthreads_or(!fine)) {
-    rows.reset();
-    for (int i = i0; i < i1; ++i) {
-      issue(i, lds);
-      XTK_WAIT_VM(0);
-      lds_barrier();
-      const int key0 = tiles.at(i) * BN;
-#pragma unroll 1
-      for (int t = 0; t < BN / 32; ++t)
-        rows.template tile<1, true>(p, lds + t * (KB / 2), lds + KB + t * (KB / 2),
-                                    reinterpret_cast<const int*>(lds + 2 * KB) + 32 * t, kdocs, key0 + 32 * t, b.len, b.pre);
-      lds_barrier();
-    }
+  rows.hold();
+  lds_barrier();
+  if (any_wave<4>(!fine, lds)) {
+    odd_rows<D, BF16>(p, b, tiles, BN, i0, i1, kdocs, first + wave, last + 1, 4, all_rows);
+    return;
   }
 
   const float l = both_halves(rows.l, false);
-  if (first + 32 * wave + rows.col >= p.rows) return;
   if (p.splits == 1) {
+    // through LDS, so that a row leaves in 16-byte pieces side by side: a lane has
+    // four columns of eight here and there.  Each wave has its own part; rows 16 bytes
+    // apart from a multiple of the banks.
+    constexpr int PITCH = 2 * D + 16;
+    unsigned char* const own = lds + wave * 32 * PITCH;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
@@ -645,10 +763,22 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(Atte
         float o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = l == 0.0f ? 0.0f : rows.acc[n][4 * w + e] * inv;
-        store4<BF16>(p, b, rows.row, 32 * n + 8 * w + 4 * rows.hi, o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint2v*>(own + rows.col * PITCH + (32 * n + 8 * w + 4 * rows.hi) * 2) =
+            uint2v{pack2<BF16>(o[0], o[1]), pack2<BF16>(o[2], o[3])};
       }
+    unsigned char* const out = p.o + p.to.at(b.x, b.y, b.z) * 2;
+    constexpr int C = D / 8;  // pieces of a row
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) {
+      const int e = i * 64 + rows.lane, r = e / C, c = e % C, row = first + 32 * wave + r;
+      if (row >= p.rows) continue;
+      const int token = (int)p.d_heads((unsigned)row), head = row - token * p.heads;
+      *reinterpret_cast<u4a*>(out + (head * p.o_head + token * p.o_row + c * 8) * 2) =
+          (u4a)(*reinterpret_cast<const uint4v*>(own + r * PITCH + c * 16));
+    }
     return;
   }
+  if (first + 32 * wave + rows.col >= p.rows) return;
   const long long row = b.block * p.rows + rows.row;
   float* const sums = sums_of(p, D, row, b.split);
 #pragma unroll
@@ -682,6 +812,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   typedef Few<D> F;
   constexpr int W = F::W, NS = F::NS, KB = 32 * D * 2, PER = D / 8;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[F::LDS];
+  const bool dma = p.dma;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const BlockAt b = block_at(p);
   const int t1 = (int)p.d_heads((unsigned)(p.rows - 1));
@@ -690,7 +821,8 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   if (kdocs)
     document_keys<W>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, 0, t1, b.len, reinterpret_cast<int*>(lds), d0, d1);
   const Tiles tiles = tiles_of(p, 32, b.start, b.start + t1, b.len, b.pre, d0, d1);
-  const int i0 = (int)((long long)tiles.n * b.split / p.splits), i1 = (int)((long long)tiles.n * (b.split + 1) / p.splits);
+  const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
+  const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
   const int mine = max(0, (i1 - i0 - wave + W - 1) / W);
 
   Fill<D, 32, false, 1> fk;
@@ -702,18 +834,19 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   auto issue = [&](int j, int slot) {
     unsigned char* const at = ring + slot * F::TILE;
     const int key0 = key_of(j);
-    fk.issue(p.dma, key0, b.len - key0, at);
-    fv.issue(p.dma, key0, b.len - key0, at + KB);
+    fk.issue(dma, key0, b.len - key0, at);
+    fv.issue(dma, key0, b.len - key0, at + KB);
   };
-  Rows<D, BF16> rows;
-  rows.begin(p, 0, b.x, b.y, b.z, b.start);
 #pragma unroll
   for (int j = 0; j < NS; ++j)
     if (j < mine) issue(j, j);
+  Rows<D, BF16> rows;
+  rows.begin(p, 0, b.x, b.y, b.z, b.start);
   bool fine = true;
   int slot = 0;
+#pragma unroll 1
   for (int j = 0; j < mine; ++j) {
-    const int ahead = p.dma ? min(mine - 1 - j, NS - 1) : 0;
+    const int ahead = dma ? min(mine - 1 - j, NS - 1) : 0;
     switch (ahead) {
       case 0: XTK_WAIT_VM(0); break;
       case 1: XTK_WAIT_VM(PER); break;
@@ -722,23 +855,17 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
     }
     asm volatile("" ::: "memory");
     unsigned char* const at = ring + slot * F::TILE;
-    fine &= rows.template tile<1, false>(p, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
+    fine &= rows.template tile<1>(p, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
     // every fragment is in registers before the slot is filled again
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     if (j + NS < mine) issue(j + NS, slot);
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
-  if (!fine) {
-    rows.reset();
-    for (int j = 0; j < mine; ++j) {
-      issue(j, 0);
-      XTK_WAIT_VM(0);
-      asm volatile("" ::: "memory");
-      rows.template tile<1, true>(p, ring, ring + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  __syncthreads();  // every ring is done with
+  if (any_wave<W>(!fine, lds)) {
+    odd_rows<D, BF16>(p, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);
+    return;
   }
 
   // the waves' results meet in the rings
@@ -796,55 +923,72 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   }
 }
 
-// The splits of a row joined, in a fixed order.  A row takes G groups of D / 4 threads
-// (a column quad each), every G-th split a group; up to 256 splits.
-template <int D, bool BF16>
+// The splits of rows joined, in a fixed order: D / 4 threads (a column quad each) take
+// every G-th split of a row.  G = 1: 256 / (D / 4) rows a workgroup, for few splits;
+// else one row with as many groups as fit, and up to 256 splits.
+template <int D, bool BF16, bool FEW>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs p, long long all_rows) {
   constexpr int Q = D / 4, G = 256 / Q;
-  __shared__ float f[256];
-  __shared__ float red[8];
-  __shared__ __attribute__((aligned(16))) float part[G][D];
-  const long long row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, g = tid / Q, d = 4 * (tid % Q);
+  const long long row = FEW ? (long long)blockIdx.x * G + g : blockIdx.x;
+  if (FEW && (g >= G || row >= all_rows)) return;
   BlockAt b;
   const int blk = (int)p.d_work((unsigned)row);
   const int r = (int)(row - (long long)blk * p.rows);
   p.blocks(blk, b.x, b.y, b.z);
-  const float2 t = tid < p.splits ? *reinterpret_cast<const float2*>(total_of(p, D, all_rows, row, tid))
-                                  : float2{-__builtin_inff(), 0.0f};
-  const int g = tid / Q, d = 4 * (tid % Q);
-  // the first sums are on their way before the maximum is known
-  float4v v[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    v[u] = g < G && g + u * G < p.splits ? *reinterpret_cast<const float4v*>(sums_of(p, D, row, g + u * G) + d)
-                                         : float4v{0, 0, 0, 0};
-  float m = wave_reduce<true>(t.x);
-  if (lane == 0) red[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  if (m == -__builtin_inff()) m = 0.0f;
-  const float own = __builtin_amdgcn_exp2f(t.x - m);
-  f[tid] = own;
-  const float l = wave_reduce<false>(t.y * own);
-  if (lane == 0) red[4 + wave] = l;
-  __syncthreads();
   float4v o = {0, 0, 0, 0};
-  if (g < G) {
+  float total = 0.0f;
+  if constexpr (FEW) {
+    float m = -__builtin_inff();
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, *total_of(p, D, all_rows, row, s));
+    if (m == -__builtin_inff()) m = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      const float2 t = *reinterpret_cast<const float2*>(total_of(p, D, all_rows, row, s));
+      const float f = __builtin_amdgcn_exp2f(t.x - m);
+      total += t.y * f;
+      o += f * *reinterpret_cast<const float4v*>(sums_of(p, D, row, s) + d);
+    }
+  } else {
+    __shared__ float f[256];
+    __shared__ float red[8];
+    __shared__ __attribute__((aligned(16))) float part[G][D];
+    const int lane = tid & 63, wave = tid >> 6;
+    const float2 t = tid < p.splits ? *reinterpret_cast<const float2*>(total_of(p, D, all_rows, row, tid))
+                                    : float2{-__builtin_inff(), 0.0f};
+    // the first sums are on their way before the maximum is known
+    float4v v[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (g + u * G < p.splits) o += f[g + u * G] * v[u];
-#pragma unroll 8
-    for (int s = g + 4 * G; s < p.splits; s += G)
-      o += f[s] * *reinterpret_cast<const float4v*>(sums_of(p, D, row, s) + d);
-    *reinterpret_cast<float4v*>(&part[g][d]) = o;
-  }
-  __syncthreads();
-  if (tid >= Q) return;
-  o = float4v{0, 0, 0, 0};
+      v[u] = g < G && g + u * G < p.splits ? *reinterpret_cast<const float4v*>(sums_of(p, D, row, g + u * G) + d)
+                                           : float4v{0, 0, 0, 0};
+    float m = wave_reduce<true>(t.x);
+    if (lane == 0) red[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (m == -__builtin_inff()) m = 0.0f;
+    const float own = __builtin_amdgcn_exp2f(t.x - m);
+    f[tid] = own;
+    const float l = wave_reduce<false>(t.y * own);
+    if (lane == 0) red[4 + wave] = l;
+    __syncthreads();
+    if (g < G) {
 #pragma unroll
-  for (int w = 0; w < G; ++w) o += *reinterpret_cast<const float4v*>(&part[w][d]);
-  const float total = (red[4] + red[5]) + (red[6] + red[7]);
+      for (int u = 0; u < 4; ++u)
+        if (g + u * G < p.splits) o += f[g + u * G] * v[u];
+#pragma unroll 8
+      for (int s = g + 4 * G; s < p.splits; s += G)
+        o += f[s] * *reinterpret_cast<const float4v*>(sums_of(p, D, row, s) + d);
+      *reinterpret_cast<float4v*>(&part[g][d]) = o;
+    }
+    __syncthreads();
+    if (tid >= Q) return;
+    o = float4v{0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < G; ++w) o += *reinterpret_cast<const float4v*>(&part[w][d]);
+    total = (red[4] + red[5]) + (red[6] + red[7]);
+  }
   if (total == 0.0f) o = float4v{0, 0, 0, 0};
   else o *= 1.0f / total;
   store4<BF16>(p, b, r, d, o[0], o[1], o[2], o[3]);
@@ -860,7 +1004,11 @@ hipError_t run_attend_elem(bool few, const AttendArgs& a, hipStream_t s) {
     if (e != hipSuccess) return e;
     AttendArgs j = a;
     j.d_work = div31(static_cast<unsigned>(a.rows));
-    attend_join_kernel<D, BF16><<<static_cast<unsigned>(all_rows), 256, 0, s>>>(j, all_rows);
+    constexpr int rows = 256 / (D / 4);
+    if (a.splits <= 16)
+      attend_join_kernel<D, BF16, true><<<static_cast<unsigned>((all_rows + rows - 1) / rows), 256, 0, s>>>(j, all_rows);
+    else
+      attend_join_kernel<D, BF16, false><<<static_cast<unsigned>(all_rows), 256, 0, s>>>(j, all_rows);
   }
   return hipGetLastError();
 }
