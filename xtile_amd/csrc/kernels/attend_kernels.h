@@ -127,8 +127,8 @@ struct Rows {
   int pos, above, below; // sees key j when below < j <= above (or j < prefix)
   int p0, p1;            // positions of the wave's first and last row
   float slope;           // times log2 e
-  int doc, one_doc;      // this lane's document; the first lane's, where alike: all rows have that
-  bool alike;
+  int doc;               // this lane's document
+  bool hidden;           // some row did not see some key of a tile that the wave worked on
   uint4v q[KK];
   float16v acc[N];
   float m, l;
@@ -148,8 +148,7 @@ struct Rows {
     below = p.window ? max(pos - p.window, -1) : -1;
     slope = p.slopes ? p.slopes[p.tslopes.at(bx, by, bz) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
     doc = p.qdocs ? p.qdocs[p.tqdocs.at(bx, by, bz) + token * p.qdoc_step] : 0;
-    one_doc = __builtin_amdgcn_readfirstlane(doc);
-    alike = __builtin_amdgcn_ballot_w64(doc != one_doc) == 0;
+    hidden = false;
     const unsigned char* at = p.q + (p.tq.at(bx, by, bz) + head * p.q_head + token * p.q_row + 8 * hi) * 2;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) q[kk] = (uint4v)(*reinterpret_cast<const u4a*>(at + kk * 32));
@@ -214,11 +213,27 @@ struct Rows {
   }
 
   // T tiles of 32 keys from key0 on.  docs: their documents in LDS, or null, then from
-  // kdocs.  False where values that are not finite lie in a tile that is masked in part
-  // (the rows' results are then of no use).
+  // kdocs.
   template <int T>
-  __device__ __forceinline__ bool tile(const AttendArgs& p, const unsigned char* K, const unsigned char* V,
+  __device__ __forceinline__ void tile(const AttendArgs& p, const unsigned char* K, const unsigned char* V,
                                        const int* docs, const int* kdocs, int key0, int len, int pre) {
+    bool part = !sees_all(p, key0, 32 * T, len, pre);
+    bool by_doc = false, by_key = false;  // rows, or keys, of several documents
+    int tile_doc = 0;
+    if (kdocs) {
+      const int i = key0 + (lane & (32 * T - 1));
+      const int d = docs ? docs[lane & (32 * T - 1)] : i < len ? kdocs[i] : 0;
+      tile_doc = __builtin_amdgcn_readfirstlane(d);
+      by_key = __builtin_amdgcn_ballot_w64(i < len && d != tile_doc) != 0;
+      if (!by_key) {
+        const unsigned long long same = __builtin_amdgcn_ballot_w64(doc == tile_doc);
+        if (same == 0) return;
+        by_doc = ~same != 0;
+      }
+      part |= by_doc || by_key;
+    }
+    hidden |= part;
+
     float16v s[T];
 #pragma unroll
     for (int t = 0; t < T; ++t)
@@ -250,15 +265,6 @@ struct Rows {
 #pragma unroll
       for (int n = 0; n < N; ++n) vf[x][n] = value_fragment(V, 0, x, n);
     __builtin_amdgcn_sched_barrier(0);
-
-    bool part = !sees_all(p, key0, 32 * T, len, pre);
-    bool by_doc = false;
-    if (kdocs) {
-      const int i = key0 + (lane & (32 * T - 1));
-      const int d = docs ? docs[lane & (32 * T - 1)] : i < len ? kdocs[i] : one_doc;
-      by_doc = !alike || __builtin_amdgcn_ballot_w64(i < len && d != one_doc) != 0;
-      part |= by_doc;
-    }
 
     float mul = p.scale_log2;
     if (p.cap_log2 > 0.0f) {
@@ -302,7 +308,8 @@ struct Rows {
       for (int t = 0; t < T; ++t) {
         const int base = key0 + t * 32 + 4 * hi;
         unsigned bits = ((up_to(above - base) & ~up_to(below - base)) | up_to(pre - 1 - base)) & up_to(len - 1 - base);
-        if (by_doc) {
+        if (by_doc && doc != tile_doc) bits = 0;
+        if (by_key) {
 #pragma unroll
           for (int w = 0; w < 4; ++w)
 #pragma unroll
@@ -340,13 +347,20 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
     }
-    bool fine = true;
-    if (part) {
-      fine = finite_values<T>(V);
-      asm volatile("" ::: "memory");  // or the fragments just looked through would be kept for the products
-    }
     add_values<T>(V, s, vf, mul);
-    return fine;
+  }
+
+  // Whether a value that a row does not see may have spoilt its sums: a weight of 0
+  // times an infinity or NaN is NaN, and stays.  (A row's own infinities look alike;
+  // odd_rows, which does such rows again, tells them apart.  Where the total is not
+  // finite either, the row's own scores are not.)
+  __device__ __forceinline__ bool spoilt() const {
+    float t = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t = fmaf(acc[n][r], 0.0f, t);
+    return hidden && __builtin_amdgcn_ballot_w64(t != 0.0f && l - l == 0.0f) != 0;
   }
 
   // Weights e^(score - m), rounded to the values' type (off by half a step each, as
@@ -396,29 +410,6 @@ struct Rows {
     }
     __builtin_amdgcn_s_setprio(0);
   }
-
-  static constexpr unsigned kExp = BF16 ? 0x7f80u : 0x7c00u;
-
-  // A weight of 0 times a hidden infinity or NaN would be NaN: a tile that is masked
-  // in part is looked through for them, and a workgroup that meets any goes through
-  // its rows again one by one (odd_rows).
-  template <int T>
-  __device__ __forceinline__ bool finite_values(const unsigned char* V) const {
-    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-    us2 most = {0, 0};
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const uint4v v = value_fragment(V, t, u, n);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, v[e] & (kExp | kExp << 16)));
-        }
-    return __builtin_amdgcn_ballot_w64(most[0] == kExp || most[1] == kExp) == 0;
-  }
 };
 
 // The tiles of BN keys that a workgroup's rows may see: tiles [a0, a0 + na) of the
@@ -442,42 +433,38 @@ __device__ __forceinline__ Tiles tiles_of(const AttendArgs& p, int bn, int p0, i
   return t;
 }
 
-// The smallest and largest over the workgroup's threads; `mem`: two ints a wave.
-template <int W>
-__device__ __forceinline__ void span(int& lo, int& hi, int* mem) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    lo = min(lo, __shfl_xor(lo, o, 64));
-    hi = max(hi, __shfl_xor(hi, o, 64));
-  }
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
-    mem[2 * wave] = lo;
-    mem[2 * wave + 1] = hi;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    lo = min(lo, mem[2 * w]);
-    hi = max(hi, mem[2 * w + 1]);
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = __builtin_amdgcn_readfirstlane(hi);
-  __syncthreads();
+// The smallest (or largest) over a wave, in every lane: wave_reduce for integers.
+template <bool IS_MAX>
+__device__ __forceinline__ int wave_extreme(int v) {
+  constexpr int id = IS_MAX ? -0x7fffffff - 1 : 0x7fffffff;
+  auto op = [](int a, int b) { return IS_MAX ? max(a, b) : min(a, b); };
+  int a = v;
+  a = op(a, __builtin_amdgcn_update_dpp(id, v, 0x111, 0xf, 0xf, false));
+  a = op(a, __builtin_amdgcn_update_dpp(id, v, 0x112, 0xf, 0xf, false));
+  a = op(a, __builtin_amdgcn_update_dpp(id, v, 0x113, 0xf, 0xf, false));
+  a = op(a, __builtin_amdgcn_update_dpp(id, a, 0x114, 0xf, 0xe, false));
+  a = op(a, __builtin_amdgcn_update_dpp(id, a, 0x118, 0xf, 0xc, false));
+  a = op(a, __builtin_amdgcn_update_dpp(id, a, 0x142, 0xa, 0xf, false));
+  a = op(a, __builtin_amdgcn_update_dpp(id, a, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(a, 63);
 }
 
-// Keys [d0, d1) outside of which no key's document lies between those of tokens
-// t0 to t1: all that packed documents need not read.
+// Keys [d0, d1), of the first `keys`, outside of which no key's document lies between
+// those of tokens t0 to t1: all that packed documents need not read.  mem: two ints a
+// wave.
 template <int W>
 __device__ __forceinline__ void document_keys(const AttendArgs& p, const int* qdocs, const int* kdocs, int t0, int t1,
                                               int keys, int* mem, int& d0, int& d1) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int lo = 0x7fffffff, hi = -0x7fffffff - 1;
-  for (int t = t0 + (int)threadIdx.x; t <= t1; t += 64 * W) {
+#pragma unroll 2
+  for (int t = t0 + lane; t <= t1; t += 64) {  // every wave by itself
     const int d = qdocs[t * p.qdoc_step];
     lo = min(lo, d);
     hi = max(hi, d);
   }
-  span<W>(lo, hi, mem);
+  lo = wave_extreme<false>(lo);
+  hi = wave_extreme<true>(hi);
   int first = keys, last = -1;
   typedef int i4a __attribute__((ext_vector_type(4), aligned(4)));
   constexpr int STEP = 256 * W;  // keys a round
@@ -497,6 +484,7 @@ __device__ __forceinline__ void document_keys(const AttendArgs& p, const int* qd
           last = max(last, at);
         }
   }
+#pragma unroll 4
   for (j += threadIdx.x; j < keys; j += 64 * W) {
     const int d = kdocs[j];
     if (d >= lo && d <= hi) {
@@ -504,9 +492,21 @@ __device__ __forceinline__ void document_keys(const AttendArgs& p, const int* qd
       last = max(last, j);
     }
   }
-  span<W>(first, last, mem);
-  d0 = first;
-  d1 = last + 1;
+  first = wave_extreme<false>(first);
+  last = wave_extreme<true>(last);
+  if (lane == 0) {
+    mem[2 * wave] = first;
+    mem[2 * wave + 1] = last;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    first = min(first, mem[2 * w]);
+    last = max(last, mem[2 * w + 1]);
+  }
+  d0 = __builtin_amdgcn_readfirstlane(first);
+  d1 = __builtin_amdgcn_readfirstlane(last) + 1;
+  __syncthreads();
 }
 
 struct BlockAt {
@@ -531,6 +531,11 @@ __device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
   b.len = __builtin_amdgcn_readfirstlane(b.len);
   b.pre = __builtin_amdgcn_readfirstlane(b.pre);
   return b;
+}
+
+// No row up to token t1 sees this key or a later one, documents aside.
+__device__ __forceinline__ int last_key(const AttendArgs& p, const BlockAt& b, int t1) {
+  return p.causal ? min(b.len, max(max(b.start + t1, -1) + 1, b.pre)) : b.len;
 }
 
 // BN keys of D values each from an array to LDS, by STEP waves: instruction i of a
@@ -710,7 +715,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(Atte
   const int* const kdocs = p.kdocs ? p.kdocs + p.tkdocs.at(b.x, b.y, b.z) : nullptr;
   int d0 = 0, d1 = b.len;
   if (kdocs)
-    document_keys<4>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, t0, t1, b.len, reinterpret_cast<int*>(lds), d0, d1);
+    document_keys<4>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, t0, t1, last_key(p, b, t1), reinterpret_cast<int*>(lds),
+                     d0, d1);
   const Tiles tiles = tiles_of(p, BN, b.start + t0, b.start + t1, b.len, b.pre, d0, d1);
   const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
   const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
@@ -728,7 +734,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(Atte
   if (i0 < i1) issue(i0, lds);
   Rows<D, BF16> rows;
   rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start);
-  bool fine = true;
 #pragma unroll 1
   for (int i = i0; i < i1; ++i) {
     // one barrier a tile: behind it this tile has landed, and every wave is done with
@@ -739,11 +744,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(Atte
     if (i + 1 < i1) issue(i + 1, lds + ((i + 1 - i0) & 1) * STAGE);
     const int key0 = tiles.at(i) * BN;
     if (!rows.sees_none(p, key0, BN, b.pre))
-      fine &= rows.template tile<2>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len, b.pre);
+      rows.template tile<2>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len, b.pre);
   }
   rows.hold();
   lds_barrier();
-  if (any_wave<4>(!fine, lds)) {
+  if (any_wave<4>(rows.spoilt(), lds)) {
     odd_rows<D, BF16>(p, b, tiles, BN, i0, i1, kdocs, first + wave, last + 1, 4, all_rows);
     return;
   }
@@ -819,7 +824,8 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   const int* const kdocs = p.kdocs ? p.kdocs + p.tkdocs.at(b.x, b.y, b.z) : nullptr;
   int d0 = 0, d1 = b.len;
   if (kdocs)
-    document_keys<W>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, 0, t1, b.len, reinterpret_cast<int*>(lds), d0, d1);
+    document_keys<W>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, 0, t1, last_key(p, b, t1), reinterpret_cast<int*>(lds),
+                     d0, d1);
   const Tiles tiles = tiles_of(p, 32, b.start, b.start + t1, b.len, b.pre, d0, d1);
   const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
   const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
@@ -842,7 +848,6 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
     if (j < mine) issue(j, j);
   Rows<D, BF16> rows;
   rows.begin(p, 0, b.x, b.y, b.z, b.start);
-  bool fine = true;
   int slot = 0;
 #pragma unroll 1
   for (int j = 0; j < mine; ++j) {
@@ -855,7 +860,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
     }
     asm volatile("" ::: "memory");
     unsigned char* const at = ring + slot * F::TILE;
-    fine &= rows.template tile<1>(p, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
+    rows.template tile<1>(p, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
     // every fragment is in registers before the slot is filled again
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -863,7 +868,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
   __syncthreads();  // every ring is done with
-  if (any_wave<W>(!fine, lds)) {
+  if (any_wave<W>(rows.spoilt(), lds)) {
     odd_rows<D, BF16>(p, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);
     return;
   }
