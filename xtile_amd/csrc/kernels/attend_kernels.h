@@ -132,7 +132,10 @@ struct Rows {
   uint4v q[KK];
   float16v acc[N];
   float m, l;
-  int koff[KK], voff[N]; // LDS offsets of this lane's part of a key and of a value fragment
+  // LDS offsets of this lane's part of a key and of a value fragment, for each step;
+  // the widest heads, short of registers, keep one of a key row and work out the rest
+  static constexpr bool LEAN = D == 256;
+  int koff[LEAN ? 1 : KK], voff[N];
 
   __device__ __forceinline__ void begin(const AttendArgs& p, int first, int bx, int by, int bz, int start) {
     lane = threadIdx.x & 63;
@@ -158,7 +161,7 @@ struct Rows {
 #pragma unroll
     for (int n = 0; n < N; ++n) voff[n] = key * PITCH + ((((chunk ^ vsw(key)) << 4) + 8 * (li & 1)) ^ (n << 6));
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) koff[kk] = col * PITCH + (((2 * kk + hi) ^ ksw(col)) << 4);
+    for (int kk = 0; kk < (LEAN ? 1 : KK); ++kk) koff[kk] = col * PITCH + (((2 * kk + hi) ^ ksw(col)) << 4);
   }
 
   __device__ __forceinline__ void reset() {
@@ -178,7 +181,12 @@ struct Rows {
   }
 
   __device__ __forceinline__ uint4v key_fragment(const unsigned char* K, int kt, int kk) const {
-    return *reinterpret_cast<const uint4v*>(K + koff[kk] + kt * 32 * PITCH);
+    if constexpr (LEAN) {
+      int at = koff[0];
+      asm volatile("" : "+v"(at));
+      return *reinterpret_cast<const uint4v*>(K + (at ^ (kk << 5)) + kt * 32 * PITCH);
+    }
+    return *reinterpret_cast<const uint4v*>(K + koff[LEAN ? 0 : kk] + kt * 32 * PITCH);
   }
 
   // Values of keys 32 kt + 16 u + {4 h + 0..3, 8 + 4 h + 0..3}, column 32 n + c.
@@ -546,36 +554,64 @@ struct Fill {
   typedef Rows<D, false> R;
   static constexpr int IN = BN * D * 2 / 1024 / STEP;
   static_assert(IN * 1024 * STEP == BN * D * 2, "whole instructions");
+  // Where an instruction takes whole rows, the swizzle of its first row and that of
+  // the lane's row among them are apart (the rows' bits are): two registers, the row's
+  // offset and the chunk's, serve all instructions.  That fits three workgroups on a CU
+  // at 64 columns (documents of 8192 tokens: 57 -> 51 us) and leaves nothing in scratch
+  // at 256.  Otherwise each has its own: at 128 the arithmetic costs more than the
+  // registers (a batch of decoded tokens: 175 us against 179).
+  static constexpr bool WHOLE = 1024 % (2 * D) == 0 && D != 128;
+  static constexpr int RPI = 512 / D;
   const unsigned char* base;
   unsigned pitch;
-  unsigned off[IN];
+  unsigned off[WHOLE ? 2 : IN];
   int lane, first;
+
+  static __device__ __forceinline__ int swizzle(int row) { return VALUES ? R::vsw(row) : R::ksw(row); }
 
   __device__ __forceinline__ void begin(const unsigned char* b, long long ld, int wave) {
     base = b;
     pitch = (unsigned)(ld * 2);
     lane = threadIdx.x & 63;
     first = wave;
+    if constexpr (WHOLE) {
+      const int row = lane / (D / 8), c = lane % (D / 8);
+      off[0] = (unsigned)row * pitch;
+      off[1] = (unsigned)(c ^ swizzle(row)) << 4;
+    } else {
 #pragma unroll
-    for (int i = 0; i < IN; ++i) {
-      const int pos = (i * STEP + first) * 1024 + lane * 16, row = pos / (2 * D), c = (pos % (2 * D)) >> 4;
-      off[i] = (unsigned)row * pitch + ((c ^ (VALUES ? R::vsw(row) : R::ksw(row))) << 4);
+      for (int i = 0; i < IN; ++i) {
+        const int pos = (i * STEP + first) * 1024 + lane * 16, row = pos / (2 * D), c = (pos % (2 * D)) >> 4;
+        off[i] = (unsigned)row * pitch + ((c ^ swizzle(row)) << 4);
+      }
+    }
+  }
+
+  // Byte offset of the chunk that instruction i of this wave brings; chunk: off[1].
+  __device__ __forceinline__ unsigned at(int i, unsigned chunk) const {
+    if constexpr (WHOLE) {
+      const int row = (i * STEP + first) * RPI;
+      return (unsigned)row * pitch + off[0] + (chunk ^ ((unsigned)swizzle(row) << 4));
+    } else {
+      return off[i];
     }
   }
 
   __device__ __forceinline__ void issue(bool dma, int key0, int left, unsigned char* to) const {
     const unsigned char* from = base + (long long)key0 * pitch;
+    unsigned chunk = off[WHOLE ? 1 : 0];
+    if constexpr (WHOLE) asm volatile("" : "+v"(chunk));  // or the offsets would be kept, a register each
     if (dma) {
       const i32x4 rs = raw_rsrc(from, (unsigned)(min(left, BN) - 1) * pitch + 2 * D);
-      const unsigned at = __builtin_amdgcn_readfirstlane(lds_at(to) + first * 1024);
+      const unsigned lds = __builtin_amdgcn_readfirstlane(lds_at(to) + first * 1024);
 #pragma unroll
-      for (int i = 0; i < IN; ++i) dma16(rs, at + i * STEP * 1024, off[i], 0);
+      for (int i = 0; i < IN; ++i) dma16(rs, lds + i * STEP * 1024, at(i, chunk), 0);
     } else {
 #pragma unroll
       for (int i = 0; i < IN; ++i) {
         const int pos = (i * STEP + first) * 1024 + lane * 16;
         uint4v v = {0, 0, 0, 0};
-        if (pos / (2 * D) < left) v = (uint4v)(*reinterpret_cast<const u4a*>(from + off[i]));
+        if (pos / (2 * D) < left) v = (uint4v)(*reinterpret_cast<const u4a*>(from + at(i, chunk)));
         *reinterpret_cast<uint4v*>(to + pos) = v;
       }
     }
@@ -704,7 +740,7 @@ __device__ __forceinline__ bool any_wave(bool x, unsigned char* lds) {
 // More than 32 rows: 128 of them, 32 a wave, the keys in tiles of 64 that the waves
 // share, two of them in LDS.
 template <int D, bool BF16>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs p, long long all_rows) {
+__global__ __launch_bounds__(256, D <= 64 ? 3 : D <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs p, long long all_rows) {
   constexpr int BN = 64, KB = BN * D * 2, STAGE = 2 * KB + 256;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
   const bool dma = p.dma;
@@ -867,6 +903,9 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
     if (j + NS < mine) issue(j + NS, slot);
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
+  // At 256 columns the accumulators would otherwise meet themselves in other registers,
+  // and scratch; narrower heads lose a few of 120 us by it.
+  if constexpr (D == 256) rows.hold();
   __syncthreads();  // every ring is done with
   if (any_wave<W>(rows.spoilt(), lds)) {
     odd_rows<D, BF16>(p, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);

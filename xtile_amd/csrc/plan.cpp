@@ -1338,9 +1338,11 @@ int attend_splits(const Plan& p) {
   const int64_t rows = a.heads * a.rows, per = rows <= kAttendFewRows ? kAttendFewRows : kAttendRows;
   const double tiles = double(p.grid[0]) * p.grid[1] * p.grid[2] * double((rows + per - 1) / per);
   // Four workgroups a CU, so that sequences of different lengths even out, but
-  // no fewer than 256 keys each.
+  // no fewer than 256 keys each, of those that a window leaves.
+  const bool band = a.causal && a.window && a.extra[3].arg < 0;
+  const int64_t keys = band ? std::min(a.keys, a.window + a.rows) : a.keys;
   const double want = 1024 / tiles;
-  const int64_t most = a.keys / 256;
+  const int64_t most = keys / 256;
   if (want < 2 || most < 2) return 1;
   return static_cast<int>(std::min<double>(std::min<double>(want, double(most)), 256));
 }
