@@ -1333,16 +1333,24 @@ GemmCover gemm_cover(const Plan& p, int64_t w, bool is_m) {
   return c;
 }
 
+// Keys are split where the tiles of rows leave compute units idle, into no more parts
+// than fill them once: a second round costs more than it evens out (a token against
+// 131072 keys, 8 heads: 256 workgroups 108 us, 512 112, 1024 121).  A part of few rows
+// has a tile for each wave; one of many rows has four tiles, and the keys are not split
+// below 1024, where joining the parts costs what they save (577 keys, 160 tiles: whole
+// 20.4 us, halves 25.7).
 int attend_splits(const Plan& p) {
   const AttendPlan& a = p.attend;
-  const int64_t rows = a.heads * a.rows, per = rows <= kAttendFewRows ? kAttendFewRows : kAttendRows;
+  const int64_t rows = a.heads * a.rows;
+  const bool few = rows <= kAttendFewRows;
+  const int64_t per = few ? kAttendFewRows : kAttendRows;
   const double tiles = double(p.grid[0]) * p.grid[1] * p.grid[2] * double((rows + per - 1) / per);
-  // Four workgroups a CU, so that sequences of different lengths even out, but
-  // no fewer than 256 keys each, of those that a window leaves.
+  // A causal window leaves only so many keys, whatever the cache holds.
   const bool band = a.causal && a.window && a.extra[3].arg < 0;
   const int64_t keys = band ? std::min(a.keys, a.window + a.rows) : a.keys;
-  const double want = 1024 / tiles;
-  const int64_t most = keys / 256;
+  const int fit = few ? (a.d > 64 ? 1 : 2) : a.d > 128 ? 1 : a.d > 64 ? 2 : 3;  // workgroups on a compute unit
+  const double want = 256 * fit / tiles;
+  const int64_t most = few ? keys / 128 : keys < 1024 ? 1 : keys / 256;
   if (want < 2 || most < 2) return 1;
   return static_cast<int>(std::min<double>(std::min<double>(want, double(most)), 256));
 }
