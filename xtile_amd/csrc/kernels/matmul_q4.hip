@@ -1,17 +1,21 @@
 // Products with 4-bit weights:
 //   y[m, n] = rs[m] sum_g s[n, g] sum_{k in group g} x[m, k] w[n, k]
 //
-// The weights are read once, 16 bytes a lane straight into registers, and bound
-// the kernel: x, of few rows, comes from L2.  A workgroup takes 16 NT rows of
-// weights and 16 MT rows of x; its waves split K in chunks of 128 and meet once,
-// in LDS, in a fixed order.
+// The weights are read once and bound the kernel: x, of few rows, comes from L2.  A
+// workgroup takes 16 rows of weights and 16 MT rows of x; its waves split K in chunks
+// of 128 and meet once, in LDS, in a fixed order.
 //
-// A chunk: lane (n = lane % 16, q = lane / 16) loads the 32 weights of row n at
-// k = 32 q.  A 4 x 4 transpose over the quarters of the wave (four swaps of lane
-// halves and rows) turns that into one word for each step of 32 K values: in step
-// t lane (n, q) has the eight weights at k = 32 t + 8 q, so a step lies within one
-// group of 32 whatever the group's size.  x goes as the MFMA's rows, the weights
-// as its columns, so a lane's results are all of one weight row and take one scale.
+// A wave brings a chunk's weights, rows of x and scales into a ring of its own in LDS
+// by DMA, so that nothing but its own loads makes it wait and neighbouring lanes read
+// neighbouring bytes.  Loaded straight into the fragments' registers, where neighbours
+// are of different rows, every load takes its 64 lookups in the cache apart: 16 rows of
+// int8 by 4096 x 11008 weights took 16.8 us so and take 9.7 us.  Two chunks in a ring
+// leave several workgroups on a CU; three and four are slower (11008 x 4096, groups of
+// 32: 11.8, 13.1 and 13.4 us), as are four waves for eight and sixteen (13.9, 16.1).
+//
+// Of the fragments, x goes as the MFMA's rows and the weights as its columns, so a
+// lane's results are all of one weight row and take one scale; lane (n, q) has the
+// eight weights at k = 32 t + 8 q in step t, one word.
 //
 // Unpacking: the bytes hold weight + 8 (0..15).  Nibbles i and i + 4 of a word are
 // neighbours along K; shifted to the top four bits of the mantissa of 16.0 (both
@@ -22,6 +26,7 @@
 // integers; x's bytes are put in the nibbles' order by two v_perm a word pair.
 #include "launch.h"
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -44,45 +49,44 @@ struct Q4Args {
   BlockDecode blocks;
   Div31 d_tiles, d_nt;  // tiles of a Block, n tiles
   int tiles, ntiles;
-  int M, N, K, chunks, group;
-  Div31 d_group;  // units of 32 FL weights in a group
+  int M, N, K, group;
+  int dma;
+  Div31 d_group;  // steps of 32 FL weights in a group
   int s_elem, y_elem;
 };
 
 typedef unsigned u4a __attribute__((ext_vector_type(4), aligned(1)));
-typedef unsigned u2a __attribute__((ext_vector_type(2), aligned(1)));
 
-// Register t of quarter q <-> register q of quarter t.
-__device__ __forceinline__ void transpose_quarters(unsigned (&d)[4]) {
-  auto swap32 = [](unsigned& a, unsigned& b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-  };
-  auto swap16 = [](unsigned& a, unsigned& b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-  };
-  swap32(d[0], d[2]);
-  swap32(d[1], d[3]);
-  swap16(d[0], d[1]);
-  swap16(d[2], d[3]);
+// Four bytes a lane into LDS by DMA; as dma16.
+__device__ __forceinline__ void dma4(i32x4 rsrc, unsigned lds, unsigned voff) {
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
 }
 
-__device__ __forceinline__ float scale_at(const void* s, int elem, long long i) {
-  if (elem == kF32) return static_cast<const float*>(s)[i];
-  if (elem == kF16) return (float)static_cast<const _Float16*>(s)[i];
-  return __builtin_bit_cast(float, (unsigned)static_cast<const unsigned short*>(s)[i] << 16);
-}
+constexpr unsigned kNone = 1u << 31;  // an offset behind every row: such lanes read zeros
+
+// What a workgroup of W waves holds.  ROWS: rows of x, of which the MFMA takes 16 at a
+// time (fewer are read again and again, for results that are not stored).
+template <bool I8, int ROWS, int W, int NS>
+struct Q4Shape {
+  static constexpr int MT = ROWS <= 16 ? 1 : ROWS / 16;
+  static constexpr int ES = I8 ? 1 : 2, PIECES = 8 * ES;  // pieces of 16 bytes in a row's 128 values
+  // a stage: the weights, x, the scales; instructions that bring x, and all three
+  static constexpr int X0 = 1024, S0 = X0 + ROWS * PIECES * 16, STAGE = S0 + 256;
+  static constexpr int XI = ROWS * PIECES / 64, PER = XI + 2;
+  static constexpr int LDS = W * NS * STAGE;
+  static_assert(XI * 64 == ROWS * PIECES && LDS <= 160 * 1024 && NS >= 2 && NS <= 4 && (NS - 1) * PER < 64, "");
+  static_assert(W * MT * 1024 <= LDS, "the waves' parts take the rings' place");
+};
 
 // FL: steps of 32 between two additions to the result (1, 2 or 4): at most the group.
-template <int ELEM, int MT, int NT, int W, int FL>
+// S32: scales of 32 bits.  NS: chunks in a wave's ring.
+template <int ELEM, int ROWS, int W, int NS, int FL, bool S32>
 __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   constexpr bool I8 = ELEM == kI8;
-  constexpr int ES = I8 ? 1 : 2;
+  typedef Q4Shape<I8, ROWS, W, NS> S;
+  constexpr int ES = S::ES, MT = S::MT, XI = S::XI, PIECES = S::PIECES, NF = 4 / FL;
   typedef typename std::conditional<I8, int4v, float4v>::type acc_t;
-  __shared__ float part[W][NT * MT][4][64];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[S::LDS];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -92,95 +96,110 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   const int tm = (int)p.d_nt(tile), tn = tile - tm * p.ntiles;
   int bx, by, bz;
   p.blocks(b, bx, by, bz);
-  const int m0 = tm * 16 * MT, n0 = tn * 16 * NT;
+  const int m0 = tm * 16 * MT, n0 = tn * 16;
+  const unsigned char* const w = p.w + p.tw.at(bx, by, bz) + n0 * p.ldw;
+  const unsigned char* const x = p.x + (p.tx.at(bx, by, bz) + m0 * p.ldx) * ES;
 
-  const unsigned char* w[NT];
-  long long sc[NT];
+  // A lane's pieces: the weights' row lane / 4, piece (lane % 4) ^ row / 2 % 4; x's row
+  // lane / PIECES of each instruction's, piece (lane % PIECES) ^ row % 8.  Neighbours
+  // read neighbours in memory, and fragments, of one piece of 16 rows, lie over all banks.
+  const int wn = lane >> 2, wt = (lane & 3) ^ ((lane >> 3) & 3);
+  const unsigned wat = wn < p.N - n0 ? (unsigned)wn * (unsigned)p.ldw + wt * 16 : kNone;
+  constexpr int XR = 64 / PIECES;  // rows of an instruction: 4 or 8
+  unsigned xat[XI];
+  const int xr = lane / PIECES;
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {  // rows past the end read the last one; their results are not stored
-    const int n = min(n0 + 16 * j + col, p.N - 1);
-    w[j] = p.w + p.tw.at(bx, by, bz) + n * p.ldw;
-    sc[j] = p.ts.at(bx, by, bz) + n * p.lds;
+  for (int i = 0; i < XI; ++i) {
+    const int row = i * XR + xr, c = (lane % PIECES) ^ (row & 7);
+    xat[i] = row < p.M - m0 ? (unsigned)row * (unsigned)p.ldx * ES + c * 16 : kNone;
   }
-  const unsigned char* x[MT];
+  // Its scale: row lane / 4, the group of step FL (lane % 4) of a chunk.  DMA takes four
+  // bytes, of which a scale of 16 bits is either half, so the address is rounded down to
+  // them; they lie within the memory that holds the scale.
+  const int sf0 = lane & 3;
+  const unsigned char* const st = static_cast<const unsigned char*>(p.s) + ((p.ts.at(bx, by, bz) + n0 * p.lds) << (S32 ? 2 : 1));
+  const unsigned odd = (unsigned)reinterpret_cast<uintptr_t>(st) & 3;  // 16 bits: 0 or 2
+  const unsigned char* const s0 = st - odd;
+  const bool sany = wn < p.N - n0 && sf0 < NF;
+  const unsigned srow = (unsigned)wn * (unsigned)p.lds;
+  unsigned char* const ring = lds + wave * NS * S::STAGE;
+  auto issue = [&](int c, int slot) {
+    unsigned char* const at = ring + slot * S::STAGE;
+    const unsigned char* const wc = w + (long long)c * 64;
+    const unsigned char* const xc = x + (long long)c * 128 * ES;
+    const int left = p.K - c * 128;  // pieces past it are zeros
+    const bool whole = left >= 128;
+    const unsigned wo = whole || wt * 32 < left ? wat : kNone;
+    const unsigned so = ((srow + p.d_group((unsigned)(c * NF + sf0))) << (S32 ? 2 : 1)) + odd;
+    const bool sin = sany && sf0 * FL * 32 < left;
+    if (p.dma) {
+      // the low half of its generic address (a cast between address spaces compares with null first)
+      const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>(at));
+      dma16(raw_rsrc(wc, kNone), to, wo, 0);
+      const i32x4 rs = raw_rsrc(xc, kNone);
 #pragma unroll
-  for (int i = 0; i < MT; ++i) x[i] = p.x + (p.tx.at(bx, by, bz) + min(m0 + 16 * i + col, p.M - 1) * p.ldx + q * 8) * ES;
-
-  float4v y[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) y[i][j] = float4v{0, 0, 0, 0};
-
-  struct Chunk {
-    unsigned w[NT][4];
-    uint4v x[MT][4];
-    float s[NT][4 / FL];
-  };
-  // steps: of 32 K values in this chunk (fewer than four in a last one)
-  auto fetch = [&](int c, int steps, Chunk& k) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const u4a v = *reinterpret_cast<const u4a*>(w[j] + (long long)c * 64 + (q < steps ? q : 0) * 16);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) k.w[j][t] = v[t];
-#pragma unroll
-      for (int f = 0; f < 4 / FL; ++f) {
-        const int g = (int)p.d_group((unsigned)(c * (4 / FL) + (f * FL < steps ? f : 0)));
-        k.s[j][f] = scale_at(p.s, p.s_elem, sc[j] + g);
+      for (int i = 0; i < XI; ++i) {
+        const int k = ((lane % PIECES) ^ ((i * XR + xr) & 7)) * (16 / ES);
+        dma16(rs, to + S::X0 + 1024 * i, whole || k < left ? xat[i] : kNone, 0);
       }
+      dma4(raw_rsrc(s0, kNone), to + S::S0, sin ? so & ~3u : kNone);
+    } else {
+      uint4v v = {0, 0, 0, 0};
+      if (wo < kNone) v = (uint4v)(*reinterpret_cast<const u4a*>(wc + wo));
+      *reinterpret_cast<uint4v*>(at + lane * 16) = v;
+#pragma unroll
+      for (int i = 0; i < XI; ++i) {
+        const int k = ((lane % PIECES) ^ ((i * XR + xr) & 7)) * (16 / ES);
+        uint4v u = {0, 0, 0, 0};
+        if (xat[i] < kNone && k < left) u = (uint4v)(*reinterpret_cast<const u4a*>(xc + xat[i]));
+        *reinterpret_cast<uint4v*>(at + S::X0 + 1024 * i + lane * 16) = u;
+      }
+      unsigned e = 0;
+      if (sin) e = *reinterpret_cast<const unsigned*>(s0 + (so & ~3u));
+      *reinterpret_cast<unsigned*>(at + S::S0 + lane * 4) = e;
     }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const unsigned char* at = x[i] + ((long long)c * 128 + (t < steps ? t : 0) * 32) * ES;
-        if constexpr (I8) {
-          const u2a v = *reinterpret_cast<const u2a*>(at);
-          k.x[i][t] = uint4v{v[0], v[1], 0, 0};
-        } else {
-          k.x[i][t] = (uint4v)(*reinterpret_cast<const u4a*>(at));
-        }
-      }
   };
-  auto compute = [&](int steps, Chunk& k) {
+
+  float4v y[MT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) transpose_quarters(k.w[j]);
+  for (int i = 0; i < MT; ++i) y[i] = float4v{0, 0, 0, 0};
+
+  // where this lane's fragments lie in a stage: a word of weights, and of x the piece of
+  // a row's step, in which int8 rows have two quarters' eight bytes
+  const int wfrag = col * 64 + q * 4, wsw = (col >> 1) & 3;
+  const int xrow = ROWS < 16 ? col % ROWS : col, xsw = xrow & 7;
+  const int xfrag = S::X0 + xrow * PIECES * 16 + (I8 ? (q & 1) * 8 : 0), xpiece = I8 ? q >> 1 : q;
+  int f16 = p.s_elem == kF16;
+  asm volatile("" : "+v"(f16));  // told apart lane by lane: a branch would part the products
+  const bool f16_scales = f16 != 0;
+  const unsigned srow_col = (unsigned)col * (unsigned)p.lds + (odd >> 1);
+
+  auto compute = [&](const unsigned (&d)[4], const uint4v (&xf)[MT][4], const unsigned (&sc)[NF], int c) {
 #pragma unroll
-    for (int f = 0; f < 4 / FL; ++f) {
-      if (f * FL >= steps) break;
-      acc_t acc[MT][NT], off[MT];
+    for (int f = 0; f < NF; ++f) {
+      // one step: its correction is where its products begin; more: two sums side by side
+      constexpr bool CHAIN = FL == 1;
+      acc_t acc[MT], off[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        off[i] = acc_t{0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
-      }
+      for (int i = 0; i < MT; ++i) acc[i] = off[i] = acc_t{0, 0, 0, 0};
 #pragma unroll
       for (int u = 0; u < FL; ++u) {
         const int t = f * FL + u;
-        if (t >= steps) break;
         if constexpr (I8) {
-          const long eights = 0x0808080808080808L;
-          long xi[MT];
+          const long eights = CHAIN ? (long)0xf8f8f8f8f8f8f8f8UL : 0x0808080808080808L;
+          const long wj = (long)(((unsigned long)((d[t] >> 4) & 0x0f0f0f0fu) << 32) | (d[t] & 0x0f0f0f0fu));
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
-            const unsigned lo = __builtin_amdgcn_perm(k.x[i][t][1], k.x[i][t][0], 0x05010400u);
-            const unsigned hi = __builtin_amdgcn_perm(k.x[i][t][1], k.x[i][t][0], 0x07030602u);
-            xi[i] = (long)(((unsigned long)hi << 32) | lo);
-            off[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xi[i], eights, off[i], 0, 0, 0);
-          }
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const unsigned d = k.w[j][t];
-            const long wj = (long)(((unsigned long)((d >> 4) & 0x0f0f0f0fu) << 32) | (d & 0x0f0f0f0fu));
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xi[i], wj, acc[i][j], 0, 0, 0);
+            const unsigned lo = __builtin_amdgcn_perm(xf[i][t][1], xf[i][t][0], 0x05010400u);
+            const unsigned hi = __builtin_amdgcn_perm(xf[i][t][1], xf[i][t][0], 0x07030602u);
+            const long xi = (long)(((unsigned long)hi << 32) | lo);
+            off[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xi, eights, off[i], 0, 0, 0);
+            acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xi, wj, CHAIN ? off[i] : acc[i], 0, 0, 0);
           }
         } else {
           // 16 + u: f16 0x4c00 | u << 6, bf16 0x4180 | u << 3
           constexpr unsigned one = ELEM == kF16 ? 0x4c004c00u : 0x41804180u, mask = ELEM == kF16 ? 0x03c003c0u : 0x00780078u;
-          constexpr unsigned c24 = ELEM == kF16 ? 0x4e004e00u : 0x41c041c0u;
+          constexpr unsigned c24 = (ELEM == kF16 ? 0x4e004e00u : 0x41c041c0u) | (CHAIN ? 0x80008000u : 0);
           constexpr int up = ELEM == kF16 ? 6 : 3;
           auto mma = [](uint4v a, uint4v bb, float4v c) {
             if constexpr (ELEM == kF16)
@@ -188,63 +207,90 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
             else
               return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, bb), c, 0, 0, 0);
           };
+          uint4v v;
 #pragma unroll
-          for (int i = 0; i < MT; ++i) off[i] = mma(k.x[i][t], uint4v{c24, c24, c24, c24}, off[i]);
+          for (int e = 0; e < 4; ++e)
+            v[e] = ((up >= 4 * e ? d[t] << (up - 4 * e) : d[t] >> (4 * e - up)) & mask) | one;
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const unsigned d = k.w[j][t];
-            uint4v v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              v[e] = ((up >= 4 * e ? d << (up - 4 * e) : d >> (4 * e - up)) & mask) | one;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i][j] = mma(k.x[i][t], v, acc[i][j]);
+          for (int i = 0; i < MT; ++i) {
+            off[i] = mma(xf[i][t], uint4v{c24, c24, c24, c24}, off[i]);
+            acc[i] = mma(xf[i][t], v, CHAIN ? off[i] : acc[i]);
           }
         }
+      }
+      float sf;
+      if constexpr (S32) {
+        sf = __builtin_bit_cast(float, sc[f]);
+      } else {
+        const unsigned half = sc[f] >> (((srow_col + p.d_group((unsigned)(c * NF + f))) & 1) * 16);
+        const float h = (float)__builtin_bit_cast(_Float16, (unsigned short)half), b = __builtin_bit_cast(float, half << 16);
+        sf = f16_scales ? h : b;
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) y[i][j][r] = fmaf((float)(acc[i][j][r] - off[i][r]), k.s[j][f], y[i][j][r]);
+        for (int r = 0; r < 4; ++r) y[i][r] = fmaf((float)(CHAIN ? acc[i][r] : acc[i][r] - off[i][r]), sf, y[i][r]);
     }
   };
 
-  auto steps_of = [&](int c) { return min(4, (p.K >> 5) - 4 * c); };
-  Chunk k0, k1;
-  int c = wave;
-  if (c < p.chunks) {
-    fetch(c, steps_of(c), k0);
-    while (true) {
-      const int c1 = c + W;
-      if (c1 < p.chunks) fetch(c1, steps_of(c1), k1);
-      compute(steps_of(c), k0);
-      if (c1 >= p.chunks) break;
-      const int c2 = c1 + W;
-      if (c2 < p.chunks) fetch(c2, steps_of(c2), k0);
-      compute(steps_of(c1), k1);
-      if (c2 >= p.chunks) break;
-      c = c2;
+  const int chunks = (p.K + 127) >> 7, mine = max(0, (chunks - wave + W - 1) / W);
+#pragma unroll
+  for (int j = 0; j < NS; ++j)
+    if (j < mine) issue(wave + j * W, j);
+  int slot = 0;
+#pragma unroll 1
+  for (int j = 0; j < mine; ++j) {
+    const int ahead = p.dma ? min(mine - 1 - j, NS - 1) : 0;
+    switch (ahead) {
+      case 0: XTK_WAIT_VM(0); break;
+      case 1: XTK_WAIT_VM(S::PER); break;
+      case 2: XTK_WAIT_VM(NS > 2 ? 2 * S::PER : 0); break;
+      default: XTK_WAIT_VM(NS > 3 ? 3 * S::PER : 0); break;
     }
+    asm volatile("" ::: "memory");
+    const unsigned char* const at = ring + slot * S::STAGE;
+    unsigned d[4], sc[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) sc[f] = *reinterpret_cast<const unsigned*>(at + S::S0 + col * 16 + f * 4);
+    uint4v xf[MT][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      d[t] = *reinterpret_cast<const unsigned*>(at + wfrag + ((t ^ wsw) << 4));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const unsigned char* const xp = at + xfrag + i * 256 * PIECES;
+        if constexpr (I8) {
+          const uint2v e = *reinterpret_cast<const uint2v*>(xp + (((2 * t + xpiece) ^ xsw) << 4));
+          xf[i][t] = uint4v{e[0], e[1], 0, 0};
+        } else {
+          xf[i][t] = *reinterpret_cast<const uint4v*>(xp + (((4 * t + xpiece) ^ xsw) << 4));
+        }
+      }
+    }
+    // every fragment is in registers before the slot is filled again
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (j + NS < mine) issue(wave + (j + NS) * W, slot);
+    slot = slot + 1 == NS ? 0 : slot + 1;
+    compute(d, xf, sc, wave + j * W);
   }
+  __syncthreads();  // every ring is done with
 
   // the waves' parts, summed in the order of the waves
+  float* const part = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) part[wave][i * NT + j][r][lane] = y[i][j][r];
+    for (int r = 0; r < 4; ++r) part[((wave * MT + i) * 4 + r) * 64 + lane] = y[i][r];
   __syncthreads();
   const long long y0 = p.ty.at(bx, by, bz), r0 = p.trs.at(bx, by, bz);
-  for (int e = threadIdx.x; e < NT * MT * 256; e += 64 * W) {
-    const int ij = e >> 8, r = (e >> 6) & 3, l = e & 63;
+  for (int e = threadIdx.x; e < MT * 256; e += 64 * W) {
+    const int i = e >> 8, r = (e >> 6) & 3, l = e & 63;
+    const int m = m0 + 16 * i + 4 * (l >> 4) + r, n = n0 + (l & 15);
+    if (m >= p.M || n >= p.N) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int u = 0; u < W; ++u) v += part[u][ij][r][l];
-    const int m = m0 + 16 * (ij / NT) + 4 * (l >> 4) + r, n = n0 + 16 * (ij % NT) + (l & 15);
-    if (m >= p.M || n >= p.N) continue;
+    for (int u = 0; u < W; ++u) v += part[u * MT * 256 + e];
     if (p.rs) v *= p.rs[r0 + m * p.ldrs];
     const long long at = y0 + m * p.ldy + n;
     if (p.y_elem == kF32) static_cast<float*>(p.y)[at] = v;
@@ -253,27 +299,32 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   }
 }
 
-template <int ELEM, int MT, int NT, int W>
+template <int ELEM, bool S32, int ROWS, int W, int NS>
 void run_fl(Q4Args& a, int wgs, hipStream_t s) {
-  a.d_group = div31(a.group / (a.group % 128 == 0 ? 128 : a.group % 64 == 0 ? 64 : 32));
-  if (a.group % 128 == 0) matmul_q4_kernel<ELEM, MT, NT, W, 4><<<wgs, 64 * W, 0, s>>>(a);
-  else if (a.group % 64 == 0) matmul_q4_kernel<ELEM, MT, NT, W, 2><<<wgs, 64 * W, 0, s>>>(a);
-  else matmul_q4_kernel<ELEM, MT, NT, W, 1><<<wgs, 64 * W, 0, s>>>(a);
+  const int fl = a.group % 128 == 0 ? 4 : a.group % 64 == 0 ? 2 : 1;
+  a.d_group = div31(a.group / (32 * fl));
+  if (fl == 4) matmul_q4_kernel<ELEM, ROWS, W, NS, 4, S32><<<wgs, 64 * W, 0, s>>>(a);
+  else if (fl == 2) matmul_q4_kernel<ELEM, ROWS, W, NS, 2, S32><<<wgs, 64 * W, 0, s>>>(a);
+  else matmul_q4_kernel<ELEM, ROWS, W, NS, 1, S32><<<wgs, 64 * W, 0, s>>>(a);
 }
 
-template <int ELEM>
+template <int ELEM, bool S32>
 bool run(Q4Args& a, long long blocks, hipStream_t s) {
-  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4, nt = 1, w = 8;
-  a.ntiles = (a.N + 16 * nt - 1) / (16 * nt);
-  const long long tiles = (long long)a.ntiles * ((a.M + 16 * mt - 1) / (16 * mt));
-  if (tiles > 0x7fffffffLL || !grid_fits(tiles * blocks, 64 * w)) return false;
+  constexpr int FEW = ELEM == kI8 ? 8 : 4;  // rows that one instruction brings
+  a.ntiles = (a.N + 15) / 16;
+  auto tiles_of = [&](int mt) { return (long long)a.ntiles * ((a.M + 16 * mt - 1) / (16 * mt)); };
+  int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  while (mt > 1 && tiles_of(mt) * blocks < 256) mt >>= 1;
+  const long long tiles = tiles_of(mt);
+  if (tiles > 0x7fffffffLL || !grid_fits(tiles * blocks, 512)) return false;
   a.tiles = (int)tiles;
   a.d_tiles = div31(a.tiles);
   a.d_nt = div31(a.ntiles);
   const int wgs = (int)(tiles * blocks);
-  if (mt == 1) run_fl<ELEM, 1, 1, 8>(a, wgs, s);
-  else if (mt == 2) run_fl<ELEM, 2, 1, 8>(a, wgs, s);
-  else run_fl<ELEM, 4, 1, 8>(a, wgs, s);
+  if (a.M <= FEW) run_fl<ELEM, S32, FEW, 8, 2>(a, wgs, s);
+  else if (mt == 1) run_fl<ELEM, S32, 16, 8, 2>(a, wgs, s);
+  else if (mt == 2) run_fl<ELEM, S32, 32, 4, 3>(a, wgs, s);
+  else run_fl<ELEM, S32, 64, 4, 2>(a, wgs, s);
   return true;
 }
 
@@ -308,14 +359,30 @@ hipError_t launch_matmul_q4(const xt::Plan& p, void* const* bufs, hipStream_t s,
   a.M = static_cast<int>(q.y.rows);
   a.N = static_cast<int>(q.y.cols);
   a.K = static_cast<int>(q.K);
-  a.chunks = (a.K + 127) / 128;
   a.group = static_cast<int>(q.group);
+  // DMA takes rows of whole 16 bytes; others go through registers
+  auto pieces = [&](const xt::Access2D& t, int per) {
+    const xt::TileAddr& d = t.addr;
+    return reinterpret_cast<uintptr_t>(bufs[t.arg]) % 16 == 0 && t.ld % per == 0 && d.c0 % per == 0 && d.sx % per == 0 &&
+           d.sy % per == 0 && d.sz % per == 0;
+  };
+  a.dma = pieces(q.x, q.x.elem == xt::Elem::I8 ? 16 : 8) && pieces(q.w, 16);
   a.s_elem = elem_of(q.scales.elem);
   a.y_elem = elem_of(q.y.elem);
+  // what a lane adds to its tile's address has 32 bits
+  auto apart = [](int rows, long long ld, int bytes) { return (long long)rows * ld * bytes < (1LL << 31); };
+  const int xs = q.x.elem == xt::Elem::I8 ? 1 : 2;
+  if (!apart(std::min(a.M, 64), a.ldx, xs) || !apart(std::min(a.N, 16), a.ldw, 1) ||
+      !apart(std::min(a.N, 16), a.lds, a.s_elem == kF32 ? 4 : 2)) {
+    why = "matmul_q4: rows that a workgroup reads together span 2^31 bytes or more";
+    return hipErrorInvalidValue;
+  }
   bool ok;
-  if (q.x.elem == xt::Elem::I8) ok = run<kI8>(a, grid_blocks(p), s);
-  else if (q.x.elem == xt::Elem::F16) ok = run<kF16>(a, grid_blocks(p), s);
-  else ok = run<kBF16>(a, grid_blocks(p), s);
+  const bool s32 = a.s_elem == kF32;
+  const long long blocks = grid_blocks(p);
+  if (q.x.elem == xt::Elem::I8) ok = s32 ? run<kI8, true>(a, blocks, s) : run<kI8, false>(a, blocks, s);
+  else if (q.x.elem == xt::Elem::F16) ok = s32 ? run<kF16, true>(a, blocks, s) : run<kF16, false>(a, blocks, s);
+  else ok = s32 ? run<kBF16, true>(a, blocks, s) : run<kBF16, false>(a, blocks, s);
   if (!ok) {
     why = "matmul_q4: " + std::to_string(a.M) + " x " + std::to_string(a.N) + " tiles exceed one launch";
     return hipErrorInvalidValue;
