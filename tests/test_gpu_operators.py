@@ -121,6 +121,14 @@ def test_rms_norm_unaligned(cuda):
     assert y[0] == 0 and bool((y[-2:] == 0).all())
 
 
+@pytest.mark.parametrize("over", [None, "x", "r"])
+@pytest.mark.parametrize("cols", [8, 9, 15, 511, 513, 1023, 2047, 4099, 8191, 9001])
+def test_rms_norm_rows_that_eight_does_not_divide(cuda, cols, over):
+    """A row's last vector begins inside its neighbour: it counts once, also in place."""
+    norm_case(cuda, 7, cols, "bf16", True, over == "x", over=over)
+    norm_case(cuda, 7, cols, "f32", True, over != "x", over=over, gamma="f16")
+
+
 def test_rms_norm_refuses_results_over_what_it_reads_elsewhere(cuda):
     import torch
 
@@ -192,6 +200,64 @@ def test_matmul_q4(cuda, m, n, k, group, dtype, out, scales):
     # the roundings of a sum do not all go one way: by their root mean square
     err = float((y.double() - want).norm() / want.norm())
     assert err <= ref.half_step(y) + 4e-6, err
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "i8"])
+@pytest.mark.parametrize("m,n,k,group", [(24, 4100, 224, 32), (50, 4090, 416, 32), (33, 4096, 384, 128), (130, 2060, 320, 64),
+                                         (5, 300, 32 * 131, 32), (9, 65, 96 * 41, 96)])
+def test_matmul_q4_exact_where_tiles_fill_the_card(cuda, m, n, k, group, dtype):
+    """Two and four tiles of rows to a workgroup, and rings that go round."""
+    test_matmul_q4_exact(cuda, m, n, k, group, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "i8"])
+@pytest.mark.parametrize("scales", ["f32", "f16"])
+@pytest.mark.parametrize("m", [1, 12, 40])
+def test_matmul_q4_of_pitched_rows(cuda, m, scales, dtype):
+    """Rows apart by more than they hold: by whole 16 bytes, and by an odd number, with
+    scales that begin at an odd element; what lies behind a row is NaN or never read."""
+    import torch
+
+    n, k, group = (4099, 160, 32) if m == 40 else (45, 160, 32)
+    x, w, s, _ = q4_inputs(cuda, m, n, k, group, dtype, scales, exact=True)
+    want, packed, el = ref.matmul_q4(x, w, s), xt.pack_q4(w), DSL[dtype]
+    for xp, wp in ((k + 32, k // 2 + 16), (k + 1, k // 2 + 3)):
+        sp = k // group + 2
+        xa, wa = xt.Array((m, xp), el), xt.Array((n, wp), xt.int8)
+        sa, ya = xt.Array((n, sp), DSL[scales]), xt.Array((m, n), xt.float32)
+
+        @xt.kernel
+        def parts(x, w, s, y):
+            t = xt.matmul_q4(xt.load(x, index=(0, 0), shape=(m, k)), xt.load(w, index=(0, 0), shape=(n, k // 2)),
+                             xt.load(s, index=(0, 0), shape=(n, k // group)))
+            xt.store(y, index=(0, 0), tile=t)
+
+        p = xt.convert(parts, args=(xa, wa, sa, ya), grid=(1, 1, 1))
+        bx = torch.full((m, xp), 99 if dtype == "i8" else math.nan, device=cuda).to(x.dtype)
+        bw = torch.full((n, wp), -1, dtype=torch.int8, device=cuda)
+        bs = torch.full((n * sp + 1,), math.nan, dtype=s.dtype, device=cuda)[1:].view(n, sp)
+        bx[:, :k], bw[:, : k // 2], bs[:, : k // group] = x, packed, s
+        y = torch.full((m, n), 7.0, device=cuda)
+        say(xt.plan(p)["kernel"], m, scales, dtype, xp, wp)
+        xt.launch(p, bx, bw, bs, y)
+        assert torch.equal(y.double(), want)
+
+
+def test_matmul_q4_refuses_rows_two_gigabytes_apart(cuda):
+    import torch
+
+    @xt.kernel
+    def part(x, w, s, y):
+        t = xt.matmul_q4(xt.load(x, index=(0, 0), shape=(2, 32)), xt.load(w, index=(0, 0), shape=(16, 16)),
+                         xt.load(s, index=(0, 0), shape=(16, 1)))
+        xt.store(y, index=(0, 0), tile=t)
+
+    x = torch.empty(2, 1 << 30, dtype=torch.float16, device=cuda)
+    w, s = torch.zeros(16, 16, dtype=torch.int8, device=cuda), torch.ones(16, 1, device=cuda)
+    p = xt.convert(part, args=(xt.Array(tuple(x.shape), xt.float16), xt.Array((16, 16), xt.int8),
+                               xt.Array((16, 1), xt.float32), xt.Array((2, 16), xt.float32)), grid=(1, 1, 1))
+    with pytest.raises(ValueError, match="2.31 bytes"):
+        xt.launch(p, x, w, s, torch.zeros(2, 16, device=cuda))
 
 
 def test_matmul_q4_of_parts_of_arrays(cuda):
@@ -336,6 +402,15 @@ def test_attend_rows_that_see_nothing(cuda, nq):
     assert bool((y == 0).all())
     y = attend_case(cuda, 1, 1, 1, nq, 70, 64, causal=True, window=5, start=[100])
     assert bool((y == 0).all()) and not torch.isnan(y).any()
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("nq,g", [(1, 1), (3, 4), (70, 1)])
+def test_attend_windows_split_by_themselves(cuda, d, nq, g):
+    """A window's keys alone are split, wherever in the cache it lies, or before it."""
+    attend_case(cuda, 4, 1, g, nq, 4100, d, "bf16", causal=True, window=1100, start=[4100 - nq, 30, 2000, -5000],
+                length=[4100, 4000, 1999, 4100])
+    attend_case(cuda, 3, 2, g, nq, 2100, d, "f16", causal=True, window=300, slopes=True, start=[2090, 0, 1111])
 
 
 def test_attend_extreme_positions(cuda):

@@ -369,11 +369,10 @@ hipError_t launch_matmul_q4(const xt::Plan& p, void* const* bufs, hipStream_t s,
   a.dma = pieces(q.x, q.x.elem == xt::Elem::I8 ? 16 : 8) && pieces(q.w, 16);
   a.s_elem = elem_of(q.scales.elem);
   a.y_elem = elem_of(q.y.elem);
-  // what a lane adds to its tile's address has 32 bits
-  auto apart = [](int rows, long long ld, int bytes) { return (long long)rows * ld * bytes < (1LL << 31); };
-  const int xs = q.x.elem == xt::Elem::I8 ? 1 : 2;
-  if (!apart(std::min(a.M, 64), a.ldx, xs) || !apart(std::min(a.N, 16), a.ldw, 1) ||
-      !apart(std::min(a.N, 16), a.lds, a.s_elem == kF32 ? 4 : 2)) {
+  // what a lane adds to its tile's address has 31 bits
+  auto near = [](int rows, long long ld, long long cols, int bytes) { return ((rows - 1) * ld + cols) * bytes < (1LL << 31); };
+  const int xs = q.x.elem == xt::Elem::I8 ? 1 : 2, ss = a.s_elem == kF32 ? 4 : 2, rows = std::min(a.N, 16);
+  if (!near(std::min(a.M, 64), a.ldx, 128, xs) || !near(rows, a.ldw, 64, 1) || !near(rows, a.lds, a.K / 32 + 1, ss)) {
     why = "matmul_q4: rows that a workgroup reads together span 2^31 bytes or more";
     return hipErrorInvalidValue;
   }
