@@ -2,7 +2,7 @@
 //   y[m, n] = rs[m] sum_g s[n, g] sum_{k in group g} x[m, k] w[n, k]
 //
 // The weights are read once and bound the kernel: x, of few rows, comes from L2.  A
-// workgroup takes 16 rows of weights and 16 MT rows of x; its waves split K in chunks
+// workgroup takes 16 NT rows of weights and 16 MT rows of x; its waves split K in chunks
 // of 128 and meet once, in LDS, in a fixed order.
 //
 // A wave brings a chunk's weights, rows of x and scales into a ring of its own in LDS
@@ -11,7 +11,9 @@
 // are of different rows, every load takes its 64 lookups in the cache apart: 16 rows of
 // int8 by 4096 x 11008 weights took 16.8 us so and take 9.7 us.  Two chunks in a ring
 // leave several workgroups on a CU; three and four are slower (11008 x 4096, groups of
-// 32: 11.8, 13.1 and 13.4 us), as are four waves for eight and sixteen (13.9, 16.1).
+// 32: 11.8, 13.1 and 13.4 us), as are four waves and sixteen in place of eight (13.9,
+// 16.1).  One token by 4096 x 4096 takes 5.8 us, by 11008 x 4096 10.7 (2.6 TB/s): with
+// 16 KB to 88 KB of weights for a CU, the way there and back is most of it.
 //
 // Of the fragments, x goes as the MFMA's rows and the weights as its columns, so a
 // lane's results are all of one weight row and take one scale; lane (n, q) has the
@@ -66,24 +68,24 @@ constexpr unsigned kNone = 1u << 31;  // an offset behind every row: such lanes 
 
 // What a workgroup of W waves holds.  ROWS: rows of x, of which the MFMA takes 16 at a
 // time (fewer are read again and again, for results that are not stored).
-template <bool I8, int ROWS, int W, int NS>
+template <bool I8, int ROWS, int NT, int W, int NS>
 struct Q4Shape {
   static constexpr int MT = ROWS <= 16 ? 1 : ROWS / 16;
   static constexpr int ES = I8 ? 1 : 2, PIECES = 8 * ES;  // pieces of 16 bytes in a row's 128 values
   // a stage: the weights, x, the scales; instructions that bring x, and all three
-  static constexpr int X0 = 1024, S0 = X0 + ROWS * PIECES * 16, STAGE = S0 + 256;
-  static constexpr int XI = ROWS * PIECES / 64, PER = XI + 2;
+  static constexpr int X0 = 1024 * NT, S0 = X0 + ROWS * PIECES * 16, STAGE = S0 + 256 * NT;
+  static constexpr int XI = ROWS * PIECES / 64, PER = XI + 2 * NT;
   static constexpr int LDS = W * NS * STAGE;
   static_assert(XI * 64 == ROWS * PIECES && LDS <= 160 * 1024 && NS >= 2 && NS <= 4 && (NS - 1) * PER < 64, "");
-  static_assert(W * MT * 1024 <= LDS, "the waves' parts take the rings' place");
+  static_assert(W * MT * NT * 1024 <= LDS, "the waves' parts take the rings' place");
 };
 
 // FL: steps of 32 between two additions to the result (1, 2 or 4): at most the group.
 // S32: scales of 32 bits.  NS: chunks in a wave's ring.
-template <int ELEM, int ROWS, int W, int NS, int FL, bool S32>
+template <int ELEM, int ROWS, int NT, int W, int NS, int FL, bool S32>
 __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   constexpr bool I8 = ELEM == kI8;
-  typedef Q4Shape<I8, ROWS, W, NS> S;
+  typedef Q4Shape<I8, ROWS, NT, W, NS> S;
   constexpr int ES = S::ES, MT = S::MT, XI = S::XI, PIECES = S::PIECES, NF = 4 / FL;
   typedef typename std::conditional<I8, int4v, float4v>::type acc_t;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[S::LDS];
@@ -96,7 +98,7 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   const int tm = (int)p.d_nt(tile), tn = tile - tm * p.ntiles;
   int bx, by, bz;
   p.blocks(b, bx, by, bz);
-  const int m0 = tm * 16 * MT, n0 = tn * 16;
+  const int m0 = tm * 16 * MT, n0 = tn * 16 * NT;
   const unsigned char* const w = p.w + p.tw.at(bx, by, bz) + n0 * p.ldw;
   const unsigned char* const x = p.x + (p.tx.at(bx, by, bz) + m0 * p.ldx) * ES;
 
@@ -104,7 +106,9 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   // lane / PIECES of each instruction's, piece (lane % PIECES) ^ row % 8.  Neighbours
   // read neighbours in memory, and fragments, of one piece of 16 rows, lie over all banks.
   const int wn = lane >> 2, wt = (lane & 3) ^ ((lane >> 3) & 3);
-  const unsigned wat = wn < p.N - n0 ? (unsigned)wn * (unsigned)p.ldw + wt * 16 : kNone;
+  unsigned wat[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) wat[n] = wn + 16 * n < p.N - n0 ? (unsigned)(wn + 16 * n) * (unsigned)p.ldw + wt * 16 : kNone;
   constexpr int XR = 64 / PIECES;  // rows of an instruction: 4 or 8
   unsigned xat[XI];
   const int xr = lane / PIECES;
@@ -120,8 +124,6 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   const unsigned char* const st = static_cast<const unsigned char*>(p.s) + ((p.ts.at(bx, by, bz) + n0 * p.lds) << (S32 ? 2 : 1));
   const unsigned odd = (unsigned)reinterpret_cast<uintptr_t>(st) & 3;  // 16 bits: 0 or 2
   const unsigned char* const s0 = st - odd;
-  const bool sany = wn < p.N - n0 && sf0 < NF;
-  const unsigned srow = (unsigned)wn * (unsigned)p.lds;
   unsigned char* const ring = lds + wave * NS * S::STAGE;
   auto issue = [&](int c, int slot) {
     unsigned char* const at = ring + slot * S::STAGE;
@@ -129,24 +131,37 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
     const unsigned char* const xc = x + (long long)c * 128 * ES;
     const int left = p.K - c * 128;  // pieces past it are zeros
     const bool whole = left >= 128;
-    const unsigned wo = whole || wt * 32 < left ? wat : kNone;
-    const unsigned so = ((srow + p.d_group((unsigned)(c * NF + sf0))) << (S32 ? 2 : 1)) + odd;
-    const bool sin = sany && sf0 * FL * 32 < left;
+    const unsigned group = p.d_group((unsigned)(c * NF + sf0));
+    unsigned wo[NT], so[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      wo[n] = whole || wt * 32 < left ? wat[n] : kNone;
+      const unsigned s = (((unsigned)(wn + 16 * n) * (unsigned)p.lds + group) << (S32 ? 2 : 1)) + odd;
+      so[n] = wn + 16 * n < p.N - n0 && sf0 < NF && sf0 * FL * 32 < left ? s & ~3u : kNone;
+    }
     if (p.dma) {
       // the low half of its generic address (a cast between address spaces compares with null first)
       const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>(at));
-      dma16(raw_rsrc(wc, kNone), to, wo, 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) dma16(raw_rsrc(wc, kNone), to + 1024 * n, wo[n], 0);
       const i32x4 rs = raw_rsrc(xc, kNone);
 #pragma unroll
       for (int i = 0; i < XI; ++i) {
         const int k = ((lane % PIECES) ^ ((i * XR + xr) & 7)) * (16 / ES);
         dma16(rs, to + S::X0 + 1024 * i, whole || k < left ? xat[i] : kNone, 0);
       }
-      dma4(raw_rsrc(s0, kNone), to + S::S0, sin ? so & ~3u : kNone);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) dma4(raw_rsrc(s0, kNone), to + S::S0 + 256 * n, so[n]);
     } else {
-      uint4v v = {0, 0, 0, 0};
-      if (wo < kNone) v = (uint4v)(*reinterpret_cast<const u4a*>(wc + wo));
-      *reinterpret_cast<uint4v*>(at + lane * 16) = v;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint4v v = {0, 0, 0, 0};
+        if (wo[n] < kNone) v = (uint4v)(*reinterpret_cast<const u4a*>(wc + wo[n]));
+        *reinterpret_cast<uint4v*>(at + 1024 * n + lane * 16) = v;
+        unsigned e = 0;
+        if (so[n] < kNone) e = *reinterpret_cast<const unsigned*>(s0 + so[n]);
+        *reinterpret_cast<unsigned*>(at + S::S0 + 256 * n + lane * 4) = e;
+      }
 #pragma unroll
       for (int i = 0; i < XI; ++i) {
         const int k = ((lane % PIECES) ^ ((i * XR + xr) & 7)) * (16 / ES);
@@ -154,15 +169,14 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
         if (xat[i] < kNone && k < left) u = (uint4v)(*reinterpret_cast<const u4a*>(xc + xat[i]));
         *reinterpret_cast<uint4v*>(at + S::X0 + 1024 * i + lane * 16) = u;
       }
-      unsigned e = 0;
-      if (sin) e = *reinterpret_cast<const unsigned*>(s0 + (so & ~3u));
-      *reinterpret_cast<unsigned*>(at + S::S0 + lane * 4) = e;
     }
   };
 
-  float4v y[MT];
+  float4v y[MT][NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) y[i] = float4v{0, 0, 0, 0};
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) y[i][n] = float4v{0, 0, 0, 0};
 
   // where this lane's fragments lie in a stage: a word of weights, and of x the piece of
   // a row's step, in which int8 rows have two quarters' eight bytes
@@ -174,27 +188,37 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   const bool f16_scales = f16 != 0;
   const unsigned srow_col = (unsigned)col * (unsigned)p.lds + (odd >> 1);
 
-  auto compute = [&](const unsigned (&d)[4], const uint4v (&xf)[MT][4], const unsigned (&sc)[NF], int c) {
+  auto compute = [&](const unsigned (&d)[NT][4], const uint4v (&xf)[MT][4], const unsigned (&sc)[NT][NF], int c) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       // one step: its correction is where its products begin; more: two sums side by side
       constexpr bool CHAIN = FL == 1;
-      acc_t acc[MT], off[MT];
+      acc_t acc[MT][NT], off[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = off[i] = acc_t{0, 0, 0, 0};
+      for (int i = 0; i < MT; ++i) {
+        off[i] = acc_t{0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[i][n] = acc_t{0, 0, 0, 0};
+      }
 #pragma unroll
       for (int u = 0; u < FL; ++u) {
         const int t = f * FL + u;
         if constexpr (I8) {
           const long eights = CHAIN ? (long)0xf8f8f8f8f8f8f8f8UL : 0x0808080808080808L;
-          const long wj = (long)(((unsigned long)((d[t] >> 4) & 0x0f0f0f0fu) << 32) | (d[t] & 0x0f0f0f0fu));
+          long xi[MT];
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             const unsigned lo = __builtin_amdgcn_perm(xf[i][t][1], xf[i][t][0], 0x05010400u);
             const unsigned hi = __builtin_amdgcn_perm(xf[i][t][1], xf[i][t][0], 0x07030602u);
-            const long xi = (long)(((unsigned long)hi << 32) | lo);
-            off[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xi, eights, off[i], 0, 0, 0);
-            acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xi, wj, CHAIN ? off[i] : acc[i], 0, 0, 0);
+            xi[i] = (long)(((unsigned long)hi << 32) | lo);
+            off[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xi[i], eights, off[i], 0, 0, 0);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const long wj = (long)(((unsigned long)((d[n][t] >> 4) & 0x0f0f0f0fu) << 32) | (d[n][t] & 0x0f0f0f0fu));
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+              acc[i][n] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xi[i], wj, CHAIN ? off[i] : acc[i][n], 0, 0, 0);
           }
         } else {
           // 16 + u: f16 0x4c00 | u << 6, bf16 0x4180 | u << 3
@@ -207,29 +231,36 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
             else
               return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, bb), c, 0, 0, 0);
           };
-          uint4v v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = ((up >= 4 * e ? d[t] << (up - 4 * e) : d[t] >> (4 * e - up)) & mask) | one;
+          for (int i = 0; i < MT; ++i) off[i] = mma(xf[i][t], uint4v{c24, c24, c24, c24}, off[i]);
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            off[i] = mma(xf[i][t], uint4v{c24, c24, c24, c24}, off[i]);
-            acc[i] = mma(xf[i][t], v, CHAIN ? off[i] : acc[i]);
+          for (int n = 0; n < NT; ++n) {
+            uint4v v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = ((up >= 4 * e ? d[n][t] << (up - 4 * e) : d[n][t] >> (4 * e - up)) & mask) | one;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i][n] = mma(xf[i][t], v, CHAIN ? off[i] : acc[i][n]);
           }
         }
       }
-      float sf;
-      if constexpr (S32) {
-        sf = __builtin_bit_cast(float, sc[f]);
-      } else {
-        const unsigned half = sc[f] >> (((srow_col + p.d_group((unsigned)(c * NF + f))) & 1) * 16);
-        const float h = (float)__builtin_bit_cast(_Float16, (unsigned short)half), b = __builtin_bit_cast(float, half << 16);
-        sf = f16_scales ? h : b;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float sf;
+        if constexpr (S32) {
+          sf = __builtin_bit_cast(float, sc[n][f]);
+        } else {
+          // rows 16 apart begin in the same half of their four bytes
+          const unsigned half = sc[n][f] >> (((srow_col + p.d_group((unsigned)(c * NF + f))) & 1) * 16);
+          const float h = (float)__builtin_bit_cast(_Float16, (unsigned short)half), b = __builtin_bit_cast(float, half << 16);
+          sf = f16_scales ? h : b;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            y[i][n][r] = fmaf((float)(CHAIN ? acc[i][n][r] : acc[i][n][r] - off[i][r]), sf, y[i][n][r]);
       }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[i][r] = fmaf((float)(CHAIN ? acc[i][r] : acc[i][r] - off[i][r]), sf, y[i][r]);
     }
   };
 
@@ -249,13 +280,16 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
     }
     asm volatile("" ::: "memory");
     const unsigned char* const at = ring + slot * S::STAGE;
-    unsigned d[4], sc[NF];
+    unsigned d[NT][4], sc[NT][NF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) sc[f] = *reinterpret_cast<const unsigned*>(at + S::S0 + col * 16 + f * 4);
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int f = 0; f < NF; ++f) sc[n][f] = *reinterpret_cast<const unsigned*>(at + S::S0 + 256 * n + col * 16 + f * 4);
     uint4v xf[MT][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      d[t] = *reinterpret_cast<const unsigned*>(at + wfrag + ((t ^ wsw) << 4));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) d[n][t] = *reinterpret_cast<const unsigned*>(at + 1024 * n + wfrag + ((t ^ wsw) << 4));
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const unsigned char* const xp = at + xfrag + i * 256 * PIECES;
@@ -281,16 +315,18 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) part[((wave * MT + i) * 4 + r) * 64 + lane] = y[i][r];
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) part[(((wave * MT + i) * NT + n) * 4 + r) * 64 + lane] = y[i][n][r];
   __syncthreads();
   const long long y0 = p.ty.at(bx, by, bz), r0 = p.trs.at(bx, by, bz);
-  for (int e = threadIdx.x; e < MT * 256; e += 64 * W) {
-    const int i = e >> 8, r = (e >> 6) & 3, l = e & 63;
-    const int m = m0 + 16 * i + 4 * (l >> 4) + r, n = n0 + (l & 15);
+  for (int e = threadIdx.x; e < MT * NT * 256; e += 64 * W) {
+    const int i = e / (256 * NT), j = (e >> 8) % NT, r = (e >> 6) & 3, l = e & 63;
+    const int m = m0 + 16 * i + 4 * (l >> 4) + r, n = n0 + 16 * j + (l & 15);
     if (m >= p.M || n >= p.N) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int u = 0; u < W; ++u) v += part[u * MT * 256 + e];
+    for (int u = 0; u < W; ++u) v += part[u * MT * NT * 256 + e];
     if (p.rs) v *= p.rs[r0 + m * p.ldrs];
     const long long at = y0 + m * p.ldy + n;
     if (p.y_elem == kF32) static_cast<float*>(p.y)[at] = v;
@@ -299,32 +335,42 @@ __global__ __launch_bounds__(64 * W) void matmul_q4_kernel(Q4Args p) {
   }
 }
 
-template <int ELEM, bool S32, int ROWS, int W, int NS>
+template <int ELEM, bool S32, int ROWS, int NT, int W, int NS>
 void run_fl(Q4Args& a, int wgs, hipStream_t s) {
   const int fl = a.group % 128 == 0 ? 4 : a.group % 64 == 0 ? 2 : 1;
   a.d_group = div31(a.group / (32 * fl));
-  if (fl == 4) matmul_q4_kernel<ELEM, ROWS, W, NS, 4, S32><<<wgs, 64 * W, 0, s>>>(a);
-  else if (fl == 2) matmul_q4_kernel<ELEM, ROWS, W, NS, 2, S32><<<wgs, 64 * W, 0, s>>>(a);
-  else matmul_q4_kernel<ELEM, ROWS, W, NS, 1, S32><<<wgs, 64 * W, 0, s>>>(a);
+  if (fl == 4) matmul_q4_kernel<ELEM, ROWS, NT, W, NS, 4, S32><<<wgs, 64 * W, 0, s>>>(a);
+  else if (fl == 2) matmul_q4_kernel<ELEM, ROWS, NT, W, NS, 2, S32><<<wgs, 64 * W, 0, s>>>(a);
+  else matmul_q4_kernel<ELEM, ROWS, NT, W, NS, 1, S32><<<wgs, 64 * W, 0, s>>>(a);
 }
 
 template <int ELEM, bool S32>
 bool run(Q4Args& a, long long blocks, hipStream_t s) {
   constexpr int FEW = ELEM == kI8 ? 8 : 4;  // rows that one instruction brings
-  a.ntiles = (a.N + 15) / 16;
-  auto tiles_of = [&](int mt) { return (long long)a.ntiles * ((a.M + 16 * mt - 1) / (16 * mt)); };
+  auto tiles_of = [&](int mt, int nt) {
+    return (long long)((a.N + 16 * nt - 1) / (16 * nt)) * ((a.M + 16 * mt - 1) / (16 * mt));
+  };
+  // As many rows of x to a workgroup as leave one for every CU.  64 rows of 16 bits are
+  // sixteen times their weights' bytes, from L2: there a workgroup takes 32 rows of
+  // weights if three quarters of the CUs still get one (42 rows by 7906 x 8192: 26.6 us,
+  // with 16 rows 37; fewer rows of x, or of int8, are better off with twice the
+  // workgroups: 24 by 11008 x 4096 18.1 us against 20.8).
   int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-  while (mt > 1 && tiles_of(mt) * blocks < 256) mt >>= 1;
-  const long long tiles = tiles_of(mt);
+  while (mt > 1 && tiles_of(mt, 1) * blocks < 256) mt >>= 1;
+  const int nt = ELEM != kI8 && mt == 4 && tiles_of(mt, 2) * blocks >= 192 ? 2 : 1;
+  const long long tiles = tiles_of(mt, nt);
   if (tiles > 0x7fffffffLL || !grid_fits(tiles * blocks, 512)) return false;
   a.tiles = (int)tiles;
+  a.ntiles = (a.N + 16 * nt - 1) / (16 * nt);
   a.d_tiles = div31(a.tiles);
   a.d_nt = div31(a.ntiles);
   const int wgs = (int)(tiles * blocks);
-  if (a.M <= FEW) run_fl<ELEM, S32, FEW, 8, 2>(a, wgs, s);
-  else if (mt == 1) run_fl<ELEM, S32, 16, 8, 2>(a, wgs, s);
-  else if (mt == 2) run_fl<ELEM, S32, 32, 4, 3>(a, wgs, s);
-  else run_fl<ELEM, S32, 64, 4, 2>(a, wgs, s);
+  if (a.M <= FEW) run_fl<ELEM, S32, FEW, 1, 8, 2>(a, wgs, s);
+  else if (mt == 1) run_fl<ELEM, S32, 16, 1, 8, 2>(a, wgs, s);
+  else if (mt == 2) run_fl<ELEM, S32, 32, 1, 8, ELEM == kI8 ? 3 : 2>(a, wgs, s);
+  else if constexpr (ELEM == kI8) run_fl<ELEM, S32, 64, 1, 8, 2>(a, wgs, s);
+  else if (nt == 1) run_fl<ELEM, S32, 64, 1, 4, 2>(a, wgs, s);
+  else run_fl<ELEM, S32, 64, 2, 4, 2>(a, wgs, s);
   return true;
 }
 
