@@ -299,6 +299,25 @@ def test_matmul_q4_unaligned_and_not_finite(cuda):
     assert bool(torch.isnan(y[1]).all()) and torch.equal(y[[0, 2]].double(), ref.matmul_q4(x, w, s)[[0, 2]])
 
 
+@pytest.mark.parametrize("m", [3, 20])
+def test_matmul_q4_large_and_infinite_values(cuda, m):
+    """Up to 2^115 a row's sums are held; an infinity makes its row NaN."""
+    import torch
+
+    p = K.matmul_q4(m, 33, 256, group=128, dtype=xt.bfloat16, scales=xt.float32, out=xt.float32)
+    x, w, s, _ = q4_inputs(cuda, m, 33, 256, 128, "bf16", "f32", exact=True)
+    s *= 2.0**-20
+    x[1] *= 2.0**113
+    y = torch.full((m, 33), 7.0, device=cuda)
+    xt.launch(p, x, xt.pack_q4(w), s, y)
+    assert torch.equal(y.double(), ref.matmul_q4(x, w, s))
+    x[2, 250] = math.inf
+    xt.launch(p, x, xt.pack_q4(w), s, y)
+    assert bool(torch.isnan(y[2]).all())
+    y[2], x[2] = 0, 0
+    assert torch.equal(y.double(), ref.matmul_q4(x, w, s))
+
+
 def test_matmul_q4_refuses_a_result_over_an_operand(cuda):
     import torch
 
@@ -402,6 +421,34 @@ def test_attend_rows_that_see_nothing(cuda, nq):
     assert bool((y == 0).all())
     y = attend_case(cuda, 1, 1, 1, nq, 70, 64, causal=True, window=5, start=[100])
     assert bool((y == 0).all()) and not torch.isnan(y).any()
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("nk", [193, 257, 321, 640])
+def test_attend_rows_whose_keys_two_groups_of_waves_share(cuda, nk, d):
+    """An odd number of tiles, groups without a visible tile, and rows without a key."""
+    attend_case(cuda, 1, 2, 1, 150, nk, d, "bf16")
+    attend_case(cuda, 3, 1, 2, 90, nk, d, "f16", causal=True, start=[nk - 90, -20, 40], length=[nk, nk - 1, 30],
+                slopes=True)
+    docs = [[t // 70 for t in range(nk)]] * 2
+    attend_case(cuda, 2, 1, 1, nk, nk, d, "bf16", causal=True, docs=(docs, docs), prefix=[3, 200], over_q=True)
+
+
+@pytest.mark.parametrize("n", [200, 500])
+def test_attend_infinite_values_where_two_groups_of_waves_share_keys(cuda, n):
+    """Values of both groups' tiles that earlier rows do not see."""
+    import torch
+
+    q, k, v = (rand((1, 1, n, 64), "f16", cuda, s) for s in (1, 2, 3))
+    v[0, 0, 40, 3], v[0, 0, 90, 4], v[0, 0, 130, 5], v[0, 0, n - 1, 6] = math.inf, -math.inf, math.nan, math.nan
+    p = K.masked_attention(1, 1, 1, n, n, 64, dtype=xt.float16, causal=True)
+    o = torch.zeros_like(q)
+    xt.launch(p, q, k, v, o)
+    o = o[0, 0].float()
+    assert bool(torch.isfinite(o[:40]).all()) and bool((o[40:, 3] == math.inf).all())
+    assert bool(torch.isfinite(o[:90, 4]).all()) and bool((o[90:, 4] == -math.inf).all())
+    assert bool(torch.isfinite(o[:130, 5]).all()) and bool(torch.isnan(o[130:, 5]).all())
+    assert bool(torch.isfinite(o[:-1, 6]).all()) and bool(torch.isnan(o[-1, 6])) and bool(torch.isfinite(o[:, 7:]).all())
 
 
 @pytest.mark.parametrize("d", [32, 64, 128, 256])

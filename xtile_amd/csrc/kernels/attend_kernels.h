@@ -737,21 +737,24 @@ __device__ __forceinline__ bool any_wave(bool x, unsigned char* lds) {
   return __builtin_amdgcn_readfirstlane(any) != 0;
 }
 
-// More than 32 rows: 128 of them, 32 a wave, the keys in tiles of 64 that the waves
-// share, two of them in LDS.
-template <int D, bool BF16>
-__global__ __launch_bounds__(256, D <= 64 ? 3 : D <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs p, long long all_rows) {
+// More than 32 rows: 128 of them, 32 a wave, the keys in tiles of 64 that four waves
+// share, two of them in LDS.  G groups of four waves have the same rows and take tiles
+// in turn, and the second's results join the first's: where workgroups are so few that
+// a SIMD would have one wave, whose products and arithmetic wait for each other.
+template <int D, bool BF16, int G>
+__global__ __launch_bounds__(256 * G, G == 2 ? 2 : D <= 64 ? 3 : D <= 128 ? 2 : 1)
+void attend_rows_kernel(AttendArgs p, long long all_rows) {
   constexpr int BN = 64, KB = BN * D * 2, STAGE = 2 * KB + 256;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * G * STAGE];
   const bool dma = p.dma;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int every = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = every & 3, group = G == 1 ? 0 : every >> 2;
   const BlockAt b = block_at(p);
   const int first = b.tile * 128, last = min(first + 127, p.rows - 1);
   const int t0 = (int)p.d_heads((unsigned)first), t1 = (int)p.d_heads((unsigned)last);
   const int* const kdocs = p.kdocs ? p.kdocs + p.tkdocs.at(b.x, b.y, b.z) : nullptr;
   int d0 = 0, d1 = b.len;
   if (kdocs)
-    document_keys<4>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, t0, t1, last_key(p, b, t1), reinterpret_cast<int*>(lds),
+    document_keys<4 * G>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, t0, t1, last_key(p, b, t1), reinterpret_cast<int*>(lds),
                      d0, d1);
   const Tiles tiles = tiles_of(p, BN, b.start + t0, b.start + t1, b.len, b.pre, d0, d1);
   const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
@@ -767,26 +770,58 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : D <= 128 ? 2 : 1) void attend_ro
     fv.issue(dma, key0, left, at + KB);
     if (kdocs) dma4(raw_rsrc(kdocs + key0, (unsigned)min(left, BN) * 4), lds_at(at + 2 * KB), (threadIdx.x & 63) * 4);
   };
-  if (i0 < i1) issue(i0, lds);
+  unsigned char* const stages = lds + group * 2 * STAGE;
+  if (i0 + group < i1) issue(i0 + group, stages);
   Rows<D, BF16> rows;
   rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start);
 #pragma unroll 1
-  for (int i = i0; i < i1; ++i) {
+  for (int i = i0 + group, n = 0; i - group < i1; i += G, n ^= 1) {
     // one barrier a tile: behind it this tile has landed, and every wave is done with
     // the one before, whose place the next one takes while this one is worked on
-    unsigned char* const at = lds + ((i - i0) & 1) * STAGE;
+    unsigned char* const at = stages + n * STAGE;
     XTK_WAIT_VM(0);
     lds_barrier();
-    if (i + 1 < i1) issue(i + 1, lds + ((i + 1 - i0) & 1) * STAGE);
+    if (i + G < i1) issue(i + G, stages + (n ^ 1) * STAGE);
+    if (G > 1 && i >= i1) continue;
     const int key0 = tiles.at(i) * BN;
     if (!rows.sees_none(p, key0, BN, b.pre))
       rows.template tile<2>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len, b.pre);
   }
   rows.hold();
   lds_barrier();
-  if (any_wave<4>(rows.spoilt(), lds)) {
-    odd_rows<D, BF16>(p, b, tiles, BN, i0, i1, kdocs, first + wave, last + 1, 4, all_rows);
+  if (any_wave<4 * G>(rows.spoilt(), lds)) {
+    odd_rows<D, BF16>(p, b, tiles, BN, i0, i1, kdocs, first + every, last + 1, 4 * G, all_rows);
     return;
+  }
+  if constexpr (G == 2) {
+    // behind what the rows leave through below
+    float* const theirs = reinterpret_cast<float*>(lds + 4 * 32 * (2 * D + 16)) + wave * (32 * D + 128);
+    static_assert(4 * 32 * (2 * D + 16) + 4 * (32 * D + 128) * 4 <= 2 * G * STAGE, "the second group's results");
+    if (group == 1) {
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          *reinterpret_cast<float4v*>(theirs + (4 * n + w) * 256 + rows.lane * 4) =
+              float4v{rows.acc[n][4 * w], rows.acc[n][4 * w + 1], rows.acc[n][4 * w + 2], rows.acc[n][4 * w + 3]};
+      theirs[32 * D + rows.lane] = rows.m;
+      theirs[32 * D + 64 + rows.lane] = rows.l;
+    }
+    __syncthreads();
+    if (group == 1) return;
+    const float m1 = theirs[32 * D + rows.lane], l1 = theirs[32 * D + 64 + rows.lane];
+    const float m = fmaxf(rows.m, m1), use = m == -__builtin_inff() ? 0.0f : m;
+    const float a0 = __builtin_amdgcn_exp2f(rows.m - use), a1 = __builtin_amdgcn_exp2f(m1 - use);
+    rows.m = m;
+    rows.l = rows.l * a0 + l1 * a1;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4v o = *reinterpret_cast<const float4v*>(theirs + (4 * n + w) * 256 + rows.lane * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rows.acc[n][4 * w + e] = rows.acc[n][4 * w + e] * a0 + o[e] * a1;
+      }
   }
 
   const float l = both_halves(rows.l, false);
@@ -1038,11 +1073,19 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs p, long lon
   store4<BF16>(p, b, r, d, o[0], o[1], o[2], o[3]);
 }
 
+// Whether two groups of waves share the rows' keys: where there is no second workgroup
+// for a CU, nor a split that would fill it, and each group gets two tiles at least (577
+// keys, 160 workgroups of 96 columns: 17.6 -> 16.6 us; 332 keys of 32: 15.5 -> 11.5; of
+// 135 keys 9.6 -> 10.6; a split of 1520 keys in five 19.8 -> 21.1).
+inline bool pairs_of(const AttendArgs& a, int d) { return d <= 128 && a.nwg <= 256 && a.splits == 1 && a.keys > 192; }
+
 template <int D, bool BF16>
 hipError_t run_attend_elem(bool few, const AttendArgs& a, hipStream_t s) {
   const long long blocks = a.nwg / ((long long)a.tiles * a.splits), all_rows = blocks * a.rows;
   if (few) attend_few_kernel<D, BF16><<<a.nwg, 64 * Few<D>::W, 0, s>>>(a, all_rows);
-  else attend_rows_kernel<D, BF16><<<a.nwg, 256, 0, s>>>(a, all_rows);
+  else if (pairs_of(a, D)) {
+    if constexpr (D <= 128) attend_rows_kernel<D, BF16, 2><<<a.nwg, 512, 0, s>>>(a, all_rows);
+  } else attend_rows_kernel<D, BF16, 1><<<a.nwg, 256, 0, s>>>(a, all_rows);
   if (a.splits > 1) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

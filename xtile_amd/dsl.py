@@ -900,7 +900,8 @@ def matmul_q4(value, weight, scales, *, row_scale=None, dtype: DType = float32):
     """`value @ w.T` with 4-bit weights: value (M, K), weight (N, K / 2) int8 as
     `pack_q4` lays them out, scales (N, K / G) with one scale a group of G weights
     of a row.  `row_scale` (M, 1) multiplies the rows of the result: with the int8
-    rows of `quantize` it is their scale."""
+    rows of `quantize` it is their scale.  Sums are held in 32 bits, of values up to
+    2**115; a row of `value` with an infinity or NaN is NaN."""
     return _trace("matmul_q4").matmul_q4(value, weight, scales, row_scale=row_scale, dtype=dtype)
 
 
