@@ -423,6 +423,32 @@ def test_attend_rows_that_see_nothing(cuda, nq):
     assert bool((y == 0).all()) and not torch.isnan(y).any()
 
 
+@pytest.mark.parametrize("n,d", [(1, 64), (20, 96), (300, 128)])
+def test_attend_one_tensor_for_queries_keys_and_values(cuda, n, d):
+    import torch
+
+    x = rand((2, 1, n, d), "bf16", cuda, 5)
+    p = K.masked_attention(2, 1, 1, n, n, d, causal=True)
+    o = torch.zeros_like(x)
+    xt.launch(p, x, x, x, o)
+    want, far = ref.attend(x, x, x, 1 / math.sqrt(d), causal=True)
+    ref.assert_within(o, want, far)
+    with pytest.raises(ValueError, match="meets buffer"):
+        xt.launch(p, x, x, x, x)
+
+
+def test_rms_norm_of_a_tensor_added_to_itself(cuda):
+    import torch
+
+    m = K.rms_norm(6, 1003, xt.float32)
+    x, g = rand((6, 1003), "f32", cuda, 1), rand((1, 1003), "f32", cuda, 2)
+    want_h, want = ref.rms_norm(x, x, g, 1e-6)
+    y = torch.zeros_like(x)
+    xt.launch(m, x, x, g, x, y)  # the sum over both
+    assert torch.equal(x.double(), want_h)
+    ref.assert_within(y, want, want.abs() * 40 * 2.0**-24 + 1e-37)
+
+
 @pytest.mark.parametrize("d", [32, 64, 96, 128])
 @pytest.mark.parametrize("nk", [193, 257, 321, 640])
 def test_attend_rows_whose_keys_two_groups_of_waves_share(cuda, nk, d):

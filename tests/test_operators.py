@@ -66,6 +66,19 @@ def test_work_of_plans():
     assert p["flops"] == 4 * 64 * 15
 
 
+def test_buffers_below_element_alignment_are_refused():
+    """Before anything is launched: the addresses are not those of any memory."""
+    from xtile_amd import _xtile
+
+    m = K.matmul_q4(1, 64, 64, group=32, dtype=xt.float16, scales=xt.float32)
+    sizes = [128, 64 * 32, 64 * 2 * 4, 64 * 4]
+    for k, at in ((0, 4097), (2, 4098), (3, 4098)):
+        ptrs = [4096] * 4
+        ptrs[k] = at
+        with pytest.raises(ValueError, match=f"buffer {k} is not aligned"):
+            _xtile.launch(m, None, ptrs, sizes, 0)
+
+
 def test_workspace():
     """Few rows over many keys work in one; the C ABI says how large."""
     assert xt.workspace(K.masked_attention(1, 8, 4, 4096, 4096, 128)) == 0

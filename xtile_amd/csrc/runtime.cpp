@@ -59,6 +59,17 @@ int get_plan(xt_module* m, const std::string& func, std::shared_ptr<const xt::Pl
   return XT_OK;
 }
 
+// A C entry's body: an exception (memory ran out while planning) becomes a status.
+template <class F>
+int guarded(char** err, F body) {
+  try {
+    return body();
+  } catch (const std::exception& e) {
+    if (err) *err = nullptr;
+    return fail(err, XT_ERR_DEVICE, e.what());
+  }
+}
+
 // Enqueues a plan over buffers known to hold its memrefs.  `work` is its workspace,
 // or null.
 int run_plan(const xt::Plan& p, void* const* bufs, void* work, size_t work_bytes, void* stream, char** err) {
@@ -70,6 +81,11 @@ int run_plan(const xt::Plan& p, void* const* bufs, void* work, size_t work_bytes
     return fail(err, XT_ERR_ARGUMENT,
                 "@" + p.func + " works in " + std::to_string(p.workspace) + " bytes at a multiple of 16, got " +
                     std::to_string(work_bytes));
+  // these kernels take any element alignment, and none below it
+  if (p.kind == xt::PlanKind::RmsNorm || p.kind == xt::PlanKind::MatmulQ4 || p.kind == xt::PlanKind::Attend)
+    for (size_t k = 0; k < p.arg_types.size(); ++k)
+      if (reinterpret_cast<uintptr_t>(bufs[k]) % xt::elem_bytes(p.arg_types[k].elem))
+        return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is not aligned to its elements");
   switch (p.kind) {
     case xt::PlanKind::EwBinary: e = xtk::launch_ew_binary(p, bufs, s, why); break;
     case xt::PlanKind::RowSoftmax: e = xtk::launch_row_softmax(p, bufs, s, why); break;
@@ -213,11 +229,13 @@ int xt_plan(xt_module* m, const char* func, char** out_desc, double* algo_bytes,
 
 int xt_workspace_bytes(xt_module* m, const char* func, size_t* bytes, char** err) {
   if (!m || !bytes) return fail(err, XT_ERR_TYPE, "expected an xtile module");
-  std::shared_ptr<const xt::Plan> plan;
-  std::lock_guard<std::mutex> lock(m->mu);
-  int st = get_plan(m, func_key(func), plan, err);
-  if (st == XT_OK) *bytes = static_cast<size_t>(plan->workspace);
-  return st;
+  return guarded(err, [&] {
+    std::shared_ptr<const xt::Plan> plan;
+    std::lock_guard<std::mutex> lock(m->mu);
+    int st = get_plan(m, func_key(func), plan, err);
+    if (st == XT_OK) *bytes = static_cast<size_t>(plan->workspace);
+    return st;
+  });
 }
 
 int xt_gpu_run(xt_module* m, const char* func, void* const* bufs, const size_t* buf_bytes,
@@ -232,54 +250,58 @@ int xt_gpu_run_buffers(xt_module* m, const char* func, const xt_buffer* bufs, in
 int xt_gpu_run_with(xt_module* m, const char* func, void* const* bufs, const size_t* buf_bytes, int nbufs, void* work,
                     size_t work_bytes, void* stream, char** err) {
   if (!m) return fail(err, XT_ERR_TYPE, "expected an xtile module");
-  std::shared_ptr<const xt::Plan> plan;
-  {
-    std::lock_guard<std::mutex> lock(m->mu);
-    int st = get_plan(m, func_key(func), plan, err);
-    if (st != XT_OK) return st;
-  }
-  const xt::Plan& p = *plan;
-  if (nbufs != static_cast<int>(p.arg_types.size()))
-    return fail(err, XT_ERR_ARGUMENT,
-                "@" + p.func + " takes " + std::to_string(p.arg_types.size()) +
-                    " buffers, got " + std::to_string(nbufs));
-  if (!bufs || !buf_bytes) return fail(err, XT_ERR_ARGUMENT, "null buffer list");
-  for (int k = 0; k < nbufs; ++k) {
-    const xt::Type& t = p.arg_types[k];
-    size_t need = static_cast<size_t>(t.numel()) * xt::elem_bytes(t.elem);
-    if (!bufs[k]) return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is null");
-    if (buf_bytes[k] < need)
+  return guarded(err, [&]() -> int {
+    std::shared_ptr<const xt::Plan> plan;
+    {
+      std::lock_guard<std::mutex> lock(m->mu);
+      int st = get_plan(m, func_key(func), plan, err);
+      if (st != XT_OK) return st;
+    }
+    const xt::Plan& p = *plan;
+    if (nbufs != static_cast<int>(p.arg_types.size()))
       return fail(err, XT_ERR_ARGUMENT,
-                  "buffer " + std::to_string(k) + " holds " + std::to_string(buf_bytes[k]) +
-                      " bytes; " + t.str() + " needs " + std::to_string(need));
-  }
-  return run_plan(p, bufs, work, work_bytes, stream, err);
+                  "@" + p.func + " takes " + std::to_string(p.arg_types.size()) +
+                      " buffers, got " + std::to_string(nbufs));
+    if (!bufs || !buf_bytes) return fail(err, XT_ERR_ARGUMENT, "null buffer list");
+    for (int k = 0; k < nbufs; ++k) {
+      const xt::Type& t = p.arg_types[k];
+      size_t need = static_cast<size_t>(t.numel()) * xt::elem_bytes(t.elem);
+      if (!bufs[k]) return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is null");
+      if (buf_bytes[k] < need)
+        return fail(err, XT_ERR_ARGUMENT,
+                    "buffer " + std::to_string(k) + " holds " + std::to_string(buf_bytes[k]) +
+                        " bytes; " + t.str() + " needs " + std::to_string(need));
+    }
+    return run_plan(p, bufs, work, work_bytes, stream, err);
+  });
 }
 
 int xt_gpu_run_buffers_with(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, void* work,
                             size_t work_bytes, void* stream, char** err) {
   if (!m) return fail(err, XT_ERR_TYPE, "expected an xtile module");
-  std::shared_ptr<const xt::Plan> plan;
-  {
-    std::lock_guard<std::mutex> lock(m->mu);
-    int st = get_plan(m, func_key(func), plan, err);
-    if (st != XT_OK) return st;
-  }
-  const xt::Plan& p = *plan;
-  constexpr int kMost = 16;
-  if (nbufs != static_cast<int>(p.arg_types.size()) || nbufs > kMost || !bufs)
-    return fail(err, XT_ERR_ARGUMENT, "@" + p.func + " takes " + std::to_string(p.arg_types.size()) +
-                                          " buffers (at most " + std::to_string(kMost) + " described ones)");
-  void* ptrs[kMost] = {};
-  for (int k = 0; k < nbufs; ++k) {
-    const xt::Type& t = p.arg_types[k];
-    bool same = bufs[k].ptr && bufs[k].dtype == elem_code(t.elem) && bufs[k].rank == static_cast<int>(t.shape.size()) &&
-                (bufs[k].shape || bufs[k].rank == 0);
-    for (int d = 0; same && d < bufs[k].rank; ++d) same = bufs[k].shape[d] == t.shape[d];
-    if (!same) return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is not a " + t.str());
-    ptrs[k] = bufs[k].ptr;
-  }
-  return run_plan(p, ptrs, work, work_bytes, stream, err);
+  return guarded(err, [&]() -> int {
+    std::shared_ptr<const xt::Plan> plan;
+    {
+      std::lock_guard<std::mutex> lock(m->mu);
+      int st = get_plan(m, func_key(func), plan, err);
+      if (st != XT_OK) return st;
+    }
+    const xt::Plan& p = *plan;
+    constexpr int kMost = 16;
+    if (nbufs != static_cast<int>(p.arg_types.size()) || nbufs > kMost || !bufs)
+      return fail(err, XT_ERR_ARGUMENT, "@" + p.func + " takes " + std::to_string(p.arg_types.size()) +
+                                            " buffers (at most " + std::to_string(kMost) + " described ones)");
+    void* ptrs[kMost] = {};
+    for (int k = 0; k < nbufs; ++k) {
+      const xt::Type& t = p.arg_types[k];
+      bool same = bufs[k].ptr && bufs[k].dtype == elem_code(t.elem) && bufs[k].rank == static_cast<int>(t.shape.size()) &&
+                  (bufs[k].shape || bufs[k].rank == 0);
+      for (int d = 0; same && d < bufs[k].rank; ++d) same = bufs[k].shape[d] == t.shape[d];
+      if (!same) return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is not a " + t.str());
+      ptrs[k] = bufs[k].ptr;
+    }
+    return run_plan(p, ptrs, work, work_bytes, stream, err);
+  });
 }
 
 }  // extern "C"
