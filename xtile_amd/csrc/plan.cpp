@@ -1336,9 +1336,10 @@ GemmCover gemm_cover(const Plan& p, int64_t w, bool is_m) {
 // Keys are split where the tiles of rows leave compute units idle, into no more parts
 // than fill them once: a second round costs more than it evens out (a token against
 // 131072 keys, 8 heads: 256 workgroups 108 us, 512 112, 1024 121).  A part of few rows
-// has a tile for each wave; one of many rows has four tiles, and the keys are not split
-// below 1024, where joining the parts costs what they save (577 keys, 160 tiles: whole
-// 20.4 us, halves 25.7).
+// has at least a tile for each wave, and two such rounds are left whole (139 keys of 160
+// columns: 10.1 us, in two parts 11.1).  One of many rows has four tiles, and the keys
+// are not split below 1024, where joining the parts costs what they save (577 keys, 160
+// tiles: whole 20.4 us, halves 25.7).
 int attend_splits(const Plan& p) {
   const AttendPlan& a = p.attend;
   const int64_t rows = a.heads * a.rows;
@@ -1350,7 +1351,8 @@ int attend_splits(const Plan& p) {
   const int64_t keys = band ? std::min(a.keys, a.window + a.rows) : a.keys;
   const int fit = few ? (a.d > 64 ? 1 : 2) : a.d > 128 ? 1 : a.d > 64 ? 2 : 3;  // workgroups on a compute unit
   const double want = 256 * fit / tiles;
-  const int64_t most = few ? keys / 128 : keys < 1024 ? 1 : keys / 256;
+  const int64_t round = a.d > 160 ? 64 : 128;  // keys of few rows that a workgroup's waves take at a time
+  const int64_t most = few ? (keys > 2 * round ? (keys + round - 1) / round : 1) : keys < 1024 ? 1 : keys / 256;
   if (want < 2 || most < 2) return 1;
   return static_cast<int>(std::min<double>(std::min<double>(want, double(most)), 256));
 }
