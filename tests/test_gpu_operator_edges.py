@@ -1,0 +1,99 @@
+"""Calls of rms_norm, matmul_q4 and attend at the edges of what they take, against 64 bits."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+import xtile_amd as xt
+from tests import operators_ref as ref
+from xtile_amd import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(shape, dtype, cuda, seed, scale=1.0):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (scale * torch.randn(shape, generator=g, device=cuda)).to(dtype)
+
+
+def say(*what):
+    print("[gpu]", *what, flush=True)
+
+
+# -- attend ------------------------------------------------------------------------
+
+
+def attend_rows(q, k, v, sees, scale, slopes=None, start=0):
+    """One head, row by row over the keys it sees alone, in 64 bits: (result, sum of
+    the weighted magnitudes).  sees: (rows, keys)."""
+    import torch
+
+    out, size = [], []
+    j = torch.arange(k.shape[0], device=k.device)
+    for t in range(q.shape[0]):
+        at = sees[t]
+        s = (k[at].double() @ q[t].double()) * scale
+        if slopes is not None:
+            s = s - slopes * (start + t - j[at]).abs().double()
+        p = torch.softmax(s, dim=0)
+        out.append(p @ v[at].double())
+        size.append(p @ v[at].double().abs())
+    return torch.stack(out), torch.stack(size)
+
+
+@pytest.mark.parametrize("n,docs", [(2, 1), (150, 75)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_attend_split_with_infinities_where_a_row_sees_nothing(cuda, dtype, n, docs):
+    """Two documents, an infinity among the second's values.  The first's rows see nothing
+    in the splits that hold it, and scores near -200 in the others."""
+    import torch
+
+    t, nk = getattr(torch, dtype), 3000
+    p = K.masked_attention(1, 1, 1, n, nk, 64, dtype=getattr(xt, dtype), docs=True)
+    say(xt.plan(p)["kernel"])
+    assert "splits=" in xt.plan(p)["kernel"]
+    q = (5 + 0.1 * rand((n, 64), torch.float32, cuda, 1)).to(t)
+    k = (-5 + 0.1 * rand((nk, 64), torch.float32, cuda, 2)).to(t)
+    v = rand((nk, 64), t, cuda, 3)
+    qd = torch.full((1, n), 2, dtype=torch.int32, device=cuda)
+    qd[0, :docs] = 1
+    kd = torch.full((1, nk), 2, dtype=torch.int32, device=cuda)
+    kd[0, :1500] = 1
+    v[2000, 5] = math.inf
+    o = torch.full_like(q, 7)
+    xt.launch(p, q.view(1, 1, n, 64), k.view(1, 1, nk, 64), v.view(1, 1, nk, 64), qd, kd, o.view(1, 1, n, 64))
+    want, size = attend_rows(q, k, v, qd[0][:, None] == kd[0], 0.125)
+    # a score is a sum of 64 products of about 25, 200 in all: off by (64 + 16) 2^-24 of it
+    far = (ref.half_step(q) + 2 * 80 * 2.0**-24 * 210 + (nk + 64) * 2.0**-24) * size + ref.half_step(q) * want.abs()
+    far = far + (2.0**-25 * nk if dtype == "float16" else 0)
+    ref.assert_within(o[:docs], want[:docs], far[:docs])
+    ref.assert_within(o[docs:], want[docs:], far[docs:].nan_to_num(1.0, posinf=1.0))
+
+
+@pytest.mark.parametrize("n", [3, 70])
+def test_attend_split_with_infinities_far_from_the_rows_keys(cuda, n):
+    """The same by a distance bias: what the first document's rows see lies far away."""
+    import torch
+
+    nk, start = 3000, 2900
+    p = K.masked_attention(1, 1, 1, n, nk, 64, slopes=True, start=True, docs=True)
+    assert "splits=" in xt.plan(p)["kernel"]
+    q, k, v = (rand(s, torch.bfloat16, cuda, i) for i, s in enumerate([(n, 64), (nk, 64), (nk, 64)]))
+    qd = torch.full((1, n), 2, dtype=torch.int32, device=cuda)
+    qd[0, : n // 2] = 1
+    kd = torch.full((1, nk), 2, dtype=torch.int32, device=cuda)
+    kd[0, :1000] = 1
+    v[1700, 9] = math.nan
+    slopes = torch.full((1, 1), 0.25, device=cuda)
+    o = torch.full_like(q, 7)
+    xt.launch(p, q.view(1, 1, n, 64), k.view(1, 1, nk, 64), v.view(1, 1, nk, 64), slopes,
+              torch.tensor([[start]], dtype=torch.int32, device=cuda), qd, kd, o.view(1, 1, n, 64))
+    want, size = attend_rows(q, k, v, qd[0][:, None] == kd[0], 0.125, 0.25, start)
+    # biases to 750, in which a score is off by 8 2^-24 of them, products by 80 2^-24 of some 10
+    far = (2.0**-8 + 2 * (8 * 750 + 80 * 10) * 2.0**-24 + (nk + 64) * 2.0**-24) * size + 2.0**-8 * want.abs()
+    ref.assert_within(o[: n // 2], want[: n // 2], far[: n // 2])
+    assert bool(torch.isnan(o[n // 2 :, 9]).all()) and bool(torch.isfinite(o[n // 2 :, 10]).all())

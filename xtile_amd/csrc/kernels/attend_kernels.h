@@ -691,7 +691,9 @@ __device__ __forceinline__ void odd_rows(const AttendArgs& p, const BlockAt& b, 
                             : s * p.scale_log2;
       return p.slopes ? fmaf(-slope, fabsf((float)(pos - j)), s) : s;
     };
-    float m = -__builtin_inff(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // the maximum, minus infinity where the row sees nothing (as in tile), and what the
+    // scores are taken relative to
+    float m = -__builtin_inff(), use = 0.0f, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll 1
@@ -703,7 +705,7 @@ __device__ __forceinline__ void odd_rows(const AttendArgs& p, const BlockAt& b, 
           m = fmaxf(m, s);
           continue;
         }
-        const float w = in ? __builtin_amdgcn_exp2f(s - m) : 0.0f;
+        const float w = in ? __builtin_amdgcn_exp2f(s - use) : 0.0f;
         l += w;
         unsigned long long left = __builtin_amdgcn_ballot_w64(in);
 #pragma unroll 1
@@ -718,7 +720,7 @@ __device__ __forceinline__ void odd_rows(const AttendArgs& p, const BlockAt& b, 
       }
       if (pass == 0) {
         m = wave_reduce<true>(m);
-        if (m == -__builtin_inff()) m = 0.0f;
+        use = m == -__builtin_inff() ? 0.0f : m;
       }
     }
     l = wave_reduce<false>(l);
