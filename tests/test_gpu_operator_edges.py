@@ -97,3 +97,36 @@ def test_attend_split_with_infinities_far_from_the_rows_keys(cuda, n):
     far = (2.0**-8 + 2 * (8 * 750 + 80 * 10) * 2.0**-24 + (nk + 64) * 2.0**-24) * size + 2.0**-8 * want.abs()
     ref.assert_within(o[: n // 2], want[: n // 2], far[: n // 2])
     assert bool(torch.isnan(o[n // 2 :, 9]).all()) and bool(torch.isfinite(o[n // 2 :, 10]).all())
+
+
+# -- matmul_q4 -----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("what", ["weights", "scales"])
+def test_matmul_q4_of_rows_whose_pitch_passes_a_tiles_31_bits(cuda, what):
+    """32 rows of weights, or of their scales, 2 GiB apart from the first to the last."""
+    import torch
+
+    m, n, k = 12288, 32, 64
+    wp, sp = (70_000_000, 2) if what == "weights" else (32, 36_000_000)
+    p16 = xt.float16
+
+    @xt.kernel
+    def part(x, w, s, y):
+        t = xt.matmul_q4(xt.load(x, index=(0, 0), shape=(m, k)), xt.load(w, index=(0, 0), shape=(n, k // 2)),
+                         xt.load(s, index=(0, 0), shape=(n, 2)))
+        xt.store(y, index=(0, 0), tile=t)
+
+    p = xt.convert(part, args=(xt.Array((m, k), p16), xt.Array((n, wp), xt.int8), xt.Array((n, sp), p16),
+                               xt.Array((m, n), xt.float32)), grid=(1, 1, 1))
+    say(xt.plan(p)["kernel"])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randint(-3, 4, (m, k), generator=g, device=cuda).half()
+    w = torch.randint(-8, 8, (n, k), generator=g, device=cuda, dtype=torch.int8)
+    s = torch.exp2(-torch.randint(0, 5, (n, 2), generator=g, device=cuda).float()).half()
+    bw = torch.zeros(n, wp, dtype=torch.int8, device=cuda)
+    bs = torch.zeros(n, sp, dtype=torch.float16, device=cuda)
+    bw[:, : k // 2], bs[:, :2] = xt.pack_q4(w), s
+    y = torch.full((m, n), 7.0, device=cuda)
+    xt.launch(p, x, bw, bs, y)
+    assert torch.equal(y.double(), ref.matmul_q4(x, w, s))

@@ -344,8 +344,9 @@ void run_fl(Q4Args& a, int wgs, hipStream_t s) {
   else matmul_q4_kernel<ELEM, ROWS, NT, W, NS, 1, S32><<<wgs, 64 * W, 0, s>>>(a);
 }
 
+// near32: 32 rows of weights, and of their scales, lie within a lane's 31 bits.
 template <int ELEM, bool S32>
-bool run(Q4Args& a, long long blocks, hipStream_t s) {
+bool run(Q4Args& a, long long blocks, bool near32, hipStream_t s) {
   constexpr int FEW = ELEM == kI8 ? 8 : 4;  // rows that one instruction brings
   auto tiles_of = [&](int mt, int nt) {
     return (long long)((a.N + 16 * nt - 1) / (16 * nt)) * ((a.M + 16 * mt - 1) / (16 * mt));
@@ -357,7 +358,7 @@ bool run(Q4Args& a, long long blocks, hipStream_t s) {
   // workgroups: 24 by 11008 x 4096 18.1 us against 20.8).
   int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
   while (mt > 1 && tiles_of(mt, 1) * blocks < 256) mt >>= 1;
-  const int nt = ELEM != kI8 && mt == 4 && tiles_of(mt, 2) * blocks >= 192 ? 2 : 1;
+  const int nt = ELEM != kI8 && mt == 4 && near32 && tiles_of(mt, 2) * blocks >= 192 ? 2 : 1;
   const long long tiles = tiles_of(mt, nt);
   if (tiles > 0x7fffffffLL || !grid_fits(tiles * blocks, 512)) return false;
   a.tiles = (int)tiles;
@@ -417,17 +418,19 @@ hipError_t launch_matmul_q4(const xt::Plan& p, void* const* bufs, hipStream_t s,
   a.y_elem = elem_of(q.y.elem);
   // what a lane adds to its tile's address has 31 bits
   auto near = [](int rows, long long ld, long long cols, int bytes) { return ((rows - 1) * ld + cols) * bytes < (1LL << 31); };
-  const int xs = q.x.elem == xt::Elem::I8 ? 1 : 2, ss = a.s_elem == kF32 ? 4 : 2, rows = std::min(a.N, 16);
-  if (!near(std::min(a.M, 64), a.ldx, 128, xs) || !near(rows, a.ldw, 64, 1) || !near(rows, a.lds, a.K / 32 + 1, ss)) {
+  const int xs = q.x.elem == xt::Elem::I8 ? 1 : 2, ss = a.s_elem == kF32 ? 4 : 2;
+  auto near_weights = [&](int rows) { return near(rows, a.ldw, 64, 1) && near(rows, a.lds, a.K / 32 + 1, ss); };
+  if (!near(std::min(a.M, 64), a.ldx, 128, xs) || !near_weights(std::min(a.N, 16))) {
     why = "matmul_q4: rows that a workgroup reads together span 2^31 bytes or more";
     return hipErrorInvalidValue;
   }
   bool ok;
   const bool s32 = a.s_elem == kF32;
+  const bool near32 = near_weights(std::min(a.N, 32));
   const long long blocks = grid_blocks(p);
-  if (q.x.elem == xt::Elem::I8) ok = s32 ? run<kI8, true>(a, blocks, s) : run<kI8, false>(a, blocks, s);
-  else if (q.x.elem == xt::Elem::F16) ok = s32 ? run<kF16, true>(a, blocks, s) : run<kF16, false>(a, blocks, s);
-  else ok = s32 ? run<kBF16, true>(a, blocks, s) : run<kBF16, false>(a, blocks, s);
+  if (q.x.elem == xt::Elem::I8) ok = s32 ? run<kI8, true>(a, blocks, near32, s) : run<kI8, false>(a, blocks, near32, s);
+  else if (q.x.elem == xt::Elem::F16) ok = s32 ? run<kF16, true>(a, blocks, near32, s) : run<kF16, false>(a, blocks, near32, s);
+  else ok = s32 ? run<kBF16, true>(a, blocks, near32, s) : run<kBF16, false>(a, blocks, near32, s);
   if (!ok) {
     why = "matmul_q4: " + std::to_string(a.M) + " x " + std::to_string(a.N) + " tiles exceed one launch";
     return hipErrorInvalidValue;
