@@ -130,3 +130,21 @@ def test_matmul_q4_of_rows_whose_pitch_passes_a_tiles_31_bits(cuda, what):
     y = torch.full((m, n), 7.0, device=cuda)
     xt.launch(p, x, bw, bs, y)
     assert torch.equal(y.double(), ref.matmul_q4(x, w, s))
+
+
+# -- rms_norm ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cols", [1, 4, 7])
+def test_rms_norm_of_many_short_rows(cuda, cols):
+    """More than 2^22 rows of fewer than eight values."""
+    import torch
+
+    rows = (1 << 22) + 37
+    m = K.rms_norm(rows, cols, xt.float32, residual=False)
+    say(xt.plan(m)["kernel"])
+    x, g = rand((rows, cols), torch.float32, cuda, 1), rand((1, cols), torch.float32, cuda, 2)
+    y = torch.full_like(x, 7)
+    xt.launch(m, x, g, y)
+    _, want = ref.rms_norm(x, None, g, 1e-6)
+    ref.assert_within(y, want, want.abs() * 40 * 2.0**-24 + 1e-37)

@@ -1,0 +1,36 @@
+"""Calls of rms_norm, matmul_q4 and attend at the edges of what they take, as far as no GPU is needed."""
+
+from __future__ import annotations
+
+import pytest
+
+import xtile_amd as xt
+from xtile_amd import _xtile
+from xtile_amd import kernels as K
+
+
+def launch_at(m, *addresses):
+    """Enqueues `m` over buffers at addresses that are none of any memory: for calls
+    that are refused before anything is launched."""
+    args = xt.signature(m)["args"]
+    sizes = []
+    for a in args:
+        n = {"f32": 4, "i32": 4, "f16": 2, "bf16": 2, "i8": 1}[a["dtype"]]
+        for e in a["shape"]:
+            n *= e
+        sizes.append(n)
+    _xtile.launch(m, None, list(addresses), sizes, 0)
+
+
+def apart(n):
+    return [(i + 1) << 44 for i in range(n)]
+
+
+@pytest.mark.parametrize("rows,cols", [(1 << 26, 4), (1 << 26, 1), ((1 << 26) - 1, 8), ((1 << 26) - 3, 1000), (1 << 24, 1025),
+                                       (1 << 22, 8193), (1 << 22, 40001)])
+def test_rms_norm_refuses_rows_beyond_one_launch(rows, cols):
+    """2^32 work-items or more, counted as they are launched: 64, 256 or 1024 threads a
+    row, rows of 8 to 1024 values four to a workgroup."""
+    m = K.rms_norm(rows, cols, xt.float32, residual=False)
+    with pytest.raises(ValueError, match="exceed one launch"):
+        launch_at(m, *apart(3))

@@ -11,7 +11,8 @@
 // HBM bounds it for many rows (8192 of 4096 bf16 values with a residual to int8: 235 MB
 // in 47.3 us, 5.0 TB/s), one group's latency for one row.  A row takes
 // 64 threads (rows to 1024 values, no barrier), 256 (to 8192) or 1024; longer
-// rows are read again for the second half (rms_norm_long_kernel).
+// rows, and those of fewer than eight values, are read again for the second half
+// (rms_norm_long_kernel).
 #include <vector>
 
 #include "common.h"
@@ -313,12 +314,11 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(NormArgs p)
 }
 
 // Rows that the registers of a workgroup do not hold, and rows of fewer than eight
-// values: x and r are read twice,
+// values (T = 64, a row a workgroup): x and r are read twice,
 // the second time from L2.  Nothing is stored before the second pass, and then by
 // the thread that has just read those values again, since it may lie over x or r.
-template <int ELEM>
-__global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs p) {
-  constexpr int T = 1024;
+template <int ELEM, int T>
+__global__ __launch_bounds__(T) void rms_norm_long_kernel(NormArgs p) {
   const RowAt at = row_at(p, blockIdx.x);
   const int t = threadIdx.x;
   const bool quantize = p.y_elem == kI8;
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs p) {
     }
     ss += s8;
   }
-  row_reduce<1024>(ss, top, quantize);
+  row_reduce<T>(ss, top, quantize);
   const float inv = inverse_root(p, ss);
   float s = 0.0f, is = 0.0f;
   if (quantize) {
@@ -363,22 +363,37 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs p) {
   }
 }
 
+// What a launch takes: threads a row, workgroups and their threads, and whether the
+// rows are read twice.
+struct NormGrid {
+  int row;
+  long long wgs;
+  int threads;
+  bool twice;
+  NormGrid(int cols, long long rows)
+      : row(cols <= 1024 ? 64 : cols <= 8192 ? 256 : 1024), twice(cols < 8 || cols > 32768) {
+    threads = twice ? row : row < 256 ? 256 : row;
+    wgs = (rows + threads / row - 1) / (threads / row);
+  }
+};
+
 template <int ELEM, int T, bool GWIDE>
-void run(const NormArgs& a, int nv, hipStream_t s) {
-  constexpr int threads = T < 256 ? 256 : T;
-  const int wgs = T < 256 ? (a.rows + 256 / T - 1) / (256 / T) : a.rows;
-  if (nv <= 1) rms_norm_kernel<ELEM, T, 1, GWIDE><<<wgs, threads, 0, s>>>(a);
-  else if (nv <= 2) rms_norm_kernel<ELEM, T, 2, GWIDE><<<wgs, threads, 0, s>>>(a);
-  else rms_norm_kernel<ELEM, T, 4, GWIDE><<<wgs, threads, 0, s>>>(a);
+void run(const NormArgs& a, const NormGrid& g, hipStream_t s) {
+  const unsigned wgs = static_cast<unsigned>(g.wgs);
+  const int nv = ((a.cols + 7) / 8 + T - 1) / T;  // vectors a thread
+  if (nv <= 1) rms_norm_kernel<ELEM, T, 1, GWIDE><<<wgs, g.threads, 0, s>>>(a);
+  else if (nv <= 2) rms_norm_kernel<ELEM, T, 2, GWIDE><<<wgs, g.threads, 0, s>>>(a);
+  else rms_norm_kernel<ELEM, T, 4, GWIDE><<<wgs, g.threads, 0, s>>>(a);
 }
 
 template <int ELEM, bool GWIDE>
-void run_elem(const NormArgs& a, hipStream_t s) {
-  const int v = (a.cols + 7) / 8;  // vectors of a row
-  if (a.cols < 8 || v > 4096) rms_norm_long_kernel<ELEM><<<a.rows, 1024, 0, s>>>(a);
-  else if (v <= 128) run<ELEM, 64, GWIDE>(a, (v + 63) / 64, s);
-  else if (v <= 1024) run<ELEM, 256, GWIDE>(a, (v + 255) / 256, s);
-  else run<ELEM, 1024, GWIDE>(a, (v + 1023) / 1024, s);
+void run_elem(const NormArgs& a, const NormGrid& g, hipStream_t s) {
+  const unsigned wgs = static_cast<unsigned>(g.wgs);
+  if (g.twice && g.row == 64) rms_norm_long_kernel<ELEM, 64><<<wgs, 64, 0, s>>>(a);
+  else if (g.twice) rms_norm_long_kernel<ELEM, 1024><<<wgs, 1024, 0, s>>>(a);
+  else if (g.row == 64) run<ELEM, 64, GWIDE>(a, g, s);
+  else if (g.row == 256) run<ELEM, 256, GWIDE>(a, g, s);
+  else run<ELEM, 1024, GWIDE>(a, g, s);
 }
 
 int elem_of(xt::Elem e) {
@@ -433,15 +448,15 @@ hipError_t launch_rms_norm(const xt::Plan& p, void* const* bufs, hipStream_t s, 
   a.gamma_elem = elem_of(n.gamma.elem);
   a.y_elem = elem_of(n.y.elem);
   a.eps = n.eps;
-  const int t = a.cols <= 1024 ? 64 : a.cols <= 8192 ? 256 : 1024;
-  if (!grid_fits(rows, t)) {
+  const NormGrid g(a.cols, rows);
+  if (!grid_fits(g.wgs, g.threads)) {
     why = "rms_norm: " + std::to_string(rows) + " rows exceed one launch";
     return hipErrorInvalidValue;
   }
   const bool wide = a.gamma_elem == kF32;
-  if (n.x.elem == xt::Elem::F32) wide ? run_elem<kF32, true>(a, s) : run_elem<kF32, false>(a, s);
-  else if (n.x.elem == xt::Elem::F16) wide ? run_elem<kF16, true>(a, s) : run_elem<kF16, false>(a, s);
-  else wide ? run_elem<kBF16, true>(a, s) : run_elem<kBF16, false>(a, s);
+  if (n.x.elem == xt::Elem::F32) wide ? run_elem<kF32, true>(a, g, s) : run_elem<kF32, false>(a, g, s);
+  else if (n.x.elem == xt::Elem::F16) wide ? run_elem<kF16, true>(a, g, s) : run_elem<kF16, false>(a, g, s);
+  else wide ? run_elem<kBF16, true>(a, g, s) : run_elem<kBF16, false>(a, g, s);
   return hipGetLastError();
 }
 
