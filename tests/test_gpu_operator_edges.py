@@ -148,3 +148,17 @@ def test_rms_norm_of_many_short_rows(cuda, cols):
     xt.launch(m, x, g, y)
     _, want = ref.rms_norm(x, None, g, 1e-6)
     ref.assert_within(y, want, want.abs() * 40 * 2.0**-24 + 1e-37)
+
+
+@pytest.mark.parametrize("over", ["x", "r"])
+def test_rms_norm_scales_of_one_column_over_an_input(cuda, over):
+    """Rows of one value, whose scales have the input's shape and type."""
+    import torch
+
+    m = K.rms_norm(37, 1, xt.float32, quantize=True)
+    x, r, g = rand((37, 1), torch.float32, cuda, 1), rand((37, 1), torch.float32, cuda, 2), torch.full((1, 1), 3.0, device=cuda)
+    want_h, want = ref.rms_norm(x, r, g, 1e-6)
+    h, q, s = torch.zeros_like(x), torch.zeros(37, 1, dtype=torch.int8, device=cuda), {"x": x, "r": r}[over]
+    xt.launch(m, x, r, g, h, q, s)
+    assert torch.equal(h, want_h.float()) and torch.equal(q, 127 * torch.sign(want_h).to(torch.int8))
+    ref.assert_within(s, want.abs() / 127, want.abs() / 127 * 40 * 2.0**-24)

@@ -350,7 +350,6 @@ __global__ __launch_bounds__(T) void rms_norm_long_kernel(NormArgs p) {
   if (quantize) {
     s = __builtin_bit_cast(float, top) * inv / 127.0f;
     is = s >= 1.0e-37f ? 1.0f / s : 0.0f;
-    if (t == 0) p.scale[at.scale] = s;
     if (s != s) is = s;
   }
   for (int c = t * 8; c < p.cols; c += T * 8) {
@@ -361,6 +360,8 @@ __global__ __launch_bounds__(T) void rms_norm_long_kernel(NormArgs p) {
     for (int e = 0; e < 8; ++e) y[e] = h[e] * inv * g[e];
     store_y8(p, at.y + c, p.cols - c, y, s, is);
   }
+  // behind the second pass: the scales of rows of one value may lie over x or r
+  if (quantize && t == 0) p.scale[at.scale] = s;
 }
 
 // What a launch takes: threads a row, workgroups and their threads, and whether the
