@@ -34,3 +34,30 @@ def test_rms_norm_refuses_rows_beyond_one_launch(rows, cols):
     m = K.rms_norm(rows, cols, xt.float32, residual=False)
     with pytest.raises(ValueError, match="exceed one launch"):
         launch_at(m, *apart(3))
+
+
+def traced(body, *arrays, grid=(1, 1, 1)):
+    return xt.convert(K._named("traced", lambda a: body(*a), len(arrays)), args=arrays, grid=grid)
+
+
+@pytest.mark.parametrize("grid", [(2, 1, 1), (1, 2, 1), (1, 1, 2)])
+def test_results_over_inputs_that_several_blocks_read_are_refused(grid):
+    """Every Block has the same tile: one would read what another has stored."""
+    x, g = xt.Array((4, 64), xt.float32), xt.Array((1, 64), xt.float32)
+
+    def norm(x, g, y):
+        xt.store(y, index=(0, 0), tile=xt.rms_norm(xt.load(x, index=(0, 0), shape=(4, 64)), xt.load(g, index=(0, 0), shape=(1, 64))))
+
+    m = traced(norm, x, g, x, grid=grid)
+    a, b, _ = apart(3)
+    with pytest.raises(ValueError, match="meets buffer 0"):
+        launch_at(m, a, b, a)
+    h = xt.Array((4, 64), xt.float16)
+
+    def attention(q, k, v, o):
+        xt.store(o, index=(0, 0), tile=xt.attend(*(xt.load(t, index=(0, 0), shape=(4, 64)) for t in (q, k, v)), scale=1.0))
+
+    m = traced(attention, h, h, h, h, grid=grid)
+    a, b, c, _ = apart(4)
+    with pytest.raises(ValueError, match="meets buffer 0"):
+        launch_at(m, a, b, c, a)

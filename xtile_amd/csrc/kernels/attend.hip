@@ -49,12 +49,12 @@ extern template hipError_t run_attend<256>(bool, bool, const AttendArgs&, hipStr
 hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipStream_t s, std::string& why) {
   const xt::AttendPlan& t = p.attend;
   // a workgroup reads its own query rows before it stores them, so the result may
-  // lie over q, element for element; over nothing else
+  // lie over q, element for element, where no two Blocks have the same; over nothing else
   auto apart = [&](int in) {
     if (in < 0 || (in != t.o.arg && !buffers_meet(p, bufs, t.o.arg, in))) return true;
     const xt::TileAddr &a = t.q.addr, &b = t.o.addr;
     if (in == t.q.arg && bufs[in] == bufs[t.o.arg] && t.q.head == t.o.head && t.q.row == t.o.row && a.c0 == b.c0 &&
-        a.sx == b.sx && a.sy == b.sy && a.sz == b.sz)
+        a.sx == b.sx && a.sy == b.sy && a.sz == b.sz && own_tiles(p, b))
       return true;
     why = "buffer " + std::to_string(t.o.arg) + " is stored and meets buffer " + std::to_string(in) +
           ", which the program reads elsewhere";

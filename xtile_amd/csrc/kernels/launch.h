@@ -77,9 +77,15 @@ inline bool accesses_meet(const xt::Plan& p, void* const* bufs, const xt::Access
   return first(x) < past(y) && first(y) < past(x);
 }
 
+// Whether no two Blocks have the same tile: every axis with more than one of them
+// moves it (each dim of an array is tiled along one axis, so moved tiles are apart).
+inline bool own_tiles(const xt::Plan& p, const xt::TileAddr& a) {
+  return (p.grid[0] == 1 || a.sx) && (p.grid[1] == 1 || a.sy) && (p.grid[2] == 1 || a.sz);
+}
+
 // Whether a result may be stored while an operand is read: their buffers do not
 // meet, or, where every thread has read what it stores over (`in_place`), they are
-// the same elements at the same places.
+// the same elements at the same places, of one Block only.
 inline bool result_apart(const xt::Plan& p, void* const* bufs, const xt::Access2D& out, const xt::Access2D& in,
                          bool in_place, std::string& why) {
   if (out.arg != in.arg && !buffers_meet(p, bufs, out.arg, in.arg)) return true;
@@ -87,7 +93,7 @@ inline bool result_apart(const xt::Plan& p, void* const* bufs, const xt::Access2
     return a.elem == b.elem && a.rows == b.rows && a.cols == b.cols && a.ld == b.ld && a.addr.c0 == b.addr.c0 &&
            a.addr.sx == b.addr.sx && a.addr.sy == b.addr.sy && a.addr.sz == b.addr.sz;
   };
-  if (in_place && bufs[out.arg] == bufs[in.arg] && same(out, in)) return true;
+  if (in_place && bufs[out.arg] == bufs[in.arg] && same(out, in) && own_tiles(p, out.addr)) return true;
   why = "buffer " + std::to_string(out.arg) + " is stored and meets buffer " + std::to_string(in.arg) +
         ", which the program reads elsewhere";
   return false;
