@@ -61,3 +61,34 @@ def test_results_over_inputs_that_several_blocks_read_are_refused(grid):
     a, b, c, _ = apart(4)
     with pytest.raises(ValueError, match="meets buffer 0"):
         launch_at(m, a, b, c, a)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "o"])
+def test_attend_refuses_rows_whose_elements_lie_apart(which):
+    """A tile of one of three interleaved arrays, reshaped to rows."""
+    rows, apart3 = xt.Array((40, 64), xt.float16), xt.Array((40, 64, 3), xt.float16)
+
+    def body(q, k, v, o):
+        def tile(name, a):
+            if name != which:
+                return xt.load(a, index=(0, 0), shape=(40, 64))
+            return xt.reshape(xt.load(a, index=(0, 0, 1), shape=(40, 64, 1)), shape=(40, 64))
+
+        y = xt.attend(tile("q", q), tile("k", k), tile("v", v), scale=1.0)
+        if which == "o":
+            xt.store(o, index=(0, 0, 1), tile=xt.reshape(y, shape=(40, 64, 1)))
+        else:
+            xt.store(o, index=(0, 0), tile=y)
+
+    m = traced(body, *(apart3 if name == which else rows for name in "qkvo"))
+    with pytest.raises(NotImplementedError, match="side by side"):
+        xt.plan(m)
+
+
+def test_attend_takes_rows_of_an_array_whose_last_dim_is_one():
+    def body(q, k, v, o):
+        q, k, v = (xt.reshape(xt.load(t, index=(0, 0, 0), shape=(40, 64, 1)), shape=(40, 64)) for t in (q, k, v))
+        xt.store(o, index=(0, 0, 0), tile=xt.reshape(xt.attend(q, k, v, scale=1.0), shape=(40, 64, 1)))
+
+    a = xt.Array((40, 64, 1), xt.float16)
+    assert "attend f16 heads=1 rows=40 keys=40 d=64" in xt.plan(traced(body, a, a, a, a))["kernel"]

@@ -694,8 +694,9 @@ bool reshaped_strides(const std::vector<int64_t>& tile, const std::vector<int64_
   return at == src.size();
 }
 
-// The load or store `o` of a tile that the program sees as `shape`.
-bool attend_access(const Analysis& an, const Op& o, const std::vector<int64_t>& shape, AttendAccess& a,
+// The load or store `o` of a tile that the program sees as `shape`; `columns`: its last
+// dim is read and stored whole, so its elements have to lie side by side.
+bool attend_access(const Analysis& an, const Op& o, const std::vector<int64_t>& shape, bool columns, AttendAccess& a,
                    std::vector<int64_t>& strides, std::string& err) {
   const bool is_load = o.name == "xt.load";
   const int mem_v = is_load ? o.operands[0] : o.operands[1];
@@ -716,6 +717,10 @@ bool attend_access(const Analysis& an, const Op& o, const std::vector<int64_t>& 
     return false;
   if (!reshaped_strides(ten.shape, strides_of(mem.shape), shape, strides)) {
     err = o.name + " of argument #" + std::to_string(a.arg) + ": the tile's dims do not reshape to evenly spaced rows";
+    return false;
+  }
+  if (columns && shape.back() > 1 && strides.back() != 1) {
+    err = o.name + " of argument #" + std::to_string(a.arg) + ": the HIP attend kernel takes rows whose elements lie side by side";
     return false;
   }
   return true;
@@ -753,7 +758,7 @@ bool match_attend(const Analysis& an, Plan& p, std::string& err) {
   std::vector<int> read;
   std::vector<int64_t> s;
   auto rows_of = [&](const Op* o, AttendAccess& x) {
-    if (!attend_access(an, *o, hrd, x, s, err)) return false;
+    if (!attend_access(an, *o, hrd, true, x, s, err)) return false;
     x.head = s[token ? 1 : 0];
     x.row = s[token ? 0 : 1];
     return true;
@@ -770,12 +775,12 @@ bool match_attend(const Analysis& an, Plan& p, std::string& err) {
     if (i == 0) {
       if (!rows_of(ld, a.q)) return false;
     } else if (i < 3) {
-      if (!attend_access(an, *ld, {a.keys, a.d}, *kv[i - 1], s, err)) return false;
+      if (!attend_access(an, *ld, {a.keys, a.d}, true, *kv[i - 1], s, err)) return false;
       kv[i - 1]->row = s[0];
     } else {
       while (!extras->ints[e]) ++e;
       const Type& t = an.f.type_of(at->operands[i]);
-      if (!attend_access(an, *ld, t.shape, a.extra[e], s, err)) return false;
+      if (!attend_access(an, *ld, t.shape, false, a.extra[e], s, err)) return false;
       a.extra[e].row = s[1];
       ++e;
     }
