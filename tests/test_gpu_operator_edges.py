@@ -99,6 +99,79 @@ def test_attend_split_with_infinities_far_from_the_rows_keys(cuda, n):
     assert bool(torch.isnan(o[n // 2 :, 9]).all()) and bool(torch.isfinite(o[n // 2 :, 10]).all())
 
 
+def capped(cuda, n, nk, d, cap, dtype, spread=1.0, seed=1, edit=None, length=None):
+    """(result, what it should be, how far it may be off)"""
+    import torch
+
+    t, scale = getattr(torch, dtype), d**-0.5
+    p = K.masked_attention(1, 1, 1, n, nk, d, dtype=getattr(xt, dtype), cap=cap, causal=False, length=length is not None)
+    say(xt.plan(p)["kernel"], cap)
+    q, k, v = (rand((s, d), t, cuda, seed + i, c) for i, (s, c) in enumerate([(n, spread), (nk, spread), (nk, 1.0)]))
+    if edit:
+        edit(q, k, v)
+    o = torch.full_like(q, 7)
+    le = [] if length is None else [torch.tensor([[length]], dtype=torch.int32, device=cuda)]
+    xt.launch(p, q.view(1, 1, n, d), k.view(1, 1, nk, d), v.view(1, 1, nk, d), *le, o.view(1, 1, n, d))
+    k, v = k[:length], v[:length]
+    qd, kd, vd = q.double(), k.double(), v.double()
+    s = qd @ kd.t() * scale
+    # the product's sum, then: up to cap / 2 a polynomial off by 6.2e-7 of the score, beyond
+    # it cap (1 - 2 / (e^2z + 1)), whose exponent, exponential, sum and reciprocal leave at
+    # most 16 2^-24 of its own size; two products by constants more.  Caps to 256 take the
+    # latter for all of a tile: 8 2^-24 of the cap
+    off = (d + 8) * 2.0**-24 * (qd.abs() @ kd.abs().t() * scale) + 24 * 2.0**-24 * s.abs()
+    off = off + (8 * 2.0**-24 * cap if cap <= 256 else 0)
+    x = cap * torch.tanh(s / cap)
+    off = torch.minimum(off, torch.full_like(off, 2 * cap))
+    w = torch.softmax(x, dim=1)
+    want, size = w @ vd, w @ vd.abs()
+    u = ref.half_step(q)
+    far = (u + 2 * off.amax(dim=1, keepdim=True) + (nk + 64) * 2.0**-24) * size + u * want.abs()
+    if dtype == "float16":
+        far = far + 2.0**-25 * vd.abs().sum(0) + 2.0**-25
+    return o, want, far
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n,nk,d", [(1, 300, 128), (90, 300, 128), (90, 150, 128), (40, 300, 256), (3, 90, 32)])
+@pytest.mark.parametrize("cap", [260.0, 884.0, 1e4, 1e5, 1e6, 1e9, 1e30, 3e38])
+def test_attend_large_caps(cuda, cap, n, nk, d, dtype):
+    """Towards no cap at all."""
+    o, want, far = capped(cuda, n, nk, d, cap, dtype, 1.5)
+    ref.assert_within(o, want, far)
+
+
+@pytest.mark.parametrize("n", [1, 90])
+@pytest.mark.parametrize("cap", [1e-38, 1e-30, 1e-6, 1e-3, 0.05])
+def test_attend_small_caps(cuda, cap, n):
+    """Towards equal scores."""
+    o, want, far = capped(cuda, n, 300, 64, cap, "bfloat16")
+    ref.assert_within(o, want, far)
+
+
+@pytest.mark.parametrize("n", [1, 90])
+@pytest.mark.parametrize("cap", [0.5, 5.0, 50.0, 257.0, 1e4])
+def test_attend_caps_of_scores_small_and_large(cuda, cap, n):
+    """Scores on both sides of half the cap in one tile, then also keys that are not
+    finite where no row sees them."""
+    import torch
+
+    def edit(q, k, v):
+        k[::3] *= 30
+        k[1::3] *= 0.05
+
+    o, want, far = capped(cuda, n, 300, 64, cap, "bfloat16", edit=edit)
+    ref.assert_within(o, want, far)
+
+    def odd(q, k, v):
+        edit(q, k, v)
+        k[251:] = math.nan
+        v[251:] = math.inf
+
+    o2, want, far = capped(cuda, n, 300, 64, cap, "bfloat16", edit=odd, length=251)
+    ref.assert_within(o2, want, far)
+
+
 # -- matmul_q4 -----------------------------------------------------------------------
 
 

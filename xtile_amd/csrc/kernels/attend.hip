@@ -19,7 +19,10 @@
 // 2^-24 cap, or, for a tile of scores with |z| <= 1/2 throughout (caps are set far
 // above ordinary scores), as z times a polynomial in z^2 fitted to tanh(z) / z there
 // (relative error 5.4e-7 by fit, 6.2e-7 in 32 bits): five operations a score in place
-// of five of which two take twice the time.
+// of five of which two take twice the time.  A few 2^-24 of a large cap are more than a
+// score may be off by, so above 256 (and where the polynomial's coefficients are no normal
+// numbers) kernels of their own take, in tiles with larger |z|, the form that each score
+// asks for.
 //
 // Tiles that no row sees are not read: the visible ones are two runs, the prefix
 // and the band between window and diagonal, cut to the keys whose documents may be
@@ -37,14 +40,14 @@
 
 namespace xtk {
 
-extern template hipError_t run_attend<32>(bool, bool, const AttendArgs&, hipStream_t);
-extern template hipError_t run_attend<64>(bool, bool, const AttendArgs&, hipStream_t);
-extern template hipError_t run_attend<96>(bool, bool, const AttendArgs&, hipStream_t);
-extern template hipError_t run_attend<128>(bool, bool, const AttendArgs&, hipStream_t);
-extern template hipError_t run_attend<160>(bool, bool, const AttendArgs&, hipStream_t);
-extern template hipError_t run_attend<192>(bool, bool, const AttendArgs&, hipStream_t);
-extern template hipError_t run_attend<224>(bool, bool, const AttendArgs&, hipStream_t);
-extern template hipError_t run_attend<256>(bool, bool, const AttendArgs&, hipStream_t);
+extern template hipError_t run_attend<32>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+extern template hipError_t run_attend<64>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+extern template hipError_t run_attend<96>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+extern template hipError_t run_attend<128>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+extern template hipError_t run_attend<160>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+extern template hipError_t run_attend<192>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+extern template hipError_t run_attend<224>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+extern template hipError_t run_attend<256>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
 
 hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipStream_t s, std::string& why) {
   const xt::AttendPlan& t = p.attend;
@@ -120,14 +123,24 @@ hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipSt
   a.d_work = div31(a.tiles * a.splits);
   a.d_splits = div31(a.splits);
   a.scale_log2 = t.scale * 1.44269504088896340736f;
+  FineCap fine{};
+  const FineCap* look = nullptr;
   if (t.cap > 0) {
-    a.cap_in = 2.0f * t.scale * 1.44269504088896340736f / t.cap;
-    a.cap_log2 = t.cap * 1.44269504088896340736f;
-    const double z = double(t.scale) / t.cap;  // of a product; its powers are normal numbers in this range
-    a.cap_near = z > 1e-4 && z < 1e4 ? static_cast<float>(0.5 / z) : -1.0f;
+    // z = s scale / cap of a product s.  The polynomial's powers of scale / cap go into its
+    // coefficients where they are normal numbers, else z is worked out (mul).  What passes
+    // half of float's range is held there: such caps leave scores alone, or near 0.
+    static constexpr double most = 1.7e38;
+    auto held = [](double v) { return static_cast<float>(v < most ? v : most); };
+    const double scale = t.scale, z = scale / t.cap, log2e = 1.4426950408889634;
+    const bool ordinary = z > 1e-4 && z < 1e4;
+    a.cap_in = held(2.0 * z * log2e);
+    a.cap_log2 = held(std::max<double>(t.cap * log2e, 1.17549435e-38));
+    fine.mul = ordinary ? 1.0f : held(z);
+    a.cap_near = held(0.5 / z);
     static const double poly[4] = {0.999999456, -0.33326318, 0.131902967, -0.0444022264};
-    for (int i = 0; i < 4; ++i)
-      a.cap_poly[i] = static_cast<float>(poly[i] * t.cap * 1.4426950408889634 * std::pow(z, 2 * i + 1));
+    for (int i = 0; i < 4; ++i) a.cap_poly[i] = held(poly[i] * scale * log2e * (ordinary ? std::pow(z, 2 * i) : 1.0));
+    // a few 2^-24 of 256 are less than half precision's rounding of a weight
+    if (!ordinary || t.cap > 256) look = &fine;
   }
   a.causal = t.causal;
   a.window = static_cast<int>(std::min<int64_t>(t.window, 1 << 30));
@@ -141,14 +154,14 @@ hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipSt
   a.dma = chunks(t.k) && chunks(t.v);
   const bool b = t.elem == xt::Elem::BF16;
   switch (t.d) {
-    case 32: return run_attend<32>(b, few, a, s);
-    case 64: return run_attend<64>(b, few, a, s);
-    case 96: return run_attend<96>(b, few, a, s);
-    case 128: return run_attend<128>(b, few, a, s);
-    case 160: return run_attend<160>(b, few, a, s);
-    case 192: return run_attend<192>(b, few, a, s);
-    case 224: return run_attend<224>(b, few, a, s);
-    default: return run_attend<256>(b, few, a, s);
+    case 32: return run_attend<32>(b, few, a, look, s);
+    case 64: return run_attend<64>(b, few, a, look, s);
+    case 96: return run_attend<96>(b, few, a, look, s);
+    case 128: return run_attend<128>(b, few, a, look, s);
+    case 160: return run_attend<160>(b, few, a, look, s);
+    case 192: return run_attend<192>(b, few, a, look, s);
+    case 224: return run_attend<224>(b, few, a, look, s);
+    default: return run_attend<256>(b, few, a, look, s);
   }
 }
 

@@ -4,7 +4,7 @@
 
 namespace xtk {
 
-template hipError_t run_attend<128>(bool, bool, const AttendArgs&, hipStream_t);
-template hipError_t run_attend<160>(bool, bool, const AttendArgs&, hipStream_t);
+template hipError_t run_attend<128>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+template hipError_t run_attend<160>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
 
 }  // namespace xtk

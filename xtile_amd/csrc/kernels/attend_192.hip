@@ -4,8 +4,8 @@
 
 namespace xtk {
 
-template hipError_t run_attend<192>(bool, bool, const AttendArgs&, hipStream_t);
-template hipError_t run_attend<224>(bool, bool, const AttendArgs&, hipStream_t);
-template hipError_t run_attend<256>(bool, bool, const AttendArgs&, hipStream_t);
+template hipError_t run_attend<192>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+template hipError_t run_attend<224>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+template hipError_t run_attend<256>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
 
 }  // namespace xtk

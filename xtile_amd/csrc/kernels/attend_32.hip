@@ -4,8 +4,8 @@
 
 namespace xtk {
 
-template hipError_t run_attend<32>(bool, bool, const AttendArgs&, hipStream_t);
-template hipError_t run_attend<64>(bool, bool, const AttendArgs&, hipStream_t);
-template hipError_t run_attend<96>(bool, bool, const AttendArgs&, hipStream_t);
+template hipError_t run_attend<32>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+template hipError_t run_attend<64>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
+template hipError_t run_attend<96>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
 
 }  // namespace xtk

@@ -29,14 +29,23 @@ struct AttendArgs {
   int tiles, splits, nwg;
   float scale_log2;  // scale * log2 e, what the products are multiplied by without a cap
   float cap_in, cap_log2;  // 2 scale log2 e / cap and cap * log2 e; cap_log2 0: no cap
-  float cap_near, cap_poly[4];  // products of at most cap_near take cap_poly (attend.hip); cap_near < 0: none do
+  // Products of at most cap_near take cap_poly (attend.hip); a tile of none above it does,
+  // and one of others takes the exponential, or, by FINE kernels, what each score asks for.
+  float cap_near, cap_poly[4];
   int causal, window, dma;
   float* work;
 };
 
-// attend_*.hip, one instantiation each for d of 32, 64, ... 256.
+// For kernels that choose for each score: the polynomial is in (mul s)^2.  An argument of
+// its own, behind the others: in their midst it moves the scalar registers of every kernel
+// (causal, 64 columns: 49 us -> 52).
+struct FineCap {
+  float mul;
+};
+
+// attend_*.hip, one instantiation each for d of 32, 64, ... 256; fine: null for none.
 template <int D>
-hipError_t run_attend(bool bf16, bool few, const AttendArgs& a, hipStream_t s);
+hipError_t run_attend(bool bf16, bool few, const AttendArgs& a, const FineCap* fine, hipStream_t s);
 
 }  // namespace xtk
 
@@ -91,6 +100,19 @@ __device__ __forceinline__ float add_pair(unsigned w, float l) {
   }
 }
 
+// The capped score, in units of log2, of a product s within cap_near (w: its square,
+// times mul^2), of a larger one, and of any.
+__device__ __forceinline__ float capped_near(const AttendArgs& p, float s, float w) {
+  return s * fmaf(w, fmaf(w, fmaf(w, p.cap_poly[3], p.cap_poly[2]), p.cap_poly[1]), p.cap_poly[0]);
+}
+__device__ __forceinline__ float capped_far(const AttendArgs& p, float s) {
+  return fmaf(-2.0f * p.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.cap_in) + 1.0f), p.cap_log2);
+}
+__device__ __forceinline__ float capped(const AttendArgs& p, const FineCap& c, float s) {
+  const float z = s * c.mul;
+  return fabsf(s) <= p.cap_near ? capped_near(p, s, z * z) : capped_far(p, s);
+}
+
 template <bool BF16>
 __device__ __forceinline__ unsigned pack2(float a, float b) {
   if constexpr (BF16) {
@@ -106,7 +128,8 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
 // h = lane / 32) holds row c; of a tile of 32 keys it holds the scores of keys
 // 8 (r / 4) + 4 h + r % 4 in register r, and of the result columns
 // 32 n + 8 (r / 4) + 4 h + r % 4 in register r of acc[n].
-template <int D, bool BF16>
+// FINE: the cap looks at each score.
+template <int D, bool BF16, bool FINE = false>
 struct Rows {
   static constexpr int N = D / 32, KK = D / 16;
   static constexpr int PITCH = 2 * D;  // bytes of a key row in LDS
@@ -223,7 +246,7 @@ struct Rows {
   // T tiles of 32 keys from key0 on.  docs: their documents in LDS, or null, then from
   // kdocs.
   template <int T>
-  __device__ __forceinline__ void tile(const AttendArgs& p, const unsigned char* K, const unsigned char* V,
+  __device__ __forceinline__ void tile(const AttendArgs& p, const FineCap& c, const unsigned char* K, const unsigned char* V,
                                        const int* docs, const int* kdocs, int key0, int len, int pre) {
     bool part = !sees_all(p, key0, 32 * T, len, pre);
     bool by_doc = false, by_key = false;  // rows, or keys, of several documents
@@ -275,7 +298,7 @@ struct Rows {
     __builtin_amdgcn_sched_barrier(0);
 
     float mul = p.scale_log2;
-    if (p.cap_log2 > 0.0f) {
+    if (FINE || p.cap_log2 > 0.0f) {
       float big[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int t = 0; t < T; ++t)
@@ -288,16 +311,14 @@ struct Rows {
         for (int t = 0; t < T; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float w = s[t][r] * s[t][r];
-            s[t][r] *= fmaf(w, fmaf(w, fmaf(w, p.cap_poly[3], p.cap_poly[2]), p.cap_poly[1]), p.cap_poly[0]);
+            const float z = FINE ? s[t][r] * c.mul : s[t][r];
+            s[t][r] = capped_near(p, s[t][r], z * z);
           }
       } else {
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[t][r] = fmaf(-2.0f * p.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[t][r] * p.cap_in) + 1.0f),
-                           p.cap_log2);
+          for (int r = 0; r < 16; ++r) s[t][r] = FINE ? capped(p, c, s[t][r]) : capped_far(p, s[t][r]);
       }
     }
     if (p.slopes) {
@@ -661,8 +682,8 @@ __device__ __forceinline__ float* total_of(const AttendArgs& p, int D, long long
 // wave each and in vector arithmetic: the way for keys among which hidden values are
 // not finite, of which only what a row sees is ever multiplied.  Lane j of 64 keys has
 // the score of key j; then the lanes have the columns.
-template <int D, bool BF16>
-__device__ __forceinline__ void odd_rows(const AttendArgs& p, const BlockAt& b, const Tiles& tiles, int bn, int i0, int i1,
+template <int D, bool BF16, bool FINE>
+__device__ __forceinline__ void odd_rows(const AttendArgs& p, const FineCap& c, const BlockAt& b, const Tiles& tiles, int bn, int i0, int i1,
                                          const int* kdocs, int first, int last, int step, long long all_rows) {
   const int lane = threadIdx.x & 63;
   auto value = [](unsigned short x) {
@@ -686,9 +707,7 @@ __device__ __forceinline__ void odd_rows(const AttendArgs& p, const BlockAt& b, 
       float s = 0.0f;
 #pragma unroll 1
       for (int d = 0; d < D; ++d) s = fmaf(value(q[d]), value(k[d]), s);
-      s = p.cap_log2 > 0.0f ? fmaf(-2.0f * p.cap_log2,
-                                   __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.cap_in) + 1.0f), p.cap_log2)
-                            : s * p.scale_log2;
+      s = FINE ? capped(p, c, s) : p.cap_log2 > 0.0f ? capped_far(p, s) : s * p.scale_log2;
       return p.slopes ? fmaf(-slope, fabsf((float)(pos - j)), s) : s;
     };
     // the maximum, minus infinity where the row sees nothing (as in tile), and what the
@@ -761,9 +780,9 @@ __device__ __forceinline__ bool any_wave(bool x, unsigned char* lds) {
 // share, two of them in LDS.  G groups of four waves have the same rows and take tiles
 // in turn, and the second's results join the first's: where workgroups are so few that
 // a SIMD would have one wave, whose products and arithmetic wait for each other.
-template <int D, bool BF16, int G>
+template <int D, bool BF16, int G, bool FINE>
 __global__ __launch_bounds__(256 * G, G == 2 ? 2 : D <= 64 ? 3 : D <= 128 ? 2 : 1)
-void attend_rows_kernel(AttendArgs p, long long all_rows) {
+void attend_rows_kernel(AttendArgs p, long long all_rows, FineCap c) {
   constexpr int BN = 64, KB = BN * D * 2, STAGE = 2 * KB + 256;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * G * STAGE];
   const bool dma = p.dma;
@@ -792,7 +811,7 @@ void attend_rows_kernel(AttendArgs p, long long all_rows) {
   };
   unsigned char* const stages = lds + group * 2 * STAGE;
   if (i0 + group < i1) issue(i0 + group, stages);
-  Rows<D, BF16> rows;
+  Rows<D, BF16, FINE> rows;
   rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start);
 #pragma unroll 1
   for (int i = i0 + group, n = 0; i - group < i1; i += G, n ^= 1) {
@@ -805,12 +824,12 @@ void attend_rows_kernel(AttendArgs p, long long all_rows) {
     if (G > 1 && i >= i1) continue;
     const int key0 = tiles.at(i) * BN;
     if (!rows.sees_none(p, key0, BN, b.pre))
-      rows.template tile<2>(p, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len, b.pre);
+      rows.template tile<2>(p, c, at, at + KB, reinterpret_cast<const int*>(at + 2 * KB), kdocs, key0, b.len, b.pre);
   }
   rows.hold();
   lds_barrier();
   if (any_wave<4 * G>(rows.spoilt(), lds)) {
-    odd_rows<D, BF16>(p, b, tiles, BN, i0, i1, kdocs, first + every, last + 1, 4 * G, all_rows);
+    odd_rows<D, BF16, FINE>(p, c, b, tiles, BN, i0, i1, kdocs, first + every, last + 1, 4 * G, all_rows);
     return;
   }
   if constexpr (G == 2) {
@@ -903,8 +922,8 @@ struct Few {
 
 // Up to 32 rows: every wave has them all and takes tiles of 32 keys in turn, each in
 // a ring of its own, so that nothing but its own loads makes a wave wait.
-template <int D, bool BF16>
-__global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p, long long all_rows) {
+template <int D, bool BF16, bool FINE>
+__global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p, long long all_rows, FineCap c) {
   typedef Few<D> F;
   constexpr int W = F::W, NS = F::NS, KB = 32 * D * 2, PER = D / 8;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[F::LDS];
@@ -937,7 +956,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
 #pragma unroll
   for (int j = 0; j < NS; ++j)
     if (j < mine) issue(j, j);
-  Rows<D, BF16> rows;
+  Rows<D, BF16, FINE> rows;
   rows.begin(p, 0, b.x, b.y, b.z, b.start);
   int slot = 0;
 #pragma unroll 1
@@ -951,7 +970,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
     }
     asm volatile("" ::: "memory");
     unsigned char* const at = ring + slot * F::TILE;
-    rows.template tile<1>(p, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
+    rows.template tile<1>(p, c, at, at + KB, nullptr, kdocs, key_of(j), b.len, b.pre);
     // every fragment is in registers before the slot is filled again
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -963,7 +982,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   if constexpr (D == 256) rows.hold();
   __syncthreads();  // every ring is done with
   if (any_wave<W>(rows.spoilt(), lds)) {
-    odd_rows<D, BF16>(p, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);
+    odd_rows<D, BF16, FINE>(p, c, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);
     return;
   }
 
@@ -1099,13 +1118,25 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs p, long lon
 // 135 keys 9.6 -> 10.6; a split of 1520 keys in five 19.8 -> 21.1).
 inline bool pairs_of(const AttendArgs& a, int d) { return d <= 128 && a.nwg <= 256 && a.splits == 1 && a.keys > 192; }
 
+template <int D, bool BF16, bool FINE>
+void run_attend_rows(bool few, const AttendArgs& a, long long all_rows, const FineCap& c, hipStream_t s) {
+  if (few) {
+    attend_few_kernel<D, BF16, FINE><<<a.nwg, 64 * Few<D>::W, 0, s>>>(a, all_rows, c);
+    return;
+  }
+  if constexpr (D <= 128)
+    if (pairs_of(a, D)) {
+      attend_rows_kernel<D, BF16, 2, FINE><<<a.nwg, 512, 0, s>>>(a, all_rows, c);
+      return;
+    }
+  attend_rows_kernel<D, BF16, 1, FINE><<<a.nwg, 256, 0, s>>>(a, all_rows, c);
+}
+
 template <int D, bool BF16>
-hipError_t run_attend_elem(bool few, const AttendArgs& a, hipStream_t s) {
+hipError_t run_attend_elem(bool few, const AttendArgs& a, const FineCap* fine, hipStream_t s) {
   const long long blocks = a.nwg / ((long long)a.tiles * a.splits), all_rows = blocks * a.rows;
-  if (few) attend_few_kernel<D, BF16><<<a.nwg, 64 * Few<D>::W, 0, s>>>(a, all_rows);
-  else if (pairs_of(a, D)) {
-    if constexpr (D <= 128) attend_rows_kernel<D, BF16, 2><<<a.nwg, 512, 0, s>>>(a, all_rows);
-  } else attend_rows_kernel<D, BF16, 1><<<a.nwg, 256, 0, s>>>(a, all_rows);
+  if (fine) run_attend_rows<D, BF16, true>(few, a, all_rows, *fine, s);
+  else run_attend_rows<D, BF16, false>(few, a, all_rows, FineCap{}, s);
   if (a.splits > 1) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1123,8 +1154,8 @@ hipError_t run_attend_elem(bool few, const AttendArgs& a, hipStream_t s) {
 }  // namespace
 
 template <int D>
-hipError_t run_attend(bool bf16, bool few, const AttendArgs& a, hipStream_t s) {
-  return bf16 ? run_attend_elem<D, true>(few, a, s) : run_attend_elem<D, false>(few, a, s);
+hipError_t run_attend(bool bf16, bool few, const AttendArgs& a, const FineCap* fine, hipStream_t s) {
+  return bf16 ? run_attend_elem<D, true>(few, a, fine, s) : run_attend_elem<D, false>(few, a, fine, s);
 }
 
 }  // namespace xtk
