@@ -172,6 +172,33 @@ def test_attend_caps_of_scores_small_and_large(cuda, cap, n):
     ref.assert_within(o2, want, far)
 
 
+@pytest.mark.parametrize("nk,split", [(131072, True), (3000, False)])
+def test_attend_float16_weights_far_below_the_largest(cuda, nk, split):
+    """One key holds nearly all of the weight, the others some 2^-25.5 each."""
+    import torch
+
+    d = 64
+    p = K.masked_attention(1, 1, 1, 1, nk, d, dtype=xt.float16)
+    q, k = torch.zeros(1, 1, 1, d, device=cuda).half(), torch.zeros(1, 1, nk, d, device=cuda).half()
+    v = torch.ones(1, 1, nk, d, device=cuda).half()
+    q[0, 0, 0, 0], k[0, 0, 7, 0] = 1.0, 25.5 * math.log(2) * 8  # the scale is 1 / 8
+    v[0, 0, 7] = 0
+    k[0, 0, 100:200, 0], v[0, 0, 100:200, 3] = 30.0, -2.0
+    o = torch.zeros_like(q)
+    bufs = [t.data_ptr() for t in (q, k, v, o)], [2 * t.numel() for t in (q, k, v, o)]
+    if split:
+        xt.launch(p, q, k, v, o)
+    else:
+        xt._native.launch(p, None, *bufs, torch.cuda.current_stream().cuda_stream)
+    w = torch.softmax(k[0, 0].double() @ q[0, 0, 0].double() / 8, 0)
+    want = w @ v[0, 0].double()
+    # a weight of the largest's 2^-25.5 is held as one of 2^-18.5: steps of 2^-24
+    far = (2.0**-11 + 200 * 2.0**-24) * (w @ v[0, 0].double().abs()) + nk * 2.0**-32 * 1.0 + 2.0**-11 * want.abs() + 2.0**-25
+    say(float(want[0]), float(o[0, 0, 0, 0]))
+    assert float(far.max()) < 0.08 * float(want.max())
+    ref.assert_within(o[0, 0, 0], want, far)
+
+
 # -- matmul_q4 -----------------------------------------------------------------------
 
 

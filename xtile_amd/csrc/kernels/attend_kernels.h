@@ -62,7 +62,10 @@ typedef unsigned u4a __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned u2a __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr int kFar = 1 << 30;  // positions are held within this
-constexpr float kSlack = 8.0f;
+// Weights may reach 2^kSlack times that of the largest score so far.  In half precision
+// they are held 2^kRaise times larger: at most 2^15, and what is lost begins at 2^-32 of the
+// largest instead of 2^-25, of which a long row may have enough to matter.
+constexpr float kSlack = 8.0f, kRaise = 7.0f;
 
 // The LDS address of a pointer into LDS: the low half of its generic address (a cast
 // between address spaces compares with null first).
@@ -363,7 +366,8 @@ struct Rows {
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) most[r & 3] = fmaxf(most[r & 3], s[t][r]);
-    const float top = both_halves(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), true) * mul;
+    float top = both_halves(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), true) * mul;
+    if constexpr (!BF16) top -= kRaise;  // and so m is, wherever it goes with l and the sums
     // weights may reach 2^kSlack: the sums are rescaled only where a row's maximum
     // has grown by more (most tiles of a long row raise some row's by a little)
     if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) {
