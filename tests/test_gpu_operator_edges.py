@@ -199,6 +199,40 @@ def test_attend_float16_weights_far_below_the_largest(cuda, nk, split):
     ref.assert_within(o[0, 0, 0], want, far)
 
 
+@pytest.mark.parametrize("n", [1, 40, 64])
+def test_attend_infinite_values_of_small_weight(cuda, n):
+    """A weight that the values' type does not hold is not zero: its infinity counts."""
+    import torch
+
+    q, k, v = (torch.zeros(1, 1, s, 64, device=cuda).half() for s in (n, 64, 64))
+    q[..., 0] = 1
+    k[0, 0, 3, 0] = 40 * math.log(2) * 8
+    v[0, 0, 50, 6], v[0, 0, 51, 7] = math.inf, -math.inf
+    p = K.masked_attention(1, 1, 1, n, 64, 64, dtype=xt.float16)
+    o = torch.zeros_like(q)
+    xt.launch(p, q, k, v, o)
+    assert bool((o[..., 6] == math.inf).all()) and bool((o[..., 7] == -math.inf).all())
+    assert bool((o[..., :6] == 0).all()) and bool((o[..., 8:] == 0).all())
+
+
+@pytest.mark.parametrize("n", [1, 64])
+def test_attend_values_near_the_largest(cuda, n):
+    """The sums hold them: weights above one, between two rescalings, do not overflow."""
+    import torch
+
+    q, k, v = (torch.zeros(1, 1, s, 64, device=cuda).bfloat16() for s in (n, 1024, 1024))
+    q[..., 0] = 1
+    k[0, 0, 1000, 0] = 38.0  # a score of 4.75: 2^6.85 times the others' weight
+    v[0, 0, 1000, 2], v[0, 0, :, 4] = 3e38, 1.0
+    p = K.masked_attention(1, 1, 1, n, 1024, 64)
+    o = torch.zeros_like(q)
+    xt.launch(p, q, k, v, o)
+    w = math.exp(38.0 / 8) / (math.exp(38.0 / 8) + 1023)
+    want = w * float(v[0, 0, 1000, 2])
+    assert bool(((o[..., 2].double() - want).abs() <= want * (2 * 2.0**-8 + 1200 * 2.0**-24)).all())
+    assert bool((o[..., 4] == 1).all())
+
+
 # -- matmul_q4 -----------------------------------------------------------------------
 
 

@@ -154,7 +154,6 @@ struct Rows {
   int p0, p1;            // positions of the wave's first and last row
   float slope;           // times log2 e
   int doc;               // this lane's document
-  bool hidden;           // some row did not see some key of a tile that the wave worked on
   uint4v q[KK];
   float16v acc[N];
   float m, l;
@@ -177,7 +176,6 @@ struct Rows {
     below = p.window ? max(pos - p.window, -1) : -1;
     slope = p.slopes ? p.slopes[p.tslopes.at(bx, by, bz) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
     doc = p.qdocs ? p.qdocs[p.tqdocs.at(bx, by, bz) + token * p.qdoc_step] : 0;
-    hidden = false;
     const unsigned char* at = p.q + (p.tq.at(bx, by, bz) + head * p.q_head + token * p.q_row + 8 * hi) * 2;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) q[kk] = (uint4v)(*reinterpret_cast<const u4a*>(at + kk * 32));
@@ -266,7 +264,6 @@ struct Rows {
       }
       part |= by_doc || by_key;
     }
-    hidden |= part;
 
     float16v s[T];
 #pragma unroll
@@ -383,17 +380,18 @@ struct Rows {
     add_values<T>(V, s, vf, mul);
   }
 
-  // Whether a value that a row does not see may have spoilt its sums: a weight of 0
-  // times an infinity or NaN is NaN, and stays.  (A row's own infinities look alike;
-  // odd_rows, which does such rows again, tells them apart.  Where the total is not
-  // finite either, the row's own scores are not.)
+  // Whether a value may have spoilt a row's sums: a weight of 0, of a key that the row does
+  // not see or by rounding, times an infinity or NaN is NaN, and stays; and a weight above
+  // one, between rescalings, may take a value near the largest past it.  (Infinities that
+  // belong in the result look alike; odd_rows, which does such rows again, tells them apart.
+  // Where the total is not finite either, the row's own scores are not.)
   __device__ __forceinline__ bool spoilt() const {
     float t = 0.0f;
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) t = fmaf(acc[n][r], 0.0f, t);
-    return hidden && __builtin_amdgcn_ballot_w64(t != 0.0f && l - l == 0.0f) != 0;
+    return __builtin_amdgcn_ballot_w64(t != 0.0f && l - l == 0.0f) != 0;
   }
 
   // Weights e^(score - m), rounded to the values' type (off by half a step each, as
@@ -682,9 +680,19 @@ __device__ __forceinline__ float* total_of(const AttendArgs& p, int D, long long
   return p.work + rows * p.splits * D + 2 * (row * p.splits + split);
 }
 
+// The kernel's arguments (AttendArgs comes first), loaded where they are used: what only the
+// way of odd rows reads would take scalar registers in every launch's loop (2048 tokens, 16
+// heads of 32 columns, causal: 30.5 us so, 26.6).
+__device__ __forceinline__ const AttendArgs& args_here() {
+  auto at = (const __attribute__((address_space(4))) AttendArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return *(const AttendArgs*)at;
+}
+
 // Rows first, first + step, ... below last over the keys of tiles [i0, i1) of bn, a
-// wave each and in vector arithmetic: the way for keys among which hidden values are
-// not finite, of which only what a row sees is ever multiplied.  Lane j of 64 keys has
+// wave each and in vector arithmetic: the way for keys among which values are not finite
+// or near the largest, of which only what a row sees is ever multiplied, by weights of 32
+// bits and at most one.  Lane j of 64 keys has
 // the score of key j; then the lanes have the columns.
 template <int D, bool BF16, bool FINE>
 __device__ __forceinline__ void odd_rows(const AttendArgs& p, const FineCap& c, const BlockAt& b, const Tiles& tiles, int bn, int i0, int i1,
@@ -833,7 +841,7 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, FineCap c) {
   rows.hold();
   lds_barrier();
   if (any_wave<4 * G>(rows.spoilt(), lds)) {
-    odd_rows<D, BF16, FINE>(p, c, b, tiles, BN, i0, i1, kdocs, first + every, last + 1, 4 * G, all_rows);
+    odd_rows<D, BF16, FINE>(args_here(), c, b, tiles, BN, i0, i1, kdocs, first + every, last + 1, 4 * G, all_rows);
     return;
   }
   if constexpr (G == 2) {
@@ -986,7 +994,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   if constexpr (D == 256) rows.hold();
   __syncthreads();  // every ring is done with
   if (any_wave<W>(rows.spoilt(), lds)) {
-    odd_rows<D, BF16, FINE>(p, c, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);
+    odd_rows<D, BF16, FINE>(args_here(), c, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);
     return;
   }
 
