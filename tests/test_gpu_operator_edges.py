@@ -296,3 +296,17 @@ def test_rms_norm_scales_of_one_column_over_an_input(cuda, over):
     xt.launch(m, x, r, g, h, q, s)
     assert torch.equal(h, want_h.float()) and torch.equal(q, 127 * torch.sign(want_h).to(torch.int8))
     ref.assert_within(s, want.abs() / 127, want.abs() / 127 * 40 * 2.0**-24)
+
+
+@pytest.mark.parametrize("rows,cols", [(4096, 4096), (2, 100000)])
+def test_rms_norm_rows_in_8_bits_are_quotients_to_the_nearest(cuda, rows, cols):
+    """Of the values and the scale in 32 bits, as float32 division rounds them."""
+    import torch
+
+    x, g = rand((rows, cols), torch.float32, cuda, 1), rand((1, cols), torch.float32, cuda, 2)
+    y, s = torch.zeros_like(x), torch.zeros(rows, 1, device=cuda)
+    q = torch.zeros(rows, cols, dtype=torch.int8, device=cuda)
+    xt.launch(K.rms_norm(rows, cols, xt.float32, residual=False), x, g, y)
+    xt.launch(K.rms_norm(rows, cols, xt.float32, residual=False, quantize=True), x, g, q, s)
+    want = torch.round(y / s).clamp(-127, 127)
+    assert int((q.float() != want).sum()) == 0

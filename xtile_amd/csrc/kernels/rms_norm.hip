@@ -127,13 +127,31 @@ __device__ __forceinline__ void load8_of(int elem, const void* base, long long a
   else load8<kBF16>(base, at, n, v);
 }
 
-// y / s to int8, half to even.  `inv` is 1 / s, 0 where s is too small for a
-// normal reciprocal: those rows divide.
-__device__ __forceinline__ int to_i8(float y, float s, float inv) {
-  const float v = inv != 0.0f ? y * inv : s != 0.0f ? y / s : 0.0f;
+// y / s to int8, half to even.
+__device__ __forceinline__ int to_i8(float y, float s) {
+  const float v = s != 0.0f ? y / s : 0.0f;
   int i;  // saturates, NaN to 0; assembly because a C++ cast of such values is undefined
   asm("v_cvt_i32_f32 %0, %1" : "=v"(i) : "v"(__builtin_rintf(v)));
   return min(max(i, -127), 127);
+}
+
+// Four of them by inv = 1 / s: y inv, and what it leaves of y once more, is the quotient as
+// division rounds it, so that halves fall where they should.  |y| is at most 127 s but for a
+// few roundings, so none of them passes 127, and 1.5 2^23 more has the integer in its low byte.
+__device__ __forceinline__ unsigned to_i8x4(const float* y, float s, float inv) {
+  unsigned u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float q = y[i] * inv;
+    u[i] = __builtin_bit_cast(unsigned, fmaf(fmaf(-q, s, y[i]), inv, q) + 12582912.0f);
+  }
+  return __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u) | __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+}
+
+// What to_i8x4 takes of a row's scale: 0 for scales that are not finite, or too small for the
+// remainders to be normal numbers.  Such rows divide.
+__device__ __forceinline__ float inverse_scale(float s) {
+  return s >= 1.0e-30f && s < __builtin_inff() ? 1.0f / s : 0.0f;
 }
 
 __device__ __forceinline__ void store_y8(const NormArgs& p, long long at, int n, const float (&y)[8], float s, float inv) {
@@ -146,8 +164,13 @@ __device__ __forceinline__ void store_y8(const NormArgs& p, long long at, int n,
   } else {
     signed char* q = static_cast<signed char*>(p.y) + at;
     unsigned w[2] = {0, 0};
+    if (__builtin_amdgcn_readfirstlane(inv != 0.0f)) {  // of the row, which every lane has
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((unsigned)to_i8(y[i], s, inv) & 255u) << (8 * (i & 3));
+      for (int i = 0; i < 2; ++i) w[i] = to_i8x4(y + 4 * i, s, inv);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i >> 2] |= ((unsigned)to_i8(y[i], s) & 255u) << (8 * (i & 3));
+    }
     if (n >= 8) {
       typedef unsigned u2 __attribute__((ext_vector_type(2), aligned(1)));
       *reinterpret_cast<u2*>(q) = u2{w[0], w[1]};
@@ -297,9 +320,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(NormArgs p)
   float s = 0.0f, is = 0.0f;
   if (quantize) {
     s = __builtin_bit_cast(float, top) * inv / 127.0f;
-    is = s >= 1.0e-37f ? 1.0f / s : 0.0f;
+    is = inverse_scale(s);
     if (t == 0) p.scale[at.scale] = s;
-    if (s != s) is = s;
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -349,8 +371,7 @@ __global__ __launch_bounds__(T) void rms_norm_long_kernel(NormArgs p) {
   float s = 0.0f, is = 0.0f;
   if (quantize) {
     s = __builtin_bit_cast(float, top) * inv / 127.0f;
-    is = s >= 1.0e-37f ? 1.0f / s : 0.0f;
-    if (s != s) is = s;
+    is = inverse_scale(s);
   }
   for (int c = t * 8; c < p.cols; c += T * 8) {
     float h[8], g[8], y[8];
