@@ -128,6 +128,14 @@ int xt_gpu_run_with(xt_module* m, const char* func, void* const* bufs, const siz
 int xt_gpu_run_buffers_with(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, void* work,
                             size_t work_bytes, void* stream, char** err);
 
+/* xt_gpu_run_buffers with a workspace from `alloc`, which is called once the
+ * buffers are known to be the program's, at most once, and only for a program
+ * that works in one: `bytes` of device memory as above, or NULL, which refuses
+ * the launch (XT_ERR_ARGUMENT).  It throws nothing. */
+typedef void* (*xt_alloc)(void* context, size_t bytes);
+int xt_gpu_run_buffers_alloc(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, xt_alloc alloc,
+                             void* context, void* stream, char** err);
+
 #ifdef __cplusplus
 }
 #endif

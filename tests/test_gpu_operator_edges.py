@@ -310,3 +310,47 @@ def test_rms_norm_rows_in_8_bits_are_quotients_to_the_nearest(cuda, rows, cols):
     xt.launch(K.rms_norm(rows, cols, xt.float32, residual=False, quantize=True), x, g, q, s)
     want = torch.round(y / s).clamp(-127, 127)
     assert int((q.float() != want).sum()) == 0
+
+
+# -- launches ------------------------------------------------------------------------
+
+
+def test_a_launch_looks_its_program_up_once(cuda):
+    """One call into the library, which asks for a workspace only where the program has one."""
+    import ctypes
+
+    import torch
+
+    xt.launch(K.add(64, 64), *(torch.zeros(64, 64, device=cuda) for _ in range(3)))  # the native call is loaded
+    module, lib = xt._launch_native.__self__, xt._native.lib
+    alloc_t = ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t)
+    run_t = ctypes.CFUNCTYPE(ctypes.c_int, *([ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int]
+                                             + [ctypes.c_void_p] * 4))
+    own = ctypes.cast(lib.xt_gpu_run_buffers_alloc, ctypes.c_void_p).value
+    calls, asked = [], []
+
+    def run(m, func, bufs, n, alloc, context, stream, err):
+        @alloc_t
+        def counted(c, size):
+            asked.append(size)
+            return alloc_t(alloc)(c, size)
+
+        calls.append(func)
+        return run_t(own)(m, func, bufs, n, ctypes.cast(counted, ctypes.c_void_p), context, stream, err)
+
+    counting, release = run_t(run), ctypes.cast(lib.xt_free, ctypes.c_void_p).value
+    module.bind(ctypes.cast(counting, ctypes.c_void_p).value, release, xt._native.NativeModule)
+    try:
+        a, c = torch.ones(64, 64, device=cuda), torch.zeros(64, 64, device=cuda)
+        xt.launch(K.add(64, 64), a, a, c)
+        assert len(calls) == 1 and not asked and bool((c == 2).all())
+        p = K.masked_attention(1, 2, 4, 1, 5000, 64)
+        q, k, v = (rand(s, torch.bfloat16, cuda, i) for i, s in enumerate([(1, 8, 1, 64), (1, 2, 5000, 64), (1, 2, 5000, 64)]))
+        o = torch.zeros_like(q)
+        xt.launch(p, q, k, v, o)
+        assert len(calls) == 2 and asked == [xt.workspace(p)]
+    finally:
+        module.bind(own, release, xt._native.NativeModule)
+    o2 = torch.zeros_like(q)
+    xt.launch(p, q, k, v, o2)
+    assert torch.equal(o, o2) and len(calls) == 2

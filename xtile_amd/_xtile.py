@@ -117,6 +117,11 @@ SIGNATURES["xt_gpu_run_buffers_with"] = (
     [*SIGNATURES["xt_gpu_run_buffers"][1][:4], ctypes.c_void_p, ctypes.c_size_t,
      *SIGNATURES["xt_gpu_run_buffers"][1][4:]],
 )
+SIGNATURES["xt_gpu_run_buffers_alloc"] = (
+    ctypes.c_int,
+    [*SIGNATURES["xt_gpu_run_buffers"][1][:4], ctypes.c_void_p, ctypes.c_void_p,
+     *SIGNATURES["xt_gpu_run_buffers"][1][4:]],
+)
 
 
 def _load() -> ctypes.CDLL:

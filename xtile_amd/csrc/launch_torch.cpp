@@ -3,12 +3,11 @@
 // A launch through the Python checks (signature JSON, six attribute reads and
 // a size product a tensor, a device context manager, ctypes arrays) took 12-16
 // us of host time, several times what a small kernel runs; this call takes the
-// tensors' fields from their C++ objects and hands them to xt_gpu_run_buffers_with.
+// tensors' fields from their C++ objects and hands them to xt_gpu_run_buffers_alloc.
 //
-//   bind(run, free, type, workspace)     xt_gpu_run_buffers_with, xt_free and
-//                                        xt_workspace_bytes of the library that owns
-//                                        the module handles, as addresses, and the
-//                                        handles' type (None: capsules)
+//   bind(run, free, type)                xt_gpu_run_buffers_alloc and xt_free of the
+//                                        library that owns the module handles, as
+//                                        addresses, and the handles' type (None: capsules)
 //   launch(handle, buffers, func, stream) True when the program was enqueued.
 //                                        False when anything is not the plain
 //                                        case: the caller then takes the checked
@@ -39,12 +38,10 @@
 
 namespace {
 
-typedef int (*RunFn)(xt_module*, const char*, const xt_buffer*, int, void*, size_t, void*, char**);
-typedef int (*WorkFn)(xt_module*, const char*, size_t*, char**);
+typedef int (*RunFn)(xt_module*, const char*, const xt_buffer*, int, xt_alloc, void*, void*, char**);
 typedef void (*FreeFn)(void*);
 RunFn g_run = nullptr;
 FreeFn g_free = nullptr;
-WorkFn g_work = nullptr;
 PyTypeObject* g_handle = nullptr;  // the ctypes binding's NativeModule; nullptr: capsules
 PyObject* g_ptr_name = nullptr;    // "_ptr"
 
@@ -101,6 +98,25 @@ struct OnDevice {
   }
 };
 
+// A launch's workspace, from torch's allocator on the launch's stream.
+struct Workspace {
+  c10::DeviceIndex device;
+  void* stream;
+  c10::DataPtr memory;
+};
+
+// As xt_alloc: null where the stream is not torch's current one, or memory ran out.
+void* torch_memory(void* context, size_t bytes) {
+  Workspace& w = *static_cast<Workspace*>(context);
+  try {
+    if (w.stream != static_cast<void*>(c10::hip::getCurrentHIPStream(w.device).stream())) return nullptr;
+    w.memory = c10::hip::HIPCachingAllocator::get()->allocate(bytes);
+    return w.memory.get();
+  } catch (const std::exception&) {
+    return nullptr;
+  }
+}
+
 PyObject* launch_plain(PyObject* const* args) {
   xt_module* m = g_run ? module_of(args[0]) : nullptr;
   if (!m || !PyTuple_CheckExact(args[1])) Py_RETURN_FALSE;
@@ -144,21 +160,11 @@ PyObject* launch_plain(PyObject* const* args) {
   }
   char* err = nullptr;
   int st = XT_ERR_ARGUMENT;
-  const bool current = stream == static_cast<void*>(c10::hip::getCurrentHIPStream(device).stream());
+  Workspace work{device, stream, {}};
   Py_BEGIN_ALLOW_THREADS;
   try {
-    size_t need = 0;
-    st = g_work(m, func, &need, &err);
-    if (st == XT_OK && need == 0) {
-      st = g_run(m, func, b, static_cast<int>(n), nullptr, 0, stream, &err);
-    } else if (st == XT_OK && current) {
-      const c10::DataPtr work = c10::hip::HIPCachingAllocator::get()->allocate(need);
-      st = g_run(m, func, b, static_cast<int>(n), work.get(), need, stream, &err);
-    } else {
-      st = XT_ERR_ARGUMENT;
-    }
-  } catch (const std::exception&) {  // out of memory: the checked path says so
-    st = XT_ERR_ARGUMENT;
+    st = g_run(m, func, b, static_cast<int>(n), torch_memory, &work, stream, &err);
+  } catch (const std::exception&) {  // out of memory while planning: the checked path says so
   }
   Py_END_ALLOW_THREADS;
   const std::string text = err ? err : "launch failed";
@@ -185,13 +191,11 @@ PyObject* launch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  void* run = nargs == 4 && PyLong_Check(args[0]) ? PyLong_AsVoidPtr(args[0]) : nullptr;
-  void* release = nargs == 4 && PyLong_Check(args[1]) ? PyLong_AsVoidPtr(args[1]) : nullptr;
-  void* work = nargs == 4 && PyLong_Check(args[3]) ? PyLong_AsVoidPtr(args[3]) : nullptr;
+  void* run = nargs == 3 && PyLong_Check(args[0]) ? PyLong_AsVoidPtr(args[0]) : nullptr;
+  void* release = nargs == 3 && PyLong_Check(args[1]) ? PyLong_AsVoidPtr(args[1]) : nullptr;
   if (PyErr_Occurred()) return nullptr;
-  if (!run || !release || !work || (args[2] != Py_None && !PyType_Check(args[2]))) {
-    PyErr_SetString(PyExc_ValueError, "bind(address of xt_gpu_run_buffers_with, address of xt_free, handle type or None, "
-                                      "address of xt_workspace_bytes)");
+  if (!run || !release || (args[2] != Py_None && !PyType_Check(args[2]))) {
+    PyErr_SetString(PyExc_ValueError, "bind(address of xt_gpu_run_buffers_alloc, address of xt_free, handle type or None)");
     return nullptr;
   }
   PyObject* const was = reinterpret_cast<PyObject*>(g_handle);
@@ -203,7 +207,6 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Py_XDECREF(was);
   g_run = reinterpret_cast<RunFn>(run);
   g_free = reinterpret_cast<FreeFn>(release);
-  g_work = reinterpret_cast<WorkFn>(work);
   Py_RETURN_NONE;
 }
 
@@ -211,7 +214,7 @@ PyMethodDef kMethods[] = {
     {"launch", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(launch)), METH_FASTCALL,
      "launch(handle, buffers, func, stream) -> bool: whether the program was enqueued"},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL,
-     "bind(xt_gpu_run_buffers_with, xt_free, type, xt_workspace_bytes): the library's functions, as addresses, and its handles' type"},
+     "bind(xt_gpu_run_buffers_alloc, xt_free, type): the library's functions, as addresses, and its handles' type"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_launch", "xt.launch over torch tensors", -1, kMethods,

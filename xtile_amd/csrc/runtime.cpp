@@ -116,6 +116,44 @@ int elem_code(xt::Elem e) {
   }
 }
 
+struct Work {
+  void* at;
+  size_t bytes;
+  bool given;  // false: the launch is refused
+};
+
+// A launch over described buffers, in the workspace that `work_of` gives for a plan.
+template <class F>
+int run_buffers(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, F work_of, void* stream, char** err) {
+  if (!m) return fail(err, XT_ERR_TYPE, "expected an xtile module");
+  return guarded(err, [&]() -> int {
+    std::shared_ptr<const xt::Plan> plan;
+    {
+      std::lock_guard<std::mutex> lock(m->mu);
+      int st = get_plan(m, func_key(func), plan, err);
+      if (st != XT_OK) return st;
+    }
+    const xt::Plan& p = *plan;
+    constexpr int kMost = 16;
+    if (nbufs != static_cast<int>(p.arg_types.size()) || nbufs > kMost || !bufs)
+      return fail(err, XT_ERR_ARGUMENT, "@" + p.func + " takes " + std::to_string(p.arg_types.size()) +
+                                            " buffers (at most " + std::to_string(kMost) + " described ones)");
+    void* ptrs[kMost] = {};
+    for (int k = 0; k < nbufs; ++k) {
+      const xt::Type& t = p.arg_types[k];
+      bool same = bufs[k].ptr && bufs[k].dtype == elem_code(t.elem) && bufs[k].rank == static_cast<int>(t.shape.size()) &&
+                  (bufs[k].shape || bufs[k].rank == 0);
+      for (int d = 0; same && d < bufs[k].rank; ++d) same = bufs[k].shape[d] == t.shape[d];
+      if (!same) return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is not a " + t.str());
+      ptrs[k] = bufs[k].ptr;
+    }
+    const Work w = work_of(p);
+    if (!w.given) return fail(err, XT_ERR_ARGUMENT, "@" + p.func + " works in " + std::to_string(p.workspace) +
+                                                        " bytes, of which none were given");
+    return run_plan(p, ptrs, w.at, w.bytes, stream, err);
+  });
+}
+
 }  // namespace
 
 extern "C" {
@@ -278,30 +316,18 @@ int xt_gpu_run_with(xt_module* m, const char* func, void* const* bufs, const siz
 
 int xt_gpu_run_buffers_with(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, void* work,
                             size_t work_bytes, void* stream, char** err) {
-  if (!m) return fail(err, XT_ERR_TYPE, "expected an xtile module");
-  return guarded(err, [&]() -> int {
-    std::shared_ptr<const xt::Plan> plan;
-    {
-      std::lock_guard<std::mutex> lock(m->mu);
-      int st = get_plan(m, func_key(func), plan, err);
-      if (st != XT_OK) return st;
-    }
-    const xt::Plan& p = *plan;
-    constexpr int kMost = 16;
-    if (nbufs != static_cast<int>(p.arg_types.size()) || nbufs > kMost || !bufs)
-      return fail(err, XT_ERR_ARGUMENT, "@" + p.func + " takes " + std::to_string(p.arg_types.size()) +
-                                            " buffers (at most " + std::to_string(kMost) + " described ones)");
-    void* ptrs[kMost] = {};
-    for (int k = 0; k < nbufs; ++k) {
-      const xt::Type& t = p.arg_types[k];
-      bool same = bufs[k].ptr && bufs[k].dtype == elem_code(t.elem) && bufs[k].rank == static_cast<int>(t.shape.size()) &&
-                  (bufs[k].shape || bufs[k].rank == 0);
-      for (int d = 0; same && d < bufs[k].rank; ++d) same = bufs[k].shape[d] == t.shape[d];
-      if (!same) return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is not a " + t.str());
-      ptrs[k] = bufs[k].ptr;
-    }
-    return run_plan(p, ptrs, work, work_bytes, stream, err);
-  });
+  return run_buffers(m, func, bufs, nbufs, [&](const xt::Plan&) { return Work{work, work_bytes, true}; }, stream, err);
+}
+
+int xt_gpu_run_buffers_alloc(xt_module* m, const char* func, const xt_buffer* bufs, int nbufs, xt_alloc alloc,
+                             void* context, void* stream, char** err) {
+  if (!alloc) return fail(err, XT_ERR_ARGUMENT, "null alloc");
+  auto work_of = [&](const xt::Plan& p) {
+    if (!p.workspace) return Work{nullptr, 0, true};
+    void* const at = alloc(context, static_cast<size_t>(p.workspace));
+    return Work{at, static_cast<size_t>(p.workspace), at != nullptr};
+  };
+  return run_buffers(m, func, bufs, nbufs, work_of, stream, err);
 }
 
 }  // extern "C"
