@@ -233,6 +233,24 @@ def test_attend_values_near_the_largest(cuda, n):
     assert bool((o[..., 4] == 1).all())
 
 
+@pytest.mark.parametrize("n,nk", [(1, 100), (3, 100), (70, 100), (2, 2000)])
+@pytest.mark.parametrize("start,window", [(2**31 - 1, 2**31 - 1), (2**31 - 50, 2**31 - 30), (2**30, 2**30 - 20),
+                                          (2**30 - 1, 2**30 + 50), (2**31 - 1, 5), (2**30 - 60, 2**30), (-(2**31), 7),
+                                          (-(2**30) - 5, 2**31 - 1), (97, 2**31 - 1)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attend_windows_at_far_positions(cuda, causal, start, window, n, nk):
+    """Positions of 31 bits and windows as large, of which a row sees none, some or all keys."""
+    import torch
+
+    p = K.masked_attention(1, 1, 1, n, nk, 64, causal=causal, window=window, start=True)
+    q, k, v = (rand((1, 1, s, 64), torch.bfloat16, cuda, i) for i, s in enumerate((n, nk, nk)))
+    st = torch.tensor([[start]], dtype=torch.int32, device=cuda)
+    o = torch.full_like(q, 7)
+    xt.launch(p, q, k, v, st, o)
+    want, far = ref.attend(q, k, v, 0.125, causal=causal, window=window, start=st)
+    ref.assert_within(o, want, far)
+
+
 # -- matmul_q4 -----------------------------------------------------------------------
 
 

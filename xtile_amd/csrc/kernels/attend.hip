@@ -143,7 +143,7 @@ hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipSt
     if (!ordinary || t.cap > 256) look = &fine;
   }
   a.causal = t.causal;
-  a.window = static_cast<int>(std::min<int64_t>(t.window, 1 << 30));
+  a.window = static_cast<int>(t.window);
   // DMA takes 16-byte aligned rows, of which 64 lie within a descriptor's 4 GiB;
   // other rows go through registers
   auto chunks = [&](const xt::AttendAccess& x) {

@@ -127,6 +127,11 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
   }
 }
 
+// The last key that a window hides from a row at pos: -1 for none, or without windows.
+__device__ __forceinline__ int before(const AttendArgs& p, int window, int pos) {
+  return !p.window || pos < window ? -1 : pos - window;
+}
+
 // What one wave's 32 query rows see, and its running softmax.  Lane (c = lane % 32,
 // h = lane / 32) holds row c; of a tile of 32 keys it holds the scores of keys
 // 8 (r / 4) + 4 h + r % 4 in register r, and of the result columns
@@ -152,6 +157,7 @@ struct Rows {
   int row, token;        // this lane's row of the Block (the last one past the end) and its token
   int pos, above, below; // sees key j when below < j <= above (or j < prefix)
   int p0, p1;            // positions of the wave's first and last row
+  int w0, w1;            // the last keys before their windows
   float slope;           // times log2 e
   int doc;               // this lane's document
   uint4v q[KK];
@@ -162,7 +168,7 @@ struct Rows {
   static constexpr bool LEAN = D == 256;
   int koff[LEAN ? 1 : KK], voff[N];
 
-  __device__ __forceinline__ void begin(const AttendArgs& p, int first, int bx, int by, int bz, int start) {
+  __device__ __forceinline__ void begin(const AttendArgs& p, int first, int bx, int by, int bz, int start, int window) {
     lane = threadIdx.x & 63;
     col = lane & 31;
     hi = lane >> 5;
@@ -173,7 +179,9 @@ struct Rows {
     p0 = start + (int)p.d_heads((unsigned)min(first, p.rows - 1));
     p1 = start + (int)p.d_heads((unsigned)min(first + 31, p.rows - 1));
     above = p.causal ? min(pos, kFar) : kFar;
-    below = p.window ? max(pos - p.window, -1) : -1;
+    below = before(p, window, pos);
+    w0 = before(p, window, p0);
+    w1 = before(p, window, p1);
     slope = p.slopes ? p.slopes[p.tslopes.at(bx, by, bz) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
     doc = p.qdocs ? p.qdocs[p.tqdocs.at(bx, by, bz) + token * p.qdoc_step] : 0;
     const unsigned char* at = p.q + (p.tq.at(bx, by, bz) + head * p.q_head + token * p.q_row + 8 * hi) * 2;
@@ -226,10 +234,10 @@ struct Rows {
 
   // Whether the wave's rows see all of keys [key0, key0 + n), documents aside, or none.
   __device__ __forceinline__ bool sees_all(const AttendArgs& p, int key0, int n, int len, int pre) const {
-    return key0 + n <= len && (key0 + n <= pre || ((!p.causal || key0 + n - 1 <= p0) && (!p.window || key0 > p1 - p.window)));
+    return key0 + n <= len && (key0 + n <= pre || ((!p.causal || key0 + n - 1 <= p0) && key0 > w1));
   }
   __device__ __forceinline__ bool sees_none(const AttendArgs& p, int key0, int n, int pre) const {
-    return key0 >= pre && ((p.causal && key0 > p1) || (p.window && key0 + n - 1 <= p0 - p.window));
+    return key0 >= pre && ((p.causal && key0 > p1) || key0 + n - 1 <= w0);
   }
 
   // Of a lane's 16 registers of a tile of 32 keys, as bits, those whose key is at most
@@ -452,8 +460,9 @@ struct Tiles {
 
 // p0, p1: the workgroup's first and last position; [d0, d1): the keys whose
 // documents may be its rows'.
-__device__ __forceinline__ Tiles tiles_of(const AttendArgs& p, int bn, int p0, int p1, int len, int pre, int d0, int d1) {
-  const int b0 = max(p.window ? max(0, p0 - p.window + 1) : 0, d0);
+__device__ __forceinline__ Tiles tiles_of(const AttendArgs& p, int bn, int p0, int p1, int window, int len, int pre, int d0,
+                                          int d1) {
+  const int b0 = max(before(p, window, p0) + 1, d0);
   const int b1 = min(p.causal ? min(len, max(p1, -1) + 1) : len, d1);
   const int a1 = min(pre, d1);
   Tiles t;
@@ -541,9 +550,16 @@ __device__ __forceinline__ void document_keys(const AttendArgs& p, const int* qd
 }
 
 struct BlockAt {
-  int x, y, z, tile, split, start, len, pre;
+  int x, y, z, tile, split, start, window, len, pre;
   long long block;
 };
+
+// A first position, held within +-kFar; so far past every key its window is shorter by what
+// that takes off, which leaves the keys that the rows see, and scores but for one constant.
+__device__ __forceinline__ void hold_start(const AttendArgs& p, int start, BlockAt& b) {
+  b.start = min(max(start, -kFar), kFar - 1);
+  if (start > kFar - 1) b.window = max(p.window - (start - (kFar - 1)), 0);
+}
 
 template <bool FEW>
 __device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
@@ -558,6 +574,7 @@ __device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
   p.blocks(blk, b.x, b.y, b.z);
   if constexpr (FEW) {
     b.start = 0;
+    b.window = p.window;
     b.len = p.keys;
     b.pre = 0;
     if (p.start || p.length || p.prefix) {
@@ -567,16 +584,19 @@ __device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
       const int start = *(p.start ? p.start + p.tstart.at(b.x, b.y, b.z) : any);
       const int len = *(p.length ? p.length + p.tlength.at(b.x, b.y, b.z) : any);
       const int pre = *(p.prefix ? p.prefix + p.tprefix.at(b.x, b.y, b.z) : any);
-      if (p.start) b.start = min(max(start, -kFar), kFar - 1);
+      if (p.start) hold_start(p, start, b);
       if (p.length) b.len = min(max(len, 0), p.keys);
       if (p.prefix) b.pre = min(max(pre, 0), b.len);
     }
   } else {
-    b.start = p.start ? min(max(p.start[p.tstart.at(b.x, b.y, b.z)], -kFar), kFar - 1) : 0;
+    b.start = 0;
+    b.window = p.window;
+    if (p.start) hold_start(p, p.start[p.tstart.at(b.x, b.y, b.z)], b);
     b.len = p.length ? min(max(p.length[p.tlength.at(b.x, b.y, b.z)], 0), p.keys) : p.keys;
     b.pre = p.prefix ? min(max(p.prefix[p.tprefix.at(b.x, b.y, b.z)], 0), b.len) : 0;
   }
   b.start = __builtin_amdgcn_readfirstlane(b.start);
+  b.window = __builtin_amdgcn_readfirstlane(b.window);
   b.len = __builtin_amdgcn_readfirstlane(b.len);
   b.pre = __builtin_amdgcn_readfirstlane(b.pre);
   return b;
@@ -711,7 +731,7 @@ __device__ __forceinline__ void odd_rows(const AttendArgs& p, const FineCap& c, 
     const float slope = p.slopes ? p.slopes[p.tslopes.at(b.x, b.y, b.z) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
     const int doc = p.qdocs ? p.qdocs[p.tqdocs.at(b.x, b.y, b.z) + token * p.qdoc_step] : 0;
     auto sees = [&](int j, int end) {
-      return j < end && j < b.len && (j < b.pre || ((!p.causal || j <= pos) && (!p.window || j > pos - p.window))) &&
+      return j < end && j < b.len && (j < b.pre || ((!p.causal || j <= pos) && j > before(p, b.window, pos))) &&
              (!kdocs || kdocs[j] == doc);
     };
     auto score = [&](int j) {
@@ -807,7 +827,7 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, FineCap c) {
   if (kdocs)
     document_keys<4 * G>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, t0, t1, last_key(p, b, t1), reinterpret_cast<int*>(lds),
                      d0, d1);
-  const Tiles tiles = tiles_of(p, BN, b.start + t0, b.start + t1, b.len, b.pre, d0, d1);
+  const Tiles tiles = tiles_of(p, BN, b.start + t0, b.start + t1, b.window, b.len, b.pre, d0, d1);
   const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
   const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
 
@@ -824,7 +844,7 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, FineCap c) {
   unsigned char* const stages = lds + group * 2 * STAGE;
   if (i0 + group < i1) issue(i0 + group, stages);
   Rows<D, BF16, FINE> rows;
-  rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start);
+  rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start, b.window);
 #pragma unroll 1
   for (int i = i0 + group, n = 0; i - group < i1; i += G, n ^= 1) {
     // one barrier a tile: behind it this tile has landed, and every wave is done with
@@ -948,7 +968,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   if (kdocs)
     document_keys<W>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, 0, t1, last_key(p, b, t1), reinterpret_cast<int*>(lds),
                      d0, d1);
-  const Tiles tiles = tiles_of(p, 32, b.start, b.start + t1, b.len, b.pre, d0, d1);
+  const Tiles tiles = tiles_of(p, 32, b.start, b.start + t1, b.window, b.len, b.pre, d0, d1);
   const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
   const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
   const int mine = max(0, (i1 - i0 - wave + W - 1) / W);
@@ -969,7 +989,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   for (int j = 0; j < NS; ++j)
     if (j < mine) issue(j, j);
   Rows<D, BF16, FINE> rows;
-  rows.begin(p, 0, b.x, b.y, b.z, b.start);
+  rows.begin(p, 0, b.x, b.y, b.z, b.start, b.window);
   int slot = 0;
 #pragma unroll 1
   for (int j = 0; j < mine; ++j) {
