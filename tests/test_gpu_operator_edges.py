@@ -330,6 +330,21 @@ def test_rms_norm_rows_in_8_bits_are_quotients_to_the_nearest(cuda, rows, cols):
     assert int((q.float() != want).sum()) == 0
 
 
+@pytest.mark.parametrize("cols", [5, 64, 2000, 40000])
+def test_rms_norm_rows_in_8_bits_of_products_below_the_normal_numbers(cuda, cols):
+    """Values and gamma so small that the largest of their products has a bit or two: the
+    integers keep their sign and stay within 127."""
+    import torch
+
+    x, g = 1e-19 * rand((9, cols), torch.float32, cuda, 1), torch.full((1, cols), 1.5e-26, device=cuda)
+    q, s = torch.full((9, cols), 99, dtype=torch.int8, device=cuda), torch.zeros(9, 1, device=cuda)
+    xt.launch(K.rms_norm(9, cols, xt.float32, residual=False, quantize=True, eps=1e-38), x, g, q, s)
+    assert int(q.min()) >= -127 and bool((q.float() * x >= 0).all())
+    _, want = ref.rms_norm(x, None, g, 1e-38)
+    # the squares, too, are near the smallest normal number: 2^-8 of a quotient at most
+    assert bool(((q.double() - (want / s.double()).clamp(-127, 127)).abs() <= 0.5 + 2.0**-1).all())
+
+
 # -- launches ------------------------------------------------------------------------
 
 

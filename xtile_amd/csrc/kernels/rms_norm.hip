@@ -149,9 +149,10 @@ __device__ __forceinline__ unsigned to_i8x4(const float* y, float s, float inv) 
 }
 
 // What to_i8x4 takes of a row's scale: 0 for scales that are not finite, or too small for the
-// remainders to be normal numbers.  Such rows divide.
-__device__ __forceinline__ float inverse_scale(float s) {
-  return s >= 1.0e-30f && s < __builtin_inff() ? 1.0f / s : 0.0f;
+// remainders to be normal numbers, or from a product `top` of too few bits for its values to
+// be at most 127 of them.  Such rows divide.
+__device__ __forceinline__ float inverse_scale(float s, unsigned top) {
+  return s >= 1.0e-30f && s < __builtin_inff() && __builtin_bit_cast(float, top) >= 1.0e-30f ? 1.0f / s : 0.0f;
 }
 
 __device__ __forceinline__ void store_y8(const NormArgs& p, long long at, int n, const float (&y)[8], float s, float inv) {
@@ -320,7 +321,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(NormArgs p)
   float s = 0.0f, is = 0.0f;
   if (quantize) {
     s = __builtin_bit_cast(float, top) * inv / 127.0f;
-    is = inverse_scale(s);
+    is = inverse_scale(s, top);
     if (t == 0) p.scale[at.scale] = s;
   }
 #pragma unroll
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(T) void rms_norm_long_kernel(NormArgs p) {
   float s = 0.0f, is = 0.0f;
   if (quantize) {
     s = __builtin_bit_cast(float, top) * inv / 127.0f;
-    is = inverse_scale(s);
+    is = inverse_scale(s, top);
   }
   for (int c = t * 8; c < p.cols; c += T * 8) {
     float h[8], g[8], y[8];
