@@ -30,8 +30,9 @@
 // m, l and sums in the workspace, and a second kernel joins them.
 //
 // Many rows are bound by the arithmetic of the softmax (4096 tokens, 32 heads of 128
-// columns on 8 key heads, causal, capped: 172 to 184 us, 0.75 to 0.80 PFLOP/s), single
-// tokens by HBM (64 heads of 128 on 8, 131072 keys: 103 to 108 us, 5.0 to 5.2 TB/s).
+// columns on 8 key heads, causal, capped: 166 to 181 us, 0.76 to 0.83 PFLOP/s; 158 without
+// the cap), single tokens by HBM (64 heads of 128 on 8, 131072 keys: 102 to 107 us, 5.0 to
+// 5.2 TB/s).
 #include "attend_kernels.h"
 
 #include <cmath>

@@ -9,7 +9,8 @@
 // max |y| = max |h gamma| / sqrt(...): one exchange over the group serves both.
 //
 // HBM bounds it for many rows (8192 of 4096 bf16 values with a residual to int8: 235 MB
-// in 47.3 us, 5.0 TB/s), one group's latency for one row.  A row takes
+// in 41.2 us by the tracer, 5.7 TB/s; 46.3 to 47.5 a launch of a graph), one group's latency
+// for one row (2.6 us by the tracer).  A row takes
 // 64 threads (rows to 1024 values, no barrier), 256 (to 8192) or 1024; longer
 // rows, and those of fewer than eight values, are read again for the second half
 // (rms_norm_long_kernel).
@@ -257,9 +258,10 @@ struct Raw8 {
 
 // T threads a row, NV vectors of eight values each; GWIDE: gamma has 32 bits.  Every
 // load is on its way before the first value is looked at: none is conditional, and none
-// is converted where it is loaded (one row of 4096 bf16 values 3.0 us, with the loads
-// one behind the other 3.6; 8192 rows to int8 47.5 us, and 61).  A vector that would pass the row's end starts eight values
-// before it: its first ones are also its neighbour's, count once and are stored twice.
+// is converted where it is loaded (launches in a graph: one row of 4096 bf16 values 3.0 us,
+// with the loads one behind the other 3.6; 8192 rows to int8 47.5 us, and 61).  A vector that
+// would pass the row's end starts eight values before it: its first ones are also its
+// neighbour's, count once and are stored twice.
 template <int ELEM, int T, int NV, bool GWIDE>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(NormArgs p) {
   constexpr int R = T < 256 ? 256 / T : 1;  // rows of a workgroup
