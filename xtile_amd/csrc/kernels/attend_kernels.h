@@ -62,9 +62,9 @@ typedef unsigned u4a __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned u2a __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr int kFar = 1 << 30;  // positions are held within this
-// Weights may reach 2^kSlack times that of the largest score so far.  In half precision
-// they are held 2^kRaise times larger: at most 2^15, and what is lost begins at 2^-32 of the
-// largest instead of 2^-25, of which a long row may have enough to matter.
+// Weights may reach 2^kSlack times that of the largest score that the sums are relative to.
+// In half precision they are held 2^kRaise times larger: at most 2^15, and what is lost
+// begins at 2^-32 of the largest instead of 2^-25, of which a long row may have enough to matter.
 constexpr float kSlack = 8.0f, kRaise = 7.0f;
 
 // The LDS address of a pointer into LDS: the low half of its generic address (a cast
@@ -702,7 +702,7 @@ __device__ __forceinline__ float* total_of(const AttendArgs& p, int D, long long
 
 // The kernel's arguments (AttendArgs comes first), loaded where they are used: what only the
 // way of odd rows reads would take scalar registers in every launch's loop (2048 tokens, 16
-// heads of 32 columns, causal: 30.5 us so, 26.6).
+// heads of 32 columns, causal: 30.5 us if kept in registers, 26.6 if loaded here).
 __device__ __forceinline__ const AttendArgs& args_here() {
   auto at = (const __attribute__((address_space(4))) AttendArgs*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(at));
@@ -715,8 +715,9 @@ __device__ __forceinline__ const AttendArgs& args_here() {
 // bits and at most one.  Lane j of 64 keys has
 // the score of key j; then the lanes have the columns.
 template <int D, bool BF16, bool FINE>
-__device__ __forceinline__ void odd_rows(const AttendArgs& p, const FineCap& c, const BlockAt& b, const Tiles& tiles, int bn, int i0, int i1,
-                                         const int* kdocs, int first, int last, int step, long long all_rows) {
+__device__ __forceinline__ void odd_rows(const AttendArgs& p, const FineCap& c, const BlockAt& b, const Tiles& tiles,
+                                         int bn, int i0, int i1, const int* kdocs, int first, int last, int step,
+                                         long long all_rows) {
   const int lane = threadIdx.x & 63;
   auto value = [](unsigned short x) {
     return BF16 ? __builtin_bit_cast(float, (unsigned)x << 16) : (float)__builtin_bit_cast(_Float16, x);
