@@ -1,0 +1,227 @@
+"""Sampling on the GPU against its definition in 64 bits: the same tokens."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import xtile_amd as xt
+from xtile_amd import kernels as K
+
+from . import answers_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": xt.float32, "f16": xt.float16, "bf16": xt.bfloat16}
+
+
+def torch_dtype(name):
+    import torch
+
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def column(v, rows, dtype):
+    """A (rows, 1) tensor of a number, or of one for each row."""
+    import torch
+
+    return torch.tensor(v, dtype=dtype).expand(rows).reshape(rows, 1).contiguous().cuda()
+
+
+def run(x, u, dtype, without_workspace=False, trow=None, **params):
+    """Tokens of a CPU tensor of logits; params: numbers or lists of one a row."""
+    import torch
+
+    rows, vocab = x.shape
+    asked = {k: v for k, v in params.items() if v is not None}
+    m = K.sample(rows, vocab, DTYPES[dtype], trow=trow, **{k: True for k in asked})
+    print(f"[gpu] {xt.plan(m)['kernel']}", flush=True)
+    y = torch.full((rows, 1), -7, dtype=torch.int32, device="cuda")
+    bufs = [x.cuda(), column(u, rows, torch.float32)]
+    for name in ("temperature", "top_k", "top_p", "min_p"):
+        if name in asked:
+            bufs.append(column(asked[name], rows, torch.int32 if name == "top_k" else torch.float32))
+    bufs.append(y)
+    if without_workspace:
+        from xtile_amd import _xtile
+
+        _xtile.launch(m, None, [t.data_ptr() for t in bufs], [t.numel() * t.element_size() for t in bufs],
+                      torch.cuda.current_stream().cuda_stream)
+    else:
+        xt.launch(m, *bufs)
+    return y.view(-1).tolist()
+
+
+def want(x, u, **params):
+    rows = x.shape[0]
+
+    def of(v, r, kind=np.float32):
+        return None if v is None else kind(v[r] if isinstance(v, (list, tuple)) else v)
+
+    return [ref.sample(x[r].double().numpy(), of(u, r),
+                       **{k: of(v, r, np.int32 if k == "top_k" else np.float32) for k, v in params.items()})
+            for r in range(rows)]
+
+
+def check(x, u, dtype="f32", **params):
+    w = want(x, u, **params)
+    assert run(x, u, dtype, **params) == w
+    assert run(x, u, dtype, without_workspace=True, **params) == w
+
+
+def logits(rows, vocab, dtype, seed, spread=2.5):
+    import torch
+
+    g = torch.Generator().manual_seed(seed)
+    return (spread * torch.randn(rows, vocab, generator=g)).to(torch_dtype(dtype))
+
+
+def uniforms(rows, seed):
+    return np.random.default_rng(seed).random(rows).astype(np.float32).tolist()
+
+
+OPTIONS = [{}, {"temperature": 0.7}, {"top_k": 40}, {"top_p": 0.9}, {"min_p": 0.05},
+           {"temperature": 1.3, "top_k": 1000, "top_p": 0.97, "min_p": 0.001}]
+
+
+@pytest.mark.parametrize("options", OPTIONS, ids=lambda o: "-".join(o) or "none")
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 32768, "f32"), (9, 50001, "bf16"), (5, 1000, "f16"), (3, 131072, "f32"),
+                                              (70, 4097, "f32")])
+def test_sizes(rows, vocab, dtype, options):
+    check(logits(rows, vocab, dtype, vocab), uniforms(rows, vocab), dtype, **options)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 3, 7, 8, 31, 63, 65, 255, 2047, 2048, 2049])
+def test_short_rows(vocab):
+    rows = 12
+    x = logits(rows, vocab, "f32", vocab)
+    check(x, uniforms(rows, vocab))
+    check(x, uniforms(rows, vocab), top_p=0.5, top_k=[1, 2, 3, vocab, vocab + 1, 0, -1, 5, vocab - 1, 9, 100, 1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("options", [{}, {"top_k": 3000}, {"top_p": 0.3}, {"top_k": 20000, "top_p": 0.6}, {"min_p": 0.3}],
+                         ids=lambda o: "-".join(o) or "none")
+def test_many_equal_logits(dtype, options):
+    """Halves, so that thousands are equal: by index."""
+    x = (logits(6, 30000, "f32", 3, 1.0) * 2).round().div(2).to(torch_dtype(dtype))
+    check(x, uniforms(6, 8), dtype, **options)
+
+
+@pytest.mark.parametrize("vocab", [6, 2048, 2049, 5000, 70000])
+def test_rows_of_one_value(vocab):
+    """Weights are all 1: the token is the one that u, and the cuts, count out."""
+    import torch
+
+    x = torch.full((5, vocab), -3.25)
+    u = [0.0, 0.5, 0.25, 0.999, 0.7]
+    assert run(x, u, "f32") == [int(np.floor(np.float64(np.float32(v)) * vocab)) for v in u]
+    check(x, u)
+    check(x, u, top_k=[1, 2, 5, 3000, vocab], top_p=[0.5, 0.1, 1.0, 0.0, 0.75])
+    check(x, u, temperature=[0.0, 1e-30, 1e30, float("inf"), 2.0])
+
+
+def test_odd_logits():
+    """Infinities, NaN and zeros of both signs."""
+    import torch
+
+    inf, nan = float("inf"), float("nan")
+    rows = [[-inf] * 9, [nan] * 9, [nan, -inf, 1.0, nan, 0.0, -inf, 1.0, 1.0, nan], [inf, 0.0, inf, -inf, nan, inf, 1.0, 2.0, 3.0],
+            [0.0, -0.0, 0.0, -0.0, -1.0, -inf, 0.0, -0.0, 0.0], [-inf] * 8 + [-1e38], [3e38, -3e38, 3e38, 0, 0, 0, 0, 0, 0],
+            [1e-45, -1e-45, 0.0, 1e-45, 0, 0, 0, 0, 0]]
+    x = torch.tensor(rows)
+    for u in (0.0, 0.3, 0.6, 0.999):
+        for options in ({}, {"temperature": 0.5}, {"temperature": 0.0}, {"temperature": inf}, {"top_k": 4}, {"top_p": 0.5},
+                        {"min_p": 0.9}, {"top_k": 2, "top_p": 0.2, "min_p": 1.0}):
+            check(x, u, **options)
+    assert run(x, 0.3, "f32")[:2] == [-1, -1]
+
+
+def test_odd_parameters():
+    """Each parameter past its range, and NaN."""
+    inf, nan = float("inf"), float("nan")
+    x = logits(8, 700, "f32", 1)
+    check(x, [0.0, -1.0, 1.0, 2.0, nan, inf, -inf, float(np.nextafter(np.float32(1), np.float32(0)))])
+    check(x, uniforms(8, 2), temperature=[0.0, -1.0, nan, inf, 1e-45, 3e38, -inf, 1e-3])
+    check(x, uniforms(8, 3), top_p=[0.0, -1.0, 1.0, 2.0, nan, inf, -inf, 1e-30])
+    check(x, uniforms(8, 4), min_p=[0.0, -1.0, 1.0, 2.0, nan, inf, -inf, 1e-30])
+    check(x, uniforms(8, 5), top_k=[0, -1, 1, 700, 701, 2**31 - 1, -2**31, 699])
+
+
+def test_every_token_can_be_drawn():
+    """u at and next to each border of a few exact weights."""
+    import torch
+
+    x = torch.zeros(1, 8)
+    for i in range(8):
+        for u, token in ((i / 8, i), (float(np.nextafter(np.float32((i + 1) / 8), np.float32(0))), i)):
+            assert run(x, u, "f32") == [token]
+
+
+@pytest.mark.parametrize("skip", [0, 1, 3])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_blocks_pitches_and_alignment(dtype, skip):
+    """Rows of a wider array from any element on, parameters in a column of theirs; what lies
+    beside the tokens stays."""
+    import torch
+
+    rows, vocab, wide, trow = 8, 3001, 3 * 3001, 2
+
+    @xt.kernel
+    def sample_kernel(x, u, p, y):
+        b = xt.bid(0)
+        t = xt.load(x, index=(b, 1), shape=(trow, vocab))
+        xt.store(y, index=(b, 2), tile=xt.sample(t, xt.load(u, index=(b, 1), shape=(trow, 1)),
+                                                 top_p=xt.load(p, index=(b, 0), shape=(trow, 1))))
+
+    m = xt.convert(sample_kernel, args=(xt.Array(shape=(rows, wide), dtype=DTYPES[dtype]),
+                                        xt.Array(shape=(rows, 3), dtype=xt.float32),
+                                        xt.Array(shape=(rows, 2), dtype=xt.float32),
+                                        xt.Array(shape=(rows, 4), dtype=xt.int32)), grid=(rows // trow, 1, 1))
+    x = logits(rows, wide, dtype, 6)
+    flat = torch.zeros(rows * wide + 8, dtype=x.dtype, device="cuda")
+    dx = flat[skip:skip + rows * wide].view(rows, wide)
+    dx.copy_(x)
+    u, p = torch.rand(rows, 3), torch.full((rows, 2), 0.8)
+    y = torch.full((rows, 4), -7, dtype=torch.int32, device="cuda")
+    xt.launch(m, dx, u.cuda(), p.cuda(), y)
+    part = x[:, vocab:2 * vocab]
+    w = [ref.sample(part[r].double().numpy(), float(u[r, 1]), top_p=float(p[r, 0])) for r in range(rows)]
+    assert y[:, 2].tolist() == w
+    assert bool((y[:, [0, 1, 3]] == -7).all())
+
+
+def test_streams_and_graphs():
+    """Two programs at once, and one captured and replayed."""
+    import torch
+
+    rows, vocab = 4, 40000
+    m = K.sample(rows, vocab, top_p=True)
+    p = torch.full((rows, 1), 0.9, device="cuda")
+    x, u = logits(rows, vocab, "f32", 1), torch.tensor(uniforms(rows, 1)).view(rows, 1)
+    jobs = []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            dx, du = (x + i).roll(i, 1).cuda(), u.cuda()
+            y = torch.empty(rows, 1, dtype=torch.int32, device="cuda")
+            for _ in range(3):
+                xt.launch(m, dx, du, p, y)
+            jobs.append((stream, dx, y))
+    for stream, dx, y in jobs:
+        stream.synchronize()
+        assert y.view(-1).tolist() == want(dx.cpu(), u.view(-1).tolist(), top_p=0.9)
+    dx, du = x.cuda(), u.cuda()
+    y = torch.empty(rows, 1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        xt.launch(m, dx, du, p, y)
+    for seed in range(3):
+        new, nu = logits(rows, vocab, "f32", 10 + seed), torch.tensor(uniforms(rows, seed)).view(rows, 1)
+        dx.copy_(new)
+        du.copy_(nu)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert y.view(-1).tolist() == want(new, nu.view(-1).tolist(), top_p=0.9)

@@ -12,7 +12,8 @@ hand-written HIP kernels: ``compile`` validates and plans the launch, and
 Extensions over the reference API: ``float16`` / ``bfloat16`` / ``int32``
 dtypes, ``canonicalize``, ``plan``, ``signature``, ``workspace`` and ``launch``,
 and the ops ``rms_norm``, ``row_scale``, ``quantize``, ``matmul_q4`` (with
-``pack_q4`` / ``unpack_q4``) and ``attend``.
+``pack_q4`` / ``unpack_q4``), ``mx4_scale``, ``quantize_mx4``, ``dequantize_mx4``,
+``matmul_mx4``, ``attend`` and ``sample``.
 """
 
 from __future__ import annotations
@@ -36,6 +37,7 @@ from .dsl import (
     bid,
     convert as _convert_impl,
     cos,
+    dequantize_mx4,
     exp,
     float16,
     float32,
@@ -45,16 +47,20 @@ from .dsl import (
     load,
     load_conv2d,
     matmul,
+    matmul_mx4,
     matmul_q4,
     max,
     mma,
     mul,
+    mx4_scale,
     quantize,
+    quantize_mx4,
     reciprocal,
     reshape,
     rms_norm,
     row_scale,
     rsqrt,
+    sample,
     sigmoid,
     silu,
     sin,
@@ -374,6 +380,7 @@ __all__ = [
     "compile",
     "convert",
     "cos",
+    "dequantize_mx4",
     "exp",
     "float16",
     "float32",
@@ -384,10 +391,12 @@ __all__ = [
     "load",
     "load_conv2d",
     "matmul",
+    "matmul_mx4",
     "matmul_q4",
     "max",
     "mma",
     "mul",
+    "mx4_scale",
     "nova_allocate",
     "nova_barrier",
     "nova_optimize",
@@ -397,11 +406,13 @@ __all__ = [
     "parse",
     "plan",
     "quantize",
+    "quantize_mx4",
     "reciprocal",
     "reshape",
     "rms_norm",
     "row_scale",
     "rsqrt",
+    "sample",
     "save_compile_results",
     "save_ir",
     "sigmoid",

@@ -169,7 +169,8 @@ bool is_pure_op(const std::string& n) {
                                "xt.sigmoid", "xt.tanh", "xt.silu", "xt.itof", "xt.ftoi",
                                "xt.matmul", "xt.mma", "xt.reduce_sum", "xt.reduce_max",
                                "xt.reshape", "xt.transpose", "xt.permute", "arith.constant",
-                               "xt.rms_norm", "xt.row_scale", "xt.quantize", "xt.matmul_q4", "xt.attend"};
+                               "xt.rms_norm", "xt.row_scale", "xt.quantize", "xt.matmul_q4", "xt.attend",
+                               "xt.mx4_scale", "xt.quantize_mx4", "xt.dequantize_mx4", "xt.matmul_mx4", "xt.sample"};
   for (const char* p : pure)
     if (n == p) return true;
   return false;
@@ -248,7 +249,12 @@ const std::unordered_map<std::string, OpInfo>& op_table() {
       {"xt.row_scale", {Fmt::Arith, 1, 1, 1}},
       {"xt.quantize", {Fmt::Arith, 2, 2, 1}},
       {"xt.matmul_q4", {Fmt::Arith, 3, 4, 1}},
-      {"xt.attend", {Fmt::Arith, 3, 9, 1}},
+      {"xt.attend", {Fmt::Arith, 3, 10, 1}},
+      {"xt.mx4_scale", {Fmt::Arith, 1, 1, 1}},
+      {"xt.quantize_mx4", {Fmt::Arith, 2, 2, 1}},
+      {"xt.dequantize_mx4", {Fmt::Arith, 2, 2, 1}},
+      {"xt.matmul_mx4", {Fmt::Arith, 4, 4, 1}},
+      {"xt.sample", {Fmt::Arith, 2, 6, 1}},
       {"func.return", {Fmt::Return, 0, -1, 0}},
       {"cf.br", {Fmt::Br, 0, -1, 0}},
       {"cf.cond_br", {Fmt::CondBr, 1, 1, 0}},

@@ -29,6 +29,11 @@
 // the rows'.  Few rows over many keys are split over workgroups that leave their
 // m, l and sums in the workspace, and a second kernel joins them.
 //
+// Drafted trees (parents): a token's ancestors are 64 bits, made in each wave by lanes that
+// double how far up they have seen, and are turned into the tiles' masks where a tile has
+// drafted tokens; the rest of the cache is seen whole.  The kernels are those of other rows,
+// in instantiations of their own.
+//
 // Many rows are bound by the arithmetic of the softmax (4096 tokens, 32 heads of 128
 // columns on 8 key heads, causal, capped: 166 to 181 us, 0.76 to 0.83 PFLOP/s; 158 without
 // the cap), single tokens by HBM (64 heads of 128 on 8, 131072 keys: 102 to 107 us, 5.0 to
@@ -50,6 +55,15 @@ extern template hipError_t run_attend<192>(bool, bool, const AttendArgs&, const 
 extern template hipError_t run_attend<224>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
 extern template hipError_t run_attend<256>(bool, bool, const AttendArgs&, const FineCap*, hipStream_t);
 
+extern template hipError_t run_attend_tree<32>(bool, bool, const AttendArgs&, const TreeCap&, bool, hipStream_t);
+extern template hipError_t run_attend_tree<64>(bool, bool, const AttendArgs&, const TreeCap&, bool, hipStream_t);
+extern template hipError_t run_attend_tree<96>(bool, bool, const AttendArgs&, const TreeCap&, bool, hipStream_t);
+extern template hipError_t run_attend_tree<128>(bool, bool, const AttendArgs&, const TreeCap&, bool, hipStream_t);
+extern template hipError_t run_attend_tree<160>(bool, bool, const AttendArgs&, const TreeCap&, bool, hipStream_t);
+extern template hipError_t run_attend_tree<192>(bool, bool, const AttendArgs&, const TreeCap&, bool, hipStream_t);
+extern template hipError_t run_attend_tree<224>(bool, bool, const AttendArgs&, const TreeCap&, bool, hipStream_t);
+extern template hipError_t run_attend_tree<256>(bool, bool, const AttendArgs&, const TreeCap&, bool, hipStream_t);
+
 hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipStream_t s, std::string& why) {
   const xt::AttendPlan& t = p.attend;
   // a workgroup reads its own query rows before it stores them, so the result may
@@ -65,7 +79,7 @@ hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipSt
     return false;
   };
   for (const xt::AttendAccess* a : {&t.q, &t.k, &t.v, &t.extra[0], &t.extra[1], &t.extra[2], &t.extra[3], &t.extra[4],
-                                    &t.extra[5]})
+                                    &t.extra[5], &t.extra[6]})
     if (!apart(a->arg)) return hipErrorInvalidValue;
   auto off = [](const xt::AttendAccess& a) {  // tile steps are not negative
     return Walk{static_cast<unsigned long long>(a.addr.sx), static_cast<unsigned long long>(a.addr.sy),
@@ -154,6 +168,24 @@ hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipSt
   };
   a.dma = chunks(t.k) && chunks(t.v);
   const bool b = t.elem == xt::Elem::BF16;
+  if (t.extra[6].arg >= 0) {
+    TreeCap tree{};
+    tree.mul = fine.mul;
+    ints(6, tree.parents, tree.tparents);
+    tree.step = t.extra[6].row;
+    tree.tokens = static_cast<int>(t.rows);
+    const bool l = look != nullptr;
+    switch (t.d) {
+      case 32: return run_attend_tree<32>(b, few, a, tree, l, s);
+      case 64: return run_attend_tree<64>(b, few, a, tree, l, s);
+      case 96: return run_attend_tree<96>(b, few, a, tree, l, s);
+      case 128: return run_attend_tree<128>(b, few, a, tree, l, s);
+      case 160: return run_attend_tree<160>(b, few, a, tree, l, s);
+      case 192: return run_attend_tree<192>(b, few, a, tree, l, s);
+      case 224: return run_attend_tree<224>(b, few, a, tree, l, s);
+      default: return run_attend_tree<256>(b, few, a, tree, l, s);
+    }
+  }
   switch (t.d) {
     case 32: return run_attend<32>(b, few, a, look, s);
     case 64: return run_attend<64>(b, few, a, look, s);

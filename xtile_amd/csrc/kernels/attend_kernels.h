@@ -43,9 +43,20 @@ struct FineCap {
   float mul;
 };
 
+// For kernels of drafted trees: beside that, each token's parent.
+struct TreeCap : FineCap {
+  const int* parents;
+  Walk tparents;
+  long long step;
+  int tokens;
+};
+
 // attend_*.hip, one instantiation each for d of 32, 64, ... 256; fine: null for none.
 template <int D>
 hipError_t run_attend(bool bf16, bool few, const AttendArgs& a, const FineCap* fine, hipStream_t s);
+// attend_tree_*.hip; fine: whether the cap looks at each score.
+template <int D>
+hipError_t run_attend_tree(bool bf16, bool few, const AttendArgs& a, const TreeCap& tree, bool fine, hipStream_t s);
 
 }  // namespace xtk
 
@@ -132,13 +143,68 @@ __device__ __forceinline__ int before(const AttendArgs& p, int window, int pos) 
   return !p.window || pos < window ? -1 : pos - window;
 }
 
+// What a kernel does beside the plain one: kFine, the cap looks at each score; kTree, the
+// rows are a tree of drafted tokens.
+constexpr int kPlain = 0, kFine = 1, kTree = 2;
+// (a type by name: an expression would be part of the kernels' names)
+template <int MODE>
+struct CapArg {
+  typedef FineCap type;
+};
+template <>
+struct CapArg<kTree> {
+  typedef TreeCap type;
+};
+template <>
+struct CapArg<kTree | kFine> {
+  typedef TreeCap type;
+};
+template <int MODE>
+using CapOf = typename CapArg<MODE>::type;
+
+// Of each of a tree's tokens, in its lane, the bits of its ancestors and its own.  A parent
+// comes before its child, whatever else is given is none; in each of six rounds a token
+// takes the bits of the farthest ancestor that it has, twice as far each time.
+__device__ __forceinline__ unsigned long long ancestors(const TreeCap& c, unsigned bx, unsigned by, unsigned bz) {
+  const int t = threadIdx.x & 63;
+  int up = -1;
+  if (t < c.tokens) up = c.parents[c.tparents.at(bx, by, bz) + t * c.step];
+  if (up >= t || up < 0) up = -1;
+  unsigned lo = t < 32 ? 1u << t : 0u, hi = t < 32 ? 0u : 1u << (t - 32);
+#pragma unroll
+  for (int i = 0; i < 6; ++i) {
+    const int from = max(up, 0);
+    const unsigned l = __shfl(lo, from, 64), h = __shfl(hi, from, 64);
+    const int farther = __shfl(up, from, 64);
+    if (up >= 0) {
+      lo |= l;
+      hi |= h;
+      up = farther;
+    }
+  }
+  return ((unsigned long long)hi << 32) | lo;
+}
+
+// Of those bits the nearest `window` (an ancestor's depth grows with its number).
+__device__ __forceinline__ unsigned long long nearest(unsigned long long bits, int window) {
+#pragma unroll 1
+  for (int over = __popcll(bits) - window; over > 0; --over) bits &= bits - 1;
+  return bits;
+}
+
+// Whether a token of these bits sees drafted token u, and how far above it that is.
+__device__ __forceinline__ bool sees_token(unsigned long long bits, int u) { return u >= 0 && u < 64 && ((bits >> u) & 1); }
+__device__ __forceinline__ int tokens_behind(unsigned long long bits, int u) {
+  return u >= 0 && u < 64 ? __popcll((bits >> u) >> 1) : 0;
+}
+
 // What one wave's 32 query rows see, and its running softmax.  Lane (c = lane % 32,
 // h = lane / 32) holds row c; of a tile of 32 keys it holds the scores of keys
 // 8 (r / 4) + 4 h + r % 4 in register r, and of the result columns
 // 32 n + 8 (r / 4) + 4 h + r % 4 in register r of acc[n].
-// FINE: the cap looks at each score.
-template <int D, bool BF16, bool FINE = false>
+template <int D, bool BF16, int MODE = kPlain>
 struct Rows {
+  static constexpr bool FINE = (MODE & kFine) != 0, TREE = (MODE & kTree) != 0;
   static constexpr int N = D / 32, KK = D / 16;
   static constexpr int PITCH = 2 * D;  // bytes of a key row in LDS
   static constexpr int VAHEAD = D < 128 ? 2 : 1;  // steps of 16 keys whose values are read ahead
@@ -160,6 +226,8 @@ struct Rows {
   int w0, w1;            // the last keys before their windows
   float slope;           // times log2 e
   int doc;               // this lane's document
+  unsigned long long tree;  // trees: the drafted tokens that this lane's row sees
+  int first;                // and the key of the first one
   uint4v q[KK];
   float16v acc[N];
   float m, l;
@@ -168,7 +236,8 @@ struct Rows {
   static constexpr bool LEAN = D == 256;
   int koff[LEAN ? 1 : KK], voff[N];
 
-  __device__ __forceinline__ void begin(const AttendArgs& p, int first, int bx, int by, int bz, int start, int window) {
+  __device__ __forceinline__ void begin(const AttendArgs& p, const CapOf<MODE>& c, int first, int bx, int by, int bz,
+                                        int start, int window) {
     lane = threadIdx.x & 63;
     col = lane & 31;
     hi = lane >> 5;
@@ -182,6 +251,21 @@ struct Rows {
     below = before(p, window, pos);
     w0 = before(p, window, p0);
     w1 = before(p, window, p1);
+    if constexpr (TREE) {
+      // depths lie between 0 and the tokens' number
+      const unsigned long long all = ancestors(c, bx, by, bz);
+      const unsigned lo = __shfl((unsigned)all, token, 64), up = __shfl((unsigned)(all >> 32), token, 64);
+      tree = ((unsigned long long)up << 32) | lo;
+      this->first = start;
+      pos = start + __popcll(tree) - 1;
+      above = start - 1;
+      below = before(p, window, pos);
+      if (p.window) tree = nearest(tree, window);
+      p0 = start;
+      p1 = start + c.tokens - 1;
+      w0 = before(p, window, p0);
+      w1 = before(p, window, p1);
+    }
     slope = p.slopes ? p.slopes[p.tslopes.at(bx, by, bz) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
     doc = p.qdocs ? p.qdocs[p.tqdocs.at(bx, by, bz) + token * p.qdoc_step] : 0;
     const unsigned char* at = p.q + (p.tq.at(bx, by, bz) + head * p.q_head + token * p.q_row + 8 * hi) * 2;
@@ -234,9 +318,11 @@ struct Rows {
 
   // Whether the wave's rows see all of keys [key0, key0 + n), documents aside, or none.
   __device__ __forceinline__ bool sees_all(const AttendArgs& p, int key0, int n, int len, int pre) const {
+    if constexpr (TREE) return key0 + n <= min(len, first) && key0 > w1;
     return key0 + n <= len && (key0 + n <= pre || ((!p.causal || key0 + n - 1 <= p0) && key0 > w1));
   }
   __device__ __forceinline__ bool sees_none(const AttendArgs& p, int key0, int n, int pre) const {
+    if constexpr (TREE) return key0 + n - 1 <= w0;
     return key0 >= pre && ((p.causal && key0 > p1) || key0 + n - 1 <= w0);
   }
 
@@ -247,6 +333,15 @@ struct Rows {
     return (1u << (4 * (y >> 3) + min((y & 7) + 1, 4))) - 1u;  // -1: 4 (-1) + 4
   }
 
+  // The bits of a lane's 16 registers of the tile of 32 keys from key0 on that are drafted
+  // tokens which its row sees.
+  __device__ __forceinline__ unsigned tree_bits(int key0) const {
+    const int u = key0 - first;  // the drafted token of the tile's first key
+    if (u <= -32 || u >= 64) return 0;
+    const unsigned w = (u >= 0 ? (unsigned)(tree >> u) : (unsigned)(tree << -u)) >> (4 * hi);
+    return (w & 15) | ((w >> 4) & 0xf0) | ((w >> 8) & 0xf00) | ((w >> 12) & 0xf000);
+  }
+
   __device__ __forceinline__ int doc_of(const int* docs, const int* kdocs, int t, int i, int base, int len) const {
     if (docs) return docs[t * 32 + 4 * hi + i];
     return base + i < len ? kdocs[base + i] : 0;
@@ -255,7 +350,7 @@ struct Rows {
   // T tiles of 32 keys from key0 on.  docs: their documents in LDS, or null, then from
   // kdocs.
   template <int T>
-  __device__ __forceinline__ void tile(const AttendArgs& p, const FineCap& c, const unsigned char* K, const unsigned char* V,
+  __device__ __forceinline__ void tile(const AttendArgs& p, const CapOf<MODE>& c, const unsigned char* K, const unsigned char* V,
                                        const int* docs, const int* kdocs, int key0, int len, int pre) {
     bool part = !sees_all(p, key0, 32 * T, len, pre);
     bool by_doc = false, by_key = false;  // rows, or keys, of several documents
@@ -334,8 +429,17 @@ struct Rows {
       for (int t = 0; t < T; ++t) {
         const float away = (float)(pos - (key0 + t * 32 + 4 * hi));
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[t][r] = fmaf(-slope, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[t][r] * mul);
+        for (int r = 0; r < 16; ++r) {
+          float far = fabsf(away - (float)(8 * (r >> 2) + (r & 3)));
+          if constexpr (TREE) {
+            // only the last tiles have drafted tokens: their distance is by depth
+            if (key0 + 32 * T > first) {
+              const int u = key0 + t * 32 + 4 * hi + 8 * (r >> 2) + (r & 3) - first;
+              if (u >= 0) far = (float)tokens_behind(tree, u);
+            }
+          }
+          s[t][r] = fmaf(-slope, far, s[t][r] * mul);
+        }
       }
       mul = 1.0f;
     }
@@ -345,6 +449,8 @@ struct Rows {
       for (int t = 0; t < T; ++t) {
         const int base = key0 + t * 32 + 4 * hi;
         unsigned bits = ((up_to(above - base) & ~up_to(below - base)) | up_to(pre - 1 - base)) & up_to(len - 1 - base);
+        if constexpr (TREE)
+          bits = ((up_to(above - base) & ~up_to(below - base)) | tree_bits(key0 + t * 32)) & up_to(len - 1 - base);
         if (by_doc && doc != tile_doc) bits = 0;
         if (by_key) {
 #pragma unroll
@@ -470,6 +576,16 @@ __device__ __forceinline__ Tiles tiles_of(const AttendArgs& p, int bn, int p0, i
   t.na = a1 > d0 ? (a1 + bn - 1) / bn - t.a0 : 0;
   t.b0 = max(b0 / bn, t.na ? t.a0 + t.na : 0);
   t.n = t.na + (b1 > b0 ? max(0, (b1 + bn - 1) / bn - t.b0) : 0);
+  return t;
+}
+
+// The same for a tree of drafted tokens behind the keys before b.start.
+__device__ __forceinline__ Tiles tree_tiles(const AttendArgs& p, int bn, int start, int window, int len, int tokens) {
+  const int b0 = before(p, window, start) + 1, b1 = min(len, max(start + tokens, 0));
+  Tiles t;
+  t.a0 = t.na = 0;
+  t.b0 = b0 / bn;
+  t.n = b1 > b0 ? max(0, (b1 + bn - 1) / bn - t.b0) : 0;
   return t;
 }
 
@@ -714,11 +830,14 @@ __device__ __forceinline__ const AttendArgs& args_here() {
 // or near the largest, of which only what a row sees is ever multiplied, by weights of 32
 // bits and at most one.  Lane j of 64 keys has
 // the score of key j; then the lanes have the columns.
-template <int D, bool BF16, bool FINE>
-__device__ __forceinline__ void odd_rows(const AttendArgs& p, const FineCap& c, const BlockAt& b, const Tiles& tiles,
+template <int D, bool BF16, int MODE>
+__device__ __forceinline__ void odd_rows(const AttendArgs& p, const CapOf<MODE>& c, const BlockAt& b, const Tiles& tiles,
                                          int bn, int i0, int i1, const int* kdocs, int first, int last, int step,
                                          long long all_rows) {
+  constexpr bool FINE = (MODE & kFine) != 0, TREE = (MODE & kTree) != 0;
   const int lane = threadIdx.x & 63;
+  unsigned long long all = 0;
+  if constexpr (TREE) all = ancestors(c, b.x, b.y, b.z);
   auto value = [](unsigned short x) {
     return BF16 ? __builtin_bit_cast(float, (unsigned)x << 16) : (float)__builtin_bit_cast(_Float16, x);
   };
@@ -726,12 +845,22 @@ __device__ __forceinline__ void odd_rows(const AttendArgs& p, const FineCap& c, 
   const unsigned short* const values = reinterpret_cast<const unsigned short*>(p.v) + p.tv.at(b.x, b.y, b.z);
 #pragma unroll 1
   for (int row = first; row < last; row += step) {
-    const int token = (int)p.d_heads((unsigned)row), head = row - token * p.heads, pos = b.start + token;
+    const int token = (int)p.d_heads((unsigned)row), head = row - token * p.heads;
+    int pos = b.start + token;
+    unsigned long long tree = 0;
+    if constexpr (TREE) {
+      const unsigned lo = __shfl((unsigned)all, token, 64), up = __shfl((unsigned)(all >> 32), token, 64);
+      tree = ((unsigned long long)up << 32) | lo;
+      pos = b.start + __popcll(tree) - 1;
+      if (p.window) tree = nearest(tree, b.window);
+    }
     const unsigned short* const q = reinterpret_cast<const unsigned short*>(p.q) + p.tq.at(b.x, b.y, b.z) +
                                     head * p.q_head + token * p.q_row;
     const float slope = p.slopes ? p.slopes[p.tslopes.at(b.x, b.y, b.z) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
     const int doc = p.qdocs ? p.qdocs[p.tqdocs.at(b.x, b.y, b.z) + token * p.qdoc_step] : 0;
     auto sees = [&](int j, int end) {
+      if constexpr (TREE)
+        return j < end && j < b.len && (j < b.start ? j > before(p, b.window, pos) : sees_token(tree, j - b.start));
       return j < end && j < b.len && (j < b.pre || ((!p.causal || j <= pos) && j > before(p, b.window, pos))) &&
              (!kdocs || kdocs[j] == doc);
     };
@@ -741,7 +870,10 @@ __device__ __forceinline__ void odd_rows(const AttendArgs& p, const FineCap& c, 
 #pragma unroll 1
       for (int d = 0; d < D; ++d) s = fmaf(value(q[d]), value(k[d]), s);
       s = FINE ? capped(p, c, s) : p.cap_log2 > 0.0f ? capped_far(p, s) : s * p.scale_log2;
-      return p.slopes ? fmaf(-slope, fabsf((float)(pos - j)), s) : s;
+      float far = fabsf((float)(pos - j));
+      if constexpr (TREE)
+        if (j >= b.start) far = (float)tokens_behind(tree, j - b.start);
+      return p.slopes ? fmaf(-slope, far, s) : s;
     };
     // the maximum, minus infinity where the row sees nothing (as in tile), and what the
     // scores are taken relative to
@@ -813,9 +945,9 @@ __device__ __forceinline__ bool any_wave(bool x, unsigned char* lds) {
 // share, two of them in LDS.  G groups of four waves have the same rows and take tiles
 // in turn, and the second's results join the first's: where workgroups are so few that
 // a SIMD would have one wave, whose products and arithmetic wait for each other.
-template <int D, bool BF16, int G, bool FINE>
+template <int D, bool BF16, int G, int MODE>
 __global__ __launch_bounds__(256 * G, G == 2 ? 2 : D <= 64 ? 3 : D <= 128 ? 2 : 1)
-void attend_rows_kernel(AttendArgs p, long long all_rows, FineCap c) {
+void attend_rows_kernel(AttendArgs p, long long all_rows, CapOf<MODE> c) {
   constexpr int BN = 64, KB = BN * D * 2, STAGE = 2 * KB + 256;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * G * STAGE];
   const bool dma = p.dma;
@@ -828,7 +960,9 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, FineCap c) {
   if (kdocs)
     document_keys<4 * G>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, t0, t1, last_key(p, b, t1), reinterpret_cast<int*>(lds),
                      d0, d1);
-  const Tiles tiles = tiles_of(p, BN, b.start + t0, b.start + t1, b.window, b.len, b.pre, d0, d1);
+  Tiles tiles;
+  if constexpr ((MODE & kTree) != 0) tiles = tree_tiles(p, BN, b.start, b.window, b.len, c.tokens);
+  else tiles = tiles_of(p, BN, b.start + t0, b.start + t1, b.window, b.len, b.pre, d0, d1);
   const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
   const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
 
@@ -844,8 +978,8 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, FineCap c) {
   };
   unsigned char* const stages = lds + group * 2 * STAGE;
   if (i0 + group < i1) issue(i0 + group, stages);
-  Rows<D, BF16, FINE> rows;
-  rows.begin(p, first + 32 * wave, b.x, b.y, b.z, b.start, b.window);
+  Rows<D, BF16, MODE> rows;
+  rows.begin(p, c, first + 32 * wave, b.x, b.y, b.z, b.start, b.window);
 #pragma unroll 1
   for (int i = i0 + group, n = 0; i - group < i1; i += G, n ^= 1) {
     // one barrier a tile: behind it this tile has landed, and every wave is done with
@@ -862,7 +996,7 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, FineCap c) {
   rows.hold();
   lds_barrier();
   if (any_wave<4 * G>(rows.spoilt(), lds)) {
-    odd_rows<D, BF16, FINE>(args_here(), c, b, tiles, BN, i0, i1, kdocs, first + every, last + 1, 4 * G, all_rows);
+    odd_rows<D, BF16, MODE>(args_here(), c, b, tiles, BN, i0, i1, kdocs, first + every, last + 1, 4 * G, all_rows);
     return;
   }
   if constexpr (G == 2) {
@@ -955,8 +1089,8 @@ struct Few {
 
 // Up to 32 rows: every wave has them all and takes tiles of 32 keys in turn, each in
 // a ring of its own, so that nothing but its own loads makes a wave wait.
-template <int D, bool BF16, bool FINE>
-__global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p, long long all_rows, FineCap c) {
+template <int D, bool BF16, int MODE>
+__global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p, long long all_rows, CapOf<MODE> c) {
   typedef Few<D> F;
   constexpr int W = F::W, NS = F::NS, KB = 32 * D * 2, PER = D / 8;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[F::LDS];
@@ -969,7 +1103,9 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   if (kdocs)
     document_keys<W>(p, p.qdocs + p.tqdocs.at(b.x, b.y, b.z), kdocs, 0, t1, last_key(p, b, t1), reinterpret_cast<int*>(lds),
                      d0, d1);
-  const Tiles tiles = tiles_of(p, 32, b.start, b.start + t1, b.window, b.len, b.pre, d0, d1);
+  Tiles tiles;
+  if constexpr ((MODE & kTree) != 0) tiles = tree_tiles(p, 32, b.start, b.window, b.len, c.tokens);
+  else tiles = tiles_of(p, 32, b.start, b.start + t1, b.window, b.len, b.pre, d0, d1);
   const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
   const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
   const int mine = max(0, (i1 - i0 - wave + W - 1) / W);
@@ -989,8 +1125,8 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
 #pragma unroll
   for (int j = 0; j < NS; ++j)
     if (j < mine) issue(j, j);
-  Rows<D, BF16, FINE> rows;
-  rows.begin(p, 0, b.x, b.y, b.z, b.start, b.window);
+  Rows<D, BF16, MODE> rows;
+  rows.begin(p, c, 0, b.x, b.y, b.z, b.start, b.window);
   int slot = 0;
 #pragma unroll 1
   for (int j = 0; j < mine; ++j) {
@@ -1015,7 +1151,7 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
   if constexpr (D == 256) rows.hold();
   __syncthreads();  // every ring is done with
   if (any_wave<W>(rows.spoilt(), lds)) {
-    odd_rows<D, BF16, FINE>(args_here(), c, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);
+    odd_rows<D, BF16, MODE>(args_here(), c, b, tiles, 32, i0, i1, kdocs, wave, p.rows, W, all_rows);
     return;
   }
 
@@ -1151,25 +1287,26 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs p, long lon
 // 135 keys 9.6 -> 10.6; a split of 1520 keys in five 19.8 -> 21.1).
 inline bool pairs_of(const AttendArgs& a, int d) { return d <= 128 && a.nwg <= 256 && a.splits == 1 && a.keys > 192; }
 
-template <int D, bool BF16, bool FINE>
-void run_attend_rows(bool few, const AttendArgs& a, long long all_rows, const FineCap& c, hipStream_t s) {
+template <int D, bool BF16, int MODE>
+void run_attend_rows(bool few, const AttendArgs& a, long long all_rows, const CapOf<MODE>& c, hipStream_t s) {
   if (few) {
-    attend_few_kernel<D, BF16, FINE><<<a.nwg, 64 * Few<D>::W, 0, s>>>(a, all_rows, c);
+    attend_few_kernel<D, BF16, MODE><<<a.nwg, 64 * Few<D>::W, 0, s>>>(a, all_rows, c);
     return;
   }
   if constexpr (D <= 128)
     if (pairs_of(a, D)) {
-      attend_rows_kernel<D, BF16, 2, FINE><<<a.nwg, 512, 0, s>>>(a, all_rows, c);
+      attend_rows_kernel<D, BF16, 2, MODE><<<a.nwg, 512, 0, s>>>(a, all_rows, c);
       return;
     }
-  attend_rows_kernel<D, BF16, 1, FINE><<<a.nwg, 256, 0, s>>>(a, all_rows, c);
+  attend_rows_kernel<D, BF16, 1, MODE><<<a.nwg, 256, 0, s>>>(a, all_rows, c);
 }
 
+inline long long all_rows_of(const AttendArgs& a) { return a.nwg / ((long long)a.tiles * a.splits) * a.rows; }
+
+// Behind the rows' kernel.
 template <int D, bool BF16>
-hipError_t run_attend_elem(bool few, const AttendArgs& a, const FineCap* fine, hipStream_t s) {
-  const long long blocks = a.nwg / ((long long)a.tiles * a.splits), all_rows = blocks * a.rows;
-  if (fine) run_attend_rows<D, BF16, true>(few, a, all_rows, *fine, s);
-  else run_attend_rows<D, BF16, false>(few, a, all_rows, FineCap{}, s);
+hipError_t run_attend_join(const AttendArgs& a, hipStream_t s) {
+  const long long all_rows = all_rows_of(a);
   if (a.splits > 1) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1184,7 +1321,26 @@ hipError_t run_attend_elem(bool few, const AttendArgs& a, const FineCap* fine, h
   return hipGetLastError();
 }
 
+template <int D, bool BF16>
+hipError_t run_attend_elem(bool few, const AttendArgs& a, const FineCap* fine, hipStream_t s) {
+  if (fine) run_attend_rows<D, BF16, kFine>(few, a, all_rows_of(a), *fine, s);
+  else run_attend_rows<D, BF16, kPlain>(few, a, all_rows_of(a), FineCap{}, s);
+  return run_attend_join<D, BF16>(a, s);
+}
+
+template <int D, bool BF16>
+hipError_t run_attend_tree_elem(bool few, const AttendArgs& a, const TreeCap& tree, bool fine, hipStream_t s) {
+  if (fine) run_attend_rows<D, BF16, kTree | kFine>(few, a, all_rows_of(a), tree, s);
+  else run_attend_rows<D, BF16, kTree>(few, a, all_rows_of(a), tree, s);
+  return run_attend_join<D, BF16>(a, s);
+}
+
 }  // namespace
+
+template <int D>
+hipError_t run_attend_tree(bool bf16, bool few, const AttendArgs& a, const TreeCap& tree, bool fine, hipStream_t s) {
+  return bf16 ? run_attend_tree_elem<D, true>(few, a, tree, fine, s) : run_attend_tree_elem<D, false>(few, a, tree, fine, s);
+}
 
 template <int D>
 hipError_t run_attend(bool bf16, bool few, const AttendArgs& a, const FineCap* fine, hipStream_t s) {

@@ -133,6 +133,10 @@ hipError_t launch_tilevm(const xt::Plan& p, void* const* bufs, hipStream_t s, st
 
 hipError_t launch_rms_norm(const xt::Plan& p, void* const* bufs, hipStream_t s, std::string& why);
 hipError_t launch_matmul_q4(const xt::Plan& p, void* const* bufs, hipStream_t s, std::string& why);
+hipError_t launch_mx4_rows(const xt::Plan& p, void* const* bufs, hipStream_t s, std::string& why);
+hipError_t launch_matmul_mx4(const xt::Plan& p, void* const* bufs, hipStream_t s, std::string& why);
+// `work`: the plan's workspace, or null (a row then has one workgroup).
+hipError_t launch_sample(const xt::Plan& p, void* const* bufs, void* work, hipStream_t s, std::string& why);
 // `work`: the plan's workspace, or null (the keys are then not split).
 hipError_t launch_attend(const xt::Plan& p, void* const* bufs, void* work, hipStream_t s, std::string& why);
 

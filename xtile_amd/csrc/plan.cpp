@@ -12,9 +12,13 @@
 //              (kernels/conv2d.py:10-37; conv slice math lib/xt/XTToNova.cpp:110-142)
 //   RmsNorm    rms_norm of a loaded tile or of the sum of two, to rows of floats
 //              or through row_scale and quantize to rows in 8 bits (no reference
-//              counterpart, like the two below)
+//              counterpart, like those below)
 //   MatmulQ4   store(matmul_q4(load X, load W, load S[, load R]))
 //   Attend     store(attend(load Q, load K, load V, ...)), reshapes in between
+//   Mx4Rows    the stores of mx4_scale(load X), quantize_mx4 and dequantize_mx4 of
+//              them, or store(dequantize_mx4(load Q, load S))
+//   MatmulMx4  store(matmul_mx4(load X, load XS, load W, load WS))
+//   Sample     store(sample(load X, load U, ...))
 #include "plan.h"
 
 #include <algorithm>
@@ -527,7 +531,7 @@ bool match_gemm_form(const Analysis& an, Plan& p, std::string& err, bool ragged)
 
 bool match_gemm(const Analysis& an, Plan& p, std::string& err) { return match_gemm_form(an, p, err, false); }
 
-// -- RmsNorm, MatmulQ4, Attend ---------------------------------------------------
+// -- RmsNorm, MatmulQ4, Mx4Rows, MatmulMx4, Sample, Attend ---------------------------------------------------
 
 const Op* load_of(const Analysis& an, int v) {
   const Op* o = def_of(an, v);
@@ -662,6 +666,156 @@ bool match_q4(const Analysis& an, Plan& p, std::string& err) {
   return true;
 }
 
+// A plan's algorithmic HBM bytes: each of these arguments once.
+void count_bytes(const Analysis& an, const std::vector<int>& args, Plan& p) {
+  for (int arg : args) {
+    const Type& t = an.f.type_of(an.f.args[arg]);
+    p.algo_bytes += double(t.numel()) * elem_bytes(t.elem);
+  }
+}
+
+bool match_mx4_rows(const Analysis& an, Plan& p, std::string& err) {
+  int ns, nq, nd, nst;
+  const Op* sc = only(an, "xt.mx4_scale", ns);
+  const Op* qz = only(an, "xt.quantize_mx4", nq);
+  const Op* dq = only(an, "xt.dequantize_mx4", nd);
+  only(an, "xt.store", nst);
+  if (ns + nq + nd == 0) return false;
+  err = "programs of rows in microscaled 4-bit floating point must be the stores of mx4_scale of a loaded tile, of "
+        "quantize_mx4 with that scale and of dequantize_mx4 of the two, or store(dequantize_mx4(rows, scales)) of loaded "
+        "tiles";
+  if (ns > 1 || nq > 1 || nd > 1) return false;
+  Mx4RowsPlan& m = p.mx4_rows;
+  m = Mx4RowsPlan{};
+  m.back = ns == 0;
+  const Op *lx = nullptr, *ls = nullptr;
+  if (m.back) {
+    if (nq || !(lx = load_of(an, dq->operands[0])) || !(ls = load_of(an, dq->operands[1])) || ls == lx) return false;
+  } else {
+    if (!(lx = load_of(an, sc->operands[0]))) return false;
+    if (nq && (qz->operands[0] != sc->operands[0] || qz->operands[1] != sc->results[0])) return false;
+    if (nd && (!nq || dq->operands[0] != qz->results[0] || dq->operands[1] != sc->results[0])) return false;
+  }
+  const Op *st_q = nullptr, *st_s = nullptr, *st_y = nullptr;
+  std::vector<int> stored, read;
+  for (const Op* o : an.compute) {
+    if (o->name != "xt.store") continue;
+    const int v = o->operands[0];
+    const Op** slot = nd && v == dq->results[0] ? &st_y : nq && v == qz->results[0] ? &st_q : ns && v == sc->results[0] ? &st_s : nullptr;
+    if (!slot || *slot) return false;
+    *slot = o;
+    stored.push_back(an.arg_index(o->operands[1]));
+  }
+  if (nst == 0 || (m.back && !st_y) || count_ops(an) != (m.back ? 2 : 1) + ns + nq + nd + nst) return false;
+  err.clear();
+  // an access that is absent has no argument
+  if (!access_of(an, *lx, m.back ? m.q : m.x, err) || (ls && !access_of(an, *ls, m.s, err)) ||
+      (st_q && !access_of(an, *st_q, m.q, err)) || (st_s && !access_of(an, *st_s, m.s, err)) ||
+      (st_y && !access_of(an, *st_y, m.y, err)))
+    return false;
+  if (!m.back && st_y && m.y.elem != m.x.elem) {
+    err = "quantize_mx4 programs store values of the operand's type";
+    return false;
+  }
+  if (m.back) read = {m.q.arg, m.s.arg};
+  // the values may lie over x, as the launch finds
+  std::vector<int> apart = read;
+  if (!m.back) {
+    read = {m.x.arg};
+    if (m.y.arg != m.x.arg) apart = read;
+    else if (m.q.arg == m.x.arg || m.s.arg == m.x.arg) return err = "the rows and scales are stored to arguments of their own", false;
+  }
+  if (!stored_apart(stored, apart, "mx4", err)) return false;
+  const Access2D& rows = m.back ? m.q : m.x;
+  m.cols = m.back ? 2 * rows.cols : rows.cols;
+  const double blocks = double(p.grid[0]) * p.grid[1] * p.grid[2], elems = double(rows.rows) * double(m.cols);
+  if (blocks * double(rows.rows) >= 2147483648.0 || m.cols >= (int64_t(1) << 30) || blocks * elems >= 17179869184.0) {
+    err = "programs of rows in microscaled 4-bit floating point take fewer than 2^31 rows of fewer than 2^30 columns, and "
+          "fewer than 2^34 values";
+    return false;
+  }
+  p.kind = PlanKind::Mx4Rows;
+  for (int a : stored)
+    if (!std::count(read.begin(), read.end(), a)) read.push_back(a);
+  count_bytes(an, read, p);
+  p.algo_flops = 4 * blocks * elems;
+  return true;
+}
+
+bool match_mx4(const Analysis& an, Plan& p, std::string& err) {
+  int nm, nst;
+  const Op* mm = only(an, "xt.matmul_mx4", nm);
+  const Op* st = only(an, "xt.store", nst);
+  if (nm == 0) return false;
+  err = "matmul_mx4 programs must be store(matmul_mx4(x, x scales, w, w scales)) with loaded operands";
+  if (nm != 1 || nst != 1 || st->operands[0] != mm->results[0]) return false;
+  Mx4Plan& m = p.mx4;
+  m = Mx4Plan{};
+  Access2D* acc[4] = {&m.x, &m.xs, &m.w, &m.ws};
+  std::set<const Op*> distinct;
+  std::vector<int> read;
+  for (int i = 0; i < 4; ++i) {
+    const Op* ld = load_of(an, mm->operands[i]);
+    if (!ld) return false;
+    distinct.insert(ld);
+    std::string e;
+    if (!access_of(an, *ld, *acc[i], e)) return err = e, false;
+    if (!std::count(read.begin(), read.end(), acc[i]->arg)) read.push_back(acc[i]->arg);
+  }
+  if (count_ops(an) != static_cast<int>(distinct.size()) + 2) return false;
+  err.clear();
+  if (!access_of(an, *st, m.y, err) || !stored_apart({m.y.arg}, read, "matmul_mx4", err)) return false;
+  m.K = 2 * m.x.cols;
+  if (m.y.rows >= (int64_t(1) << 30) || m.y.cols >= (int64_t(1) << 30) || m.K >= (int64_t(1) << 24)) {
+    err = "matmul_mx4 takes tiles of fewer than 2^30 rows and columns and K below 2^24";
+    return false;
+  }
+  p.kind = PlanKind::MatmulMx4;
+  const double blocks = double(p.grid[0]) * p.grid[1] * p.grid[2];
+  p.algo_flops = blocks * 2.0 * double(m.y.rows) * double(m.y.cols) * double(m.K);
+  read.push_back(m.y.arg);
+  count_bytes(an, read, p);
+  return true;
+}
+
+bool match_sample(const Analysis& an, Plan& p, std::string& err) {
+  int ns, nst;
+  const Op* sm = only(an, "xt.sample", ns);
+  const Op* st = only(an, "xt.store", nst);
+  if (ns == 0) return false;
+  err = "sample programs must be store(sample(...)) with loaded operands";
+  if (ns != 1 || nst != 1 || st->operands[0] != sm->results[0]) return false;
+  SamplePlan& s = p.sample;
+  s = SamplePlan{};
+  const Attr* extras = find_attr(sm->attrs, "extras");
+  std::set<const Op*> distinct;
+  std::vector<int> read;
+  for (size_t i = 0, e = 0; i < sm->operands.size(); ++i) {
+    const Op* ld = load_of(an, sm->operands[i]);
+    if (!ld) return false;
+    distinct.insert(ld);
+    if (i >= 2)
+      while (!extras->ints[e]) ++e;
+    Access2D& a = i == 0 ? s.x : i == 1 ? s.u : s.extra[e++];
+    std::string why;
+    if (!access_of(an, *ld, a, why)) return err = why, false;
+    if (!std::count(read.begin(), read.end(), a.arg)) read.push_back(a.arg);
+  }
+  if (count_ops(an) != static_cast<int>(distinct.size()) + 2) return false;
+  err.clear();
+  if (!access_of(an, *st, s.y, err) || !stored_apart({s.y.arg}, read, "sample", err)) return false;
+  const double blocks = double(p.grid[0]) * p.grid[1] * p.grid[2];
+  if (blocks * double(s.x.rows) >= double(1 << 22) || s.x.cols > kSampleVocab) {
+    err = "the HIP sample kernel takes fewer than 2^22 rows of at most 2^22 logits";
+    return false;
+  }
+  p.kind = PlanKind::Sample;
+  read.push_back(s.y.arg);
+  count_bytes(an, read, p);
+  p.algo_flops = 8 * blocks * double(s.x.rows) * double(s.x.cols);
+  return true;
+}
+
 // `shape` over the elements of a tile with dims `tile` and strides `st`, in row-major
 // order: its strides, where each of its dims is one run of evenly spaced elements.
 bool reshaped_strides(const std::vector<int64_t>& tile, const std::vector<int64_t>& st,
@@ -792,6 +946,11 @@ bool match_attend(const Analysis& an, Plan& p, std::string& err) {
     return false;
   }
   if (!stored_apart({a.o.arg}, read, "attend", err)) return false;
+  if (a.extra[6].arg >= 0 && a.rows > kAttendTree) {
+    err = "the HIP attend kernel takes trees of at most " + std::to_string(kAttendTree) + " drafted tokens; got " +
+          std::to_string(a.rows);
+    return false;
+  }
   if (a.d % 32 || a.d > 256) {
     err = "the HIP attend kernel takes heads of 32 to 256 columns, a multiple of 32; got " + std::to_string(a.d);
     return false;
@@ -1287,10 +1446,29 @@ std::string Plan::describe() const {
       if (attend.cap > 0) os << " cap";
       if (attend.causal) os << " causal";
       if (attend.window) os << " window=" << attend.window;
-      static const char* names[6] = {"slopes", "start", "length", "prefix", "docs", ""};
-      for (int e = 0; e < 5; ++e)
+      static const char* names[7] = {"slopes", "start", "length", "prefix", "docs", "", "parents"};
+      for (int e : {0, 1, 2, 3, 4, 6})
         if (attend.extra[e].arg >= 0) os << " " << names[e];
       if (attend.splits > 1) os << " splits=" << attend.splits;
+      break;
+    }
+    case PlanKind::Mx4Rows:
+      if (mx4_rows.back)
+        os << "dequantize_mx4 " << elem_name(mx4_rows.y.elem) << " tile=" << mx4_rows.q.rows << "x" << mx4_rows.cols;
+      else
+        os << "quantize_mx4 " << elem_name(mx4_rows.x.elem) << (mx4_rows.q.arg >= 0 ? " rows" : "")
+           << (mx4_rows.s.arg >= 0 ? " scales" : "") << (mx4_rows.y.arg >= 0 ? " values" : "") << " tile=" << mx4_rows.x.rows
+           << "x" << mx4_rows.cols;
+      break;
+    case PlanKind::MatmulMx4:
+      os << "matmul_mx4 " << elem_name(mx4.y.elem) << " tile=" << mx4.y.rows << "x" << mx4.y.cols << " k=" << mx4.K;
+      break;
+    case PlanKind::Sample: {
+      os << "sample " << elem_name(sample.x.elem) << " tile=" << sample.x.rows << "x" << sample.x.cols;
+      static const char* names[4] = {"temperature", "top_k", "top_p", "min_p"};
+      for (int e = 0; e < 4; ++e)
+        if (sample.extra[e].arg >= 0) os << " " << names[e];
+      if (sample.slices > 1) os << " slices=" << sample.slices;
       break;
     }
     case PlanKind::Conv2d:
@@ -1352,7 +1530,7 @@ int attend_splits(const Plan& p) {
   const int64_t per = few ? kAttendFewRows : kAttendRows;
   const double tiles = double(p.grid[0]) * p.grid[1] * p.grid[2] * double((rows + per - 1) / per);
   // A causal window leaves only so many keys, whatever the cache holds.
-  const bool band = a.causal && a.window && a.extra[3].arg < 0;
+  const bool band = (a.causal || a.extra[6].arg >= 0) && a.window && a.extra[3].arg < 0;
   const int64_t keys = band ? std::min(a.keys, a.window + a.rows) : a.keys;
   const int fit = few ? (a.d > 64 ? 1 : 2) : a.d > 128 ? 1 : a.d > 64 ? 2 : 3;  // workgroups on a compute unit
   const double want = 256 * fit / tiles;
@@ -1433,7 +1611,8 @@ bool build_plan(const Module& m, const std::string& func, Plan& p, std::string& 
   // the tile interpreter, and the first reason is reported if that fails too
   err.clear();
   std::string first;
-  for (auto match : {match_ew, match_softmax, match_gemm, match_conv, match_rms_norm, match_q4, match_attend}) {
+  for (auto match : {match_ew, match_softmax, match_gemm, match_conv, match_rms_norm, match_q4, match_attend, match_mx4_rows, match_mx4,
+                     match_sample}) {
     std::string why;
     if (match(an, p, why)) return true;
     if (first.empty()) first = why;

@@ -41,7 +41,7 @@ struct Coord {
   int64_t value = 0;
 };
 
-enum class PlanKind { EwBinary, RowSoftmax, Gemm, Conv2d, TileVM, Fused, RmsNorm, MatmulQ4, Attend };
+enum class PlanKind { EwBinary, RowSoftmax, Gemm, Conv2d, TileVM, Fused, RmsNorm, MatmulQ4, Attend, Mx4Rows, MatmulMx4, Sample };
 enum class EwOp { Add = 0, Sub = 1, Mul = 2 };
 
 struct ConvPlan {
@@ -129,6 +129,30 @@ struct Q4Plan {
   int64_t K = 0, group = 0;
 };
 
+// The stores of mx4_scale(load x), of quantize_mx4 with that scale and of the values
+// that dequantize_mx4 makes of the two, each where it is wanted (arg -1: not); or
+// store(dequantize_mx4(load q, load s)).
+struct Mx4RowsPlan {
+  bool back = false;
+  Access2D x, q, s, y;  // cols in elements of each: C, C / 2, C / 32 and C
+  int64_t cols = 0;     // C
+};
+
+// store(matmul_mx4(load x, load xs, load w, load ws)).
+struct Mx4Plan {
+  Access2D x, xs, w, ws, y;
+  int64_t K = 0;
+};
+
+// store(sample(load x, load u[, load extras])).
+struct SamplePlan {
+  Access2D x, u, y;
+  Access2D extra[4];  // temperature, top_k, top_p, min_p; arg -1: absent
+  // Few rows of many logits: workgroups that share a row where the launch is given a
+  // workspace (1: never).
+  int slices = 1;
+};
+
 // One operand of an attend program as heads x rows x D (or rows x columns) of a
 // strided array; strides in elements, D contiguous.
 struct AttendAccess {
@@ -143,7 +167,7 @@ struct AttendPlan {
   Elem elem = Elem::None;
   int64_t heads = 0, rows = 0, keys = 0, d = 0;  // of a Block; `heads` query heads share its keys
   AttendAccess q, k, v, o;
-  AttendAccess extra[6];  // slopes, start, length, prefix, q_docs, k_docs; arg -1: absent
+  AttendAccess extra[7];  // slopes, start, length, prefix, q_docs, k_docs, parents; arg -1: absent
   float scale = 1, cap = 0;  // cap 0: none
   bool causal = false;
   int64_t window = 0;        // 0: none
@@ -155,6 +179,10 @@ struct AttendPlan {
 // Rows of one attend workgroup: up to 32 take one wave's width with the keys
 // dealt to the waves, more take 128 with the keys shared.
 constexpr int64_t kAttendFewRows = 32, kAttendRows = 128;
+// Logits of a row that `sample` takes.
+constexpr int64_t kSampleVocab = int64_t(1) << 22;
+// Drafted tokens of a tree: their ancestors are a lane's 64 bits.
+constexpr int64_t kAttendTree = 64;
 
 struct Plan {
   PlanKind kind = PlanKind::EwBinary;
@@ -182,6 +210,9 @@ struct Plan {
   NormPlan norm;
   Q4Plan q4;
   AttendPlan attend;
+  Mx4RowsPlan mx4_rows;
+  Mx4Plan mx4;
+  SamplePlan sample;
   int64_t workspace = 0;  // bytes a launch may work in beside its buffers
   VmPlan vm;
   std::shared_ptr<FusedPlan> fused;  // Fused: the generated kernel (vm keeps the accesses)

@@ -82,7 +82,8 @@ int run_plan(const xt::Plan& p, void* const* bufs, void* work, size_t work_bytes
                 "@" + p.func + " works in " + std::to_string(p.workspace) + " bytes at a multiple of 16, got " +
                     std::to_string(work_bytes));
   // these kernels take any element alignment, and none below it
-  if (p.kind == xt::PlanKind::RmsNorm || p.kind == xt::PlanKind::MatmulQ4 || p.kind == xt::PlanKind::Attend)
+  if (p.kind == xt::PlanKind::RmsNorm || p.kind == xt::PlanKind::MatmulQ4 || p.kind == xt::PlanKind::Attend ||
+      p.kind == xt::PlanKind::Mx4Rows || p.kind == xt::PlanKind::MatmulMx4 || p.kind == xt::PlanKind::Sample)
     for (size_t k = 0; k < p.arg_types.size(); ++k)
       if (reinterpret_cast<uintptr_t>(bufs[k]) % xt::elem_bytes(p.arg_types[k].elem))
         return fail(err, XT_ERR_ARGUMENT, "buffer " + std::to_string(k) + " is not aligned to its elements");
@@ -96,6 +97,9 @@ int run_plan(const xt::Plan& p, void* const* bufs, void* work, size_t work_bytes
     case xt::PlanKind::RmsNorm: e = xtk::launch_rms_norm(p, bufs, s, why); break;
     case xt::PlanKind::MatmulQ4: e = xtk::launch_matmul_q4(p, bufs, s, why); break;
     case xt::PlanKind::Attend: e = xtk::launch_attend(p, bufs, work, s, why); break;
+    case xt::PlanKind::Mx4Rows: e = xtk::launch_mx4_rows(p, bufs, s, why); break;
+    case xt::PlanKind::MatmulMx4: e = xtk::launch_matmul_mx4(p, bufs, s, why); break;
+    case xt::PlanKind::Sample: e = xtk::launch_sample(p, bufs, work, s, why); break;
   }
   if (!why.empty()) return fail(err, XT_ERR_ARGUMENT, why);
   if (e != hipSuccess)

@@ -10,7 +10,8 @@
 //   reshape / transpose / permute    lib/xt/XTOps.cpp:309-397
 // Extension (not in the reference): matmul and load_conv2d also accept
 // f16 x f16 and bf16 x bf16 inputs with an f32 result; the ops rms_norm,
-// row_scale, quantize, matmul_q4 and attend.
+// row_scale, quantize, matmul_q4, mx4_scale, quantize_mx4, dequantize_mx4, matmul_mx4,
+// attend and sample.
 #include <algorithm>
 #include <cmath>
 
@@ -115,8 +116,8 @@ struct Verifier {
     if (const Attr* w = find_attr(o.attrs, "window"))
       if (w->kind != Attr::Int || w->i <= 0 || w->i > 0x7fffffff)
         return fail(o.loc, n, "window attribute must be positive and below 2^31");
-    if (extras->kind != Attr::DenseArray || extras->ints.size() != 6)
-      return fail(o.loc, n, "extras attribute must have exactly 6 entries");
+    if (extras->kind != Attr::DenseArray || (extras->ints.size() != 6 && extras->ints.size() != 7))
+      return fail(o.loc, n, "extras attribute must have exactly 6 entries, or 7 with parents");
     size_t count = 3;
     for (int64_t e : extras->ints) {
       if (e != 0 && e != 1) return fail(o.loc, n, "extras attribute entries must be 0 or 1");
@@ -124,14 +125,78 @@ struct Verifier {
     }
     if (count != o.operands.size()) return fail(o.loc, n, "extras attribute does not match the operand count");
     if (extras->ints[4] != extras->ints[5]) return fail(o.loc, n, "q_docs and k_docs come together");
-    static const char* names[6] = {"slopes", "start", "length", "prefix", "q_docs", "k_docs"};
-    const int64_t cols[6] = {heads, 1, 1, 1, rows, nk};
-    for (size_t e = 0, at = 3; e < 6; ++e) {
+    const Attr* causal = find_attr(o.attrs, "causal");
+    if (extras->ints.size() == 7 && extras->ints[6] && (extras->ints[3] || extras->ints[4] || (causal && causal->i)))
+      return fail(o.loc, n, "takes parents without causal, prefix, q_docs and k_docs");
+    static const char* names[7] = {"slopes", "start", "length", "prefix", "q_docs", "k_docs", "parents"};
+    const int64_t cols[7] = {heads, 1, 1, 1, rows, nk, rows};
+    for (size_t e = 0, at = 3; e < extras->ints.size(); ++e) {
       if (!extras->ints[e]) continue;
       const Type want = Type::tensor(e == 0 ? Elem::F32 : Elem::I32, {1, cols[e]});
       if (T(o.operands[at++]) != want) return fail(o.loc, n, std::string(names[e]) + " must be a " + want.str());
     }
     return true;
+  }
+
+  // Rows in microscaled 4-bit floating point and their scales.
+  bool mx4_rows(const Op& o, const Type& q, const Type& s) {
+    if (q.elem != Elem::I8 || s.elem != Elem::I8) return fail(o.loc, o.name, "requires i8 rows and scales");
+    if (q.shape[1] % 16 || s.shape[0] != q.shape[0] || s.shape[1] != q.shape[1] / 16)
+      return fail(o.loc, o.name, "requires (R, C / 2) rows with (R, C / 32) scales");
+    return true;
+  }
+
+  bool verify_mx4(const Func& f, const Op& o) {
+    const std::string& n = o.name;
+    if (!rank2(f, o)) return false;
+    auto T = [&](int v) -> const Type& { return f.type_of(v); };
+    const Type &x = T(o.operands[0]), &r = T(o.results[0]);
+    if (n == "xt.mx4_scale" || n == "xt.quantize_mx4") {
+      if (!narrow_or_f32(x.elem)) return fail(o.loc, n, "requires an f32, f16 or bf16 operand");
+      if (x.shape[1] % 32) return fail(o.loc, n, "requires rows of whole blocks of 32");
+      const Type scale = Type::tensor(Elem::I8, {x.shape[0], x.shape[1] / 32});
+      if (n == "xt.mx4_scale")
+        return r == scale || fail(o.loc, n, "requires an i8 result with one scale a block of 32");
+      if (T(o.operands[1]) != scale) return fail(o.loc, n, "requires an i8 scale a block of 32");
+      return r == Type::tensor(Elem::I8, {x.shape[0], x.shape[1] / 2}) ||
+             fail(o.loc, n, "requires an i8 result with two values a byte");
+    }
+    if (!mx4_rows(o, x, T(o.operands[1]))) return false;
+    if (!narrow_or_f32(r.elem)) return fail(o.loc, n, "requires an f32, f16 or bf16 result");
+    if (n == "xt.dequantize_mx4")
+      return (r.shape[0] == x.shape[0] && r.shape[1] == 2 * x.shape[1]) ||
+             fail(o.loc, n, "requires a result with two values for each byte of the rows");
+    const Type& w = T(o.operands[2]);
+    if (!mx4_rows(o, w, T(o.operands[3]))) return false;
+    if (x.shape[1] != w.shape[1]) return fail(o.loc, n, "requires value and weight rows of one length");
+    return (r.shape[0] == x.shape[0] && r.shape[1] == w.shape[0]) ||
+           fail(o.loc, n, "result shape must match matmul output shape");
+  }
+
+  bool verify_sample(const Func& f, const Op& o) {
+    const std::string& n = o.name;
+    if (!rank2(f, o)) return false;
+    auto T = [&](int v) -> const Type& { return f.type_of(v); };
+    const Type& x = T(o.operands[0]);
+    if (!narrow_or_f32(x.elem)) return fail(o.loc, n, "requires f32, f16 or bf16 logits");
+    const Attr* extras = need_attr(o, "extras");
+    if (!extras) return false;
+    if (extras->kind != Attr::DenseArray || extras->ints.size() != 4)
+      return fail(o.loc, n, "extras attribute must have exactly 4 entries");
+    size_t count = 2;
+    for (int64_t e : extras->ints) {
+      if (e != 0 && e != 1) return fail(o.loc, n, "extras attribute entries must be 0 or 1");
+      count += static_cast<size_t>(e);
+    }
+    if (count != o.operands.size()) return fail(o.loc, n, "extras attribute does not match the operand count");
+    static const char* names[5] = {"uniform", "temperature", "top_k", "top_p", "min_p"};
+    for (size_t e = 0, at = 1; e < 5; ++e) {
+      if (e && !extras->ints[e - 1]) continue;
+      const Type want = Type::tensor(e == 2 ? Elem::I32 : Elem::F32, {x.shape[0], 1});
+      if (T(o.operands[at++]) != want) return fail(o.loc, n, std::string(names[e]) + " must be a " + want.str());
+    }
+    return T(o.results[0]) == Type::tensor(Elem::I32, {x.shape[0], 1}) ||
+           fail(o.loc, n, "requires an i32 result with one token a row");
   }
 
   bool verify_op(const Func& f, const Op& o) {
@@ -425,6 +490,9 @@ struct Verifier {
       return true;
     }
     if (n == "xt.attend") return verify_attend(f, o);
+    if (n == "xt.mx4_scale" || n == "xt.quantize_mx4" || n == "xt.dequantize_mx4" || n == "xt.matmul_mx4")
+      return verify_mx4(f, o);
+    if (n == "xt.sample") return verify_sample(f, o);
     if (n == "func.return") {
       if (o.operands.size() != f.result_types.size())
         return fail(o.loc, n, "has " + std::to_string(o.operands.size()) +

@@ -23,7 +23,9 @@ result, mirroring the reference's int8 -> float32 rule (xtile/dsl.py:369-370).
 Also an extension: `int32` arrays (positions, lengths, documents), and the
 operators of a language model's layer, each one op over whole tiles:
 `rms_norm`, `row_scale` and `quantize` (rows in 8 bits), `matmul_q4` (4-bit
-weights) and `attend` (masked attention).
+weights), `mx4_scale`, `quantize_mx4`, `dequantize_mx4` and `matmul_mx4`
+(microscaled 4-bit floating point), `attend` (masked attention) and `sample`
+(a token from its logits).
 """
 
 from __future__ import annotations
@@ -669,9 +671,85 @@ class TraceContext:
         self.ops.append(_Operator("xt.matmul_q4", result, operands))
         return result
 
+    def _float_rows(self, op: str, value) -> None:
+        self._need_tensor(value)
+        if len(value.shape) != 2:
+            raise ValueError(f"{op} currently supports rank-2 tensors only")
+        if value.dtype not in _FLOATS:
+            raise TypeError(f"{op} requires a float32, float16 or bfloat16 tensor")
+        if value.shape[1] % 32:
+            raise ValueError(f"{op} requires rows of whole blocks of 32")
+
+    def _mx4_rows(self, op: str, value, scale) -> tuple[int, int]:
+        """(rows, values a row) of packed rows and their scales."""
+        self._need_tensor(value)
+        self._need_tensor(scale)
+        if len(value.shape) != 2 or len(scale.shape) != 2:
+            raise ValueError(f"{op} currently supports rank-2 tensors only")
+        if value.dtype != int8 or scale.dtype != int8:
+            raise TypeError(f"{op} requires int8 rows and scales, as quantize_mx4 and mx4_scale give them")
+        if value.shape[1] % 16 or scale.shape != (value.shape[0], value.shape[1] // 16):
+            raise ValueError(f"{op} requires (R, C / 2) rows with (R, C / 32) scales")
+        return value.shape[0], 2 * value.shape[1]
+
+    def mx4_scale(self, value) -> TensorValue:
+        self._float_rows("xt.mx4_scale", value)
+        result = self._value("mx4_scale", (value.shape[0], value.shape[1] // 32), int8)
+        self.ops.append(_Operator("xt.mx4_scale", result, (value,)))
+        return result
+
+    def quantize_mx4(self, value, scale) -> TensorValue:
+        self._float_rows("xt.quantize_mx4", value)
+        self._need_tensor(scale)
+        if scale.shape != (value.shape[0], value.shape[1] // 32) or scale.dtype != int8:
+            raise ValueError("xt.quantize_mx4 requires the int8 (R, C / 32) scale of mx4_scale")
+        result = self._value("quantized", (value.shape[0], value.shape[1] // 2), int8)
+        self.ops.append(_Operator("xt.quantize_mx4", result, (value, scale)))
+        return result
+
+    def dequantize_mx4(self, value, scale, dtype: DType = float32) -> TensorValue:
+        shape = self._mx4_rows("xt.dequantize_mx4", value, scale)
+        if dtype not in _FLOATS:
+            raise TypeError("xt.dequantize_mx4 requires a float32, float16 or bfloat16 result")
+        result = self._value("values", shape, dtype)
+        self.ops.append(_Operator("xt.dequantize_mx4", result, (value, scale)))
+        return result
+
+    def matmul_mx4(self, value, value_scale, weight, weight_scale, dtype: DType = float32) -> TensorValue:
+        m, k = self._mx4_rows("xt.matmul_mx4", value, value_scale)
+        n, wk = self._mx4_rows("xt.matmul_mx4", weight, weight_scale)
+        if dtype not in _FLOATS:
+            raise TypeError("xt.matmul_mx4 requires a float32, float16 or bfloat16 result")
+        if k != wk:
+            raise ValueError("xt.matmul_mx4 requires value and weight rows of one length")
+        result = self._value("matmul", (m, n), dtype)
+        self.ops.append(_Operator("xt.matmul_mx4", result, (value, value_scale, weight, weight_scale)))
+        return result
+
+    def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None) -> TensorValue:
+        extras = (temperature, top_k, top_p, min_p)
+        for t in (logits, uniform, *(e for e in extras if e is not None)):
+            self._need_tensor(t)
+        if len(logits.shape) != 2:
+            raise ValueError("xt.sample currently supports rank-2 tensors only")
+        if logits.dtype not in _FLOATS:
+            raise TypeError("xt.sample requires float32, float16 or bfloat16 logits")
+        rows = (logits.shape[0], 1)
+        for name, t in zip(("uniform", "temperature", "top_k", "top_p", "min_p"), (uniform, *extras)):
+            dtype = int32 if name == "top_k" else float32
+            if t is not None and (t.shape != rows or t.dtype != dtype):
+                raise ValueError(f"xt.sample requires {name} of shape {rows} and dtype {dtype.name}")
+        present = ", ".join("1" if e is not None else "0" for e in extras)
+        result = self._value("token", rows, int32)
+        operands = (logits, uniform, *(e for e in extras if e is not None))
+        self.ops.append(_Operator("xt.sample", result, operands, (("extras", f"array<i32: {present}>"),)))
+        return result
+
     def attend(self, q, k, v, scale, cap=None, causal=False, window=None, slopes=None, start=None, length=None,
-               prefix=None, q_docs=None, k_docs=None) -> TensorValue:
+               prefix=None, q_docs=None, k_docs=None, parents=None) -> TensorValue:
         extras = (slopes, start, length, prefix, q_docs, k_docs)
+        if parents is not None:
+            extras = (*extras, parents)
         for t in (q, k, v, *(e for e in extras if e is not None)):
             self._need_tensor(t)
         if q.dtype not in _NARROW_FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -687,8 +765,10 @@ class TraceContext:
             raise ValueError("xt.attend requires a (heads, rows, D) or (rows, heads * D) query tensor")
         if (q_docs is None) != (k_docs is None):
             raise ValueError("xt.attend requires q_docs and k_docs together")
-        wants = ((1, heads), (1, 1), (1, 1), (1, 1), (1, rows), (1, nk))
-        for name, t, shape in zip(("slopes", "start", "length", "prefix", "q_docs", "k_docs"), extras, wants):
+        if parents is not None and (causal or prefix is not None or q_docs is not None):
+            raise ValueError("xt.attend takes parents without causal, prefix, q_docs and k_docs")
+        wants = ((1, heads), (1, 1), (1, 1), (1, 1), (1, rows), (1, nk), (1, rows))
+        for name, t, shape in zip(("slopes", "start", "length", "prefix", "q_docs", "k_docs", "parents"), extras, wants):
             dtype = float32 if name == "slopes" else int32
             if t is not None and (t.shape != shape or t.dtype != dtype):
                 raise ValueError(f"xt.attend requires {name} of shape {shape} and dtype {dtype.name}")
@@ -905,8 +985,56 @@ def matmul_q4(value, weight, scales, *, row_scale=None, dtype: DType = float32):
     return _trace("matmul_q4").matmul_q4(value, weight, scales, row_scale=row_scale, dtype=dtype)
 
 
+def mx4_scale(value):
+    """(R, C / 32) int8 scales of rows in microscaled 4-bit floating point: of each
+    block of 32 neighbours the byte e + 127 (0 to 254 unsigned) of the power 2**e that the block's values are
+    multiples of, e = floor(log2(largest magnitude)) - 2, at least -127; 0 for a
+    block of zeros, 255 for one with an infinity or NaN."""
+    return _trace("mx4_scale").mx4_scale(value)
+
+
+def quantize_mx4(value, scale):
+    """(R, C / 2) int8 rows: `value / 2**e` of each block of 32, with the `scale` that
+    mx4_scale gave for them, to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4 and 6 with a
+    sign (halfway to the one whose last bit is 0; magnitudes above 6 are 6).  Two
+    values a byte, the first in the lower half: sign, two bits of exponent, one of
+    mantissa.  All 0 in blocks with an infinity or NaN."""
+    return _trace("quantize_mx4").quantize_mx4(value, scale)
+
+
+def dequantize_mx4(value, scale, *, dtype: DType = float32):
+    """The (R, C) values of rows of quantize_mx4 and their scales, rounded once to
+    `dtype`; NaN in blocks whose scale is 255."""
+    return _trace("dequantize_mx4").dequantize_mx4(value, scale, dtype=dtype)
+
+
+def matmul_mx4(value, value_scale, weight, weight_scale, *, dtype: DType = float32):
+    """`value @ weight.T` of rows in microscaled 4-bit floating point: value (M, K / 2)
+    and weight (N, K / 2) with scales (M, K / 32) and (N, K / 32), as quantize_mx4
+    and mx4_scale give them.  Sums are held in 32 bits; a row with a scale of 255 is
+    NaN."""
+    return _trace("matmul_mx4").matmul_mx4(value, value_scale, weight, weight_scale, dtype=dtype)
+
+
+def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=None):
+    """(R, 1) int32 tokens, one drawn from each row of (R, V) logits.
+
+    A token's weight is `exp((logit - largest) / temperature)`; temperatures of 0
+    or less, and NaN, leave the largest logits alone, and logits of plus infinity
+    leave nothing but themselves.  Tokens are ordered by logit, the largest first,
+    equal ones by index.  Of the order's beginning remain: the first `top_k` tokens
+    (0 or less: all); of those the fewest whose weights reach `top_p` of their total
+    (1 or more, and NaN: all; at least one); and those whose weight is at least `min_p` of the largest
+    (above 1: as 1; NaN: as 0).  The result is the first whose weights, summed in that order, exceed
+    `uniform` times the sum of what remains: `uniform` is held within 0 and what is just
+    below 1, NaN as 0.  Weights and sums are held in 64 bits.  Logits of NaN
+    count as minus infinity, and a row of nothing else gives -1.  All but the logits
+    are (R, 1) tiles, float32 or, top_k, int32."""
+    return _trace("sample").sample(logits, uniform, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
 def attend(q, k, v, *, scale, cap=None, causal=False, window=None, slopes=None, start=None, length=None, prefix=None,
-           q_docs=None, k_docs=None):
+           q_docs=None, k_docs=None, parents=None):
     """`softmax(scores) v` over the keys that each query row sees.
 
     q is (heads, rows, D) or (rows, heads * D); its heads share k and v, (keys,
@@ -918,9 +1046,18 @@ def attend(q, k, v, *, scale, cap=None, causal=False, window=None, slopes=None, 
     rows), k_docs (1, keys), int32); and j < prefix (a (1, 1) int32 tile), or
     j <= p if `causal` and p - j < window if `window` is given.  Rows that see
     nothing, or only scores of minus infinity, are 0.  What hidden keys and
-    values hold, NaN included, has no effect."""
+    values hold, NaN included, has no effect.
+
+    With `parents`, a (1, rows) int32 tile, the rows are a tree of drafted tokens
+    that follows the keys before `start`, and key start + u is drafted token u's.
+    parents[t] is the drafted token that t continues, one before t; any other
+    value is none: t continues the keys before `start`.  Row t is at position
+    start + its depth (the number of its ancestors), key start + u at that of token
+    u.  Of the drafted tokens a row sees its ancestors and itself (under `window`
+    and `length` as above), of the keys behind them none.  Not with `causal`,
+    `prefix` or documents."""
     return _trace("attend").attend(q, k, v, scale, cap=cap, causal=causal, window=window, slopes=slopes, start=start,
-                                   length=length, prefix=prefix, q_docs=q_docs, k_docs=k_docs)
+                                   length=length, prefix=prefix, q_docs=q_docs, k_docs=k_docs, parents=parents)
 
 
 def convert(kernel_fn, *, args, grid, double_buffering, parse_module):

@@ -13,7 +13,8 @@ the tile sizes of the five benchmark configurations:
               A shared along axis 0 (`shared = 1`)
 
 Beside them: `layernorm`, `column_softmax`, `bias_add` and `attention`, and the
-operators of a language model's layer: `rms_norm`, `matmul_q4`, `masked_attention`.
+operators of a language model's layer: `rms_norm`, `matmul_q4`, `quantize_mx4`,
+`dequantize_mx4`, `matmul_mx4`, `masked_attention` and `sample`.
 """
 
 from __future__ import annotations
@@ -27,6 +28,7 @@ from . import (
     bid,
     cdiv,
     convert,
+    dequantize_mx4 as tile_dequantize_mx4,
     exp,
     float16,
     float32,
@@ -36,15 +38,19 @@ from . import (
     load,
     load_conv2d,
     matmul,
+    matmul_mx4 as tile_matmul_mx4,
     matmul_q4 as tile_matmul_q4,
     max as tile_max,
     mul as tile_mul,
+    mx4_scale,
     quantize,
+    quantize_mx4 as tile_quantize_mx4,
     reciprocal,
     rms_norm as tile_rms_norm,
     row_scale as tile_row_scale,
     rsqrt,
     reshape,
+    sample as tile_sample,
     store,
     sub as tile_sub,
     sum as tile_sum,
@@ -393,17 +399,91 @@ def matmul_q4(m: int, n: int, k: int, *, group: int = 128, dtype=bfloat16, scale
     return convert(_named("matmul_q4_kernel", body, len(args)), args=args, grid=(1, 1, 1))
 
 
+def quantize_mx4(rows: int, cols: int, dtype=bfloat16, *, values: bool = False):
+    """Rows in microscaled 4-bit floating point: blocks of 32 values with a scale each.
+
+    Buffers: x (rows, cols), the rows (rows, cols / 2) int8, their scales (rows,
+    cols / 32) int8 and, with `values`, what they stand for (rows, cols) of `dtype`."""
+    arrays = [Array(shape=(rows, cols), dtype=dtype), *_mx4_arrays(rows, cols)]
+    if values:
+        arrays.append(arrays[0])
+
+    def body(args):
+        x = load(args[0], index=(0, 0), shape=(rows, cols))
+        s = mx4_scale(x)
+        q = tile_quantize_mx4(x, s)
+        store(args[1], index=(0, 0), tile=q)
+        store(args[2], index=(0, 0), tile=s)
+        if values:
+            store(args[3], index=(0, 0), tile=tile_dequantize_mx4(q, s, dtype=dtype))
+
+    return convert(_named("quantize_mx4_kernel", body, len(arrays)), args=tuple(arrays), grid=(1, 1, 1))
+
+
+def dequantize_mx4(rows: int, cols: int, dtype=bfloat16):
+    """The values of such rows.  Buffers: the rows (rows, cols / 2) int8, their scales
+    (rows, cols / 32) int8, y (rows, cols) of `dtype`."""
+    arrays = [*_mx4_arrays(rows, cols), Array(shape=(rows, cols), dtype=dtype)]
+
+    def body(args):
+        q, s = (load(a, index=(0, 0), shape=t.shape) for a, t in zip(args, arrays[:2]))
+        store(args[2], index=(0, 0), tile=tile_dequantize_mx4(q, s, dtype=dtype))
+
+    return convert(_named("dequantize_mx4_kernel", body, 3), args=tuple(arrays), grid=(1, 1, 1))
+
+
+def matmul_mx4(m: int, n: int, k: int, *, out=float32):
+    """x (m, k) against n rows of k weights, both in microscaled 4-bit floating point.
+
+    Buffers: the rows of x (m, k / 2) int8 and their scales (m, k / 32) int8, the
+    weights (n, k / 2) and theirs (n, k / 32), y (m, n) of `out`."""
+    arrays = [*_mx4_arrays(m, k), *_mx4_arrays(n, k)]
+
+    def body(args):
+        tiles = [load(a, index=(0, 0), shape=t.shape) for a, t in zip(args, arrays)]
+        store(args[4], index=(0, 0), tile=tile_matmul_mx4(*tiles, dtype=out))
+
+    args = (*arrays, Array(shape=(m, n), dtype=out))
+    return convert(_named("matmul_mx4_kernel", body, len(args)), args=args, grid=(1, 1, 1))
+
+
+def sample(rows: int, vocab: int, dtype=float32, *, temperature: bool = False, top_k: bool = False,
+           top_p: bool = False, min_p: bool = False, trow: int | None = None):
+    """One token of each row of logits; `xtile_amd.sample` states which.
+
+    Buffers: logits (rows, vocab), uniform (rows, 1) float32, those of temperature
+    (float32), top_k (int32), top_p and min_p (float32) that are asked for, (rows, 1)
+    each, then the tokens (rows, 1) int32.  `trow` rows a Block (default: all)."""
+    trow = rows if trow is None else trow
+    if trow < 1 or rows % trow:
+        raise ValueError("trow must divide rows")
+    one = Array(shape=(rows, 1), dtype=float32)
+    asked = {"temperature": (temperature, one), "top_k": (top_k, Array(shape=(rows, 1), dtype=int32)),
+             "top_p": (top_p, one), "min_p": (min_p, one)}
+    extras = {name: array for name, (wanted, array) in asked.items() if wanted}
+
+    def body(args):
+        r = bid(0)
+        x = load(args[0], index=(r, 0), shape=(trow, vocab))
+        u, *rest = (load(a, index=(r, 0), shape=(trow, 1)) for a in args[1:-1])
+        store(args[-1], index=(r, 0), tile=tile_sample(x, u, **dict(zip(extras, rest))))
+
+    args = (Array(shape=(rows, vocab), dtype=dtype), one, *extras.values(), Array(shape=(rows, 1), dtype=int32))
+    return convert(_named("sample_kernel", body, len(args)), args=args, grid=(rows // trow, 1, 1))
+
+
 def masked_attention(batch: int, kv_heads: int, group: int, nq: int, nk: int, d: int, *, dtype=bfloat16, scale=None,
                      cap=None, causal: bool = False, window=None, slopes: bool = False, start: bool = False,
-                     length: bool = False, prefix: bool = False, docs: bool = False, token_major: bool = False):
+                     length: bool = False, prefix: bool = False, docs: bool = False, parents: bool = False,
+                     token_major: bool = False):
     """Attention of `group` query heads to each key head, one Block a key head.
 
     Buffers: q and the result [batch, kv_heads * group, nq, d], k and v [batch,
     kv_heads, nk, d], or, `token_major`, [batch, nq, kv_heads * group * d] and
     [batch, nk, kv_heads * d]; between v and the result, where asked for: slopes
     (kv_heads, group) float32; start, length, prefix (batch, 1) int32; the documents
-    of the queries (batch, nq) and of the keys (batch, nk) int32.  Their meaning is
-    `attend`'s.  `scale` defaults to d ** -0.5."""
+    of the queries (batch, nq) and of the keys (batch, nk) int32; the parents of
+    drafted tokens (batch, nq) int32.  Their meaning is `attend`'s.  `scale` defaults to d ** -0.5."""
     if min(batch, kv_heads, group, nq, nk, d) < 1:
         raise ValueError("masked_attention sizes must be positive")
     heads = kv_heads * group
@@ -413,7 +493,8 @@ def masked_attention(batch: int, kv_heads: int, group: int, nq: int, nk: int, d:
     named = {"slopes": (slopes, Array(shape=(kv_heads, group), dtype=float32)), "start": (start, per_batch),
              "length": (length, per_batch), "prefix": (prefix, per_batch),
              "q_docs": (docs, Array(shape=(batch, nq), dtype=int32)),
-             "k_docs": (docs, Array(shape=(batch, nk), dtype=int32))}
+             "k_docs": (docs, Array(shape=(batch, nk), dtype=int32)),
+             "parents": (parents, Array(shape=(batch, nq), dtype=int32))}
     extras = {name: array for name, (wanted, array) in named.items() if wanted}
     scale = d**-0.5 if scale is None else scale
 
@@ -441,6 +522,13 @@ def masked_attention(batch: int, kv_heads: int, group: int, nq: int, nk: int, d:
 
 
 _quantize = quantize
+
+
+def _mx4_arrays(rows: int, cols: int):
+    """Packed rows and their scales."""
+    if cols % 32:
+        raise ValueError("rows in microscaled 4-bit floating point are whole blocks of 32")
+    return Array(shape=(rows, cols // 2), dtype=int8), Array(shape=(rows, cols // 32), dtype=int8)
 
 
 def _named(name: str, body, count: int):
