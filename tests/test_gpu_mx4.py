@@ -9,6 +9,7 @@ import xtile_amd as xt
 from xtile_amd import kernels as K
 
 from . import answers_ref as ref
+from .gpu_util import kernels_of
 from .operators_ref import HALF
 
 pytestmark = pytest.mark.gpu
@@ -230,6 +231,44 @@ def test_products(m, n, k, out):
     rng = np.random.default_rng(m * n + k)
     x, w = random_rows(rng, m, k, 122, 130), random_rows(rng, n, k, 122, 130)
     check_product(run_product(x, w, out), x, w, out)
+
+
+def product_buffers(x, w, out="f32"):
+    import torch
+
+    m, n = x[0].shape[0], w[0].shape[0]
+    return [int8(ref.pack(x[0])), int8(x[1]), int8(ref.pack(w[0])), int8(w[1]),
+            torch.full((m, n), 3.0, dtype=torch_dtype(out), device="cuda")]
+
+
+# Sizes of which each kernel takes some; none is a multiple of a tile, nor K of a stage.
+KERNELS = [(3, 100, 1056, "few_kernel<8, 8>"), (5, 9000, 1056, "few_kernel<8, 4>"), (15, 100, 4128, "few_kernel<16, 8>"),
+           (12, 9000, 1056, "few_kernel<16, 4>"), (63, 4090, 2080, "mid_kernel<1, 1, 8>"), (125, 4090, 1056, "mid_kernel<1, 2, 4>"),
+           (250, 4090, 1056, "mid_kernel<2, 2, 4>"), (1001, 4090, 544, "many_kernel<128, 128, 4, 3>"),
+           (1500, 4090, 1056, "many_kernel<128, 128, 4, 2>"), (4090, 4000, 288, "many_kernel<256, 256, 8, 2>")]
+
+
+@pytest.mark.parametrize("m,n,k,kernel", KERNELS)
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_every_kernel(m, n, k, kernel, out):
+    rng = np.random.default_rng(k)
+    x, w = random_rows(rng, m, k, 122, 130), random_rows(rng, n, k, 122, 130)
+    bufs = product_buffers(x, w, out)
+    program = K.matmul_mx4(m, n, k, out=DTYPES[out])
+    print(f"[gpu] matmul_mx4 {m} x {n} x {k} -> {out}: {kernel}", flush=True)
+    assert kernels_of(program, bufs) == ["matmul_mx4_" + kernel]
+    check_product(bufs[4].cpu().double().numpy(), x, w, out)
+
+
+@pytest.mark.parametrize("k", [32, 64, 96, 224, 256, 288, 480, 512, 544, 768, 800, 1056, 1312])
+@pytest.mark.parametrize("m,n", [(1000, 4090), (1500, 4090), (4090, 4000)])
+def test_large_tiles_of_every_depth(m, n, k):
+    """From fewer stages than buffers to more, with and without a part of one; scales of 255 in
+    the last row and column."""
+    rng = np.random.default_rng(k)
+    x, w = random_rows(rng, m, k, 122, 130), random_rows(rng, n, k, 122, 130)
+    x[1][-1, -1] = w[1][-1, 0] = 255
+    check_product(run_product(x, w, "f32"), x, w, "f32")
 
 
 @pytest.mark.parametrize("m,n,k", [(5, 40, 512), (40, 60, 288), (300, 290, 544)])

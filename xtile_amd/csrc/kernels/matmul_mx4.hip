@@ -13,6 +13,7 @@
 #include "launch.h"
 
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 
@@ -35,7 +36,8 @@ struct Mx4Args {
   long long ldx, ldxs, ldw, ldws, ldy;  // bytes; y: elements
   BlockDecode blocks;
   Div31 d_tiles, d_nt;  // tiles of a Block, n tiles
-  int tiles, ntiles;
+  Div31 d_group, d_width, d_last;  // of many rows: a group's tiles, its columns, the last one's
+  int tiles, ntiles, mtiles, group, nwg;
   int M, N, blocks_k;  // blocks of 32 of a row
   int dma;
   int y_elem;
@@ -73,17 +75,17 @@ struct Pieces {
   }
 };
 
-// Three words of 21 rows' scales that one instruction brings (lane 3 r + i: word i of row
-// first + r), at most `count` of them.  Rows begin at any byte: a word that holds none of
-// the eight bytes, or none of a row's, is not read.
+// Three words a row of scales, 64 of which one instruction brings: words first on, of rows
+// below `count`.  Rows begin at any byte: a word that holds none of the eight bytes, or none
+// of a row's, is not read.
 struct Scales {
   unsigned off;  // of the word, less the bytes before it
   int before;    // bytes of the word before the row's first
   __device__ __forceinline__ void begin(const unsigned char* base, int first, int count, int rows, long long ld) {
-    const int lane = threadIdx.x & 63, r = lane / 3, i = lane - 3 * r, row = first + r;
+    const int word = first + (threadIdx.x & 63), row = word / 3, i = word - 3 * row;
     const unsigned at = (unsigned)row * (unsigned)ld, odd = ((unsigned)reinterpret_cast<uintptr_t>(base) + at) & 3;
     before = (int)odd - 4 * i;
-    off = r < count && row < rows && before > -kBlocks ? at - (unsigned)before : kNone;
+    off = row < min(count, rows) && before > -kBlocks ? at - (unsigned)before : kNone;
   }
   // from: the scales at this stage's first block.  The descriptor begins three bytes
   // earlier, for words that begin before their row.
@@ -116,20 +118,34 @@ __device__ __forceinline__ void put(void* y, int elem, long long at, float v) {
   else static_cast<__bf16*>(y)[at] = (__bf16)v;
 }
 
-// Few rows of x: a workgroup has 16 rows of weights and 16 MT of x, its W waves split K in
-// stages, each in a ring of its own, and meet once, in LDS, in a fixed order.
-// XR: rows of x in LDS (8, of which the MFMA's 16 are the same ones twice, or 16 MT).
-template <int MT, int XR, int W, int NS>
+// Four neighbours of a row, at element alignment.
+__device__ __forceinline__ void put4(void* y, int elem, long long at, float4v v) {
+  if (elem == kF32) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    *reinterpret_cast<f4*>(static_cast<float*>(y) + at) = (f4)v;
+  } else if (elem == kF16) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4), aligned(2)));
+    *reinterpret_cast<h4*>(static_cast<_Float16*>(y) + at) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+  } else {
+    typedef __bf16 b4 __attribute__((ext_vector_type(4), aligned(2)));
+    *reinterpret_cast<b4*>(static_cast<__bf16*>(y) + at) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+  }
+}
+
+// Few rows of x: a workgroup has 16 rows of weights and 16 of x, its W waves split K in
+// stages, each in a ring of two of its own, and meet once, in LDS, in a fixed order.
+// XR: rows of x in LDS (8, of which the MFMA's 16 are the same ones twice, or 16).
+template <int XR, int W>
 struct FewShape {
-  static constexpr int X0 = 2048, S0 = X0 + XR * 128, STAGE = S0 + 256 * (1 + MT);
-  static constexpr int XI = XR / 8, PER = 2 + XI + 1 + MT;  // instructions of a stage
-  static constexpr int LDS = W * NS * STAGE;
-  static_assert(LDS <= 160 * 1024 && (NS - 1) * PER < 64 && W * MT * 1024 <= LDS, "");
+  static constexpr int X0 = 2048, S0 = X0 + XR * 128, STAGE = S0 + 512;
+  static constexpr int XI = XR / 8, PER = 2 + XI + 2;  // instructions of a stage
+  static constexpr int LDS = W * 2 * STAGE;
+  static_assert(LDS <= 160 * 1024 && W * 1024 <= LDS, "");
 };
 
-template <int MT, int XR, int W, int NS>
+template <int XR, int W>
 __global__ __launch_bounds__(64 * W) void matmul_mx4_few_kernel(Mx4Args p) {
-  typedef FewShape<MT, XR, W, NS> S;
+  typedef FewShape<XR, W> S;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[S::LDS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -139,22 +155,21 @@ __global__ __launch_bounds__(64 * W) void matmul_mx4_few_kernel(Mx4Args p) {
   const int tm = (int)p.d_nt(tile), tn = tile - tm * p.ntiles;
   int bx, by, bz;
   p.blocks(b, bx, by, bz);
-  const int m0 = tm * 16 * MT, n0 = tn * 16, mrows = p.M - m0, nrows = p.N - n0;
+  const int m0 = tm * 16, n0 = tn * 16, mrows = p.M - m0, nrows = p.N - n0;
   const unsigned char* const w = p.w + p.tw.at(bx, by, bz) + n0 * p.ldw;
   const unsigned char* const ws = p.ws + p.tws.at(bx, by, bz) + n0 * p.ldws;
   const unsigned char* const x = p.x + p.tx.at(bx, by, bz) + m0 * p.ldx;
   const unsigned char* const xs = p.xs + p.txs.at(bx, by, bz) + m0 * p.ldxs;
 
   Pieces pw[2], px[S::XI];
-  Scales sw, sx[MT];
+  Scales sw, sx;
 #pragma unroll
   for (int i = 0; i < 2; ++i) pw[i].begin(8 * i, nrows, p.ldw);
 #pragma unroll
   for (int i = 0; i < S::XI; ++i) px[i].begin(8 * i, mrows, p.ldx);
   sw.begin(ws, 0, 16, nrows, p.ldws);
-#pragma unroll
-  for (int i = 0; i < MT; ++i) sx[i].begin(xs, 16 * i, 16, mrows, p.ldxs);
-  unsigned char* const ring = lds + wave * NS * S::STAGE;
+  sx.begin(xs, 0, XR, mrows, p.ldxs);
+  unsigned char* const ring = lds + wave * 2 * S::STAGE;
   auto issue = [&](int c, int slot) {
     unsigned char* const at = ring + slot * S::STAGE;
     const int left = p.blocks_k - c * kBlocks;
@@ -164,94 +179,542 @@ __global__ __launch_bounds__(64 * W) void matmul_mx4_few_kernel(Mx4Args p) {
 #pragma unroll
     for (int i = 0; i < S::XI; ++i) px[i].issue(p.dma, x + d, left, at + S::X0 + 1024 * i);
     sw.issue(ws + c * kBlocks, left, at + S::S0);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sx[i].issue(xs + c * kBlocks, left, at + S::S0 + 256 * (1 + i));
+    sx.issue(xs + c * kBlocks, left, at + S::S0 + 256);
   };
 
-  float4v y[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) y[i] = float4v{0, 0, 0, 0};
+  float4v y = {0, 0, 0, 0};
   const int stages = (p.blocks_k + kBlocks - 1) / kBlocks, mine = max(0, (stages - wave + W - 1) / W);
-#pragma unroll
-  for (int j = 0; j < NS; ++j)
-    if (j < mine) issue(wave + j * W, j);
-  // this lane's row of each operand: where it lies, and its scales' first byte
-  const int xrow = XR < 16 ? col % XR : col;
-  const int wodd = odd_of(ws, col, p.ldws);
-  int xodd[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) xodd[i] = odd_of(xs, 16 * i + xrow, p.ldxs);
+  if (mine > 0) issue(wave, 0);
+  if (mine > 1) issue(wave + W, 1);
+  // this lane's row of x, and where the scales of its two rows begin
+  const int xrow = col % XR, wodd = odd_of(ws, col, p.ldws), xodd = odd_of(xs, xrow, p.ldxs);
   int slot = 0;
 #pragma unroll 1
   for (int j = 0; j < mine; ++j) {
-    const int ahead = p.dma ? min(mine - 1 - j, NS - 1) : 0;
-    switch (ahead) {
-      case 0: XTK_WAIT_VM(0); break;
-      case 1: XTK_WAIT_VM(S::PER); break;
-      case 2: XTK_WAIT_VM(NS > 2 ? 2 * S::PER : 0); break;
-      default: XTK_WAIT_VM(NS > 3 ? 3 * S::PER : 0); break;
-    }
+    if (p.dma && j + 1 < mine) XTK_WAIT_VM(S::PER);
+    else XTK_WAIT_VM(0);
     asm volatile("" ::: "memory");
     const int left = p.blocks_k - (wave + j * W) * kBlocks;
     const unsigned char* const at = ring + slot * S::STAGE;
     // MFMA i has blocks 2 g + i; a lane's two scale bytes are moved to the low half
-    uint4v wf[2], xf[MT][2];
-    int sc[1 + MT];
+    uint4v wf[2], xf[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       wf[i] = *reinterpret_cast<const uint4v*>(at + col * 128 + piece_of(col, 2 * g + i) * 16);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int row = XR < 16 ? xrow : 16 * t + col;
-        xf[t][i] = *reinterpret_cast<const uint4v*>(at + S::X0 + row * 128 + piece_of(row, 2 * g + i) * 16);
-      }
+      xf[i] = *reinterpret_cast<const uint4v*>(at + S::X0 + xrow * 128 + piece_of(xrow, 2 * g + i) * 16);
     }
-    sc[0] = scale_word(at + S::S0 + col * 12, g >> 1, wodd, left) >> (16 * (g & 1));
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-      sc[1 + t] = scale_word(at + S::S0 + 256 * (1 + t) + xrow * 12, g >> 1, xodd[t], left) >> (16 * (g & 1));
+    const int sa = scale_word(at + S::S0 + 256 + xrow * 12, g >> 1, xodd, left) >> (16 * (g & 1));
+    const int sb = scale_word(at + S::S0 + col * 12, g >> 1, wodd, left) >> (16 * (g & 1));
     // every fragment is in registers before the slot is filled again
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    if (j + NS < mine) issue(wave + (j + NS) * W, slot);
-    slot = slot + 1 == NS ? 0 : slot + 1;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      y[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(xf[t][0]), wide(wf[0]), y[t], 4, 4, 0, sc[1 + t], 0, sc[0]);
-      y[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(xf[t][1]), wide(wf[1]), y[t], 4, 4, 1, sc[1 + t], 1, sc[0]);
-    }
+    if (j + 2 < mine) issue(wave + (j + 2) * W, slot);
+    slot ^= 1;
+    y = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(xf[0]), wide(wf[0]), y, 4, 4, 0, sa, 0, sb);
+    y = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(xf[1]), wide(wf[1]), y, 4, 4, 1, sa, 1, sb);
   }
   __syncthreads();  // every ring is done with
 
   // the waves' parts, summed in the order of the waves
   float* const part = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) part[((wave * MT + i) * 4 + r) * 64 + lane] = y[i][r];
+  for (int r = 0; r < 4; ++r) part[(wave * 4 + r) * 64 + lane] = y[r];
   __syncthreads();
-  const long long y0 = p.ty.at(bx, by, bz);
-  for (int e = threadIdx.x; e < MT * 256; e += 64 * W) {
-    const int i = e >> 8, r = (e >> 6) & 3, l = e & 63;
-    const int m = m0 + 16 * i + 4 * (l >> 4) + r, n = n0 + (l & 15);
-    if (m >= p.M || n >= p.N) continue;
-    float v = 0.0f;
+  const int e = threadIdx.x, r = e >> 6, l = e & 63;
+  const int m = m0 + 4 * (l >> 4) + r, n = n0 + (l & 15);
+  if (e >= 256 || m >= p.M || n >= p.N) return;
+  float v = 0.0f;
 #pragma unroll
-    for (int u = 0; u < W; ++u) v += part[u * MT * 256 + e];
-    put(p.y, p.y_elem, y0 + m * p.ldy + n, v);
-  }
+  for (int u = 0; u < W; ++u) v += part[u * 256 + e];
+  put(p.y, p.y_elem, p.ty.at(bx, by, bz) + m * p.ldy + n, v);
 }
 
-template <int MT, int XR, int W, int NS>
+template <int XR, int W>
 bool run_few(Mx4Args& a, long long blocks, hipStream_t s) {
-  const long long nt = (a.N + 15) / 16, tiles = nt * ((a.M + 16 * MT - 1) / (16 * MT));
+  const long long nt = (a.N + 15) / 16, tiles = nt * ((a.M + 15) / 16);
   if (tiles > 0x7fffffffLL || !grid_fits(tiles * blocks, 64 * W)) return false;
   a.tiles = static_cast<int>(tiles);
   a.ntiles = static_cast<int>(nt);
   a.d_tiles = div31(a.tiles);
   a.d_nt = div31(a.ntiles);
-  matmul_mx4_few_kernel<MT, XR, W, NS><<<static_cast<unsigned>(tiles * blocks), 64 * W, 0, s>>>(a);
+  matmul_mx4_few_kernel<XR, W><<<static_cast<unsigned>(tiles * blocks), 64 * W, 0, s>>>(a);
   return true;
+}
+
+// Tiles of 32 MT x 32 NT of the result, between the two: the waves split K as above, on
+// 32 x 32 x 64 MFMAs; a lane's half has blocks 4 h + i of a stage in step i.
+template <int MT, int NT, int W>
+struct MidShape {
+  static constexpr int X0 = NT * 4096, S0 = X0 + MT * 4096;
+  static constexpr int WI = (NT * 96 + 63) / 64, XI = (MT * 96 + 63) / 64;  // instructions for scales
+  static constexpr int STAGE = S0 + 256 * (WI + XI), PER = 4 * (MT + NT) + WI + XI;
+  static constexpr int PARTS = W * MT * NT * 4096;
+  static constexpr int LDS = W * 2 * STAGE > PARTS ? W * 2 * STAGE : PARTS;
+  static_assert(LDS <= 160 * 1024 && PER < 64, "");
+};
+
+template <int MT, int NT, int W>
+__global__ __launch_bounds__(64 * W) void matmul_mx4_mid_kernel(Mx4Args p) {
+  typedef MidShape<MT, NT, W> S;
+  typedef float float16v __attribute__((ext_vector_type(16)));
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[S::LDS];
+  const int lane = threadIdx.x & 63, lrow = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = (int)p.d_tiles(blockIdx.x);
+  const int tile = blockIdx.x - b * p.tiles;
+  const int tm = (int)p.d_nt(tile), tn = tile - tm * p.ntiles;
+  int bx, by, bz;
+  p.blocks(b, bx, by, bz);
+  const int m0 = tm * 32 * MT, n0 = tn * 32 * NT, mrows = p.M - m0, nrows = p.N - n0;
+  const unsigned char* const w = p.w + p.tw.at(bx, by, bz) + n0 * p.ldw;
+  const unsigned char* const ws = p.ws + p.tws.at(bx, by, bz) + n0 * p.ldws;
+  const unsigned char* const x = p.x + p.tx.at(bx, by, bz) + m0 * p.ldx;
+  const unsigned char* const xs = p.xs + p.txs.at(bx, by, bz) + m0 * p.ldxs;
+
+  Pieces pw[4 * NT], px[4 * MT];
+  Scales sw[S::WI], sx[S::XI];
+#pragma unroll
+  for (int i = 0; i < 4 * NT; ++i) pw[i].begin(8 * i, nrows, p.ldw);
+#pragma unroll
+  for (int i = 0; i < 4 * MT; ++i) px[i].begin(8 * i, mrows, p.ldx);
+#pragma unroll
+  for (int i = 0; i < S::WI; ++i) sw[i].begin(ws, 64 * i, 32 * NT, nrows, p.ldws);
+#pragma unroll
+  for (int i = 0; i < S::XI; ++i) sx[i].begin(xs, 64 * i, 32 * MT, mrows, p.ldxs);
+  unsigned char* const ring = lds + wave * 2 * S::STAGE;
+  auto issue = [&](int c, int slot) {
+    unsigned char* const at = ring + slot * S::STAGE;
+    const int left = p.blocks_k - c * kBlocks;
+    const long long d = (long long)c * 128;
+#pragma unroll
+    for (int i = 0; i < 4 * NT; ++i) pw[i].issue(p.dma, w + d, left, at + 1024 * i);
+#pragma unroll
+    for (int i = 0; i < 4 * MT; ++i) px[i].issue(p.dma, x + d, left, at + S::X0 + 1024 * i);
+#pragma unroll
+    for (int i = 0; i < S::WI; ++i) sw[i].issue(ws + c * kBlocks, left, at + S::S0 + 256 * i);
+#pragma unroll
+    for (int i = 0; i < S::XI; ++i) sx[i].issue(xs + c * kBlocks, left, at + S::S0 + 256 * (S::WI + i));
+  };
+
+  float16v acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
+  const int stages = (p.blocks_k + kBlocks - 1) / kBlocks, mine = max(0, (stages - wave + W - 1) / W);
+  if (mine > 0) issue(wave, 0);
+  if (mine > 1) issue(wave + W, 1);
+  const int wodd = odd_of(ws, lrow, p.ldws), xodd = odd_of(xs, lrow, p.ldxs);  // of rows 32 apart alike
+  const int row = lrow * 128, piece = piece_of(lrow, 4 * hi) * 16;  // block 4 hi + ks: its last bits changed by ks
+  int slot = 0;
+#pragma unroll 1
+  for (int j = 0; j < mine; ++j) {
+    if (p.dma && j + 1 < mine) XTK_WAIT_VM(S::PER);
+    else XTK_WAIT_VM(0);
+    asm volatile("" ::: "memory");
+    const int left = p.blocks_k - (wave + j * W) * kBlocks;
+    const unsigned char* const at = ring + slot * S::STAGE;
+    uint4v wf[4][NT], xf[4][MT];
+    int ss[NT + MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) ss[i] = scale_word(at + S::S0 + (32 * i + lrow) * 12, hi, wodd, left);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) ss[NT + i] = scale_word(at + S::S0 + 256 * S::WI + (32 * i + lrow) * 12, hi, xodd, left);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) wf[ks][i] = *reinterpret_cast<const uint4v*>(at + 4096 * i + row + (piece ^ (16 * ks)));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xf[ks][i] = *reinterpret_cast<const uint4v*>(at + S::X0 + 4096 * i + row + (piece ^ (16 * ks)));
+    }
+    // every fragment is in registers before the slot is filled again
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (j + 2 < mine) issue(wave + (j + 2) * W, slot);
+    slot ^= 1;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float16v& d = acc[i][n];
+        const int sa = ss[NT + i], sb = ss[n];
+        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(xf[0][i]), wide(wf[0][n]), d, 4, 4, 0, sa, 0, sb);
+        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(xf[1][i]), wide(wf[1][n]), d, 4, 4, 1, sa, 1, sb);
+        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(xf[2][i]), wide(wf[2][n]), d, 4, 4, 2, sa, 2, sb);
+        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(xf[3][i]), wide(wf[3][n]), d, 4, 4, 3, sa, 3, sb);
+      }
+  }
+  __syncthreads();  // every ring is done with
+
+  // the waves' parts, summed in the order of the waves; four neighbours of a row a thread
+  float* const part = reinterpret_cast<float*>(lds);
+  constexpr int COLS = 32 * NT, ALL = 1024 * MT * NT;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        part[wave * ALL + (32 * i + 8 * (v >> 2) + 4 * hi + (v & 3)) * COLS + 32 * n + lrow] = acc[i][n][v];
+  __syncthreads();
+  const long long y0 = p.ty.at(bx, by, bz);
+  for (int e = 4 * threadIdx.x; e < ALL; e += 256 * W) {
+    const int m = m0 + e / COLS, n = n0 + e % COLS;
+    if (m >= p.M || n >= p.N) continue;
+    float4v v = {0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < W; ++u) v += *reinterpret_cast<const float4v*>(part + u * ALL + e);
+    const long long to = y0 + m * p.ldy + n;
+    if (n + 4 <= p.N) put4(p.y, p.y_elem, to, v);
+    else
+      for (int k = 0; k < p.N - n; ++k) put(p.y, p.y_elem, to + k, k == 0 ? v[0] : k == 1 ? v[1] : v[2]);
+  }
+}
+
+template <int MT, int NT, int W>
+bool run_mid(Mx4Args& a, long long blocks, hipStream_t s) {
+  const long long nt = (a.N + 32 * NT - 1) / (32 * NT), tiles = nt * ((a.M + 32 * MT - 1) / (32 * MT));
+  if (tiles > 0x7fffffffLL || !grid_fits(tiles * blocks, 64 * W)) return false;
+  a.tiles = static_cast<int>(tiles);
+  a.ntiles = static_cast<int>(nt);
+  a.d_tiles = div31(a.tiles);
+  a.d_nt = div31(a.ntiles);
+  matmul_mx4_mid_kernel<MT, NT, W><<<static_cast<unsigned>(tiles * blocks), 64 * W, 0, s>>>(a);
+  return true;
+}
+
+// Many rows of x: BM x BN of the result a workgroup, NW waves of WM x WN on 32 x 32 x 64
+// MFMAs.  A stage has 256 of K, rows of 128 bytes (whole cache lines: rows of 64 bytes ask
+// L2 twice as often, which bounded the kernel), in one of NB buffers, and four steps of
+// products; a lane's half has blocks 4 h + i of it in step i.  A stage's last fragments are
+// read before its last step.  The barrier there says that every wave is done with the
+// stage's buffer and that the next stage has landed: behind it the last step runs, the next
+// stage's first fragments are read, and the DMA into that buffer begins, which has until the
+// NB - 1st such barrier to land.  So no barrier is followed by an LDS round trip (a bare
+// s_barrier: __syncthreads would wait for LDS reads too).
+//
+// The result is computed transposed (the weights are the MFMA's rows), so that a lane has
+// four neighbours of a row, and leaves through LDS in 16-byte pieces.
+template <int BM, int BN, int NW, int NB>
+struct ManyShape {
+  static constexpr int WC = NW / 2, WM = BM / 2, WN = BN / WC, MI = WM / 32, NI = WN / 32;
+  // Scales of SG stages at a time, WORDS a row.  Two halve what they ask of L2 (4096 by 11008
+  // x 4096: 126 us with one, 120 with two); a wait that leaves DMA in flight has to count
+  // it, so with more than two buffers each stage has its own.
+  static constexpr int SG = NB == 2 ? 2 : 1, WORDS = 2 * SG + 1;
+  static constexpr int AB = BM * 128, SCALES = (BM + BN) * WORDS * 4, STAGE = (BM + BN) * 128 + (SG == 1 ? SCALES : 0);
+  static constexpr int LDS = NB * STAGE + (SG == 1 ? 0 : 2 * SCALES);
+  static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, PD = PA + PB;  // data instructions of a wave and stage
+  static constexpr int PS = SCALES / 256 / NW, PER = PD + PS;              // and for scales, of SG stages
+  static constexpr int PRODUCTS = MI * NI, HALF = PD / 2, EVERY = PRODUCTS / HALF;  // of a step; data instructions
+  static_assert(PS * 256 * NW == SCALES && BM * WORDS / 64 % PS == 0, "a wave has scales of one operand");
+  static_assert(PRODUCTS % HALF == 0 && PA % 2 == 0 && MI >= NI && (MI == 4 || MI == 2) && (PS + SG - 1) / SG <= PRODUCTS, "the steps' schedule");
+  static_assert(LDS <= 160 * 1024 && (NB - 1) * PER < 64, "");
+};
+
+template <int BM, int BN, int NW, int NB>
+__global__ __launch_bounds__(64 * NW, BM * BN > 128 * 128 || NB > 2 ? 1 : 2)
+void matmul_mx4_many_kernel(Mx4Args p) {
+  typedef ManyShape<BM, BN, NW, NB> S;
+  typedef float float16v __attribute__((ext_vector_type(16)));
+  constexpr int MI = S::MI, NI = S::NI, PA = S::PA, PB = S::PB, PS = S::PS, SG = S::SG, WORDS = S::WORDS;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[S::LDS];
+
+  const int lane = threadIdx.x & 63, lrow = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / S::WC, wn = wave % S::WC;
+  const int id = xcd_contiguous(blockIdx.x, p.nwg);
+  const int b = (int)p.d_tiles(id);
+  int tile = id - b * p.tiles;
+  // tiles in groups of p.group tile columns, row by row, so that neighbours share panels in L2
+  const int gi = (int)p.d_group(tile), first = gi * p.group;
+  tile -= gi * p.group * p.mtiles;
+  const int width = min(p.group, p.ntiles - first);
+  const int tm = width == p.group ? (int)p.d_width(tile) : (int)p.d_last(tile), tn = first + tile - tm * width;
+  int bx, by, bz;
+  p.blocks(b, bx, by, bz);
+  const int m0 = tm * BM, n0 = tn * BN, mrows = min(BM, p.M - m0), nrows = min(BN, p.N - n0);
+  const unsigned char* const x = p.x + p.tx.at(bx, by, bz) + m0 * p.ldx;
+  const unsigned char* const xs = p.xs + p.txs.at(bx, by, bz) + m0 * p.ldxs;
+  const unsigned char* const w = p.w + p.tw.at(bx, by, bz) + n0 * p.ldw;
+  const unsigned char* const ws = p.ws + p.tws.at(bx, by, bz) + n0 * p.ldws;
+  const int nk = (p.blocks_k + kBlocks - 1) / kBlocks;  // stages
+
+  // What this lane brings: of rows 8 i + lane / 8 of its wave's instructions the piece that
+  // lies at lane % 8; it is another, 4 apart, in every second instruction.  Rows past the
+  // last lie behind the descriptors' ends and read as zeros, and so does all that comes
+  // behind the last stage: its place in LDS is filled without a branch, which would part the
+  // products from what goes between them.
+  const int piece = piece_of(lane >> 3, lane & 7);
+  const unsigned va = (8u * wave * PA + (lane >> 3)) * (unsigned)p.ldx, vb = (8u * wave * PB + (lane >> 3)) * (unsigned)p.ldw;
+  const unsigned aend = (unsigned)mrows * (unsigned)p.ldx, bend = (unsigned)nrows * (unsigned)p.ldw;
+  auto dma_one = [&](int s, unsigned char* to, int q) {
+    const int left = p.blocks_k - kBlocks * s, c = piece ^ (4 * (q & 1));
+    const bool of_a = q < PA;
+    const unsigned skip = (unsigned)s * 128, end = s < nk ? (of_a ? aend : bend) - skip : 0u;
+    const unsigned row8 = 8u * (unsigned)(of_a ? q : q - PA) * (unsigned)(of_a ? p.ldx : p.ldw);
+    const unsigned at = (of_a ? va : vb) + row8 + c * 16;
+    const unsigned lds_to = lds_at(to + (of_a ? wave * PA + q : BM / 8 + wave * PB + q - PA) * 1024);
+    dma16(raw_rsrc((of_a ? x : w) + skip, end), __builtin_amdgcn_readfirstlane(lds_to), c < left ? at : kNone, 0);
+  };
+  // Scales, eight bytes a row and stage in a word more, since rows begin at any byte; this
+  // wave's are of x's rows or of the weights'.  The descriptor ends with the last row's last scale, in
+  // whole words.
+  const bool of_x = wave * PS < BM * WORDS / 64;
+  const unsigned char* const sbase = of_x ? xs : ws;
+  const unsigned sodd = (unsigned)reinterpret_cast<uintptr_t>(sbase) & 3;
+  const unsigned sld = (unsigned)(of_x ? p.ldxs : p.ldws);
+  unsigned vs[PS];
+#pragma unroll
+  for (int q = 0; q < PS; ++q) {
+    const unsigned word = (unsigned)((wave * PS + q) * 64 + lane - (of_x ? 0 : BM * WORDS)), row = word / WORDS;
+    vs[q] = ((sodd + row * sld) & ~3u) + 4 * (word - WORDS * row);
+  }
+  const unsigned send = (sodd + (unsigned)((of_x ? mrows : nrows) - 1) * sld + (unsigned)p.blocks_k + 3) & ~3u;
+  // where the scales of stage s lie, whose buffer is `at`
+  auto scales_at = [&](int s, unsigned char* at) {
+    return SG == 1 ? at + (BM + BN) * 128 : lds + NB * S::STAGE + (s >> 1 & 1) * S::SCALES;
+  };
+  auto dma_scales = [&](int s, unsigned char* at, int q) {
+    const unsigned skip = 8u * (unsigned)s;
+    dma4(raw_rsrc(sbase - sodd + skip, s < nk ? send - skip : 0u),
+         __builtin_amdgcn_readfirstlane(lds_at(scales_at(s, at) + (wave * PS + q) * 256)), vs[q]);
+  };
+
+  const int xodd = odd_of(xs, lrow, p.ldxs), wodd = odd_of(ws, lrow, p.ldws);  // of rows 32 apart alike
+  // a row's block 4 hi + ks lies at the place of its block 4 hi, less or more: its last bits
+  // changed by ks; rows 32 apart have theirs at the same places
+  const int arow = (wm * S::WM + lrow) * 128 + piece_of(lrow, 4 * hi) * 16;
+  const int brow = S::AB + (wn * S::WN + lrow) * 128 + piece_of(lrow, 4 * hi) * 16;
+  const int xword = (wm * S::WM + lrow) * WORDS * 4 + 4 * hi, wword = (BM + wn * S::WN + lrow) * WORDS * 4 + 4 * hi;
+
+  float16v acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
+  uint4v af[2][MI], bf[2][NI];
+  unsigned raw[MI + NI][2];  // the next stage's scale words as they lie
+  int sx[MI], sw[NI];        // this stage's, a byte a step
+  auto read_a = [&](const unsigned char* at, int ks, int i) {
+    af[ks & 1][i] = *reinterpret_cast<const uint4v*>(at + (ks * 16 ^ arow) + i * 4096);
+  };
+  auto read_b = [&](const unsigned char* at, int ks, int j) {
+    bf[ks & 1][j] = *reinterpret_cast<const uint4v*>(at + (ks * 16 ^ brow) + j * 4096);
+  };
+  auto read_scale = [&](const unsigned char* at, int i) {  // at: the stage's first ones
+    const unsigned* const from =
+        reinterpret_cast<const unsigned*>(at + (i < MI ? xword + i * 128 * WORDS : wword + (i - MI) * 128 * WORDS));
+    raw[i][0] = from[0];
+    raw[i][1] = from[1];
+  };
+  auto take_scales = [&](int s) {
+    // those past the row's end as 0: 255 would make NaN of the zeros there
+    const int n = p.blocks_k - kBlocks * s - 4 * hi;
+    const unsigned mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+#pragma unroll
+    for (int i = 0; i < MI + NI; ++i) {
+      const unsigned v = __builtin_amdgcn_alignbyte(raw[i][1], raw[i][0], i < MI ? xodd : wodd) & mask;
+      if (i < MI) sx[i < MI ? i : 0] = (int)v;
+      else sw[i < MI ? 0 : i - MI] = (int)v;
+    }
+  };
+  auto mma = [&](int ks, int i, int j) {
+    const int8w a = wide(bf[ks & 1][j]), c = wide(af[ks & 1][i]);
+    float16v& d = acc[i][j];
+    if (ks == 0) d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, c, d, 4, 4, 0, sw[j], 0, sx[i]);
+    else if (ks == 1) d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, c, d, 4, 4, 1, sw[j], 1, sx[i]);
+    else if (ks == 2) d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, c, d, 4, 4, 2, sw[j], 2, sx[i]);
+    else d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, c, d, 4, 4, 3, sw[j], 3, sx[i]);
+  };
+  // Step ks: its MI NI products; behind product n issue(n), a DMA instruction or nothing,
+  // and what the next step needs, the fragments that its first products take first.
+  constexpr int PRODUCTS = S::PRODUCTS, EVERY = S::EVERY, HALF = S::HALF;
+  auto step = [&](int ks, const unsigned char* at, int next, auto issue) {
+#pragma unroll
+    for (int n = 0; n < PRODUCTS; ++n) {
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (MI == NI) {  // shells of the larger index
+        const int k = n < 1 ? 0 : n < 4 ? 1 : n < 9 ? 2 : 3, r = n - k * k;
+        mma(ks, r < k ? r : k, r < k ? k : r - k);
+      } else {
+        mma(ks, 2 * (n >> 2) + (n & 1), (n >> 1) & 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      issue(n);
+      __builtin_amdgcn_sched_barrier(0);
+      if (n < MI) read_a(at, next, n);
+      if (n < NI) read_b(at, next, n);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto none = [](int) {};
+
+  // prologue: as much as the buffers hold, of the last one half the data
+#pragma unroll
+  for (int s = 0; s < NB; ++s) {
+#pragma unroll
+    for (int q = 0; q < (s < NB - 1 ? S::PD : HALF); ++q) dma_one(s, lds + s * S::STAGE, q);
+    if (s < NB - 1) {
+#pragma unroll
+      for (int q = 0; q < PS; ++q) dma_scales(s, lds + s * S::STAGE, q);
+    }
+  }
+  static_assert(SG == 1 || NB == 2, "the first wait leaves the second stage's data");
+  XTK_WAIT_VM((NB - 2) * S::PER + HALF);
+  asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < MI; ++i) read_a(lds, 0, i);
+#pragma unroll
+  for (int j = 0; j < NI; ++j) read_b(lds, 0, j);
+#pragma unroll
+  for (int i = 0; i < MI + NI; ++i) read_scale(scales_at(0, lds), i);
+  take_scales(0);
+
+  // stage s in `at`, with `last` the buffer before it and `next` the one behind it
+  auto stage = [&](int s, unsigned char* at, unsigned char* last, unsigned char* next, bool odd) {
+    step(0, at, 1, [&](int n) {
+      if (n % EVERY == 0) dma_one(s + NB - 1, last, HALF + n / EVERY);
+    });
+    step(1, at, 2, [&](int n) {
+      if constexpr (SG == 1) {
+        if (n < PS) dma_scales(s + NB - 1, last, n);
+      } else {  // of the two stages from the next even one on, in two halves
+        constexpr int FIRST = (PS + 1) / 2;
+        if (!odd && n < FIRST) dma_scales(s + 2, at, n);
+        if (odd && n < PS - FIRST) dma_scales(s + 1, at, FIRST + n);
+      }
+    });
+    step(2, at, 3, none);
+    XTK_WAIT_VM((NB - 2) * S::PER);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const unsigned char* const scales = scales_at(s + 1, next) + (SG == 2 && !odd ? 8 : 0);
+    step(3, next, 0, [&](int n) {
+      if (n % EVERY == 0) dma_one(s + NB, at, n / EVERY);
+      if (n >= PRODUCTS - MI) {
+        read_scale(scales, n - (PRODUCTS - MI));
+        if (n - (PRODUCTS - MI) < NI) read_scale(scales, MI + n - (PRODUCTS - MI));
+      }
+    });
+    take_scales(s + 1);
+  };
+  if constexpr (SG == 2) {
+#pragma unroll 1
+    for (int s = 0; s < nk; s += 2) {
+      stage(s, lds, lds + S::STAGE, lds + S::STAGE, false);
+      if (s + 1 < nk) stage(s + 1, lds + S::STAGE, lds, lds, true);
+    }
+  } else {
+    unsigned char *at = lds, *last = lds + (NB - 1) * S::STAGE;
+#pragma unroll 1
+    for (int s = 0; s < nk; ++s) {
+      unsigned char* const next = at == lds + (NB - 1) * S::STAGE ? lds : at + S::STAGE;
+      stage(s, at, last, next, false);
+      last = at;
+      at = next;
+    }
+  }
+  XTK_WAIT_VM(0);
+
+  // each wave's 32 rows at a time through a part of LDS of its own
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+  static_assert(S::LDS >= NW * 32 * (S::WN * 4 + 16), "the waves' parts");
+  unsigned char* const own = lds + wave * 32 * (S::WN * 4 + 16);
+  const long long y0 = p.ty.at(bx, by, bz);
+  auto leave = [&](auto zero) {
+    typedef decltype(zero) T;
+    constexpr int ES = sizeof(T), PER16 = 16 / ES, PITCH = S::WN * ES + 16, PIECES = S::WN / PER16;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          typedef T t4 __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<t4*>(own + lrow * PITCH + (32 * j + 8 * g + 4 * hi) * ES) =
+              t4{(T)acc[i][j][4 * g], (T)acc[i][j][4 * g + 1], (T)acc[i][j][4 * g + 2], (T)acc[i][j][4 * g + 3]};
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes
+#pragma unroll
+      for (int e = lane; e < 32 * PIECES; e += 64) {
+        const int r = e / PIECES, c = e % PIECES;
+        const int m = m0 + wm * S::WM + 32 * i + r, n = n0 + wn * S::WN + c * PER16;
+        if (m >= p.M || n >= p.N) continue;
+        const T* const from = reinterpret_cast<const T*>(own + r * PITCH + c * 16);
+        T* const to = static_cast<T*>(p.y) + y0 + m * p.ldy + n;
+        if (n + PER16 <= p.N) {
+          typedef unsigned u4e __attribute__((ext_vector_type(4), aligned(2)));
+          *reinterpret_cast<u4e*>(to) = (u4e)(*reinterpret_cast<const uint4v*>(from));
+        } else {
+          for (int k = 0; k < p.N - n; ++k) to[k] = from[k];
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  };
+  if (p.y_elem == kF32) leave(0.0f);
+  else if (p.y_elem == kF16) leave((_Float16)0);
+  else leave((__bf16)0.0f);
+}
+
+template <int BM, int BN, int NW, int NB>
+bool run_many(Mx4Args& a, long long blocks, hipStream_t s) {
+  const long long mt = (a.M + BM - 1) / BM, nt = (a.N + BN - 1) / BN, tiles = mt * nt;
+  if (tiles > 0x7fffffffLL || !grid_fits(tiles * blocks, 64 * NW)) return false;
+  a.tiles = static_cast<int>(tiles);
+  a.mtiles = static_cast<int>(mt);
+  a.ntiles = static_cast<int>(nt);
+  a.nwg = static_cast<int>(tiles * blocks);
+  a.group = static_cast<int>(std::min(nt, 8LL));
+  a.d_tiles = div31(a.tiles);
+  a.d_group = div31(a.group * a.mtiles);
+  a.d_width = div31(a.group);
+  a.d_last = div31(a.ntiles % a.group ? a.ntiles % a.group : a.group);
+  matmul_mx4_many_kernel<BM, BN, NW, NB><<<a.nwg, 64 * NW, 0, s>>>(a);
+  return true;
+}
+
+// The kernel by estimated time, in us, fitted to graph replays of 34 products from 1 x 840 x
+// 1696 to 4096 x 11008 x 4096: a round of tiles costs its start and end and its stages; a
+// wave of few and mid tiles has a W-th of them.  (Measured: 64 x 4096 x 4096 in tiles of 16 x
+// 16 8.5 us, 32 x 32 6.6, 64 x 64 10.2; 256 x 4096 x 4096 in 32 x 64 14.8, 64 x 64 11.9, 128
+// x 128 18.6; 512 x 11008 x 4096 in 128 x 128 with three buffers 32.8, with two and twice
+// the workgroups on a CU 25.8, in 256 x 256 37.5; 1024 x 11008 x 4096 in 128 x 128 46.1, in
+// 256 x 256 40.9.)
+bool run(Mx4Args& a, long long blocks, hipStream_t s) {
+  const int stages = (a.blocks_k + kBlocks - 1) / kBlocks;
+  auto tiles = [&](int bm, int bn) { return double(blocks) * double((a.M + bm - 1) / bm) * double((a.N + bn - 1) / bn); };
+  auto share = [&](int waves) { return double((stages + waves - 1) / waves); };
+  auto rounds = [](double t, int at_once) { return std::ceil(t / at_once); };
+  // more workgroups than two a CU: four waves each, of which four fit on one
+  const double small = tiles(16, 16);
+  const bool eight = small <= 512;
+  const double by_16 = 2.2 + (eight ? std::max(1.0 + 0.9 * share(8), small / 256 * (0.5 + 0.78 * share(8)))
+                                    : std::max(1.0 + 0.55 * share(4), small / 256 * (0.37 + 0.3 * share(4))));
+  const double us[7] = {by_16,
+                        2.4 + rounds(tiles(32, 32), 256) * (2.0 + 0.95 * share(8)),
+                        2.3 + rounds(tiles(32, 64), 256) * (2.3 + 0.95 * share(4)),
+                        2.5 + rounds(tiles(64, 64), 256) * (3.9 + 1.35 * share(4)),
+                        2.0 + rounds(tiles(128, 128), 256) * (2.5 + 1.0 * stages),
+                        2.0 + rounds(tiles(128, 128), 512) * (2.2 + 1.35 * stages),
+                        2.0 + rounds(tiles(256, 256), 256) * (4.0 + 2.2 * stages)};
+  // large tiles take their rows by DMA only
+  switch (std::min_element(us, us + (a.dma ? 7 : 4)) - us) {
+    case 0:
+      if (a.M <= 8) return eight ? run_few<8, 8>(a, blocks, s) : run_few<8, 4>(a, blocks, s);
+      return eight ? run_few<16, 8>(a, blocks, s) : run_few<16, 4>(a, blocks, s);
+    case 1: return run_mid<1, 1, 8>(a, blocks, s);
+    case 2: return run_mid<1, 2, 4>(a, blocks, s);
+    case 3: return run_mid<2, 2, 4>(a, blocks, s);
+    case 4: return run_many<128, 128, 4, 3>(a, blocks, s);
+    case 5: return run_many<128, 128, 4, 2>(a, blocks, s);
+    default: return run_many<256, 256, 8, 2>(a, blocks, s);
+  }
 }
 
 }  // namespace
@@ -292,16 +755,13 @@ hipError_t launch_matmul_mx4(const xt::Plan& p, void* const* bufs, hipStream_t s
   a.dma = pieces(m.x) && pieces(m.w);
   // what a lane adds to its tile's address has 31 bits
   auto near = [](long long rows, long long ld) { return rows * ld + 256 < (1LL << 31); };
-  const int mr = std::min(a.M, 64), nr = std::min(a.N, 16);
+  const int mr = std::min(a.M, 256), nr = std::min(a.N, 256);
   if (!near(mr, a.ldx) || !near(mr, a.ldxs) || !near(nr, a.ldw) || !near(nr, a.ldws)) {
     why = "matmul_mx4: rows that a workgroup reads together span 2^31 bytes or more";
     return hipErrorInvalidValue;
   }
   const long long blocks = grid_blocks(p);
-  const bool ok = a.M <= 8    ? run_few<1, 8, 8, 2>(a, blocks, s)
-                  : a.M <= 16 ? run_few<1, 16, 8, 2>(a, blocks, s)
-                  : a.M <= 32 ? run_few<2, 32, 8, 2>(a, blocks, s)
-                              : run_few<4, 64, 4, 2>(a, blocks, s);
+  const bool ok = run(a, blocks, s);
   if (!ok) {
     why = "matmul_mx4: " + std::to_string(a.M) + " x " + std::to_string(a.N) + " tiles exceed one launch";
     return hipErrorInvalidValue;
