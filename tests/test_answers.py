@@ -74,6 +74,16 @@ def test_work_of_plans():
     assert p["flops"] == 4 * 64 * 2 * 3 * 2 * 5 * 77
 
 
+def test_slices_of_sampled_rows():
+    def slices(*a, **kw):
+        return xt.workspace(K.sample(*a, **kw)) // 123248
+
+    assert [slices(r, v) for r, v in ((1, 32767), (1, 32768), (32, 32768), (33, 32768), (128, 131072), (129, 2**20))] == [0, 1, 32, 0, 128, 0]
+    assert [slices(r, v, top_k=True) for r, v in ((1, 65535), (1, 65536), (32, 131072), (33, 131072))] == [0, 1, 32, 0]
+    assert "slices=4" in xt.plan(K.sample(128, 131072))["kernel"]
+    assert "slices" not in xt.plan(K.sample(1, 1000))["kernel"]
+
+
 def test_buffers_below_element_alignment_are_refused():
     """Before anything is launched: the addresses are not those of any memory."""
     from xtile_amd import _xtile

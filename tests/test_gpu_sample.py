@@ -121,6 +121,37 @@ def test_rows_of_one_value(vocab):
     check(x, u, temperature=[0.0, 1e-30, 1e30, float("inf"), 2.0])
 
 
+def long_rows(rows, vocab, kind):
+    """Rows dealt to several workgroups: of halves, of two values, and with most in one bin."""
+    import torch
+
+    x = logits(rows, vocab, "f32", vocab, 1.0)
+    if kind == "halves":
+        return (x * 2).round() / 2
+    if kind == "two":
+        return torch.where(x > 1.5, 1.0, -1.0)
+    x = x * 1e-4
+    x[:, 7] = 9.0
+    return x
+
+
+@pytest.mark.parametrize("options", [{}, {"top_k": [3000, 50, 60000, 1]}, {"top_p": 0.3}, {"top_k": 20000, "top_p": 0.6},
+                                     {"min_p": [0.3, 0.0, 1.0, 1e-9]}, {"top_k": 256, "top_p": 0.9, "min_p": 0.01},
+                                     {"temperature": [0.0, 100.0, 0.01, 1.0], "top_p": 0.99}],
+                         ids=lambda o: "-".join(o) or "none")
+@pytest.mark.parametrize("kind", ["halves", "two", "narrow"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sliced_rows(dtype, kind, options):
+    """Runs that fit a list, ones that do not, and rows of nothing between them."""
+    rows, vocab = 4, 66001
+    assert xt.workspace(K.sample(rows, vocab, DTYPES[dtype], **{k: True for k in options}))
+    x = long_rows(rows, vocab, kind).to(torch_dtype(dtype))
+    check(x, uniforms(rows, 11), dtype, **options)
+    x[2] = -float("inf")
+    x[1, ::3] = float("nan")
+    check(x, uniforms(rows, 12), dtype, **options)
+
+
 def test_odd_logits():
     """Infinities, NaN and zeros of both signs."""
     import torch

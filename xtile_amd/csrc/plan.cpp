@@ -810,6 +810,8 @@ bool match_sample(const Analysis& an, Plan& p, std::string& err) {
     return false;
   }
   p.kind = PlanKind::Sample;
+  s.slices = sample_slices(p);
+  if (s.slices > 1) p.workspace = static_cast<int64_t>(blocks) * s.x.rows * kSampleRowWork;
   read.push_back(s.y.arg);
   count_bytes(an, read, p);
   p.algo_flops = 8 * blocks * double(s.x.rows) * double(s.x.cols);
@@ -1538,6 +1540,23 @@ int attend_splits(const Plan& p) {
   const int64_t most = few ? (keys > 2 * round ? (keys + round - 1) / round : 1) : keys < 1024 ? 1 : keys / 256;
   if (want < 2 || most < 2) return 1;
   return static_cast<int>(std::min<double>(std::min<double>(want, double(most)), 256));
+}
+
+// A row alone has one workgroup, in one kernel; its slices take four, which cost 10 us more
+// where there is little to do and share what grows with the row.  Measured, alone against
+// sliced as below: 1 row of 131072 logits cut by top-p 86 and 31 us, 64 rows 105 and 67, 128
+// rows 116 and 107, 256 rows 136 against 168 with 4 slices; 1 row of 32768 26 and 23, 64 rows
+// 42 against 45; 8 rows of 8192 24 against 30.  With top-k, of few tokens, a row has no weights
+// but those of a list: 1 row of 131072 32 and 23 us, 32 rows 38 and 34, 64 rows 38 against 40,
+// 1 row of 65536 22 and 22, of 32768 17 against 22.  More than 512 workgroups, or slices
+// below 2048 logits, gain nothing.
+int sample_slices(const Plan& p) {
+  const double rows = double(p.grid[0]) * p.grid[1] * p.grid[2] * double(p.sample.x.rows);
+  const int64_t vocab = p.sample.x.cols;
+  const bool some = p.sample.extra[1].arg >= 0;
+  if (vocab < (some ? 65536 : 32768) || double(vocab) < rows * (some ? 4096 : 1024)) return 1;
+  const int64_t slices = std::min<int64_t>(static_cast<int64_t>(512 / rows), vocab / 2048);
+  return static_cast<int>(slices < 4 ? 1 : std::min<int64_t>(slices, kSampleSlices));
 }
 
 bool gemm_tile(const GemmCover& m, const GemmCover& n, bool over_a, bool over_b) {

@@ -179,8 +179,11 @@ struct AttendPlan {
 // Rows of one attend workgroup: up to 32 take one wave's width with the keys
 // dealt to the waves, more take 128 with the keys shared.
 constexpr int64_t kAttendFewRows = 32, kAttendRows = 128;
-// Logits of a row that `sample` takes.
+// Logits of a row that `sample` takes, the most slices of one, and the bytes of workspace
+// that a sliced row takes.
 constexpr int64_t kSampleVocab = int64_t(1) << 22;
+constexpr int kSampleSlices = 64;
+constexpr int64_t kSampleRowWork = 123248;
 // Drafted tokens of a tree: their ancestors are a lane's 64 bits.
 constexpr int64_t kAttendTree = 64;
 
@@ -269,6 +272,9 @@ GemmCover gemm_cover(const Plan& p, int64_t w, bool is_m);
 // B) in LDS before it stores, and another tile of the Block would still read
 // them.
 bool gemm_tile(const GemmCover& m, const GemmCover& n, bool over_a, bool over_b);
+
+// Workgroups that share a row of logits, of a plan whose sizes are set.
+int sample_slices(const Plan& p);
 
 // Workgroups that share an attend tile's keys, of a plan whose sizes are set.
 int attend_splits(const Plan& p);
