@@ -100,7 +100,8 @@ def test_shapes(shape, options, g):
 
 
 def test_a_chain_is_a_causal_row():
-    """Tokens that follow each other see what causal ones do."""
+    """Tokens that follow each other see what causal ones do.  The two take keys in other orders:
+    each is within `far` of the formula, so they are within twice that of each other."""
     import torch
 
     nq, nk, start = 20, 500, 411
@@ -112,7 +113,20 @@ def test_a_chain_is_a_causal_row():
     at = torch.tensor([[start]], dtype=torch.int32, device="cuda")
     xt.launch(K.masked_attention(1, 2, 3, nq, nk, 128, causal=True, window=100, start=True, length=True), q, k, v, at,
               at + nq, o)
-    assert torch.equal(got, o.cpu())
+    sees, distance = (torch.from_numpy(x)[None] for x in ref.tree_seen([t - 1 for t in range(nq)], start, start + nq, nk, 100))
+    want, far = ref.attend_seen(q.cpu(), k.cpu(), v.cpu(), 128**-0.5, sees, distance, None, None)
+    assert_within(o.cpu(), want, far)
+    assert bool(((got.double() - o.cpu().double()).abs() <= 2 * far).all())
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("nq,g,nk,start", [(11, 3, 64, 50), (64, 1, 65, 0), (7, 5, 1000, 700), (16, 4, 577, 561)])
+def test_33_to_64_rows(d, nq, g, nk, start):
+    """Tiles in turn, of which the last is part of one, in the wave's half of them or not."""
+    rng = np.random.default_rng(d + nk)
+    parents = [random_parents(rng, nq), random_parents(rng, nq, 2)]
+    run(2, 1, g, nq, nk, d, parents, start=[start, 3], length=[start + nq, nk], dtype="f16" if d % 64 else "bf16")
+    run(2, 1, g, nq, nk, d, parents, start=[start, 31], length=[start + nq, 31 + nq], window=40, token_major=True)
 
 
 @pytest.mark.parametrize("start,length", [

@@ -32,7 +32,13 @@
 // Drafted trees (parents): a token's ancestors are 64 bits, made in each wave by lanes that
 // double how far up they have seen, and are turned into the tiles' masks where a tile has
 // drafted tokens; the rest of the cache is seen whole.  The kernels are those of other rows,
-// in instantiations of their own.
+// in instantiations of their own, and one more for 33 to 64 rows.  What only needs to know the
+// Block (parents, slopes, q) is on its way first, and where no other workgroup reads the same
+// keys a Block's are on all XCDs (16 sequences of different lengths: 107 -> 101 us).
+// 4 x 16 rows on 8 key heads of 128 over 4096 keys take 15 us, most of it a chain of waits:
+// two launches 4, what the first loads wait for 4, four tiles 4, the join 3.  4 x 32 rows in
+// 16 sequences of up to 8192 keys take 101 us, 0.5 PFLOP/s and 3.6 TB/s; 8 x 64 rows over
+// 131072 keys, capped, 356 to 376, 0.73 to 0.78 PFLOP/s.
 //
 // Many rows are bound by the arithmetic of the softmax (4096 tokens, 32 heads of 128
 // columns on 8 key heads, causal, capped: 166 to 181 us, 0.76 to 0.83 PFLOP/s; 158 without

@@ -162,13 +162,17 @@ struct CapArg<kTree | kFine> {
 template <int MODE>
 using CapOf = typename CapArg<MODE>::type;
 
-// Of each of a tree's tokens, in its lane, the bits of its ancestors and its own.  A parent
-// comes before its child, whatever else is given is none; in each of six rounds a token
-// takes the bits of the farthest ancestor that it has, twice as far each time.
-__device__ __forceinline__ unsigned long long ancestors(const TreeCap& c, unsigned bx, unsigned by, unsigned bz) {
+// Of each of a tree's tokens, in its lane, its parent as given.
+__device__ __forceinline__ int parent_of(const TreeCap& c, unsigned bx, unsigned by, unsigned bz) {
   const int t = threadIdx.x & 63;
-  int up = -1;
-  if (t < c.tokens) up = c.parents[c.tparents.at(bx, by, bz) + t * c.step];
+  return t < c.tokens ? c.parents[c.tparents.at(bx, by, bz) + t * c.step] : -1;
+}
+
+// And the bits of its ancestors and its own.  A parent comes before its child, whatever else
+// is given is none; in each of six rounds a token takes the bits of the farthest ancestor
+// that it has, twice as far each time.
+__device__ __forceinline__ unsigned long long ancestors(int up) {
+  const int t = threadIdx.x & 63;
   if (up >= t || up < 0) up = -1;
   unsigned lo = t < 32 ? 1u << t : 0u, hi = t < 32 ? 0u : 1u << (t - 32);
 #pragma unroll
@@ -226,7 +230,8 @@ struct Rows {
   int w0, w1;            // the last keys before their windows
   float slope;           // times log2 e
   int doc;               // this lane's document
-  unsigned long long tree;  // trees: the drafted tokens that this lane's row sees
+  int up;                   // trees: the parent of the lane's token,
+  unsigned long long tree;  // the drafted tokens that its row sees
   int first;                // and the key of the first one
   uint4v q[KK];
   float16v acc[N];
@@ -236,6 +241,34 @@ struct Rows {
   static constexpr bool LEAN = D == 256;
   int koff[LEAN ? 1 : KK], voff[N];
 
+  // Trees: what needs no more than to know the Block, on its way before the keys, behind
+  // whose arrival it would be waited for.
+  __device__ __forceinline__ void ask(const AttendArgs& p, const CapOf<MODE>& c, int first, int bx, int by, int bz) {
+    if constexpr (TREE) {
+      up = parent_of(c, bx, by, bz);
+      const int row = min(first + (int)(threadIdx.x & 31), p.rows - 1), token = (int)p.d_heads((unsigned)row);
+      load(p, token, row - token * p.heads, (threadIdx.x >> 5) & 1, bx, by, bz);
+    }
+  }
+
+  // It has come.  A ring's loop waits for some of the tiles on their way, but the compiler, which
+  // does not know of those, would wait in it for every load before q's first use.
+  __device__ __forceinline__ void have() {
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(q[kk]));
+    asm volatile("" : "+v"(up), "+v"(slope));
+  }
+
+  // A row's slope and its part of q.
+  __device__ __forceinline__ void load(const AttendArgs& p, int token, int head, int hi, int bx, int by, int bz) {
+    slope = p.slopes ? p.slopes[p.tslopes.at(bx, by, bz) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
+    if constexpr (!TREE) doc = p.qdocs ? p.qdocs[p.tqdocs.at(bx, by, bz) + token * p.qdoc_step] : 0;
+    const unsigned char* at = p.q + (p.tq.at(bx, by, bz) + head * p.q_head + token * p.q_row + 8 * hi) * 2;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) q[kk] = (uint4v)(*reinterpret_cast<const u4a*>(at + kk * 32));
+  }
+
+  // Of trees, behind ask.
   __device__ __forceinline__ void begin(const AttendArgs& p, const CapOf<MODE>& c, int first, int bx, int by, int bz,
                                         int start, int window) {
     lane = threadIdx.x & 63;
@@ -253,9 +286,9 @@ struct Rows {
     w1 = before(p, window, p1);
     if constexpr (TREE) {
       // depths lie between 0 and the tokens' number
-      const unsigned long long all = ancestors(c, bx, by, bz);
-      const unsigned lo = __shfl((unsigned)all, token, 64), up = __shfl((unsigned)(all >> 32), token, 64);
-      tree = ((unsigned long long)up << 32) | lo;
+      const unsigned long long all = ancestors(up);
+      const unsigned lo = __shfl((unsigned)all, token, 64), high = __shfl((unsigned)(all >> 32), token, 64);
+      tree = ((unsigned long long)high << 32) | lo;
       this->first = start;
       pos = start + __popcll(tree) - 1;
       above = start - 1;
@@ -266,11 +299,7 @@ struct Rows {
       w0 = before(p, window, p0);
       w1 = before(p, window, p1);
     }
-    slope = p.slopes ? p.slopes[p.tslopes.at(bx, by, bz) + head * p.slope_step] * 1.44269504088896340736f : 0.0f;
-    doc = p.qdocs ? p.qdocs[p.tqdocs.at(bx, by, bz) + token * p.qdoc_step] : 0;
-    const unsigned char* at = p.q + (p.tq.at(bx, by, bz) + head * p.q_head + token * p.q_row + 8 * hi) * 2;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) q[kk] = (uint4v)(*reinterpret_cast<const u4a*>(at + kk * 32));
+    if constexpr (!TREE) load(p, token, head, hi, bx, by, bz);
     reset();
     const int g = lane >> 4, li = lane & 15;
     const int key = 4 * hi + (li >> 2), chunk = 2 * (g & 1) + ((li & 3) >> 1);
@@ -677,10 +706,11 @@ __device__ __forceinline__ void hold_start(const AttendArgs& p, int start, Block
   if (start > kFar - 1) b.window = max(p.window - (start - (kFar - 1)), 0);
 }
 
-template <bool FEW>
-__device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
+// Where a workgroup is, without its start, window, length and prefix.  `spread`: neighbours on
+// different XCDs.
+__device__ __forceinline__ BlockAt place_of(const AttendArgs& p, bool spread) {
   BlockAt b;
-  const int id = xcd_contiguous(blockIdx.x, p.nwg);
+  const int id = spread ? (int)blockIdx.x : xcd_contiguous(blockIdx.x, p.nwg);
   const int blk = (int)p.d_work((unsigned)id);
   const int rest = id - blk * p.tiles * p.splits;
   const int tile = (int)p.d_splits((unsigned)rest);
@@ -688,6 +718,12 @@ __device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
   b.tile = p.tiles - 1 - tile;  // a causal Block's last rows see the most keys: they go first
   b.block = blk;
   p.blocks(blk, b.x, b.y, b.z);
+  return b;
+}
+
+template <bool FEW>
+__device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
+  BlockAt b = place_of(p, false);
   if constexpr (FEW) {
     b.start = 0;
     b.window = p.window;
@@ -715,6 +751,25 @@ __device__ __forceinline__ BlockAt block_at(const AttendArgs& p) {
   b.window = __builtin_amdgcn_readfirstlane(b.window);
   b.len = __builtin_amdgcn_readfirstlane(b.len);
   b.pre = __builtin_amdgcn_readfirstlane(b.pre);
+  return b;
+}
+
+// The same for a tree; `early` is what needs no more than its place, behind loads that are all
+// on their way (what is absent reads a parent).
+template <class F>
+__device__ __forceinline__ BlockAt tree_block_at(const AttendArgs& p, const TreeCap& c, F early) {
+  BlockAt b = place_of(p, p.tiles == 1);  // no other reads its keys
+  const int* const any = c.parents + c.tparents.at(b.x, b.y, b.z);
+  const int start = *(p.start ? p.start + p.tstart.at(b.x, b.y, b.z) : any);
+  const int len = *(p.length ? p.length + p.tlength.at(b.x, b.y, b.z) : any);
+  early(b);
+  b.start = 0;
+  b.window = p.window;
+  if (p.start) hold_start(p, start, b);
+  b.start = __builtin_amdgcn_readfirstlane(b.start);
+  b.window = __builtin_amdgcn_readfirstlane(b.window);
+  b.len = __builtin_amdgcn_readfirstlane(p.length ? min(max(len, 0), p.keys) : p.keys);
+  b.pre = 0;
   return b;
 }
 
@@ -837,7 +892,7 @@ __device__ __forceinline__ void odd_rows(const AttendArgs& p, const CapOf<MODE>&
   constexpr bool FINE = (MODE & kFine) != 0, TREE = (MODE & kTree) != 0;
   const int lane = threadIdx.x & 63;
   unsigned long long all = 0;
-  if constexpr (TREE) all = ancestors(c, b.x, b.y, b.z);
+  if constexpr (TREE) all = ancestors(parent_of(c, b.x, b.y, b.z));
   auto value = [](unsigned short x) {
     return BF16 ? __builtin_bit_cast(float, (unsigned)x << 16) : (float)__builtin_bit_cast(_Float16, x);
   };
@@ -941,6 +996,57 @@ __device__ __forceinline__ bool any_wave(bool x, unsigned char* lds) {
   return __builtin_amdgcn_readfirstlane(any) != 0;
 }
 
+// The results of a wave that had other keys of the same rows join those of its fellow: through
+// `theirs`, 32 D + 128 floats.
+template <class R>
+__device__ __forceinline__ void join_halves(R& rows, float* theirs, bool leaves) {
+  constexpr int N = R::N, D = 32 * N;
+  if (leaves) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        *reinterpret_cast<float4v*>(theirs + (4 * n + w) * 256 + rows.lane * 4) =
+            float4v{rows.acc[n][4 * w], rows.acc[n][4 * w + 1], rows.acc[n][4 * w + 2], rows.acc[n][4 * w + 3]};
+    theirs[32 * D + rows.lane] = rows.m;
+    theirs[32 * D + 64 + rows.lane] = rows.l;
+  }
+  __syncthreads();
+  if (leaves) return;
+  const float m1 = theirs[32 * D + rows.lane], l1 = theirs[32 * D + 64 + rows.lane];
+  const float m = fmaxf(rows.m, m1), use = m == -__builtin_inff() ? 0.0f : m;
+  const float a0 = __builtin_amdgcn_exp2f(rows.m - use), a1 = __builtin_amdgcn_exp2f(m1 - use);
+  rows.m = m;
+  rows.l = rows.l * a0 + l1 * a1;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float4v o = *reinterpret_cast<const float4v*>(theirs + (4 * n + w) * 256 + rows.lane * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) rows.acc[n][4 * w + e] = rows.acc[n][4 * w + e] * a0 + o[e] * a1;
+    }
+}
+
+// A wave's rows to the workspace; l: their totals.
+template <class R>
+__device__ __forceinline__ void leave_part(const AttendArgs& p, const R& rows, const BlockAt& b, float l, long long all_rows) {
+  constexpr int N = R::N, D = 32 * N;
+  const long long row = b.block * p.rows + rows.row;
+  float* const sums = sums_of(p, D, row, b.split);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      *reinterpret_cast<float4v*>(sums + 32 * n + 8 * w + 4 * rows.hi) =
+          float4v{rows.acc[n][4 * w], rows.acc[n][4 * w + 1], rows.acc[n][4 * w + 2], rows.acc[n][4 * w + 3]};
+  if (rows.hi == 0) {
+    float* const t = total_of(p, D, all_rows, row, b.split);
+    t[0] = rows.m;
+    t[1] = l;
+  }
+}
+
 // More than 32 rows: 128 of them, 32 a wave, the keys in tiles of 64 that four waves
 // share, two of them in LDS.  G groups of four waves have the same rows and take tiles
 // in turn, and the second's results join the first's: where workgroups are so few that
@@ -952,7 +1058,11 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, CapOf<MODE> c) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * G * STAGE];
   const bool dma = p.dma;
   const int every = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = every & 3, group = G == 1 ? 0 : every >> 2;
-  const BlockAt b = block_at<false>(p);
+  Rows<D, BF16, MODE> rows;
+  BlockAt b;
+  if constexpr ((MODE & kTree) != 0)
+    b = tree_block_at(p, c, [&](const BlockAt& at) { rows.ask(p, c, at.tile * 128 + 32 * wave, at.x, at.y, at.z); });
+  else b = block_at<false>(p);
   const int first = b.tile * 128, last = min(first + 127, p.rows - 1);
   const int t0 = (int)p.d_heads((unsigned)first), t1 = (int)p.d_heads((unsigned)last);
   const int* const kdocs = p.kdocs ? p.kdocs + p.tkdocs.at(b.x, b.y, b.z) : nullptr;
@@ -978,7 +1088,6 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, CapOf<MODE> c) {
   };
   unsigned char* const stages = lds + group * 2 * STAGE;
   if (i0 + group < i1) issue(i0 + group, stages);
-  Rows<D, BF16, MODE> rows;
   rows.begin(p, c, first + 32 * wave, b.x, b.y, b.z, b.start, b.window);
 #pragma unroll 1
   for (int i = i0 + group, n = 0; i - group < i1; i += G, n ^= 1) {
@@ -1061,19 +1170,85 @@ void attend_rows_kernel(AttendArgs p, long long all_rows, CapOf<MODE> c) {
     return;
   }
   if (first + 32 * wave + rows.col >= p.rows) return;
-  const long long row = b.block * p.rows + rows.row;
-  float* const sums = sums_of(p, D, row, b.split);
+  leave_part(p, rows, b, l, all_rows);
+}
+
+// Trees of 33 to 64 rows: two waves have them for the first half of each tile of keys, and
+// two for the second, and their results meet at the end: a wave waits for its own products and
+// arithmetic in turn, so four at half a tile each take 0.9 us where two with all of it take
+// 1.4.  In LDS are as many tiles, up to four, as leave room for a second workgroup, and all but
+// one are on their way.  (Eight waves for 128 rows, with a tile more on its way, gain nothing:
+// 16 x 8 Blocks over 8192 keys of 128 columns 117 us against 121, over 700 keys 28 against 27.)
+template <int D, bool BF16, int MODE>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_half_kernel(AttendArgs p, long long all_rows, CapOf<MODE> c) {
+  constexpr int BN = 64, KB = BN * D * 2, STAGE = 2 * KB, PER = STAGE / 4096;
+  constexpr int NS = 4 * STAGE <= 80 * 1024 ? 4 : 3 * STAGE <= 80 * 1024 ? 3 : 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[NS * STAGE];
+  const bool dma = p.dma;
+  const int every = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = every & 1, half = every >> 1;
+  Rows<D, BF16, MODE> rows;
+  Fill<D, BN, false, 4> fk;
+  Fill<D, BN, true, 4> fv;
+  const BlockAt b = tree_block_at(p, c, [&](const BlockAt& at) {
+    rows.ask(p, c, 32 * mine, at.x, at.y, at.z);
+    fk.begin(p.k + p.tk.at(at.x, at.y, at.z) * 2, p.ldk, every);
+    fv.begin(p.v + p.tv.at(at.x, at.y, at.z) * 2, p.ldv, every);
+  });
+  const Tiles tiles = tree_tiles(p, BN, b.start, b.window, b.len, c.tokens);
+  const int share = (int)p.d_splits((unsigned)(tiles.n + p.splits - 1));  // tiles of a split
+  const int i0 = min(b.split * share, tiles.n), i1 = min(i0 + share, tiles.n);
+  auto issue = [&](int i, int slot) {
+    const int key0 = tiles.at(i) * BN, left = b.len - key0;
+    fk.issue(dma, key0, left, lds + slot * STAGE);
+    fv.issue(dma, key0, left, lds + slot * STAGE + KB);
+  };
+  rows.have();
+#pragma unroll
+  for (int n = 0; n < NS - 1; ++n)
+    if (i0 + n < i1) issue(i0 + n, n);
+  rows.begin(p, c, 32 * mine, b.x, b.y, b.z, b.start, b.window);
+  int slot = 0;
+#pragma unroll 1
+  for (int i = i0; i < i1; ++i) {
+    switch (dma ? min(i1 - 1 - i, NS - 2) : 0) {
+      case 0: XTK_WAIT_VM(0); break;
+      case 1: XTK_WAIT_VM(NS > 2 ? PER : 0); break;
+      default: XTK_WAIT_VM(NS > 3 ? 2 * PER : 0); break;
+    }
+    // behind the barrier this tile has landed, and every wave is done with the one before
+    lds_barrier();
+    if (i + NS - 1 < i1) issue(i + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+    const int key0 = tiles.at(i) * BN + 32 * half;
+    unsigned char* const at = lds + slot * STAGE + half * (KB / 2);
+    if (key0 < b.len && !rows.sees_none(p, key0, 32, 0))
+      rows.template tile<1>(p, c, at, at + KB, nullptr, nullptr, key0, b.len, 0);
+    slot = slot + 1 == NS ? 0 : slot + 1;
+  }
+  rows.hold();
+  lds_barrier();
+  if (any_wave<4>(rows.spoilt(), lds)) {
+    odd_rows<D, BF16, MODE>(args_here(), c, b, tiles, BN, i0, i1, nullptr, every, p.rows, 4, all_rows);
+    return;
+  }
+  static_assert(2 * (32 * D + 128) * 4 <= NS * STAGE, "the halves' results");
+  join_halves(rows, reinterpret_cast<float*>(lds) + mine * (32 * D + 128), half == 1);
+  if (half == 1) return;
+  const float l = both_halves(rows.l, false);
+  if (32 * mine + rows.col >= p.rows) return;
+  if (p.splits > 1) {
+    leave_part(p, rows, b, l, all_rows);
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int n = 0; n < D / 32; ++n)
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-      *reinterpret_cast<float4v*>(sums + 32 * n + 8 * w + 4 * rows.hi) =
-          float4v{rows.acc[n][4 * w], rows.acc[n][4 * w + 1], rows.acc[n][4 * w + 2], rows.acc[n][4 * w + 3]};
-  if (rows.hi == 0) {
-    float* const t = total_of(p, D, all_rows, row, b.split);
-    t[0] = rows.m;
-    t[1] = l;
-  }
+    for (int w = 0; w < 4; ++w) {
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = l == 0.0f ? 0.0f : rows.acc[n][4 * w + e] * inv;
+      store4<BF16>(p, b, rows.row, 32 * n + 8 * w + 4 * rows.hi, o[0], o[1], o[2], o[3]);
+    }
 }
 
 // Waves of a workgroup of few rows, and tiles of 32 keys in a wave's ring: what
@@ -1093,10 +1268,15 @@ template <int D, bool BF16, int MODE>
 __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p, long long all_rows, CapOf<MODE> c) {
   typedef Few<D> F;
   constexpr int W = F::W, NS = F::NS, KB = 32 * D * 2, PER = D / 8;
+  constexpr bool TREE = (MODE & kTree) != 0;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[F::LDS];
   const bool dma = p.dma;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const BlockAt b = block_at<true>(p);
+  Rows<D, BF16, MODE> rows;
+  BlockAt b;
+  if constexpr ((MODE & kTree) != 0)
+    b = tree_block_at(p, c, [&](const BlockAt& at) { rows.ask(p, c, 0, at.x, at.y, at.z); });
+  else b = block_at<true>(p);
   const int t1 = (int)p.d_heads((unsigned)(p.rows - 1));
   const int* const kdocs = p.kdocs ? p.kdocs + p.tkdocs.at(b.x, b.y, b.z) : nullptr;
   int d0 = 0, d1 = b.len;
@@ -1122,10 +1302,10 @@ __global__ __launch_bounds__(64 * Few<D>::W) void attend_few_kernel(AttendArgs p
     fk.issue(dma, key0, b.len - key0, at);
     fv.issue(dma, key0, b.len - key0, at + KB);
   };
+  if constexpr (TREE) rows.have();
 #pragma unroll
   for (int j = 0; j < NS; ++j)
     if (j < mine) issue(j, j);
-  Rows<D, BF16, MODE> rows;
   rows.begin(p, c, 0, b.x, b.y, b.z, b.start, b.window);
   int slot = 0;
 #pragma unroll 1
@@ -1288,32 +1468,39 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs p, long lon
 inline bool pairs_of(const AttendArgs& a, int d) { return d <= 128 && a.nwg <= 256 && a.splits == 1 && a.keys > 192; }
 
 template <int D, bool BF16, int MODE>
-void run_attend_rows(bool few, const AttendArgs& a, long long all_rows, const CapOf<MODE>& c, hipStream_t s) {
+hipError_t run_attend_rows(bool few, const AttendArgs& a, long long all_rows, const CapOf<MODE>& c, hipStream_t s) {
   if (few) {
     attend_few_kernel<D, BF16, MODE><<<a.nwg, 64 * Few<D>::W, 0, s>>>(a, all_rows, c);
-    return;
+    return hipGetLastError();
   }
+  if constexpr ((MODE & kTree) != 0)
+    if (a.rows <= xt::kAttendHalfRows) {
+      attend_half_kernel<D, BF16, MODE><<<a.nwg, 256, 0, s>>>(a, all_rows, c);
+      return hipGetLastError();
+    }
   if constexpr (D <= 128)
     if (pairs_of(a, D)) {
       attend_rows_kernel<D, BF16, 2, MODE><<<a.nwg, 512, 0, s>>>(a, all_rows, c);
-      return;
+      return hipGetLastError();
     }
   attend_rows_kernel<D, BF16, 1, MODE><<<a.nwg, 256, 0, s>>>(a, all_rows, c);
+  return hipGetLastError();
 }
 
 inline long long all_rows_of(const AttendArgs& a) { return a.nwg / ((long long)a.tiles * a.splits) * a.rows; }
 
-// Behind the rows' kernel.
+// Behind the rows' kernel, whose status is e.  A workgroup a row has its splits on their way
+// together: for up to 2048 rows of trees also where there are more than four (32 rows in 16
+// splits 17.3 -> 16.2 us; 4096 rows in 8 splits 39.3 against 41.5).
 template <int D, bool BF16>
-hipError_t run_attend_join(const AttendArgs& a, hipStream_t s) {
+hipError_t run_attend_join(const AttendArgs& a, bool tree, hipError_t e, hipStream_t s) {
+  if (e != hipSuccess) return e;
   const long long all_rows = all_rows_of(a);
   if (a.splits > 1) {
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
     AttendArgs j = a;
     j.d_work = div31(static_cast<unsigned>(a.rows));
     constexpr int rows = 256 / (D / 4);
-    if (a.splits <= 16)
+    if (a.splits <= (tree && all_rows <= 2048 ? 4 : 16))
       attend_join_kernel<D, BF16, true><<<static_cast<unsigned>((all_rows + rows - 1) / rows), 256, 0, s>>>(j, all_rows);
     else
       attend_join_kernel<D, BF16, false><<<static_cast<unsigned>(all_rows), 256, 0, s>>>(j, all_rows);
@@ -1323,16 +1510,16 @@ hipError_t run_attend_join(const AttendArgs& a, hipStream_t s) {
 
 template <int D, bool BF16>
 hipError_t run_attend_elem(bool few, const AttendArgs& a, const FineCap* fine, hipStream_t s) {
-  if (fine) run_attend_rows<D, BF16, kFine>(few, a, all_rows_of(a), *fine, s);
-  else run_attend_rows<D, BF16, kPlain>(few, a, all_rows_of(a), FineCap{}, s);
-  return run_attend_join<D, BF16>(a, s);
+  const hipError_t e = fine ? run_attend_rows<D, BF16, kFine>(few, a, all_rows_of(a), *fine, s)
+                            : run_attend_rows<D, BF16, kPlain>(few, a, all_rows_of(a), FineCap{}, s);
+  return run_attend_join<D, BF16>(a, false, e, s);
 }
 
 template <int D, bool BF16>
 hipError_t run_attend_tree_elem(bool few, const AttendArgs& a, const TreeCap& tree, bool fine, hipStream_t s) {
-  if (fine) run_attend_rows<D, BF16, kTree | kFine>(few, a, all_rows_of(a), tree, s);
-  else run_attend_rows<D, BF16, kTree>(few, a, all_rows_of(a), tree, s);
-  return run_attend_join<D, BF16>(a, s);
+  const hipError_t e = fine ? run_attend_rows<D, BF16, kTree | kFine>(few, a, all_rows_of(a), tree, s)
+                            : run_attend_rows<D, BF16, kTree>(few, a, all_rows_of(a), tree, s);
+  return run_attend_join<D, BF16>(a, true, e, s);
 }
 
 }  // namespace

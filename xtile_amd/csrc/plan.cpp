@@ -1534,7 +1534,8 @@ int attend_splits(const Plan& p) {
   // A causal window leaves only so many keys, whatever the cache holds.
   const bool band = (a.causal || a.extra[6].arg >= 0) && a.window && a.extra[3].arg < 0;
   const int64_t keys = band ? std::min(a.keys, a.window + a.rows) : a.keys;
-  const int fit = few ? (a.d > 64 ? 1 : 2) : a.d > 128 ? 1 : a.d > 64 ? 2 : 3;  // workgroups on a compute unit
+  const bool half = a.extra[6].arg >= 0 && rows <= kAttendHalfRows;
+  const int fit = few ? (a.d > 64 ? 1 : 2) : a.d > 128 ? 1 : a.d > 64 || half ? 2 : 3;  // workgroups on a compute unit
   const double want = 256 * fit / tiles;
   const int64_t round = a.d > 160 ? 64 : 128;  // keys of few rows that a workgroup's waves take at a time
   const int64_t most = few ? (keys > 2 * round ? (keys + round - 1) / round : 1) : keys < 1024 ? 1 : keys / 256;

@@ -184,8 +184,9 @@ constexpr int64_t kAttendFewRows = 32, kAttendRows = 128;
 constexpr int64_t kSampleVocab = int64_t(1) << 22;
 constexpr int kSampleSlices = 64;
 constexpr int64_t kSampleRowWork = 123248;
-// Drafted tokens of a tree: their ancestors are a lane's 64 bits.
-constexpr int64_t kAttendTree = 64;
+// Drafted tokens of a tree: their ancestors are a lane's 64 bits.  Rows of a Block up to which
+// a tree has kernels of its own.
+constexpr int64_t kAttendTree = 64, kAttendHalfRows = 64;
 
 struct Plan {
   PlanKind kind = PlanKind::EwBinary;
