@@ -18,12 +18,13 @@
 // index) as often as it takes, at most five times.
 //
 // What bounds it is the arithmetic of a row on one CU: a weight is some twenty 64-bit
-// operations, so 32768 weights and their bins take 13 us there, against 3 for their loads; a
+// operations, so 32768 weights and their bins take 10 us there, against 3 for their loads; a
 // scan of the bins takes 1, a list with its search 5.  Rows of few top-k tokens make no weights
 // but those of a list of at most kList.  Few long rows are dealt to many workgroups in slices,
 // a kernel for each pass (xt::sample_slices has the rule).  Replayed in a graph: 1 row of 32768
-// logits, top-k 50 and top-p, 17 us, without cuts 23; 1 row of 131072, top-p, 31, top-k 50, 23;
-// 64 rows of 131072, top-p and min-p, 67 (34 MB, 6 us of HBM), 256 rows of 32768 48.
+// logits, top-k 50 and top-p, 17 us, without cuts 23; 1 row of 131072, top-p, 31 to 38, top-k
+// 50, 23; 256 rows of 32768 44; 64 rows of 131072, top-p and min-p, 65, of which the largest
+// logit takes 8 (34 MB at 4 TB/s), the bins 18, the lists 18, and what is left of a row 16.
 #include "launch.h"
 
 #include <algorithm>
@@ -39,6 +40,7 @@ typedef unsigned long long u64;
 
 constexpr int kBins = 2048, kList = 2048;
 constexpr int kIndexBits = 22;  // xt::kSampleVocab
+constexpr u64 kAll = 1ull << 62;  // more than any sum: what is kept where nothing is dropped
 static_assert(xt::kSampleVocab == 1LL << kIndexBits && kBins == kList, "");
 
 struct RowWork;
@@ -212,9 +214,9 @@ struct Weights {
 
   // Never more for a larger logit: each step here is monotonic.
   __device__ __forceinline__ int bin(float x) const {
-    if (only_top) return x == top ? 0 : kBins - 1;
-    return (int)fminf((top - x) * per_bin, (float)(kBins - 1));
+    return only_top ? (x == top ? 0 : kBins - 1) : bin_of_many(x);
   }
+  __device__ __forceinline__ int bin_of_many(float x) const { return (int)fminf((top - x) * per_bin, (float)(kBins - 1)); }
 
   // A logit that no logit of bins up to `last` is below.
   __device__ __forceinline__ float least_of(int last) const {
@@ -235,7 +237,9 @@ struct Weights {
   // rint(2^S 2^z): 2^z as 2^k 2^r, |r| <= 1/2, by eleven terms of its series (off by
   // 2.2e-13), and a sum with 2^52, whose low bits are the integer.
   __device__ __forceinline__ u64 weight(float x) const {
-    if (only_top) return x == top ? 1ull << shift : 0;
+    return only_top ? (x == top ? 1ull << shift : 0) : weight_of_many(x);
+  }
+  __device__ __forceinline__ u64 weight_of_many(float x) const {
     const double z = ((double)x - (double)top) * c;
     // z to the nearest integer in the low bits of a sum with 3 2^51
     const double sum = z + 6755399441055744.0, r = z - (sum - 6755399441055744.0);
@@ -356,56 +360,91 @@ __device__ __forceinline__ int bin_with(const T* running, T value, Found& found,
   return __builtin_amdgcn_readfirstlane(*at);
 }
 
-// Adds logits first to last - 1 to the bins, in LDS: counts, and with SUMS weights and, to
-// `kept`, those of what min-p keeps.
-template <int ELEM, bool SUMS>
-__device__ __forceinline__ void add_bins(const unsigned char* row, int first, int last, int threads, const Weights& w, u64 least,
-                                         u64* sum, unsigned* count, u64* kept) {
+// Adds logits first to last - 1 to the bins, in LDS: counts, and with SUMS weights and, where
+// there is a min-p (KEPT), to `kept` those of what it keeps.  MANY: not only the largest have
+// weights; these are questions for a whole row, and a branch for each logit would keep the
+// arithmetic of one from filling another's waits.
+template <int ELEM, bool SUMS, bool KEPT, bool MANY>
+__device__ __forceinline__ void add_bins_of(const unsigned char* row, int first, int last, int threads, const Weights& w,
+                                            u64 least, u64* sum, unsigned* count, u64* kept) {
   u64 mine = 0;
   each4<ELEM, 4>(row, first, last, threads, [&](const float (&v)[4], int, int n) {
+    int b[4];
+    u64 is[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = clean(v[e]);
+      b[e] = MANY ? w.bin_of_many(x) : w.bin(x);
+      if constexpr (SUMS) is[e] = MANY ? w.weight_of_many(x) : w.weight(x);
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (e >= n) break;
-      const float x = clean(v[e]);
-      const int b = w.bin(x);
-      atomicAdd(&count[b], 1u);
+      atomicAdd(&count[b[e]], 1u);
       if constexpr (SUMS) {
-        const u64 is = w.weight(x);
-        atomicAdd(&sum[b], is);
-        if (least && is >= least) mine += is;
+        atomicAdd(&sum[b[e]], is[e]);
+        if constexpr (KEPT) mine += is[e] >= least ? is[e] : 0;
       }
     }
   });
-  if constexpr (SUMS) {
-    // without min-p: all
-    if (least) {
-      mine = wave_scan(mine);
-      if ((threadIdx.x & 63) == 63) atomicAdd(kept, mine);
-    } else if (threadIdx.x == 0) {
-      *kept = 1ull << 62;
-    }
+  if constexpr (KEPT) {
+    mine = wave_scan(mine);
+    if ((threadIdx.x & 63) == 63) atomicAdd(kept, mine);
   }
 }
 
-// give(order, logit) of each of logits first to last - 1 that lies in bins lo to hi.
-template <int ELEM, class F>
-__device__ __forceinline__ void each_in(const unsigned char* row, int first, int last, int threads, const Weights& w, int lo,
-                                        int hi, F give) {
-  const float least = w.least_of(hi), most = w.most_of(lo);
-  const bool tail = least == -__builtin_inff();  // which has NaN too
-  each4<ELEM, ELEM == kF32 ? 8 : 4>(row, first, last, threads, [&](const float (&v)[4], int i, int n) {
-    // of four one is rarely among them: a value between the two is the median of the three
-    unsigned in = 0;
+template <int ELEM>
+__device__ __forceinline__ void add_bins(const unsigned char* row, int first, int last, int threads, const Weights& w,
+                                         bool sums, u64 least, u64* sum, unsigned* count, u64* kept) {
+  if (w.only_top) {
+    add_bins_of<ELEM, true, true, false>(row, first, last, threads, w, least, sum, count, kept);
+    return;
+  }
+  if (!sums) {
+    add_bins_of<ELEM, false, false, true>(row, first, last, threads, w, least, sum, count, kept);
+  } else if (least) {
+    add_bins_of<ELEM, true, true, true>(row, first, last, threads, w, least, sum, count, kept);
+  } else {
+    add_bins_of<ELEM, true, false, true>(row, first, last, threads, w, least, sum, count, kept);
+    if (threadIdx.x == 0) *kept = kAll;
+  }
+}
+
+// Bins lo to hi of a row's logits; none of them where lo > hi.
+struct Between {
+  int lo, hi;
+  float least, most;  // no logit of them is outside; minus infinity stands for NaN too
+  __device__ __forceinline__ void begin(const Weights& w, int l, int h) {
+    lo = l;
+    hi = h;
+    least = l > h ? w.top : w.least_of(h);
+    most = l > h ? w.top : w.most_of(l);
+  }
+  __device__ __forceinline__ bool tail() const { return least == -__builtin_inff(); }
+};
+
+// give(run, order, logit) of each of logits first to last - 1 that lies in one of R runs of bins.
+template <int ELEM, int R, class F>
+__device__ __forceinline__ void each_in(const unsigned char* row, int first, int last, int threads, const Weights& w,
+                                        const Between (&run)[R], F give) {
+  bool tail = false;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) in |= (__builtin_amdgcn_fmed3f(v[e], least, most) == v[e] ? 1u : 0u) << e;
-    if (tail) in = 15;
-    if (in == 0) return;
+  for (int q = 0; q < R; ++q) tail |= run[q].tail();
+  each4<ELEM, ELEM == kF32 ? 8 : 4>(row, first, last, threads, [&](const float (&v)[4], int i, int n) {
+    // of a wave's 256 few are among them: between two is what is the median of the three
+    bool in[4] = {tail, tail, tail, tail};
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in[e] |= __builtin_amdgcn_fmed3f(v[e], run[q].least, run[q].most) == v[e];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (!((in >> e) & 1) || e >= n) continue;
+      if (!in[e] || e >= n) continue;
       const float x = clean(v[e]);
       const int b = w.bin(x);
-      if (b >= lo && b <= hi) give(order_of(x, i + e), x);
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+        if (b >= run[q].lo && b <= run[q].hi) give(q, order_of(x, i + e), x);
     }
   });
 }
@@ -433,11 +472,13 @@ __device__ __forceinline__ void sort_list(List& s, int n) {
     s.rank[t] = 0;
     if (t == 0 && n % 2) s.order[n] = ~0ull;  // two are read at a time
     __syncthreads();
+    // compared as doubles, in half the time: orders are below 2^54, whose doubles rise as they do
+    const double key = __builtin_bit_cast(double, mine);
     unsigned before = 0;
 #pragma unroll 4
     for (int j = part * each; j < min(n, (part + 1) * each); j += 2) {
-      const ulong2 o = *reinterpret_cast<const ulong2*>(s.order + j);
-      before += (o.x < mine) + (o.y < mine);
+      const double2 o = *reinterpret_cast<const double2*>(s.order + j);
+      before += (o.x < key) + (o.y < key);
     }
     if (i < n && before) atomicAdd(&s.rank[i], before);
     __syncthreads();
@@ -539,7 +580,9 @@ __device__ __forceinline__ void make_list(Shared& s, const unsigned char* row, i
                                           int shift, u64 prefix, int n) {
   if (threadIdx.x == 0) s.list.n = 0;
   __syncthreads();
-  each_in<ELEM>(row, 0, vocab, kThreads, w, lo, hi, [&](u64 o, float x) {
+  Between run[1];
+  run[0].begin(w, lo, hi);
+  each_in<ELEM>(row, 0, vocab, kThreads, w, run, [&](int, u64 o, float x) {
     if ((o >> shift) != prefix) return;
     const int at = atomicAdd(&s.list.n, 1);
     if (at >= kList) return;  // as counted, there are no more
@@ -589,7 +632,9 @@ __device__ __forceinline__ u64 search(Shared& s, const unsigned char* row, int v
         s.fine.count[i] = 0;
       }
       __syncthreads();
-      each_in<ELEM>(row, 0, vocab, kThreads, w, bin, bin, [&](u64 o, float x) {
+      Between run[1];
+      run[0].begin(w, bin, bin);
+      each_in<ELEM>(row, 0, vocab, kThreads, w, run, [&](int, u64 o, float x) {
         if ((o >> shift) != prefix) return;
         const int d = (int)(o >> next) & ((1 << (shift - next)) - 1);
         atomicAdd(&s.fine.sum[d], w.weight(x));
@@ -645,7 +690,7 @@ __device__ __forceinline__ int pick(Shared& s, const unsigned char* row, int voc
     }
     if (threadIdx.x == 0) s.kept = 0;
     __syncthreads();
-    add_bins<ELEM, true>(row, 0, vocab, kThreads, w, a.least, s.sum, s.count, &s.kept);
+    add_bins<ELEM>(row, 0, vocab, kThreads, w, true, a.least, s.sum, s.count, &s.kept);
     __syncthreads();
   }
   scan<kThreads, true, true>(s.sum, s.count, s.mem);
@@ -682,8 +727,7 @@ __device__ __forceinline__ int sample_row(const SampleArgs& p, const RowAt& at, 
   if (threadIdx.x == 0) s.kept = 0;
   const Weights w = weights_of(p, a, top);
   __syncthreads();
-  if (a.few(p.vocab)) add_bins<ELEM, false>(row, 0, p.vocab, kThreads, w, a.least, s.sum, s.count, &s.kept);
-  else add_bins<ELEM, true>(row, 0, p.vocab, kThreads, w, a.least, s.sum, s.count, &s.kept);
+  add_bins<ELEM>(row, 0, p.vocab, kThreads, w, !a.few(p.vocab), a.least, s.sum, s.count, &s.kept);
   __syncthreads();
   return pick<ELEM>(s, row, p.vocab, w, a);
 }
@@ -789,8 +833,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs p
   slice_of(p, slice, first, last);
   const bool few = a.few(p.vocab);
   const unsigned char* const row = logits_of<ELEM>(p, at);
-  if (few) add_bins<ELEM, false>(row, first, last, kSliceThreads, w, a.least, sum, count, &kept);
-  else add_bins<ELEM, true>(row, first, last, kSliceThreads, w, a.least, sum, count, &kept);
+  add_bins<ELEM>(row, first, last, kSliceThreads, w, !few, a.least, sum, count, &kept);
   __syncthreads();
   // integers: in whatever order they are added, the sums are the same
   for (int i = threadIdx.x; i < kBins; i += kSliceThreads)
@@ -799,8 +842,8 @@ __global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs p
       if (!few && sum[i]) add_to(&work.sum[i], sum[i]);
     }
   if (!few && threadIdx.x == 0) {
-    if (a.least) add_to(&work.kept, kept);
-    else if (slice == 0) work.kept = kept;
+    if (a.least || w.only_top) add_to(&work.kept, kept);
+    else if (slice == 0) work.kept = kAll;
   }
 }
 
@@ -881,19 +924,19 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs p
   int first, last;
   slice_of(p, slice, first, last);
   const unsigned char* const row = logits_of<ELEM>(p, at);
+  auto take = [&](int q, u64 o, float x) {
+    const int to = atomicAdd(&near[q], 1);
+    if (to < kNear) {
+      sum[q * kNear + to] = o;
+      logits[q * kNear + to] = x;
+    } else {
+      hand_on(q, add_to(&work.listed[q], 1), o, x);
+    }
+  };
+  Between in[3];
 #pragma unroll
-  for (int q = 0; q < 3; ++q) {
-    if (run[q].n == 0) continue;
-    each_in<ELEM>(row, first, last, kSliceThreads, w, run[q].lo, run[q].hi, [&](u64 o, float x) {
-      const int to = atomicAdd(&near[q], 1);
-      if (to < kNear) {
-        sum[q * kNear + to] = o;
-        logits[q * kNear + to] = x;
-      } else {
-        hand_on(q, add_to(&work.listed[q], 1), o, x);
-      }
-    });
-  }
+  for (int q = 0; q < 3; ++q) in[q].begin(w, run[q].lo, run[q].n ? run[q].hi : -1);
+  each_in<ELEM>(row, first, last, kSliceThreads, w, in, take);
   __syncthreads();
   if (threadIdx.x < 3) {
     const int n = min(near[threadIdx.x], kNear);
@@ -921,12 +964,25 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs p) {
     put_token(p, at, sample_row<ELEM>(p, at, a, s, top));
     return;
   }
+  // the runs' tokens, on their way together
+  constexpr int PER = kList / kThreads;
+  u64 order[3][PER], weight[3][PER];
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int i = threadIdx.x + e * kThreads;
+      const bool in = i < work.run[q].n;
+      order[q][e] = in ? work.order[q][i] : 0;
+      weight[q][e] = in ? work.weight[q][i] : 0;
+    }
   auto take = [&](int q) {
     __syncthreads();
     const int n = work.run[q].n;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      s.list.order[i] = work.order[q][i];
-      s.list.weight[i] = work.weight[q][i];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      s.list.order[threadIdx.x + e * kThreads] = order[q][e];
+      s.list.weight[threadIdx.x + e * kThreads] = weight[q][e];
     }
     __syncthreads();
     sort_list(s.list, n);
@@ -951,7 +1007,8 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs p) {
     if (!work.run[2].n) q = 1;
     __syncthreads();
   }
-  const int n = q == 2 ? take(2) : work.run[1].n;
+  int n = work.run[1].n;
+  if (q == 2) n = take(2);
   search_list(s.list, n, work.run[q].base_sum, a.drawn(kept));
   put_token(p, at, s.list.index);
 }
