@@ -252,6 +252,44 @@ def test_products_past_32_bits(m, n):
     assert not bool(y[:-last].any()) and not bool(y[:, :-last].any())
 
 
+def test_a_product_with_a_result_past_32_bits():
+    import torch
+
+    m, n, k, last = 70000, 16400, 64, 24
+    rng = np.random.default_rng(2)
+    x, w = (torch.from_numpy(rng.integers(-128, 128, (r, k // 2)).astype(np.int8)).cuda() for r in (m, n))
+    xs, ws = (torch.from_numpy(rng.integers(100, 128, (r, k // 32)).astype(np.int8)).cuda() for r in (m, n))
+    y = torch.full((m, n), 7.0, dtype=torch.float32, device="cuda")
+    p = K.matmul_mx4(m, n, k)
+    print(f"[gpu] {xt.plan(p)['kernel']}", flush=True)
+    xt.launch(p, x, xs, w, ws, y)
+    for at in (slice(0, last), slice(m // 2, m // 2 + last), slice(m - last, m)):
+        for to in (slice(0, last), slice(n - last, n)):
+            want, far = ref.matmul_mx4(of_mx4(x[at], xs[at]), of_mx4(w[to], ws[to]))
+            assert bool((np.abs(y[at, to].cpu().double().numpy() - want) <= far).all())
+
+
+@pytest.mark.parametrize("nq,g", [(2, 1), (8, 5), (40, 4)])
+def test_trees_at_the_end_of_keys_past_32_bits(nq, g):
+    """Keys of more than 4 GiB: the last ones, against the same on their own."""
+    import torch
+
+    nk, d, window = (1 << 25) + 100, 64, 90
+    k = torch.zeros(1, 1, nk, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    q = rand((1, g, nq, d), 1)
+    k[:, :, -300:], v[:, :, -300:] = rand((1, 1, 300, d), 2), rand((1, 1, 300, d), 3)
+    tree = [int(max(-1, t - 1 - t % 2)) for t in range(nq)]
+    o = torch.zeros_like(q)
+    p = K.masked_attention(1, 1, g, nq, nk, d, window=window, start=True, parents=True)
+    print(f"[gpu] {xt.plan(p)['kernel']}", flush=True)
+    xt.launch(p, q, k, v, torch.tensor([[nk - nq]], dtype=torch.int32, device="cuda"),
+              torch.tensor([tree], dtype=torch.int32, device="cuda"), o)
+    sees, distance = (torch.from_numpy(m)[None] for m in ref.tree_seen(tree, 300 - nq, 300, 300, window))
+    want, far = ref.attend_seen(q.cpu(), k[:, :, -300:].cpu(), v[:, :, -300:].cpu(), d**-0.5, sees, distance, None, None)
+    operators_ref.assert_within(o.cpu(), want, far)
+
+
 def test_logits_past_32_bits():
     """The last row of more than 4 GiB of logits."""
     import torch

@@ -152,6 +152,18 @@ def test_sliced_rows(dtype, kind, options):
     check(x, uniforms(rows, 12), dtype, **options)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("vocab", [8192, 8193, 8199, 20001, 32760, 32767, 32768, 32769])
+def test_rows_kept_in_registers(dtype, vocab):
+    """Around the sizes of 16-bit rows that are read once, with equal logits and NaN among them."""
+    x = logits(7, vocab, dtype, vocab)
+    x[2, ::2] = float("nan")
+    x[3, :] = float("-inf")
+    x[4, 1:] = x[4, 0]
+    for options in ({}, {"top_k": [50, 1, 300, 5, vocab - 1, 0, 9000]}, {"top_p": 0.7, "min_p": 0.01}):
+        check(x, uniforms(7, vocab), dtype, **options)
+
+
 def test_odd_logits():
     """Infinities, NaN and zeros of both signs."""
     import torch
@@ -190,13 +202,13 @@ def test_every_token_can_be_drawn():
 
 
 @pytest.mark.parametrize("skip", [0, 1, 3])
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_blocks_pitches_and_alignment(dtype, skip):
+@pytest.mark.parametrize("dtype,vocab", [("f32", 3001), ("bf16", 3001), ("bf16", 9001), ("f32", 40001)], ids=str)
+def test_blocks_pitches_and_alignment(dtype, vocab, skip):
     """Rows of a wider array from any element on, parameters in a column of theirs; what lies
     beside the tokens stays."""
     import torch
 
-    rows, vocab, wide, trow = 8, 3001, 3 * 3001, 2
+    rows, wide, trow = 8, 3 * vocab, 2
 
     @xt.kernel
     def sample_kernel(x, u, p, y):
