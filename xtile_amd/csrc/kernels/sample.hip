@@ -404,6 +404,27 @@ __device__ __forceinline__ int bin_with(const T* running, T value, Found& found,
   return __builtin_amdgcn_readfirstlane(*at);
 }
 
+// The same of two values, the first at most the second.
+struct FoundBoth {
+  int at[2][2];
+};
+template <int THREADS>
+__device__ __forceinline__ void bins_with(const u64* running, u64 low, u64 high, FoundBoth& found, int& turn, int& lo, int& hi) {
+  constexpr int PER = kBins / THREADS;
+  int* const at = found.at[turn ^= 1];
+  u64 before = threadIdx.x ? running[PER * threadIdx.x - 1] : 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const u64 upto = running[PER * threadIdx.x + i];
+    if (before < low && low <= upto) at[0] = PER * threadIdx.x + i;
+    if (before < high && high <= upto) at[1] = PER * threadIdx.x + i;
+    before = upto;
+  }
+  __syncthreads();
+  lo = __builtin_amdgcn_readfirstlane(at[0]);
+  hi = __builtin_amdgcn_readfirstlane(at[1]);
+}
+
 // Adds logits to the bins, in LDS: counts, and with SUMS weights and, where
 // there is a min-p (KEPT), to `kept` those of what it keeps.  MANY: not only the largest have
 // weights; these are questions for a whole row, and a branch for each logit would keep the
@@ -898,6 +919,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs p
   __shared__ unsigned count[kBins];
   __shared__ ScanMem<kSliceThreads> mem;
   __shared__ Found found;
+  __shared__ FoundBoth both;
   __shared__ int near[3], far[3];
   const int r = (int)p.d_slices(blockIdx.x), slice = blockIdx.x - r * p.slices;
   const RowAt at = row_at(p, r);
@@ -919,7 +941,6 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs p
     const unsigned before = lo ? count[lo - 1] : 0;
     return Run{lo, hi, (int)(count[hi] - before), before, lo ? sum[lo - 1] : 0};
   };
-  auto with_weight = [&](u64 value) { return bin_with<kSliceThreads, u64>(sum, value, found, turn); };
   auto before_bin = [&](int b) { return b ? sum[b - 1] : 0; };
   Run run[3] = {{0, 0, 0, 0, 0}, {0, 0, 0, 0, 0}, {0, 0, 0, 0, 0}};
   u64 total = sum[kBins - 1];
@@ -937,7 +958,8 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs p
       else run[0] = run_of(b, b);
     }
     if (a.cuts()) {
-      const int lo = with_weight(a.cut(low)), hi = with_weight(a.cut(high));
+      int lo, hi;
+      bins_with<kSliceThreads>(sum, a.cut(low), a.cut(high), both, turn, lo, hi);
       head = count[hi] <= kHead;
       run[1] = run_of(head ? 0 : lo, hi);
       low = min(low, before_bin(lo) + 1);
@@ -945,7 +967,8 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs p
     }
     const u64 by_min = work.kept;
     if (!head) {
-      const int lo = with_weight(a.drawn(min(low, by_min))), hi = with_weight(a.drawn(min(high, by_min)));
+      int lo, hi;
+      bins_with<kSliceThreads>(sum, a.drawn(min(low, by_min)), a.drawn(min(high, by_min)), both, turn, lo, hi);
       run[2] = run_of(count[hi] <= kHead ? 0 : lo, hi);
     }
   }
