@@ -453,24 +453,32 @@ struct Rows {
           for (int r = 0; r < 16; ++r) s[t][r] = FINE ? capped(p, c, s[t][r]) : capped_far(p, s[t][r]);
       }
     }
-    if (p.slopes) {
+    // of a tree's tiles only the last have drafted tokens, whose distance is by depth
+    const bool drafted = TREE && key0 + 32 * T > first;
+    if (p.slopes && !drafted) {
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         const float away = (float)(pos - (key0 + t * 32 + 4 * hi));
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float far = fabsf(away - (float)(8 * (r >> 2) + (r & 3)));
-          if constexpr (TREE) {
-            // only the last tiles have drafted tokens: their distance is by depth
-            if (key0 + 32 * T > first) {
-              const int u = key0 + t * 32 + 4 * hi + 8 * (r >> 2) + (r & 3) - first;
-              if (u >= 0) far = (float)tokens_behind(tree, u);
-            }
-          }
-          s[t][r] = fmaf(-slope, far, s[t][r] * mul);
-        }
+        for (int r = 0; r < 16; ++r)
+          s[t][r] = fmaf(-slope, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[t][r] * mul);
       }
       mul = 1.0f;
+    }
+    if constexpr (TREE) {
+      if (p.slopes && drafted) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const int base = key0 + t * 32 + 4 * hi;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = base + 8 * (r >> 2) + (r & 3);
+            const float far = key >= first ? (float)tokens_behind(tree, key - first) : fabsf((float)(pos - key));
+            s[t][r] = fmaf(-slope, far, s[t][r] * mul);
+          }
+        }
+        mul = 1.0f;
+      }
     }
     if (part) {
       unsigned seen[T];  // bit r for register r
