@@ -244,8 +244,11 @@ def product_buffers(x, w, out="f32"):
 # Sizes of which each kernel takes some; none is a multiple of a tile, nor K of a stage.
 KERNELS = [(3, 100, 1056, "few_kernel<8, 8>"), (5, 9000, 1056, "few_kernel<8, 4>"), (15, 100, 4128, "few_kernel<16, 8>"),
            (12, 9000, 1056, "few_kernel<16, 4>"), (63, 4090, 2080, "mid_kernel<1, 1, 8>"), (125, 4090, 1056, "mid_kernel<1, 2, 4>"),
-           (250, 4090, 1056, "mid_kernel<2, 2, 4>"), (1001, 4090, 544, "many_kernel<128, 128, 4, 3>"),
-           (1500, 4090, 1056, "many_kernel<128, 128, 4, 2>"), (4090, 4000, 288, "many_kernel<256, 256, 8, 2>")]
+           (250, 4090, 1056, "mid_kernel<2, 2, 4>"), (1001, 4090, 544, "many_kernel<128, 128, 4, 3, 0>"),
+           (1500, 4090, 1056, "many_kernel<128, 128, 4, 2, 0>"), (4090, 4000, 288, "many_kernel<256, 256, 8, 2, 0>"),
+           # rows of scales that begin at whole words
+           (1001, 4090, 640, "many_kernel<128, 128, 4, 3, 1>"), (1500, 4090, 1152, "many_kernel<128, 128, 4, 2, 1>"),
+           (4090, 4000, 384, "many_kernel<256, 256, 8, 2, 1>")]
 
 
 @pytest.mark.parametrize("m,n,k,kernel", KERNELS)
@@ -260,7 +263,8 @@ def test_every_kernel(m, n, k, kernel, out):
     check_product(bufs[4].cpu().double().numpy(), x, w, out)
 
 
-@pytest.mark.parametrize("k", [32, 64, 96, 224, 256, 288, 480, 512, 544, 768, 800, 1056, 1312])
+@pytest.mark.parametrize("k", [32, 64, 96, 128, 224, 256, 288, 384, 480, 512, 544, 640, 768, 800, 896, 1024, 1056, 1152, 1280,
+                               1312, 1408, 2176, 2304])
 @pytest.mark.parametrize("m,n", [(1000, 4090), (1500, 4090), (4090, 4000)])
 def test_large_tiles_of_every_depth(m, n, k):
     """From fewer stages than buffers to more, with and without a part of one; scales of 255 in

@@ -39,7 +39,7 @@ struct Mx4Args {
   Div31 d_group, d_width, d_last;  // of many rows: a group's tiles, its columns, the last one's
   int tiles, ntiles, mtiles, group, nwg;
   int M, N, blocks_k;  // blocks of 32 of a row
-  int dma;
+  int dma, whole;  // whole: scales in rows of whole words
   int y_elem;
 };
 
@@ -397,27 +397,37 @@ bool run_mid(Mx4Args& a, long long blocks, hipStream_t s) {
 //
 // The result is computed transposed (the weights are the MFMA's rows), so that a lane has
 // four neighbours of a row, and leaves through LDS in 16-byte pieces.
-template <int BM, int BN, int NW, int NB>
+//
+// A row's scales are a few bytes of a line that L2 is asked for each time: WHOLE, rows of them
+// that begin at whole words, takes those of four stages at once (SG), 32 bytes by two
+// neighbouring lanes, and others two stages' five words, or, with more than two buffers, where a
+// wait that leaves DMA in flight has to count it, one stage's three: 1024 x 4096 x 4096 in 128 x
+// 128 17.9 us against 20.8, 1024 x 11008 x 4096 in 256 x 256 36.1 against 39.3 (without any
+// scales they take 17.4 and 34.4).
+template <int P>
+struct Phase {
+  static constexpr int value = P;
+};
+template <int BM, int BN, int NW, int NB, bool WHOLE>
 struct ManyShape {
   static constexpr int WC = NW / 2, WM = BM / 2, WN = BN / WC, MI = WM / 32, NI = WN / 32;
-  // Scales of SG stages at a time, WORDS a row.  Two halve what they ask of L2 (4096 by 11008
-  // x 4096: 126 us with one, 120 with two); a wait that leaves DMA in flight has to count
-  // it, so with more than two buffers each stage has its own.
-  static constexpr int SG = NB == 2 ? 2 : 1, WORDS = 2 * SG + 1;
+  static constexpr int SG = WHOLE ? 4 : NB == 2 ? 2 : 1, WORDS = WHOLE ? 8 : 2 * SG + 1;
   static constexpr int AB = BM * 128, SCALES = (BM + BN) * WORDS * 4, STAGE = (BM + BN) * 128 + (SG == 1 ? SCALES : 0);
   static constexpr int LDS = NB * STAGE + (SG == 1 ? 0 : 2 * SCALES);
   static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, PD = PA + PB;  // data instructions of a wave and stage
-  static constexpr int PS = SCALES / 256 / NW, PER = PD + PS;              // and for scales, of SG stages
+  static constexpr int ONE = WHOLE ? 1024 : 256;                          // bytes of an instruction for scales
+  static constexpr int PS = SCALES / ONE / NW;                            // of them, of SG stages
+  static constexpr int PER = PD + (WHOLE ? 0 : PS);                       // that a wait counts a stage
   static constexpr int PRODUCTS = MI * NI, HALF = PD / 2, EVERY = PRODUCTS / HALF;  // of a step; data instructions
-  static_assert(PS * 256 * NW == SCALES && BM * WORDS / 64 % PS == 0, "a wave has scales of one operand");
-  static_assert(PRODUCTS % HALF == 0 && PA % 2 == 0 && MI >= NI && (MI == 4 || MI == 2) && (PS + SG - 1) / SG <= PRODUCTS, "the steps' schedule");
-  static_assert(LDS <= 160 * 1024 && (NB - 1) * PER < 64, "");
+  static_assert(PS * ONE * NW == SCALES && BM * WORDS * 4 / ONE % PS == 0, "a wave has scales of one operand");
+  static_assert(PRODUCTS % HALF == 0 && PA % 2 == 0 && MI >= NI && (MI == 4 || MI == 2) && (PS + SG - 1) / SG <= PRODUCTS && (!WHOLE || PS <= SG), "the steps' schedule");
+  static_assert(LDS <= 160 * 1024 && (NB - 1) * (PD + PS) < 64, "");
 };
 
-template <int BM, int BN, int NW, int NB>
+template <int BM, int BN, int NW, int NB, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, BM * BN > 128 * 128 || NB > 2 ? 1 : 2)
 void matmul_mx4_many_kernel(Mx4Args p) {
-  typedef ManyShape<BM, BN, NW, NB> S;
+  typedef ManyShape<BM, BN, NW, NB, WHOLE> S;
   typedef float float16v __attribute__((ext_vector_type(16)));
   constexpr int MI = S::MI, NI = S::NI, PA = S::PA, PB = S::PB, PS = S::PS, SG = S::SG, WORDS = S::WORDS;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[S::LDS];
@@ -459,28 +469,31 @@ void matmul_mx4_many_kernel(Mx4Args p) {
     const unsigned lds_to = lds_at(to + (of_a ? wave * PA + q : BM / 8 + wave * PB + q - PA) * 1024);
     dma16(raw_rsrc((of_a ? x : w) + skip, end), __builtin_amdgcn_readfirstlane(lds_to), c < left ? at : kNone, 0);
   };
-  // Scales, eight bytes a row and stage in a word more, since rows begin at any byte; this
+  // Scales, eight bytes a row and stage, in a word more where rows begin at any byte; this
   // wave's are of x's rows or of the weights'.  The descriptor ends with the last row's last scale, in
-  // whole words.
-  const bool of_x = wave * PS < BM * WORDS / 64;
+  // whole words, of which each is held against it.
+  const bool of_x = wave * PS < BM * WORDS * 4 / S::ONE;
   const unsigned char* const sbase = of_x ? xs : ws;
   const unsigned sodd = (unsigned)reinterpret_cast<uintptr_t>(sbase) & 3;
   const unsigned sld = (unsigned)(of_x ? p.ldxs : p.ldws);
   unsigned vs[PS];
 #pragma unroll
   for (int q = 0; q < PS; ++q) {
-    const unsigned word = (unsigned)((wave * PS + q) * 64 + lane - (of_x ? 0 : BM * WORDS)), row = word / WORDS;
-    vs[q] = ((sodd + row * sld) & ~3u) + 4 * (word - WORDS * row);
+    constexpr unsigned PIECES = WORDS * 256 / S::ONE;  // lanes of a row
+    const unsigned at = (unsigned)((wave * PS + q) * 64 + lane) - (of_x ? 0 : BM * PIECES), row = at / PIECES;
+    vs[q] = ((sodd + row * sld) & ~3u) + S::ONE / 64 * (at - PIECES * row);
   }
   const unsigned send = (sodd + (unsigned)((of_x ? mrows : nrows) - 1) * sld + (unsigned)p.blocks_k + 3) & ~3u;
   // where the scales of stage s lie, whose buffer is `at`
   auto scales_at = [&](int s, unsigned char* at) {
-    return SG == 1 ? at + (BM + BN) * 128 : lds + NB * S::STAGE + (s >> 1 & 1) * S::SCALES;
+    return SG == 1 ? at + (BM + BN) * 128 : lds + NB * S::STAGE + (s / SG & 1) * S::SCALES;
   };
   auto dma_scales = [&](int s, unsigned char* at, int q) {
     const unsigned skip = 8u * (unsigned)s;
-    dma4(raw_rsrc(sbase - sodd + skip, s < nk ? send - skip : 0u),
-         __builtin_amdgcn_readfirstlane(lds_at(scales_at(s, at) + (wave * PS + q) * 256)), vs[q]);
+    const i32x4 rs = raw_rsrc(sbase - sodd + skip, s < nk ? send - skip : 0u);
+    const unsigned to = __builtin_amdgcn_readfirstlane(lds_at(scales_at(s, at) + (wave * PS + q) * S::ONE));
+    if constexpr (WHOLE) dma16(rs, to, vs[q], 0);
+    else dma4(rs, to, vs[q]);
   };
 
   const int xodd = odd_of(xs, lrow, p.ldxs), wodd = odd_of(ws, lrow, p.ldws);  // of rows 32 apart alike
@@ -510,7 +523,7 @@ void matmul_mx4_many_kernel(Mx4Args p) {
     const unsigned* const from =
         reinterpret_cast<const unsigned*>(at + (i < MI ? xword + i * 128 * WORDS : wword + (i - MI) * 128 * WORDS));
     raw[i][0] = from[0];
-    raw[i][1] = from[1];
+    raw[i][1] = WHOLE ? 0u : from[1];
   };
   auto take_scales = [&](int s) {
     // those past the row's end as 0: 255 would make NaN of the zeros there
@@ -554,17 +567,23 @@ void matmul_mx4_many_kernel(Mx4Args p) {
   };
   auto none = [](int) {};
 
-  // prologue: as much as the buffers hold, of the last one half the data
+  // prologue: as much as the buffers hold, of the last one half the data; WHOLE: before it the
+  // scales of the first four stages and the first ones of the next
+  if constexpr (WHOLE) {
+#pragma unroll
+    for (int q = 0; q < PS; ++q) dma_scales(0, lds, q);
+    dma_scales(SG, lds, 0);
+  }
 #pragma unroll
   for (int s = 0; s < NB; ++s) {
 #pragma unroll
     for (int q = 0; q < (s < NB - 1 ? S::PD : HALF); ++q) dma_one(s, lds + s * S::STAGE, q);
-    if (s < NB - 1) {
+    if (!WHOLE && s < NB - 1) {
 #pragma unroll
       for (int q = 0; q < PS; ++q) dma_scales(s, lds + s * S::STAGE, q);
     }
   }
-  static_assert(SG == 1 || NB == 2, "the first wait leaves the second stage's data");
+  static_assert(WHOLE || SG == 1 || NB == 2, "the first wait leaves the second stage's data");
   XTK_WAIT_VM((NB - 2) * S::PER + HALF);
   asm volatile("s_barrier" ::: "memory");
 #pragma unroll
@@ -575,25 +594,31 @@ void matmul_mx4_many_kernel(Mx4Args p) {
   for (int i = 0; i < MI + NI; ++i) read_scale(scales_at(0, lds), i);
   take_scales(0);
 
-  // stage s in `at`, with `last` the buffer before it and `next` the one behind it
-  auto stage = [&](int s, unsigned char* at, unsigned char* last, unsigned char* next, bool odd) {
+  // stage s, of phase s % SG, in `at`, with `last` the buffer before it and `next` the one
+  // behind it.  WHOLE: in the last step, behind whose barrier no wave reads the scales of the
+  // group before this one, and before its data, so that a wait which leaves those leaves
+  // none of them, part of the group behind the next stage's.
+  auto stage = [&](int s, unsigned char* at, unsigned char* last, unsigned char* next, auto phase) {
+    constexpr int PHASE = decltype(phase)::value, AFTER = (PHASE + 1) % SG;
     step(0, at, 1, [&](int n) {
       if (n % EVERY == 0) dma_one(s + NB - 1, last, HALF + n / EVERY);
     });
     step(1, at, 2, [&](int n) {
       if constexpr (SG == 1) {
         if (n < PS) dma_scales(s + NB - 1, last, n);
-      } else {  // of the two stages from the next even one on, in two halves
+      } else if constexpr (SG == 2) {  // of the two stages from the next even one on, in two halves
         constexpr int FIRST = (PS + 1) / 2;
-        if (!odd && n < FIRST) dma_scales(s + 2, at, n);
-        if (odd && n < PS - FIRST) dma_scales(s + 1, at, FIRST + n);
+        if (PHASE == 0 && n < FIRST) dma_scales(s + 2, at, n);
+        if (PHASE == 1 && n < PS - FIRST) dma_scales(s + 1, at, FIRST + n);
       }
     });
     step(2, at, 3, none);
     XTK_WAIT_VM((NB - 2) * S::PER);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const unsigned char* const scales = scales_at(s + 1, next) + (SG == 2 && !odd ? 8 : 0);
+    const unsigned char* const scales = scales_at(s + 1, next) + 8 * AFTER;
     step(3, next, 0, [&](int n) {
+      if constexpr (WHOLE && AFTER < PS)
+        if (n == 0) dma_scales(s + 1 - AFTER + SG, at, AFTER);
       if (n % EVERY == 0) dma_one(s + NB, at, n / EVERY);
       if (n >= PRODUCTS - MI) {
         read_scale(scales, n - (PRODUCTS - MI));
@@ -602,20 +627,22 @@ void matmul_mx4_many_kernel(Mx4Args p) {
     });
     take_scales(s + 1);
   };
-  if constexpr (SG == 2) {
+  unsigned char *at = lds, *last = lds + (NB - 1) * S::STAGE;
+  auto turn = [&](int s, auto phase) {
+    unsigned char* const next = at == lds + (NB - 1) * S::STAGE ? lds : at + S::STAGE;
+    stage(s, at, last, next, phase);
+    last = at;
+    at = next;
+  };
 #pragma unroll 1
-    for (int s = 0; s < nk; s += 2) {
-      stage(s, lds, lds + S::STAGE, lds + S::STAGE, false);
-      if (s + 1 < nk) stage(s + 1, lds + S::STAGE, lds, lds, true);
+  for (int s = 0; s < nk; s += SG) {
+    turn(s, Phase<0>{});
+    if constexpr (SG >= 2) {
+      if (s + 1 < nk) turn(s + 1, Phase<1 % SG>{});
     }
-  } else {
-    unsigned char *at = lds, *last = lds + (NB - 1) * S::STAGE;
-#pragma unroll 1
-    for (int s = 0; s < nk; ++s) {
-      unsigned char* const next = at == lds + (NB - 1) * S::STAGE ? lds : at + S::STAGE;
-      stage(s, at, last, next, false);
-      last = at;
-      at = next;
+    if constexpr (SG == 4) {
+      if (s + 2 < nk) turn(s + 2, Phase<2>{});
+      if (s + 3 < nk) turn(s + 3, Phase<3>{});
     }
   }
   XTK_WAIT_VM(0);
@@ -675,7 +702,8 @@ bool run_many(Mx4Args& a, long long blocks, hipStream_t s) {
   a.d_group = div31(a.group * a.mtiles);
   a.d_width = div31(a.group);
   a.d_last = div31(a.ntiles % a.group ? a.ntiles % a.group : a.group);
-  matmul_mx4_many_kernel<BM, BN, NW, NB><<<a.nwg, 64 * NW, 0, s>>>(a);
+  if (a.whole) matmul_mx4_many_kernel<BM, BN, NW, NB, true><<<a.nwg, 64 * NW, 0, s>>>(a);
+  else matmul_mx4_many_kernel<BM, BN, NW, NB, false><<<a.nwg, 64 * NW, 0, s>>>(a);
   return true;
 }
 
@@ -683,9 +711,9 @@ bool run_many(Mx4Args& a, long long blocks, hipStream_t s) {
 // 1696 to 4096 x 11008 x 4096: a round of tiles costs its start and end and its stages; a
 // wave of few and mid tiles has a W-th of them.  (Measured: 64 x 4096 x 4096 in tiles of 16 x
 // 16 8.5 us, 32 x 32 6.6, 64 x 64 10.2; 256 x 4096 x 4096 in 32 x 64 14.8, 64 x 64 11.9, 128
-// x 128 18.6; 512 x 11008 x 4096 in 128 x 128 with three buffers 32.8, with two and twice
-// the workgroups on a CU 25.8, in 256 x 256 37.5; 1024 x 11008 x 4096 in 128 x 128 46.1, in
-// 256 x 256 40.9.)
+// x 128 15.4; 512 x 11008 x 4096 in 128 x 128 with three buffers 29.4, with two and twice
+// the workgroups on a CU 24.8, in 256 x 256 34.1; 1024 x 11008 x 4096 in 128 x 128 41.7, in
+// 256 x 256 36.1.)
 bool run(Mx4Args& a, long long blocks, hipStream_t s) {
   const int stages = (a.blocks_k + kBlocks - 1) / kBlocks;
   auto tiles = [&](int bm, int bn) { return double(blocks) * double((a.M + bm - 1) / bm) * double((a.N + bn - 1) / bn); };
@@ -700,9 +728,9 @@ bool run(Mx4Args& a, long long blocks, hipStream_t s) {
                         2.4 + rounds(tiles(32, 32), 256) * (2.0 + 0.95 * share(8)),
                         2.3 + rounds(tiles(32, 64), 256) * (2.3 + 0.95 * share(4)),
                         2.5 + rounds(tiles(64, 64), 256) * (3.9 + 1.35 * share(4)),
-                        2.0 + rounds(tiles(128, 128), 256) * (2.5 + 1.0 * stages),
-                        2.0 + rounds(tiles(128, 128), 512) * (2.2 + 1.35 * stages),
-                        2.0 + rounds(tiles(256, 256), 256) * (4.0 + 2.2 * stages)};
+                        2.0 + rounds(tiles(128, 128), 256) * (2.5 + (a.whole ? 0.82 : 1.0) * stages),
+                        2.0 + rounds(tiles(128, 128), 512) * (2.2 + (a.whole ? 1.28 : 1.35) * stages),
+                        2.0 + rounds(tiles(256, 256), 256) * (4.0 + (a.whole ? 1.95 : 2.2) * stages)};
   // large tiles take their rows by DMA only
   switch (std::min_element(us, us + (a.dma ? 7 : 4)) - us) {
     case 0:
@@ -747,12 +775,13 @@ hipError_t launch_matmul_mx4(const xt::Plan& p, void* const* bufs, hipStream_t s
   a.blocks_k = static_cast<int>(m.K / 32);
   a.y_elem = m.y.elem == xt::Elem::F32 ? kF32 : m.y.elem == xt::Elem::F16 ? kF16 : kBF16;
   // DMA takes rows of whole 16 bytes; others go through registers
-  auto pieces = [&](const xt::Access2D& t) {
+  auto pieces = [&](const xt::Access2D& t, int of) {
     const xt::TileAddr& d = t.addr;
-    return reinterpret_cast<uintptr_t>(bufs[t.arg]) % 16 == 0 && t.ld % 16 == 0 && d.c0 % 16 == 0 && d.sx % 16 == 0 &&
-           d.sy % 16 == 0 && d.sz % 16 == 0;
+    return reinterpret_cast<uintptr_t>(bufs[t.arg]) % of == 0 && t.ld % of == 0 && d.c0 % of == 0 && d.sx % of == 0 &&
+           d.sy % of == 0 && d.sz % of == 0;
   };
-  a.dma = pieces(m.x) && pieces(m.w);
+  a.dma = pieces(m.x, 16) && pieces(m.w, 16);
+  a.whole = pieces(m.xs, 4) && pieces(m.ws, 4);
   // what a lane adds to its tile's address has 31 bits
   auto near = [](long long rows, long long ld) { return rows * ld + 256 < (1LL << 31); };
   const int mr = std::min(a.M, 256), nr = std::min(a.N, 256);

@@ -23,8 +23,9 @@
 // but those of a list of at most kList.  Few long rows are dealt to many workgroups in slices,
 // a kernel for each pass (xt::sample_slices has the rule).  Replayed in a graph: 1 row of 32768
 // logits, top-k 50 and top-p, 17 us, without cuts 23; 1 row of 131072, top-p, 31 to 38, top-k
-// 50, 23; 256 rows of 32768 44; 64 rows of 131072, top-p and min-p, 65, of which the largest
-// logit takes 8 (34 MB at 4 TB/s), the bins 18, the lists 18, and what is left of a row 16.
+// 50, 23; 256 rows of 32768 44; 64 rows of 131072, top-p and min-p, 59 to 63, of which the
+// largest logit takes 8 (34 MB at 4 TB/s), the bins 18, the lists 18, and what is left of a row
+// 17.
 #include "launch.h"
 
 #include <algorithm>
