@@ -322,7 +322,8 @@ def pitched_product_program(m, n, k, tm, tn, wide, at, out):
 
 
 @pytest.mark.parametrize("skip", [0, 1, 6])
-@pytest.mark.parametrize("m,n,k,tm,tn", [(6, 96, 96, 3, 48), (40, 64, 160, 20, 64), (512, 384, 288, 256, 192)])
+@pytest.mark.parametrize("m,n,k,tm,tn", [(6, 96, 96, 3, 48), (40, 64, 160, 20, 64), (512, 384, 288, 256, 192),
+                                           (2048, 3840, 640, 1024, 1920), (4096, 4096, 384, 2048, 2048)])
 def test_product_blocks_pitches_and_alignment(m, n, k, tm, tn, skip):
     """Tiles of wider arrays at any byte; what lies beside them, scales of 255, has no effect."""
     import torch

@@ -481,7 +481,9 @@ void matmul_mx4_many_kernel(Mx4Args p) {
   for (int q = 0; q < PS; ++q) {
     constexpr unsigned PIECES = WORDS * 256 / S::ONE;  // lanes of a row
     const unsigned at = (unsigned)((wave * PS + q) * 64 + lane) - (of_x ? 0 : BM * PIECES), row = at / PIECES;
-    vs[q] = ((sodd + row * sld) & ~3u) + S::ONE / 64 * (at - PIECES * row);
+    // WHOLE: every second eight rows have their two pieces the other way round, or four rows'
+    // words would lie in one bank
+    vs[q] = ((sodd + row * sld) & ~3u) + S::ONE / 64 * (WHOLE ? (at ^ row >> 3) & 1 : at - PIECES * row);
   }
   const unsigned send = (sodd + (unsigned)((of_x ? mrows : nrows) - 1) * sld + (unsigned)p.blocks_k + 3) & ~3u;
   // where the scales of stage s lie, whose buffer is `at`
@@ -501,7 +503,8 @@ void matmul_mx4_many_kernel(Mx4Args p) {
   // changed by ks; rows 32 apart have theirs at the same places
   const int arow = (wm * S::WM + lrow) * 128 + piece_of(lrow, 4 * hi) * 16;
   const int brow = S::AB + (wn * S::WN + lrow) * 128 + piece_of(lrow, 4 * hi) * 16;
-  const int xword = (wm * S::WM + lrow) * WORDS * 4 + 4 * hi, wword = (BM + wn * S::WN + lrow) * WORDS * 4 + 4 * hi;
+  const int turned = WHOLE ? (lrow >> 3 & 1) * 16 : 0;
+  const int xword = ((wm * S::WM + lrow) * WORDS * 4 + 4 * hi) ^ turned, wword = ((BM + wn * S::WN + lrow) * WORDS * 4 + 4 * hi) ^ turned;
 
   float16v acc[MI][NI];
 #pragma unroll
@@ -519,9 +522,9 @@ void matmul_mx4_many_kernel(Mx4Args p) {
   auto read_b = [&](const unsigned char* at, int ks, int j) {
     bf[ks & 1][j] = *reinterpret_cast<const uint4v*>(at + (ks * 16 ^ brow) + j * 4096);
   };
-  auto read_scale = [&](const unsigned char* at, int i) {  // at: the stage's first ones
-    const unsigned* const from =
-        reinterpret_cast<const unsigned*>(at + (i < MI ? xword + i * 128 * WORDS : wword + (i - MI) * 128 * WORDS));
+  auto read_scale = [&](const unsigned char* at, int phase, int i) {  // of a stage whose group lies at `at`
+    const int word = i < MI ? xword + i * 128 * WORDS : wword + (i - MI) * 128 * WORDS;
+    const unsigned* const from = reinterpret_cast<const unsigned*>(at + (WHOLE ? word ^ 8 * phase : word + 8 * phase));
     raw[i][0] = from[0];
     raw[i][1] = WHOLE ? 0u : from[1];
   };
@@ -591,7 +594,7 @@ void matmul_mx4_many_kernel(Mx4Args p) {
 #pragma unroll
   for (int j = 0; j < NI; ++j) read_b(lds, 0, j);
 #pragma unroll
-  for (int i = 0; i < MI + NI; ++i) read_scale(scales_at(0, lds), i);
+  for (int i = 0; i < MI + NI; ++i) read_scale(scales_at(0, lds), 0, i);
   take_scales(0);
 
   // stage s, of phase s % SG, in `at`, with `last` the buffer before it and `next` the one
@@ -615,14 +618,14 @@ void matmul_mx4_many_kernel(Mx4Args p) {
     step(2, at, 3, none);
     XTK_WAIT_VM((NB - 2) * S::PER);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const unsigned char* const scales = scales_at(s + 1, next) + 8 * AFTER;
+    const unsigned char* const scales = scales_at(s + 1, next);
     step(3, next, 0, [&](int n) {
       if constexpr (WHOLE && AFTER < PS)
         if (n == 0) dma_scales(s + 1 - AFTER + SG, at, AFTER);
       if (n % EVERY == 0) dma_one(s + NB, at, n / EVERY);
       if (n >= PRODUCTS - MI) {
-        read_scale(scales, n - (PRODUCTS - MI));
-        if (n - (PRODUCTS - MI) < NI) read_scale(scales, MI + n - (PRODUCTS - MI));
+        read_scale(scales, AFTER, n - (PRODUCTS - MI));
+        if (n - (PRODUCTS - MI) < NI) read_scale(scales, AFTER, MI + n - (PRODUCTS - MI));
       }
     });
     take_scales(s + 1);
