@@ -191,6 +191,22 @@ def test_odd_parameters():
     check(x, uniforms(8, 5), top_k=[0, -1, 1, 700, 701, 2**31 - 1, -2**31, 699])
 
 
+@pytest.mark.parametrize("vocab", [9, 700, 3000, 40000, 70000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_only_the_largest_with_cuts(vocab, dtype):
+    """Temperatures that leave the largest logits alone, and infinities, under every cut."""
+    x = logits(6, vocab, dtype, vocab)
+    x[1, [vocab // 3, vocab - 1]] = 50.0
+    x[2, [0, vocab // 2]] = float("inf")
+    x[3, :] = float("inf")
+    x[4, :] = -2.0
+    x[5, 1:] = float("-inf")
+    heat = [0.0, 0.0, 1.0, 2.0, -1.0, 0.5]
+    for options in ({"top_k": 50}, {"top_k": 1000, "min_p": 0.5}, {"top_p": 0.5}, {"top_k": 3, "top_p": 0.5, "min_p": 1.0}):
+        for seed in (1, 2):
+            check(x, uniforms(6, seed), dtype, temperature=heat, **options)
+
+
 def test_every_token_can_be_drawn():
     """u at and next to each border of a few exact weights."""
     import torch

@@ -1524,7 +1524,10 @@ GemmCover gemm_cover(const Plan& p, int64_t w, bool is_m) {
 // has at least a tile for each wave, and two such rounds are left whole (139 keys of 160
 // columns: 10.1 us, in two parts 11.1).  One of many rows has four tiles, and the keys
 // are not split below 1024, where joining the parts costs what they save (577 keys, 160
-// tiles: whole 20.4 us, halves 25.7).
+// tiles: whole 20.4 us, halves 25.7).  Trees, whose rows are few, are split from 512 keys on,
+// and up to 16 tiles of them into parts of two tiles of keys (6 tiles over 595 keys in four
+// 13.6 -> 10.8 us, 8 over 512 15.1 -> 12.7, 8 over 1024 in eight 16.4 -> 15.0, 64 over 700 in two
+// 20.0 -> 19.2; 32 over 2000 in fifteen 28, in seven 25.8).
 int attend_splits(const Plan& p) {
   const AttendPlan& a = p.attend;
   const int64_t rows = a.heads * a.rows;
@@ -1534,11 +1537,13 @@ int attend_splits(const Plan& p) {
   // A causal window leaves only so many keys, whatever the cache holds.
   const bool band = (a.causal || a.extra[6].arg >= 0) && a.window && a.extra[3].arg < 0;
   const int64_t keys = band ? std::min(a.keys, a.window + a.rows) : a.keys;
-  const bool half = a.extra[6].arg >= 0 && rows <= kAttendHalfRows;
+  const bool tree = a.extra[6].arg >= 0, half = tree && rows <= kAttendHalfRows;
   const int fit = few ? (a.d > 64 ? 1 : 2) : a.d > 128 ? 1 : a.d > 64 || half ? 2 : 3;  // workgroups on a compute unit
   const double want = 256 * fit / tiles;
   const int64_t round = a.d > 160 ? 64 : 128;  // keys of few rows that a workgroup's waves take at a time
-  const int64_t most = few ? (keys > 2 * round ? (keys + round - 1) / round : 1) : keys < 1024 ? 1 : keys / 256;
+  int64_t most = 1;
+  if (few) most = keys > 2 * round ? (keys + round - 1) / round : 1;
+  else if (keys >= (tree ? 512 : 1024)) most = keys / (tree && tiles <= 16 ? 128 : 256);
   if (want < 2 || most < 2) return 1;
   return static_cast<int>(std::min<double>(std::min<double>(want, double(most)), 256));
 }
