@@ -987,9 +987,9 @@ def matmul_q4(value, weight, scales, *, row_scale=None, dtype: DType = float32):
 
 def mx4_scale(value):
     """(R, C / 32) int8 scales of rows in microscaled 4-bit floating point: of each
-    block of 32 neighbours the byte e + 127 (0 to 254 unsigned) of the power 2**e that the block's values are
-    multiples of, e = floor(log2(largest magnitude)) - 2, at least -127; 0 for a
-    block of zeros, 255 for one with an infinity or NaN."""
+    block of 32 neighbours the byte e + 127 (0 to 254 unsigned) of the power 2**e that
+    the block's values are multiples of, e = floor(log2(largest magnitude)) - 2, at
+    least -127; 0 for a block of zeros, 255 for one with an infinity or NaN."""
     return _trace("mx4_scale").mx4_scale(value)
 
 
@@ -1024,12 +1024,12 @@ def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=N
     leave nothing but themselves.  Tokens are ordered by logit, the largest first,
     equal ones by index.  Of the order's beginning remain: the first `top_k` tokens
     (0 or less: all); of those the fewest whose weights reach `top_p` of their total
-    (1 or more, and NaN: all; at least one); and those whose weight is at least `min_p` of the largest
-    (above 1: as 1; NaN: as 0).  The result is the first whose weights, summed in that order, exceed
-    `uniform` times the sum of what remains: `uniform` is held within 0 and what is just
-    below 1, NaN as 0.  Weights and sums are held in 64 bits.  Logits of NaN
-    count as minus infinity, and a row of nothing else gives -1.  All but the logits
-    are (R, 1) tiles, float32 or, top_k, int32."""
+    (1 or more, and NaN: all; at least one); and those whose weight is at least
+    `min_p` of the largest (above 1: as 1; NaN: as 0).  The result is the first whose
+    weights, summed in that order, exceed `uniform` times the sum of what remains:
+    `uniform` is held within 0 and what is just below 1, NaN as 0.  Weights and sums
+    are held in 64 bits.  Logits of NaN count as minus infinity, and a row of nothing
+    else gives -1.  All but the logits are (R, 1) tiles, float32 or, top_k, int32."""
     return _trace("sample").sample(logits, uniform, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
 

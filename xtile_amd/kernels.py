@@ -483,7 +483,8 @@ def masked_attention(batch: int, kv_heads: int, group: int, nq: int, nk: int, d:
     [batch, nk, kv_heads * d]; between v and the result, where asked for: slopes
     (kv_heads, group) float32; start, length, prefix (batch, 1) int32; the documents
     of the queries (batch, nq) and of the keys (batch, nk) int32; the parents of
-    drafted tokens (batch, nq) int32.  Their meaning is `attend`'s.  `scale` defaults to d ** -0.5."""
+    drafted tokens (batch, nq) int32, at most 64 of them.  Their meaning is `attend`'s.
+    `scale` defaults to d ** -0.5."""
     if min(batch, kv_heads, group, nq, nk, d) < 1:
         raise ValueError("masked_attention sizes must be positive")
     heads = kv_heads * group
