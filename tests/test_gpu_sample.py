@@ -284,3 +284,22 @@ def test_streams_and_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert y.view(-1).tolist() == want(new, nu.view(-1).tolist(), top_p=0.9)
+
+
+@pytest.mark.parametrize("rows,vocab", [(7, 70000), (3, 700)], ids=["sliced", "alone"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("end", ["hidden", "far"])
+def test_top_k_past_the_last_weight(rows, vocab, dtype, end):
+    """Top-k reaches into tokens without a weight, in the bin of the last one that it takes; with
+    uniforms of every kind and the other cuts."""
+    inf, nan = float("inf"), float("nan")
+    assert bool(xt.workspace(K.sample(rows, vocab, DTYPES[dtype], top_k=True))) == (vocab > 10000)
+    x = logits(rows, vocab, dtype, vocab, 1.0)
+    few = vocab // 70
+    x[:, ::70] = -inf if end == "hidden" else -2000.0  # whose weight is 0 in 64 bits too
+    below = float(np.nextafter(np.float32(1), np.float32(0)))
+    u = [1.0, 2.0, inf, nan, below, 0.0, 0.5][:rows]
+    for k in (vocab - few // 2, vocab - 1, vocab - few, vocab - few + 1):
+        for options in ({}, {"top_p": 0.9}, {"min_p": 0.001}, {"top_p": below, "min_p": 1e-30}):
+            check(x, u, dtype, top_k=k, **options)
+            check(x, u[::-1], dtype, top_k=k, **options)

@@ -954,9 +954,13 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs p
     if (a.some(p.vocab)) {
       const int b = bin_with<kSliceThreads, unsigned>(count, (unsigned)a.top_k, found, turn);
       total = high = sum[b];
-      low = before_bin(b) + 1;
-      if (count[b] == (unsigned)a.top_k) low = high;
-      else run[0] = run_of(b, b);
+      // the whole bin, or one without a weight, of which no token adds to those before it
+      if (count[b] == (unsigned)a.top_k || before_bin(b) == high) {
+        low = high;
+      } else {
+        low = before_bin(b) + 1;
+        run[0] = run_of(b, b);
+      }
     }
     if (a.cuts()) {
       int lo, hi;
