@@ -303,3 +303,81 @@ def test_top_k_past_the_last_weight(rows, vocab, dtype, end):
         for options in ({}, {"top_p": 0.9}, {"min_p": 0.001}, {"top_p": below, "min_p": 1e-30}):
             check(x, u, dtype, top_k=k, **options)
             check(x, u[::-1], dtype, top_k=k, **options)
+
+
+def time_of(program, bufs):
+    """Microseconds of a launch, from replays of a graph of ten."""
+    import torch
+
+    xt.launch(program, *bufs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(10):
+            xt.launch(program, *bufs)
+    times = []
+    for _ in range(7):
+        first, last = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        first.record()
+        graph.replay()
+        last.record()
+        torch.cuda.synchronize()
+        times.append(first.elapsed_time(last) * 100)
+    return sorted(times)[3]
+
+
+def weightless_rows(rows, vocab, dtype, kind):
+    """Rows of which few tokens have a weight: (logits, temperature)."""
+    x = logits(rows, vocab, dtype, vocab)
+    if kind == "masked":
+        x[:, 30:] = -float("inf")
+    return x, {"masked": 1.0, "greedy": 0.0, "cold": 0.02}[kind]
+
+
+@pytest.mark.parametrize("kind", ["masked", "greedy", "cold"])
+@pytest.mark.parametrize("rows,vocab,dtype", [(2, 131072, "f32"), (3, 20000, "bf16")])
+def test_top_k_of_more_than_have_a_weight(rows, vocab, dtype, kind):
+    """The same tokens as without top-k, in little more time: the kernel need not tell tokens
+    without a weight apart."""
+    x, heat = weightless_rows(rows, vocab, dtype, kind)
+    u = uniforms(rows, 3)
+    for options in ({}, {"top_p": 0.9, "min_p": 0.01}):
+        for k in (50, 256, 257, 1000):
+            check(x, u, dtype, temperature=heat, top_k=k, **options)
+            assert run(x, u, dtype, temperature=heat, top_k=k, **options) == run(x, u, dtype, temperature=heat, **options)
+
+
+@pytest.mark.parametrize("k", [50, 1000])
+@pytest.mark.parametrize("kind", ["masked", "greedy", "cold"])
+@pytest.mark.parametrize("rows,vocab,dtype", [(2, 131072, "f32"), (3, 20000, "bf16")])
+def test_time_of_top_k_of_more_than_have_a_weight(rows, vocab, dtype, kind, k):
+    """Less than four times that without top-k."""
+    import torch
+
+    x, heat = weightless_rows(rows, vocab, dtype, kind)
+    y = torch.empty(rows, 1, dtype=torch.int32, device="cuda")
+    bufs = [x.cuda(), column(uniforms(rows, 3), rows, torch.float32), column(heat, rows, torch.float32)]
+    without = time_of(K.sample(rows, vocab, DTYPES[dtype], temperature=True), [*bufs, y])
+    with_it = time_of(K.sample(rows, vocab, DTYPES[dtype], temperature=True, top_k=True), [*bufs, column(k, rows, torch.int32), y])
+    assert with_it < 4 * without, (with_it, without)
+
+
+@pytest.mark.parametrize("vocab", [9, 66001])
+def test_distances_past_the_range(vocab):
+    """Logits farther apart than float's largest, whose weights are not 0 at the temperatures above
+    it: 2^-3 for the farthest at 3.3e38.  At 1e36 those of the third token on are below 2^-400,
+    which moves no sum: a uniform of 1, held just below it, gives the last one before them."""
+    x = logits(4, vocab, "f32", vocab).abs().neg() * 1e37
+    x[:, 0], x[:, 1], x[:, 2:4] = 3.3e38, 3.2e38, -3.3e38
+    if vocab > 9:
+        x[:, 5000:] = -float("inf")
+    below = np.nextafter(1.0, 0.0)
+    for heat in (3.3e38, 1e38, 1e36):
+        for k in (2, 4, 9, 200, 1000):
+            for options in ({}, {"top_p": 0.9}, {"min_p": 0.2}):
+                asked = {"temperature": heat, "top_k": min(k, vocab), **options}
+                for u in ([0.0, 0.5, 0.9, 1.0], [0.3, 0.99, 0.75, 0.125]):
+                    w = [ref.sample(x[r].double().numpy(), min(np.float64(np.float32(u[r])), below),
+                                    **{n: np.float32(v) if n != "top_k" else v for n, v in asked.items()}) for r in range(4)]
+                    assert run(x, u, "f32", **asked) == w
+                    assert run(x, u, "f32", without_workspace=True, **asked) == w

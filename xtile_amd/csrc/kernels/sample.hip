@@ -263,6 +263,13 @@ struct Weights {
   }
   __device__ __forceinline__ int bin_of_many(float x) const { return (int)fminf((top - x) * per_bin, (float)(kBins - 1)); }
 
+  // The first tokens of the order, all that have a weight among them, from running counts: those
+  // before the last bin, which begins where weights are a quarter.  At temperatures near float's
+  // largest it begins at distances past float's range, and may have any.
+  __device__ __forceinline__ int weighted(const unsigned* running, int vocab) const {
+    return only_top || per_bin >= 1e-35f ? (int)running[kBins - 2] : vocab;
+  }
+
   // A logit that no logit of bins up to `last` is below.
   __device__ __forceinline__ float least_of(int last) const {
     if (last >= kBins - 1 || !(per_bin > 0.0f)) return -__builtin_inff();
@@ -592,9 +599,10 @@ __device__ __forceinline__ void search_list(List& s, int n, u64 base_sum, u64 va
   __syncthreads();
 }
 
-// The drawn token from a sorted list of the first n tokens, which has all that remains.
+// The drawn token from a sorted list of the first n tokens, which has all that remains: top-k of
+// them, or all that have a weight.
 __device__ __forceinline__ int pick_few(List& s, int n, const Asked& a) {
-  const u64 total = s.weight[a.top_k - 1];
+  const u64 total = s.weight[min(a.top_k, n) - 1];
   u64 kept = total;
   if (a.least > 0) {  // min-p: the running sum before the first token that it does not keep
     if (threadIdx.x == 0) s.n = n;
@@ -671,7 +679,8 @@ __device__ __forceinline__ u64 search(Shared& s, const X& logits, const Weights&
   if constexpr (BY_COUNT) bin = bin_with<kThreads, unsigned>(s.count, (unsigned)value, s.found, l.turn);
   else bin = bin_with<kThreads, u64>(s.sum, value, s.found, l.turn);
   const unsigned with = s.count[bin];
-  if (BY_COUNT && with == (unsigned)value) return s.sum[bin];  // whose token is last is not asked
+  // whose token is last is not asked, nor which of those that add nothing
+  if (BY_COUNT && (with == (unsigned)value || s.sum[bin] == (bin ? s.sum[bin - 1] : 0))) return s.sum[bin];
   if (bin < l.lo || bin > l.hi) {
     int shift = kIndexBits + 32;  // bits of the order not yet looked at
     u64 prefix = 0, base_sum = bin ? s.sum[bin - 1] : 0;
@@ -736,7 +745,8 @@ __device__ __forceinline__ int pick(Shared& s, const X& logits, int vocab, const
   Listed l;
   if (a.few(vocab)) {
     scan<kThreads, false, true>(nullptr, s.count, s.mem);
-    const int bin = bin_with<kThreads, unsigned>(s.count, (unsigned)a.top_k, s.found, l.turn);
+    const int k = min(a.top_k, w.weighted(s.count, vocab));
+    const int bin = bin_with<kThreads, unsigned>(s.count, (unsigned)k, s.found, l.turn);
     const int with = (int)s.count[bin];
     if (with <= kList) {
       make_list(s, logits, w, 0, bin, kIndexBits + 32, 0, with);
@@ -946,7 +956,8 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs p
   Run run[3] = {{0, 0, 0, 0, 0}, {0, 0, 0, 0, 0}, {0, 0, 0, 0, 0}};
   u64 total = sum[kBins - 1];
   if (few) {
-    run[0] = run_of(0, bin_with<kSliceThreads, unsigned>(count, (unsigned)a.top_k, found, turn));
+    const int k = min(a.top_k, w.weighted(count, p.vocab));
+    run[0] = run_of(0, bin_with<kSliceThreads, unsigned>(count, (unsigned)k, found, turn));
   } else {
     // the least and the most that top-k, top-p and min-p leave
     u64 low = total, high = total;
