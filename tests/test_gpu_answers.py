@@ -269,6 +269,24 @@ def test_a_product_with_a_result_past_32_bits():
             assert bool((np.abs(y[at, to].cpu().double().numpy() - want) <= far).all())
 
 
+def test_a_product_of_more_small_tiles_than_one_launch_has():
+    """Larger tiles take it: weights beside 16-byte places, which the largest do not take."""
+    import torch
+
+    n, k, last = 1 << 28, 32, 40
+    rng = np.random.default_rng(3)
+    w = int8((n * k // 2 + 16,))[1 : 1 + n * k // 2].view(n, k // 2)
+    ws = torch.full((n, 1), 127, dtype=torch.int8, device="cuda")
+    w[-last:] = torch.from_numpy(rng.integers(-128, 128, (last, k // 2)).astype(np.int8)).cuda()
+    x, xs = torch.from_numpy(rng.integers(-128, 128, (1, k // 2)).astype(np.int8)).cuda(), ws[:1].clone()
+    y = torch.full((1, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    print("[gpu] matmul_mx4 1 x 2^28 x 32", flush=True)
+    xt.launch(K.matmul_mx4(1, n, k, out=xt.bfloat16), x, xs, w, ws, y)
+    want, far = ref.matmul_mx4(of_mx4(x, xs), of_mx4(w[-last:], ws[-last:]))
+    assert bool((np.abs(y[:, -last:].cpu().double().numpy() - want) <= far + 2.0**-8 * np.abs(want)).all())
+    assert not bool(y[:, :-last].any())
+
+
 @pytest.mark.parametrize("nq,g", [(2, 1), (8, 5), (40, 4)])
 def test_trees_at_the_end_of_keys_past_32_bits(nq, g):
     """Keys of more than 4 GiB: the last ones, against the same on their own."""

@@ -727,7 +727,7 @@ bool run(Mx4Args& a, long long blocks, hipStream_t s) {
   const bool eight = small <= 512;
   const double by_16 = 2.2 + (eight ? std::max(1.0 + 0.9 * share(8), small / 256 * (0.5 + 0.78 * share(8)))
                                     : std::max(1.0 + 0.55 * share(4), small / 256 * (0.37 + 0.3 * share(4))));
-  const double us[7] = {by_16,
+  double us[7] = {by_16,
                         2.4 + rounds(tiles(32, 32), 256) * (2.0 + 0.95 * share(8)),
                         2.3 + rounds(tiles(32, 64), 256) * (2.3 + 0.95 * share(4)),
                         2.5 + rounds(tiles(64, 64), 256) * (3.9 + 1.35 * share(4)),
@@ -735,17 +735,27 @@ bool run(Mx4Args& a, long long blocks, hipStream_t s) {
                         2.0 + rounds(tiles(128, 128), 512) * (2.2 + (a.whole ? 1.28 : 1.35) * stages),
                         2.0 + rounds(tiles(256, 256), 256) * (4.0 + (a.whole ? 1.95 : 2.2) * stages)};
   // large tiles take their rows by DMA only
-  switch (std::min_element(us, us + (a.dma ? 7 : 4)) - us) {
-    case 0:
-      if (a.M <= 8) return eight ? run_few<8, 8>(a, blocks, s) : run_few<8, 4>(a, blocks, s);
-      return eight ? run_few<16, 8>(a, blocks, s) : run_few<16, 4>(a, blocks, s);
-    case 1: return run_mid<1, 1, 8>(a, blocks, s);
-    case 2: return run_mid<1, 2, 4>(a, blocks, s);
-    case 3: return run_mid<2, 2, 4>(a, blocks, s);
-    case 4: return run_many<128, 128, 4, 3>(a, blocks, s);
-    case 5: return run_many<128, 128, 4, 2>(a, blocks, s);
-    default: return run_many<256, 256, 8, 2>(a, blocks, s);
+  const int kernels = a.dma ? 7 : 4;
+  auto launch = [&](int kernel) {
+    switch (kernel) {
+      case 0:
+        if (a.M <= 8) return eight ? run_few<8, 8>(a, blocks, s) : run_few<8, 4>(a, blocks, s);
+        return eight ? run_few<16, 8>(a, blocks, s) : run_few<16, 4>(a, blocks, s);
+      case 1: return run_mid<1, 1, 8>(a, blocks, s);
+      case 2: return run_mid<1, 2, 4>(a, blocks, s);
+      case 3: return run_mid<2, 2, 4>(a, blocks, s);
+      case 4: return run_many<128, 128, 4, 3>(a, blocks, s);
+      case 5: return run_many<128, 128, 4, 2>(a, blocks, s);
+      default: return run_many<256, 256, 8, 2>(a, blocks, s);
+    }
+  };
+  // the next where one's tiles exceed a launch
+  for (int i = 0; i < kernels; ++i) {
+    double* const least = std::min_element(us, us + kernels);
+    if (launch(static_cast<int>(least - us))) return true;
+    *least = HUGE_VAL;
   }
+  return false;
 }
 
 }  // namespace
