@@ -305,6 +305,24 @@ def test_top_k_past_the_last_weight(rows, vocab, dtype, end):
             check(x, u[::-1], dtype, top_k=k, **options)
 
 
+@pytest.mark.parametrize("vocab,shift", [(9, 50), (2048, 50), (2049, 49), (1 << 17, 44), ((1 << 17) + 1, 43), (1 << 22, 39)])
+def test_units_of_weights(vocab, shift):
+    """A tail of one unit each, rounded up from 2**-0.99 of one, counts; of 2**-1.01 nothing does."""
+    import torch
+
+    below = float(np.nextafter(np.float32(1), np.float32(0)))
+    for octaves, unit in ((shift + 0.99, 1), (shift + 1.01, 0)):
+        x = torch.full((4, vocab), -octaves * np.log(2.0))
+        x[:, 0] = 0.0
+        u = [1.0, below, 0.5, 0.0]
+        total = 2**shift + unit * (vocab - 1)
+        # token t > 0 ends at 2**shift + t units; the first that exceeds u of them all, in whole numbers
+        past = [total - 1 if v >= 1 else int(v * 2**24) * total // 2**24 for v in u]
+        tokens = [max(0, p + 1 - 2**shift) for p in past]
+        assert run(x, u, "f32") == tokens
+        assert run(x, u, "f32", without_workspace=True) == tokens
+
+
 def time_of(program, bufs):
     """Microseconds of a launch, from replays of a graph of ten."""
     import torch

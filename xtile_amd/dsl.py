@@ -1027,8 +1027,14 @@ def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=N
     (1 or more, and NaN: all; at least one); and those whose weight is at least
     `min_p` of the largest (above 1: as 1; NaN: as 0).  The result is the first whose
     weights, summed in that order, exceed `uniform` times the sum of what remains:
-    `uniform` is held within 0 and what is just below 1, NaN as 0.  Weights and sums
-    are held in 64 bits.  Logits of NaN count as minus infinity, and a row of nothing
+    `uniform` is held within 0 and what is just below 1, NaN as 0.
+
+    Weights are whole numbers of units in 64 bits, and their sums exact: 2**S units are
+    the largest's, S = 61 less the bits of V - 1 and at most 50 (44 for 131072 logits).
+    Each is off by half a unit and 3e-13 of itself at most, so a token below half a
+    unit is never drawn.  V such tokens are less than 2**-24 of the largest's weight,
+    the step of a float32 uniform next to 1, up to 2**19 logits, and 2**-18 at 2**22,
+    the most that the kernel takes.  Logits of NaN count as minus infinity, and a row of nothing
     else gives -1.  All but the logits are (R, 1) tiles, float32 or, top_k, int32."""
     return _trace("sample").sample(logits, uniform, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
