@@ -74,6 +74,19 @@ def test_work_of_plans():
     assert p["flops"] == 4 * 64 * 2 * 3 * 2 * 5 * 77
 
 
+def splits_of(kv_heads, nk, d=128):
+    kernel = xt.plan(K.masked_attention(1, kv_heads, 4, 16, nk, d, start=True, length=True, parents=True))["kernel"]
+    return int(kernel.split("splits=")[1].split()[0]) if "splits=" in kernel else 1
+
+
+@pytest.mark.parametrize("kv_heads,nk,splits", [
+    (1, 300, 1), (8, 512, 4), (8, 1024, 8), (8, 3000, 23), (4, 4096, 32), (1, 8192, 64),  # two tiles of keys each
+    (8, 4096, 16), (4, 8192, 32), (8, 8192, 32), (12, 4096, 16), (16, 2048, 8)])          # four
+def test_splits_of_trees(kv_heads, nk, splits):
+    """Few tiles over short caches have small parts, until the workgroups are many."""
+    assert splits_of(kv_heads, nk) == splits
+
+
 def test_slices_of_sampled_rows():
     def slices(*a, **kw):
         return xt.workspace(K.sample(*a, **kw)) // 123248

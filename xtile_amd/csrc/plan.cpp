@@ -1524,10 +1524,13 @@ GemmCover gemm_cover(const Plan& p, int64_t w, bool is_m) {
 // has at least a tile for each wave, and two such rounds are left whole (139 keys of 160
 // columns: 10.1 us, in two parts 11.1).  One of many rows has four tiles, and the keys
 // are not split below 1024, where joining the parts costs what they save (577 keys, 160
-// tiles: whole 20.4 us, halves 25.7).  Trees, whose rows are few, are split from 512 keys on,
-// and up to 16 tiles of them into parts of two tiles of keys (6 tiles over 595 keys in four
-// 13.6 -> 10.8 us, 8 over 512 15.1 -> 12.7, 8 over 1024 in eight 16.4 -> 15.0, 64 over 700 in two
-// 20.0 -> 19.2; 32 over 2000 in fifteen 28, in seven 25.8).
+// tiles: whole 20.4 us, halves 25.7).  Trees, whose rows are few, are split from 512 keys on (64
+// tiles over 700 keys in two 20.0 -> 19.2), and up to 16 tiles of them into parts of two tiles
+// of keys where that makes up to 192 workgroups, more of which cost the join what they save
+// (parts of two tiles of keys against four, 128 columns: 4 tiles over 4096 keys 13.6 us and 14.4,
+// over 8192 16.2 and 15.1; 8 over 1024 12.1 and 12.5, over 3000 15.0 and 15.5, over 4096 15.5 and
+// 14.9, over 8192 19.0 and 16.7; 12 over 2048 14.3 and 14.4, over 4096 18.2 and 15.7; 32 over 2000
+// 28 and 25.8).
 int attend_splits(const Plan& p) {
   const AttendPlan& a = p.attend;
   const int64_t rows = a.heads * a.rows;
@@ -1543,7 +1546,7 @@ int attend_splits(const Plan& p) {
   const int64_t round = a.d > 160 ? 64 : 128;  // keys of few rows that a workgroup's waves take at a time
   int64_t most = 1;
   if (few) most = keys > 2 * round ? (keys + round - 1) / round : 1;
-  else if (keys >= (tree ? 512 : 1024)) most = keys / (tree && tiles <= 16 ? 128 : 256);
+  else if (keys >= (tree ? 512 : 1024)) most = keys / (tree && tiles <= 16 && tiles * double(keys) <= 192 * 128 ? 128 : 256);
   if (want < 2 || most < 2) return 1;
   return static_cast<int>(std::min<double>(std::min<double>(want, double(most)), 256));
 }
