@@ -38,7 +38,9 @@
 // 4 x 16 rows on 8 key heads of 128 over 4096 keys take 15 us, most of it a chain of waits:
 // two launches 4, what the first loads wait for 4, four tiles 4, the join 3.  4 x 32 rows in
 // 16 sequences of up to 8192 keys take 101 us, 0.5 PFLOP/s and 3.6 TB/s; 8 x 64 rows over
-// 131072 keys, capped, 356 to 376, 0.73 to 0.78 PFLOP/s.
+// 131072 keys, capped, 356 to 376, 0.73 to 0.78 PFLOP/s.  Weights are rounded to the values' type,
+// as other rows' are: against 64 bits these three are off by 0.0020, 0.0022 and (f16) 0.00028,
+// with weights of 32 bits by 0.0017, 0.0017 and 0.00021, most of it the result's own rounding.
 //
 // Many rows are bound by the arithmetic of the softmax (4096 tokens, 32 heads of 128
 // columns on 8 key heads, causal, capped: 166 to 181 us, 0.76 to 0.83 PFLOP/s; 158 without

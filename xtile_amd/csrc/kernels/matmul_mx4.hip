@@ -728,12 +728,12 @@ bool run(Mx4Args& a, long long blocks, hipStream_t s) {
   const double by_16 = 2.2 + (eight ? std::max(1.0 + 0.9 * share(8), small / 256 * (0.5 + 0.78 * share(8)))
                                     : std::max(1.0 + 0.55 * share(4), small / 256 * (0.37 + 0.3 * share(4))));
   double us[7] = {by_16,
-                        2.4 + rounds(tiles(32, 32), 256) * (2.0 + 0.95 * share(8)),
-                        2.3 + rounds(tiles(32, 64), 256) * (2.3 + 0.95 * share(4)),
-                        2.5 + rounds(tiles(64, 64), 256) * (3.9 + 1.35 * share(4)),
-                        2.0 + rounds(tiles(128, 128), 256) * (2.5 + (a.whole ? 0.82 : 1.0) * stages),
-                        2.0 + rounds(tiles(128, 128), 512) * (2.2 + (a.whole ? 1.28 : 1.35) * stages),
-                        2.0 + rounds(tiles(256, 256), 256) * (4.0 + (a.whole ? 1.95 : 2.2) * stages)};
+                  2.4 + rounds(tiles(32, 32), 256) * (2.0 + 0.95 * share(8)),
+                  2.3 + rounds(tiles(32, 64), 256) * (2.3 + 0.95 * share(4)),
+                  2.5 + rounds(tiles(64, 64), 256) * (3.9 + 1.35 * share(4)),
+                  2.0 + rounds(tiles(128, 128), 256) * (2.5 + (a.whole ? 0.82 : 1.0) * stages),
+                  2.0 + rounds(tiles(128, 128), 512) * (2.2 + (a.whole ? 1.28 : 1.35) * stages),
+                  2.0 + rounds(tiles(256, 256), 256) * (4.0 + (a.whole ? 1.95 : 2.2) * stages)};
   // large tiles take their rows by DMA only
   const int kernels = a.dma ? 7 : 4;
   auto launch = [&](int kernel) {

@@ -10,10 +10,13 @@
 // largest magnitude meets by two DPP steps; the conversions are the hardware's, two values
 // at a time with the scale applied.
 //
-// Results are stored past the caches, which otherwise drop what is still to be read for them:
-// 8192 rows of 4096 in bf16 with their values 24.7 us, 6.2 TB/s, against 31.1; 11008 such rows
-// back to fp16 21.6 us, 5.3 TB/s, against 25.6.  Where no values are stored the rows are read
-// past them: the 8192 rows 17.7 us, 4.8 TB/s, against 19.3; with values that costs 4 us.
+// Results are stored past the caches, which otherwise drop for them what is still to be read.
+// In a graph over 3 sets of buffers, whose inputs the Infinity Cache then keeps, and over 24,
+// whose inputs come from HBM: 8192 rows of 4096 in bf16 with their values 24.3 us (6.2 TB/s) and
+// 28.0 (5.4), stored through the caches 31.6 and 31.3; 11008 such rows back to fp16 18 to 19 us
+// and 23.0 (4.9 TB/s), through them 25 and 24.3.  Where no values are stored the rows are read
+// past them too: the 8192 rows 17.7 us and 19.0 (4.5 TB/s), read through them 17.3 and 19.8; with
+// values that costs 3 us of the 24.3 and saves 0.7 of the 28.0.
 #include "common.h"
 #include "launch.h"
 
@@ -196,9 +199,10 @@ void run_of(const Mx4RowsArgs& a, bool back, hipStream_t s) {
   else quantize_mx4_kernel<ELEM, U, false><<<wgs, 256, 0, s>>>(a);
 }
 
-// One unit a thread for few of them: 64 rows of 4096 in 2.2 us against 2.5 with two, 1024 in
-// f32 5.8 against 6.1; the large ones above with one 27.1 against 24.7 us and 22.9 against
-// 21.6, with four 26.4 and 20.5 but 3.3 for the 64 rows.
+// One unit a thread for few of them: 64 rows of 4096 with values in 2.5 us against 2.8 with two,
+// 1024 in f32 8.5 against 8.9.  The large ones above over 3 sets of buffers: with one 26 us
+// against 24.3, without values 20 against 17.7, back to fp16 21.3 against 18 to 19; with four 24.4, 18.3
+// and 18.9.
 template <int ELEM>
 void run(const Mx4RowsArgs& a, bool back, hipStream_t s) {
   if (a.units <= 1u << 19) run_of<ELEM, 1>(a, back, s);

@@ -28,7 +28,8 @@
 // logits, top-k 50 and top-p, 17 us, without cuts 23; 1 row of 131072, top-p, 31 to 38, top-k
 // 50, 23; 256 rows of 32768 44; 64 rows of 131072, top-p and min-p, 59 to 63, of which the
 // largest logit takes 8 (34 MB at 4 TB/s), the bins 18, the lists 18, and what is left of a row
-// 17.
+// 17.  Where few tokens have a weight most logits are added to one bin, one after the other: of
+// 1 row of 131072 23 to 27, of 64 of them 86 to 96, and with top-k, a workgroup a row, 130 to 262.
 #include "launch.h"
 
 #include <algorithm>

@@ -1011,8 +1011,8 @@ def dequantize_mx4(value, scale, *, dtype: DType = float32):
 def matmul_mx4(value, value_scale, weight, weight_scale, *, dtype: DType = float32):
     """`value @ weight.T` of rows in microscaled 4-bit floating point: value (M, K / 2)
     and weight (N, K / 2) with scales (M, K / 32) and (N, K / 32), as quantize_mx4
-    and mx4_scale give them.  Sums are held in 32 bits; a row with a scale of 255 is
-    NaN."""
+    and mx4_scale give them.  Sums are held in 32 bits (parts of one past float32's largest
+    make infinities or NaN); a row with a scale of 255 is NaN."""
     return _trace("matmul_mx4").matmul_mx4(value, value_scale, weight, weight_scale, dtype=dtype)
 
 
@@ -1052,7 +1052,9 @@ def attend(q, k, v, *, scale, cap=None, causal=False, window=None, slopes=None, 
     rows), k_docs (1, keys), int32); and j < prefix (a (1, 1) int32 tile), or
     j <= p if `causal` and p - j < window if `window` is given.  Rows that see
     nothing, or only scores of minus infinity, are 0.  What hidden keys and
-    values hold, NaN included, has no effect.
+    values hold, NaN included, has no effect.  Scores, maxima, totals and sums are held
+    in 32 bits; a softmax weight is rounded to v's type, in its product with v and in the
+    total alike.
 
     With `parents`, a (1, rows) int32 tile, the rows are a tree of drafted tokens
     that follows the keys before `start`, and key start + u is drafted token u's.
