@@ -191,6 +191,21 @@ def test_odd_parameters():
     check(x, uniforms(8, 5), top_k=[0, -1, 1, 700, 701, 2**31 - 1, -2**31, 699])
 
 
+@pytest.mark.parametrize("dtype,vocab", [("f32", 70000), ("bf16", 70000), ("bf16", 20000)])
+def test_odd_parameters_of_long_rows(dtype, vocab):
+    """The same of rows dealt to slices, and of ones kept in registers."""
+    inf, nan = float("inf"), float("nan")
+    x = logits(8, vocab, dtype, 1)
+    assert (xt.workspace(K.sample(8, vocab, DTYPES[dtype])) > 0) == (vocab == 70000)
+    u = [0.0, -1.0, 1.0, 2.0, nan, inf, -inf, float(np.nextafter(np.float32(1), np.float32(0)))]
+    for options in ({}, {"top_k": 40}, {"top_k": 9000}, {"top_p": 0.5}, {"min_p": 0.01}, {"top_k": 9000, "top_p": 0.9, "min_p": 0.001}):
+        check(x, u, dtype, **options)
+    check(x, uniforms(8, 2), dtype, temperature=[0.0, -1.0, nan, inf, 1e-45, 3e38, -inf, 1e-3])
+    check(x, uniforms(8, 3), dtype, top_p=[0.0, -1.0, 1.0, 2.0, nan, inf, -inf, 1e-30])
+    check(x, uniforms(8, 4), dtype, min_p=[0.0, -1.0, 1.0, 2.0, nan, inf, -inf, 1e-30])
+    check(x, uniforms(8, 5), dtype, top_k=[0, -1, 1, vocab, vocab + 1, 2**31 - 1, -2**31, vocab - 1])
+
+
 @pytest.mark.parametrize("vocab", [9, 700, 3000, 40000, 70000])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_only_the_largest_with_cuts(vocab, dtype):
